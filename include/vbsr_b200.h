@@ -268,6 +268,106 @@ vbsr_status vbsr_plan_work_info(const vbsr_plan* p, vbsr_plan_work* out);
 /* Number of CTAs (tasks) one execution launches. */
 vbsr_status vbsr_plan_num_tasks(const vbsr_plan* p, int* out);
 
+/* ---- Block-sparse layers of language models ------------------------------------------------ */
+
+/* No reference counterpart. A VBSR matrix is the weight of a block-sparse linear layer, and a dense
+ * column-major K x tokens panel (ld K) is the row-major [tokens, K] activation. The operators below
+ * work on such weights for any tokens >= 0 (0 does nothing; at most 2^22). Packed value arrays
+ * (gradients, updates, 8-bit weights) are in the reference's value layout: blocks in row order, each
+ * h x w block column-major, as HostMatrix::values.
+ *
+ * Every call is asynchronous on `stream` and allocates nothing. A call's temporary memory is the
+ * caller's workspace: device memory on the matrix's device, 256-byte aligned, at least as long as
+ * the plan's workspace function says for that number of tokens. The call keeps nothing in it for
+ * later, so calls on several streams, or in several captured graphs, are independent as long as
+ * each has its own workspace (and its own outputs). Outputs must not overlap inputs or one another
+ * unless stated. Panels need 4-byte alignment; 16-byte aligned ones are read and written faster. */
+
+enum {
+  VBSR_ACT_SILU = 0,   /* x / (1 + exp(-x))               */
+  VBSR_ACT_GELU = 1,   /* x (1 + erf(x / sqrt 2)) / 2     */
+  VBSR_ACT_RELU = 2,   /* max(x, 0), derivative 0 at 0    */
+  VBSR_ACT_SIGMOID = 3 /* 1 / (1 + exp(-x))               */
+};
+
+/* Gated feed-forward block: with G = A_gate B and U = A_up B, H = act(G) * U (element by element).
+ * Both matrices have the same block-row and block-column partition and device; their block patterns
+ * may differ. The plan keeps its own copy of both weights, taken from the matrices at creation and
+ * replaced by vbsr_gated_set_values; the matrices must outlive the plan (it reads their structure).
+ * Products are formed at FP32 accuracy. */
+typedef struct vbsr_gated vbsr_gated;
+vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, int activation,
+                              vbsr_gated** out);
+vbsr_status vbsr_gated_destroy(vbsr_gated* p);
+/* Replaces the weights by packed device arrays (value_count floats each), as after an optimiser
+ * step. Ordered on `stream`; calls of the plan on other streams must be ordered after it by the
+ * caller. */
+vbsr_status vbsr_gated_set_values(vbsr_gated* p, const float* gate_values, const float* up_values,
+                                  vbsr_stream_t stream);
+/* Workspace bytes of a forward call, or (backward != 0) the larger of a forward and a backward. */
+vbsr_status vbsr_gated_workspace_bytes(const vbsr_gated* p, int64_t tokens, int backward,
+                                       int64_t* bytes);
+/* H (M x tokens, ld M) = act(G) * U. G and U are optional (both or neither): when given, the
+ * pre-activations are written there for the backward pass. Rows without blocks have G = U = 0. */
+vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t tokens, float* H,
+                               float* G, float* U, void* workspace, int64_t workspace_bytes,
+                               vbsr_stream_t stream);
+/* Gradients of a scalar loss from dH (M x tokens), with the B of the forward call and its G and U:
+ *   dG = dH * U * act'(G), dU = dH * act(G); dB = A_gate^T dG + A_up^T dU (K x tokens);
+ *   dgate, dup: dG B^T and dU B^T at the blocks of each matrix, packed.
+ * dB, or dgate and dup together, may be NULL to leave that part out. Outputs are overwritten, not
+ * accumulated into. With tokens = 0 dgate and dup are set to zero. */
+vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float* G,
+                                const float* U, const float* dH, int64_t tokens, float* dB,
+                                float* dgate, float* dup, void* workspace,
+                                int64_t workspace_bytes, vbsr_stream_t stream);
+/* Synchronises `stream`, then reads and clears the plan's device status word: VBSR_OK, or
+ * VBSR_TIMEOUT if a bounded in-kernel wait gave up since the last check (outputs are then wrong). */
+vbsr_status vbsr_gated_check_status(const vbsr_gated* p, vbsr_stream_t stream);
+
+/* Product in 8-bit integers, C[r, t] = row_scale[r] * token_scale[t] * sum_k Aq[r, k] Q[k, t]: the
+ * sum is exact (32-bit integers), then rounded to fp32 and scaled. Weights are packed int8 device
+ * values with one scale per scalar row (output channel), laid out at creation; `m` gives the
+ * structure (its own values are not read) and must outlive the plan. A block row wider than
+ * 131072 columns in total could overflow the 32-bit sum and is refused. */
+typedef struct vbsr_int8 vbsr_int8;
+vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const float* row_scale,
+                             vbsr_int8** out);
+vbsr_status vbsr_int8_destroy(vbsr_int8* p);
+vbsr_status vbsr_int8_workspace_bytes(const vbsr_int8* p, int64_t tokens, int64_t* bytes);
+/* C from a quantised panel: Q is K x tokens int8 (ld K), token_scale has `tokens` floats. */
+vbsr_status vbsr_int8_execute(const vbsr_int8* p, const int8_t* Q, const float* token_scale,
+                              int64_t tokens, float* C, void* workspace, int64_t workspace_bytes,
+                              vbsr_stream_t stream);
+/* C from an fp32 panel, quantised within the call as vbsr_quantize_panel does. */
+vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t tokens, float* C,
+                                    void* workspace, int64_t workspace_bytes,
+                                    vbsr_stream_t stream);
+vbsr_status vbsr_int8_check_status(const vbsr_int8* p, vbsr_stream_t stream);
+/* Symmetric quantisation of a K x tokens panel, one scale per token:
+ *   token_scale[t] = max_k |B[k, t]| / 127 (fp32 division);
+ *   Q[k, t] = B[k, t] / token_scale[t] rounded to the nearest integer, ties to even, as of the exact
+ *   quotient, and clamped to [-127, 127]; a token whose scale is 0 has Q = 0.
+ * A token that holds a NaN or an infinity has scale NaN and Q = 0, so its products are NaN. Runs on
+ * the current device. */
+vbsr_status vbsr_quantize_panel(const float* B, int64_t K, int64_t tokens, int8_t* Q,
+                                float* token_scale, vbsr_stream_t stream);
+/* The same of the matrix's own weights, one scale per scalar row: packed int8 values and M scales,
+ * as vbsr_int8_create takes them. A row without blocks has scale 0. */
+vbsr_status vbsr_matrix_quantize(const vbsr_matrix* m, int8_t* values, float* row_scale,
+                                 vbsr_stream_t stream);
+
+/* Orthogonalised block update: every h x w block V of a packed value array (a gradient or momentum
+ * of the matrix's values) is replaced by `steps` Newton-Schulz steps
+ *   X = V / (|V|_F + eps); then X <- a X + (b A + c A A) X with A = X X^T
+ * with (a, b, c) = coefficients[0..2]. `out` may be `values` itself. A block of zeros gives zeros.
+ * steps in [0, 64]; `m` gives the structure and must outlive the plan. */
+typedef struct vbsr_ortho vbsr_ortho;
+vbsr_status vbsr_ortho_create(const vbsr_matrix* m, vbsr_ortho** out);
+vbsr_status vbsr_ortho_destroy(vbsr_ortho* p);
+vbsr_status vbsr_ortho_execute(const vbsr_ortho* p, const float* values, float* out, int steps,
+                               float eps, const float* coefficients, vbsr_stream_t stream);
+
 /* ---- Raw launchers kept for source compatibility ------------------------------------------ */
 
 /* launch_row_owned (row_owned.cu:397-423): C = A * B from a device view alone (no plan), one

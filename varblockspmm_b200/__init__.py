@@ -177,6 +177,24 @@ _sig = {
     "vbsr_multi_plan_execute": [_vp],
     "vbsr_multi_plan_synchronize": [_vp, C.POINTER(C.c_float)],
     "vbsr_multi_plan_gather_C": [_vp, _vp, C.c_int],
+    "vbsr_gated_create": [_vp, _vp, C.c_int, C.POINTER(_vp)],
+    "vbsr_gated_destroy": [_vp],
+    "vbsr_gated_set_values": [_vp, _vp, _vp, _vp],
+    "vbsr_gated_workspace_bytes": [_vp, C.c_int64, C.c_int, _p64],
+    "vbsr_gated_forward": [_vp, _vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_int64, _vp],
+    "vbsr_gated_backward": [_vp, _vp, _vp, _vp, _vp, C.c_int64, _vp, _vp, _vp, _vp, C.c_int64, _vp],
+    "vbsr_gated_check_status": [_vp, _vp],
+    "vbsr_int8_create": [_vp, _vp, _vp, C.POINTER(_vp)],
+    "vbsr_int8_destroy": [_vp],
+    "vbsr_int8_workspace_bytes": [_vp, C.c_int64, _p64],
+    "vbsr_int8_execute": [_vp, _vp, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp],
+    "vbsr_int8_execute_panel": [_vp, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp],
+    "vbsr_int8_check_status": [_vp, _vp],
+    "vbsr_quantize_panel": [_vp, C.c_int64, C.c_int64, _vp, _vp, _vp],
+    "vbsr_matrix_quantize": [_vp, _vp, _vp, _vp],
+    "vbsr_ortho_create": [_vp, C.POINTER(_vp)],
+    "vbsr_ortho_destroy": [_vp],
+    "vbsr_ortho_execute": [_vp, _vp, _vp, C.c_int, C.c_float, C.POINTER(C.c_float), _vp],
 }
 for _name, _args in _sig.items():
     _f = getattr(_lib, _name)
@@ -213,6 +231,14 @@ class Kernel(enum.IntEnum):
     Auto = 0
     RowOwned = 1
     SplitRow = 2
+
+
+class Activation(enum.IntEnum):
+    """Gate activations of GatedPlan."""
+    SiLU = 0
+    GELU = 1  # x (1 + erf(x / sqrt 2)) / 2
+    ReLU = 2
+    Sigmoid = 3
 
 
 # ---- host matrix -------------------------------------------------------------------------------
@@ -438,7 +464,7 @@ def compulsory_bytes(host: HostMatrix, rhs: int, r0: int = 0, r1: int | None = N
 
 # ---- device objects ----------------------------------------------------------------------------
 
-def _dev_ptr(x) -> int:
+def _dev_ptr(x, dtype: str = "float32") -> int:
     if x is None:
         return 0
     if isinstance(x, int):
@@ -446,8 +472,8 @@ def _dev_ptr(x) -> int:
     if hasattr(x, "data_ptr"):
         if not x.is_cuda:
             raise InvalidArgument("expected a CUDA tensor")
-        if x.dtype.__repr__() != "torch.float32":
-            raise InvalidArgument("expected a float32 tensor")
+        if x.dtype.__repr__() != "torch." + dtype:
+            raise InvalidArgument(f"expected a {dtype} tensor")
         if not x.is_contiguous():
             raise InvalidArgument("expected a contiguous tensor")
         return x.data_ptr()
@@ -616,6 +642,273 @@ class Plan:
             pass
 
 
+# ---- block-sparse layers of language models ----------------------------------------------------
+
+def _panel(x, rows: int, tokens: int, name: str, device: int, dtype: str = "float32") -> int:
+    """Device pointer of a rows x tokens column-major panel (a [tokens, rows] row-major tensor)."""
+    p = _dev_ptr(x, dtype)
+    if hasattr(x, "numel"):
+        if x.numel() != rows * tokens:
+            raise InvalidArgument(f"{name} has {x.numel()} elements, expected {rows} x {tokens}")
+        if rows > 1 and x.dim() > 1 and x.shape[-1] != rows:
+            raise InvalidArgument(f"{name} has shape {tuple(x.shape)}, expected [{tokens}, {rows}]")
+        if x.device.index != device:
+            raise InvalidArgument(f"{name} is on another device than the matrix")
+    return p
+
+
+def _tokens(x, rows: int, tokens: int | None, name: str) -> int:
+    """The number of tokens of a panel: given, or from the tensor's size."""
+    if tokens is not None:
+        return int(tokens)
+    if not hasattr(x, "numel"):
+        raise InvalidArgument(f"tokens must be given when {name} is a device pointer")
+    if x.numel() % rows:
+        raise InvalidArgument(f"{name} has {x.numel()} elements, expected a multiple of {rows}")
+    return x.numel() // rows
+
+
+def _empty(n: int, dtype: str, device: int, stream):
+    """A new tensor from torch's caching allocator, made on `stream` so that its memory is not handed
+    on before the work enqueued there has run."""
+    import torch
+    s = _stream_ptr(stream) or 0
+    with torch.cuda.device(device):
+        # 0 is the legacy default stream, which is torch's default stream
+        ts = torch.cuda.default_stream(device) if s == 0 else (
+            stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(s, device))
+        with torch.cuda.stream(ts):
+            return torch.empty(n, dtype=getattr(torch, dtype), device=f"cuda:{device}")
+
+
+def _workspace(nbytes: int, device: int, stream, given):
+    """(pointer, bytes, owner) of a call's workspace: the given uint8 tensor or (pointer, bytes), or a
+    new tensor."""
+    if given is not None:
+        if hasattr(given, "numel"):
+            p = _dev_ptr(given, "uint8")
+            if given.device.index != device:
+                raise InvalidArgument("workspace is on another device than the matrix")
+            return p, given.numel(), given
+        return int(given[0]), int(given[1]), given
+    if nbytes == 0:
+        return 0, 0, None
+    t = _empty(nbytes, "uint8", device, stream)
+    return t.data_ptr(), nbytes, t
+
+
+class GatedPlan:
+    """Gated feed-forward block on two VBSR weights, H = act(A_gate B) * (A_up B), with its backward
+    pass (vbsr_gated_*). No reference counterpart.
+
+        plan = GatedPlan(gate, up, Activation.SiLU)      # two Matrix of one block partition
+        plan.execute(X, H)                               # X [tokens, K], H [tokens, M]
+        plan.execute(X, H, G, U)                         # keeps the pre-activations for
+        plan.backward(X, G, U, dH, dX, dgate, dup)       # the gradients (dgate, dup packed)
+        plan.set_values(gate_values, up_values)          # packed weights after an update
+
+    Panels are K x tokens or M x tokens, column-major (a contiguous [tokens, K] tensor), for any
+    number of tokens. Calls are asynchronous on `stream` (None: the legacy default stream). Each
+    call's temporary memory is `workspace` (a uint8 CUDA tensor of workspace_bytes(tokens), or a
+    (pointer, bytes) pair), by default a new tensor per call; calls that may overlap, or captured
+    graphs that may run at the same time, need their own."""
+
+    def __init__(self, gate: Matrix, up: Matrix, activation: Activation = Activation.SiLU):
+        self._matrices = (gate, up)  # keep them alive
+        self._h = _vp()
+        _check(_lib.vbsr_gated_create(gate._h, up._h, int(activation), C.byref(self._h)))
+        info, self._up_values = gate.info(), up.info().value_count
+        self._gate_values, self._device = info.value_count, info.device
+        self._M, self._K = info.scalar_rows, info.scalar_cols
+
+    def workspace_bytes(self, tokens: int, backward: bool = False) -> int:
+        n = C.c_int64()
+        _check(_lib.vbsr_gated_workspace_bytes(self._h, tokens, int(backward), C.byref(n)))
+        return n.value
+
+    def _flat(self, x, n, name):
+        return _panel(x, n, 1, name, self._device)
+
+    def set_values(self, gate_values, up_values, stream=None):
+        """Replaces the weights by packed device arrays (the layout of HostMatrix.values)."""
+        _check(_lib.vbsr_gated_set_values(self._h,
+                                          self._flat(gate_values, self._gate_values, "gate_values"),
+                                          self._flat(up_values, self._up_values, "up_values"),
+                                          _stream_ptr(stream)))
+
+    def execute(self, B, H, G=None, U=None, tokens=None, workspace=None, stream=None):
+        """H = act(G) * U with G = A_gate B, U = A_up B; G and U are written when given."""
+        T = _tokens(B, self._K, tokens, "B")
+        ws, nb, _own = _workspace(0 if workspace is not None else self.workspace_bytes(T),
+                                  self._device, stream, workspace)
+        dev, M = self._device, self._M
+        _check(_lib.vbsr_gated_forward(self._h, _panel(B, self._K, T, "B", dev), T,
+                                       _panel(H, M, T, "H", dev), _panel(G, M, T, "G", dev),
+                                       _panel(U, M, T, "U", dev), ws, nb, _stream_ptr(stream)))
+
+    def backward(self, B, G, U, dH, dB=None, dgate=None, dup=None, tokens=None, workspace=None,
+                 stream=None):
+        """Gradients from dH: dB = A_gate^T dG + A_up^T dU, and dgate = dG B^T, dup = dU B^T at the
+        matrices' blocks (packed). dB, or dgate and dup together, may be left out."""
+        T = _tokens(B, self._K, tokens, "B")
+        ws, nb, _own = _workspace(0 if workspace is not None else self.workspace_bytes(T, True),
+                                  self._device, stream, workspace)
+        dev, M = self._device, self._M
+        _check(_lib.vbsr_gated_backward(
+            self._h, _panel(B, self._K, T, "B", dev), _panel(G, M, T, "G", dev),
+            _panel(U, M, T, "U", dev), _panel(dH, M, T, "dH", dev), T,
+            _panel(dB, self._K, T, "dB", dev), self._flat(dgate, self._gate_values, "dgate"),
+            self._flat(dup, self._up_values, "dup"), ws, nb, _stream_ptr(stream)))
+
+    def check_status(self, stream=None):
+        """Synchronises `stream` and raises if a kernel of the plan recorded a timeout."""
+        _check(_lib.vbsr_gated_check_status(self._h, _stream_ptr(stream)))
+
+    def close(self):
+        if self._h:
+            _lib.vbsr_gated_destroy(self._h)
+            self._h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Int8Plan:
+    """Product with 8-bit weights, C[r, t] = row_scale[r] token_scale[t] sum_k Aq[r, k] Q[k, t], the
+    sum exact in 32-bit integers (vbsr_int8_*). No reference counterpart.
+
+        q, s = quantize_values(matrix)                   # or weights quantised elsewhere
+        plan = Int8Plan(matrix, q, s)
+        plan.execute_panel(X, C)                         # X [tokens, K] float32, quantised per token
+        plan.execute(Q, token_scale, C)                  # or an int8 panel with its scales
+
+    `matrix` gives the structure (its own values are not read). Streams and workspaces as for
+    GatedPlan."""
+
+    def __init__(self, matrix: Matrix, values, row_scale):
+        self._matrix = matrix  # keep it alive
+        self._h = _vp()
+        info = matrix.info()
+        self._M, self._K, self._device = info.scalar_rows, info.scalar_cols, info.device
+        v = _panel(values, info.value_count, 1, "values", self._device, "int8")
+        s = _panel(row_scale, self._M, 1, "row_scale", self._device)
+        if hasattr(values, "device"):
+            import torch
+            torch.cuda.current_stream(values.device).synchronize()  # the layout runs on its own
+        _check(_lib.vbsr_int8_create(matrix._h, v, s, C.byref(self._h)))
+
+    def workspace_bytes(self, tokens: int) -> int:
+        n = C.c_int64()
+        _check(_lib.vbsr_int8_workspace_bytes(self._h, tokens, C.byref(n)))
+        return n.value
+
+    def execute(self, Q, token_scale, C_out, tokens=None, workspace=None, stream=None):
+        """C from a quantised panel Q (int8, K x tokens) and one scale per token."""
+        T = _tokens(Q, self._K, tokens, "Q")
+        ws, nb, _own = _workspace(0 if workspace is not None else self.workspace_bytes(T),
+                                  self._device, stream, workspace)
+        dev = self._device
+        _check(_lib.vbsr_int8_execute(self._h, _panel(Q, self._K, T, "Q", dev, "int8"),
+                                      _panel(token_scale, 1, T, "token_scale", dev), T,
+                                      _panel(C_out, self._M, T, "C", dev), ws, nb,
+                                      _stream_ptr(stream)))
+
+    def execute_panel(self, B, C_out, tokens=None, workspace=None, stream=None):
+        """C from a float32 panel, quantised within the call as quantize_panel does."""
+        T = _tokens(B, self._K, tokens, "B")
+        ws, nb, _own = _workspace(0 if workspace is not None else self.workspace_bytes(T),
+                                  self._device, stream, workspace)
+        dev = self._device
+        _check(_lib.vbsr_int8_execute_panel(self._h, _panel(B, self._K, T, "B", dev), T,
+                                            _panel(C_out, self._M, T, "C", dev), ws, nb,
+                                            _stream_ptr(stream)))
+
+    def check_status(self, stream=None):
+        """Synchronises `stream` and raises if a kernel of the plan recorded a timeout."""
+        _check(_lib.vbsr_int8_check_status(self._h, _stream_ptr(stream)))
+
+    def close(self):
+        if self._h:
+            _lib.vbsr_int8_destroy(self._h)
+            self._h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def quantize_panel(B, Q, token_scale, K: int, tokens=None, stream=None):
+    """Symmetric 8-bit quantisation of a K x tokens panel, one scale per token (see
+    vbsr_quantize_panel). Tensors decide the device; raw pointers are on the current one."""
+    T = _tokens(B, K, tokens, "B")
+    _dev_ptr(B)  # refuses a tensor that is not on a GPU
+    dev = B.device.index if hasattr(B, "device") else -1
+
+    def call():
+        _check(_lib.vbsr_quantize_panel(_panel(B, K, T, "B", dev), K, T,
+                                        _panel(Q, K, T, "Q", dev, "int8"),
+                                        _panel(token_scale, 1, T, "token_scale", dev),
+                                        _stream_ptr(stream)))
+    if dev < 0:
+        return call()
+    import torch
+    with torch.cuda.device(dev):
+        call()
+
+
+def quantize_values(matrix: Matrix, stream=None):
+    """(packed int8 values, row scales) of the matrix's own weights as new CUDA tensors, symmetric
+    with one scale per scalar row, as Int8Plan takes them."""
+    info = matrix.info()
+    q = _empty(info.value_count, "int8", info.device, stream)
+    s = _empty(info.scalar_rows, "float32", info.device, stream)
+    _check(_lib.vbsr_matrix_quantize(matrix._h, q.data_ptr(), s.data_ptr(), _stream_ptr(stream)))
+    return q, s
+
+
+class OrthoPlan:
+    """Orthogonalised block updates: `steps` Newton-Schulz steps on every block of a packed value
+    array (a gradient or momentum of the matrix's values; vbsr_ortho_*). No reference counterpart.
+
+        plan = OrthoPlan(matrix)
+        plan.execute(dgate, update)                      # update may be dgate itself
+    """
+
+    def __init__(self, matrix: Matrix):
+        self._matrix = matrix  # keep it alive
+        self._h = _vp()
+        info = matrix.info()
+        self._values, self._device = info.value_count, info.device
+        _check(_lib.vbsr_ortho_create(matrix._h, C.byref(self._h)))
+
+    def execute(self, values, out, steps: int = 5, eps: float = 1e-7,
+                coefficients=(3.4445, -4.7750, 2.0315), stream=None):
+        """Per block V: X = V / (|V| + eps), then `steps` times X <- a X + (b A + c A A) X with
+        A = X X^T and (a, b, c) = coefficients."""
+        if len(coefficients) != 3:
+            raise InvalidArgument("coefficients are three numbers")
+        _check(_lib.vbsr_ortho_execute(self._h, _panel(values, self._values, 1, "values", self._device),
+                                       _panel(out, self._values, 1, "out", self._device), int(steps),
+                                       float(eps), (C.c_float * 3)(*coefficients),
+                                       _stream_ptr(stream)))
+
+    def close(self):
+        if self._h:
+            _lib.vbsr_ortho_destroy(self._h)
+            self._h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class MultiPlan:
     """Multi-GPU plan: the block rows of `host` split into len(devices) balanced shards, one per
     entry of `devices` (entries may repeat), each with its own plan, B replica, C block and
@@ -730,6 +1023,7 @@ __all__ = [
     "HostMatrix", "DeviceMatrix", "Matrix", "Distribution", "Profile", "GeneratorOptions",
     "generate", "Kernel", "PlanOptions", "Plan", "launch_row_owned", "launch_row_owned_scalar",
     "partition_rows", "compulsory_bytes", "fill_uniform", "fill_uniform_device", "fill_mt19937",
+    "Activation", "GatedPlan", "Int8Plan", "OrthoPlan", "quantize_panel", "quantize_values",
     "from_csr", "load_matrix_market", "load_matrix", "block_sizes",
     "InvalidArgument", "CudaError", "VbsrError", "TimeoutError_", "BoundsViolation", "last_error",
     "STREAM_VALUES", "STREAM_DENSE", "PLAN_BOUNDS_CHECK", "PLAN_NO_SPLIT", "LIB_PATH",

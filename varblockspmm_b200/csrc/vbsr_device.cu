@@ -29,26 +29,6 @@ using namespace vbsr_b200;
 
 namespace {
 
-// ---- error helpers -------------------------------------------------------------------------------
-
-#define VBSR_CUDA(call)                                                          \
-  do {                                                                           \
-    const cudaError_t e_ = (call);                                               \
-    if (e_ != cudaSuccess) return set_error(VBSR_CUDA_ERROR, cudaGetErrorString(e_)); \
-  } while (0)
-
-// Restores the caller's current device on scope exit.
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (dev >= 0 && dev != prev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) cudaSetDevice(prev);
-  }
-};
-
 // ---- format kernels ------------------------------------------------------------------------------
 
 // Row of block b (binary search over the matrix-local row_ptr).
@@ -325,6 +305,8 @@ vbsr_status build_matrix(const vbsr_host_matrix_view* v, int r0, int r1, int mod
       d.h_row_off[i] = v->row_scalar_off[r0 + i] - v->row_scalar_off[r0];
     }
     std::vector<int64_t> voff(size_t(d.nnzb) + 1);
+    d.h_block_col.assign(v->block_col + b0, v->block_col + b1);
+    d.h_col_size.assign(v->col_size, v->col_size + S);
     std::vector<uint32_t>& desc = d.h_blk_desc;
     desc.resize(d.nnzb);
     for (int64_t b = 0; b <= d.nnzb; ++b) voff[b] = v->value_off[b0 + b] - v0;

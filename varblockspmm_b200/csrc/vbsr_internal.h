@@ -84,6 +84,27 @@ inline uint32_t pack_block(int64_t col_off, int w) { return uint32_t(col_off) | 
 // Device status word layout.
 enum { kStatusCode = 0, kStatusInfo = 1, kStatusWords = 4 };
 
+// ---- errors and device selection in the CUDA sources -------------------------------------------
+#define VBSR_CUDA(call)                                                          \
+  do {                                                                           \
+    const cudaError_t e_ = (call);                                               \
+    if (e_ != cudaSuccess) return set_error(VBSR_CUDA_ERROR, cudaGetErrorString(e_)); \
+  } while (0)
+
+#if defined(__CUDACC__)
+// Restores the caller's current device on scope exit.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    cudaGetDevice(&prev);
+    if (dev >= 0 && dev != prev) cudaSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+#endif
+
 // ---- owning matrix -------------------------------------------------------------------------
 struct MatrixData {
   int device = 0;
@@ -93,6 +114,7 @@ struct MatrixData {
   std::vector<int32_t> h_row_ptr, h_row_size;
   std::vector<int64_t> h_row_off, h_val_off_row, h_sum_w;
   std::vector<uint32_t> h_blk_desc;  // per block: col_scalar_off | (w/8 - 1)
+  std::vector<int32_t> h_block_col, h_col_size;
   // device arrays in the reference layout (device_view) ...
   int32_t *d_row_ptr = nullptr, *d_block_col = nullptr, *d_row_size = nullptr,
           *d_col_size = nullptr;

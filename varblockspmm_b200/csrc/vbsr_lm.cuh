@@ -1,0 +1,94 @@
+// vbsr_lm.cuh — pieces shared by the operators for block-sparse layers of language models
+// (vbsr_gated.cu, vbsr_int8.cu, vbsr_ortho.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "vbsr_internal.h"
+
+namespace vbsr_b200 {
+
+constexpr int64_t kMaxTokens = int64_t(1) << 22;
+
+inline int64_t align256(int64_t bytes) { return (bytes + 255) & ~int64_t(255); }
+
+inline vbsr_status check_workspace(const void* ws, int64_t bytes, int64_t need) {
+  if (need == 0) return VBSR_OK;
+  if (ws == nullptr || bytes < need)
+    return set_error(VBSR_INVALID_ARGUMENT, "workspace too small: " + std::to_string(need) +
+                                                " bytes are needed");
+  if (reinterpret_cast<uintptr_t>(ws) & 255u)
+    return set_error(VBSR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+  return VBSR_OK;
+}
+
+// Device copy of a host array (one element at least).
+template <class T>
+cudaError_t upload_array(T** dst, const std::vector<T>& src) {
+  const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(dst),
+                                   (src.empty() ? 1 : src.size()) * sizeof(T));
+  if (e != cudaSuccess || src.empty()) return e;
+  return cudaMemcpy(*dst, src.data(), src.size() * sizeof(T), cudaMemcpyHostToDevice);
+}
+
+// Reads and clears a plan's device status word after the work on `s`.
+inline vbsr_status read_status(int* d_status, cudaStream_t s) {
+  int st[kStatusWords] = {};
+  VBSR_CUDA(cudaMemcpyAsync(st, d_status, sizeof(st), cudaMemcpyDeviceToHost, s));
+  VBSR_CUDA(cudaMemsetAsync(d_status, 0, sizeof(st), s));
+  VBSR_CUDA(cudaStreamSynchronize(s));
+  if (st[kStatusCode] == VBSR_OK) return VBSR_OK;
+  if (st[kStatusCode] == VBSR_TIMEOUT)
+    return set_error(VBSR_TIMEOUT, "an in-kernel wait gave up (CTA " +
+                                       std::to_string(st[kStatusInfo]) + ")");
+  return set_error(VBSR_CUDA_ERROR, "kernel status " + std::to_string(st[kStatusCode]));
+}
+
+// Non-owning view of a matrix's device arrays (values in the device format).
+inline vbsr_device_matrix view_of(const MatrixData& d) {
+  return {d.block_rows, d.block_cols, int32_t(d.nnzb), d.M, d.K, d.d_row_ptr, d.d_block_col,
+          d.d_row_size, d.d_col_size, d.d_row_off, d.d_col_off, d.d_value_off, d.d_values};
+}
+
+// Row of block b: row_ptr[row] <= b < row_ptr[row + 1].
+__device__ __forceinline__ int row_of_block(const int32_t* row_ptr, int rows, int b) {
+  int lo = 0, hi = rows;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (row_ptr[mid] <= b) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// An activation and its derivative. expf overflows to infinity for x < -88, where silu and sigmoid
+// are then 0, as they should be; the derivative of silu is written without infinity times zero.
+__device__ __forceinline__ void act_both(int act, float x, float& a, float& da) {
+  if (act == VBSR_ACT_RELU) {
+    a = x > 0.0f ? x : (x != x ? x : 0.0f);
+    da = x > 0.0f ? 1.0f : 0.0f;
+  } else if (act == VBSR_ACT_GELU) {
+    const float cdf = 0.5f * (1.0f + erff(x * 0.70710678118654752f));
+    a = x * cdf;
+    da = cdf + x * expf(-0.5f * x * x) * 0.39894228040143268f;
+  } else {
+    const float s = 1.0f / (1.0f + expf(-x));
+    if (act == VBSR_ACT_SIGMOID) {
+      a = s;
+      da = s * (1.0f - s);
+    } else {
+      a = x * s;
+      da = s * (1.0f + x * (1.0f - s));
+    }
+  }
+}
+__device__ __forceinline__ float act_value(int act, float x) {
+  float a, da;
+  act_both(act, x, a, da);
+  return a;
+}
+
+}  // namespace vbsr_b200
