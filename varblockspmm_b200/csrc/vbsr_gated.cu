@@ -3,156 +3,286 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "vbsr_internal.h"
 #include "vbsr_lm.cuh"
-#include "vbsr_tiles.h"
+#include "vbsr_pair.cuh"
+#include "vbsr_panels.cuh"
 
 using namespace vbsr_b200;
 
 struct vbsr_gated {
   const vbsr_matrix *gate = nullptr, *up = nullptr;
-  int device = 0, act = 0;
-  int32_t block_cols = 0;
+  int device = 0, act = 0, num_sm = 148;
   int64_t M = 0, K = 0;
-  float* values[2] = {nullptr, nullptr};  // packed weights: gate, up
-  // blocks by block column, gate then up: col_ptr[2 * j + which] .. col_ptr[2 * j + which + 1]
-  int32_t* d_col_ptr = nullptr;
-  int32_t* d_col_blk = nullptr;
-  int32_t* d_col_row = nullptr;
+  char* w = nullptr;      // both weights in pairs
+  int64_t up_byte = 0;    // where up's begin
+  int* w_exp = nullptr;   // their exponent
+  float* w_partial = nullptr;
+  uint32_t* group_col = nullptr;
+  PackRow* pack = nullptr;
+  int pack_rows = 0;
+  // work units with every block row (column) whole, and cut into 2, 4 and 8 parts
+  RowUnit* rows[4] = {};
+  int row_units[4] = {};
+  ColUnit* cols[4] = {};
+  int col_units[4] = {};
+  ColEntry* entries = nullptr;
+  GradUnit* grads = nullptr;
+  int grad_units = 0;
   int* d_status = nullptr;
 };
 
 namespace {
 
-constexpr int kTok = 8;  // tokens per CTA
+// Geometry of a call's panels.
+struct Panels {
+  int R = 0;        // tokens per tile
+  int64_t tiles = 0;
+  int64_t x_at = 0, dy_at = 0, bytes = 0;
+};
+constexpr int64_t kPartialBytes = 4 * kAmaxCtas + (256 - 4 * kAmaxCtas % 256) % 256;
 
-// Packed values of a matrix from its device format.
-__global__ void unpack_blocks(vbsr_device_matrix a, float* out) {
-  const int b = blockIdx.x;
-  const int h = a.row_size[row_of_block(a.row_ptr, a.block_rows, b)], w = a.col_size[a.block_col[b]];
-  const long long vo = a.value_off[b];
-  for (int i = threadIdx.x; i < h * w; i += blockDim.x)
-    out[vo + i] = a.values[vo + blk_pos(h, w, i % h, i / h)];
+// Tiles of at most 128 tokens, as even as their step allows: 8 tokens (core matrices), or 16 where
+// the tokens are summed over (K = 16).
+Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
+  Panels g;
+  if (tokens == 0) return g;
+  const int64_t step = backward ? 16 : 8;
+  g.tiles = (tokens + 127) / 128;
+  g.R = int(((tokens + g.tiles - 1) / g.tiles + step - 1) / step * step);
+  g.x_at = 2 * kPartialBytes + 256;  // largest magnitudes of both panels, exponents
+  g.dy_at = g.x_at + align256(g.tiles * g.R * (p->K / 8) * 32);
+  g.bytes = backward ? g.dy_at + align256(g.tiles * g.R * (p->M / 4) * 32) : g.dy_at;
+  return g;
 }
 
-// One CTA per block row and kTok tokens; a thread sums one (row, token) of G and U.
-__global__ void gated_forward_kernel(vbsr_device_matrix ga, vbsr_device_matrix ua, const float* gv,
-                                     const float* uv, const float* B, long long tokens, int act,
-                                     float* H, float* G, float* U) {
-  const int row = blockIdx.x, h = ga.row_size[row];
-  const long long M = ga.scalar_rows, K = ga.scalar_cols, t0 = (long long)blockIdx.y * kTok;
-  for (int i = threadIdx.x; i < h * kTok; i += blockDim.x) {
-    const int r = i % h;
-    const long long t = t0 + i / h;
-    if (t >= tokens) continue;
-    float s[2];
-    for (int which = 0; which < 2; ++which) {
-      const vbsr_device_matrix& a = which ? ua : ga;
-      const float* v = which ? uv : gv;
-      float sum = 0.0f;
-      for (int b = a.row_ptr[row]; b < a.row_ptr[row + 1]; ++b) {
-        const int c = a.block_col[b], w = a.col_size[c];
-        const float* x = B + t * K + a.col_scalar_off[c];
-        const float* av = v + a.value_off[b] + r;
-        float part = 0.0f;
-        for (int k = 0; k < w; ++k) part = fmaf(av[(long long)k * h], x[k], part);
-        sum += part;
-      }
-      s[which] = sum;
-    }
-    const long long o = t * M + ga.row_scalar_off[row] + r;
-    H[o] = act_value(act, s[0]) * s[1];
-    if (G != nullptr) {
-      G[o] = s[0];
-      U[o] = s[1];
-    }
+int ctas_for(int64_t threads, int most) {
+  return int(std::max<int64_t>(1, std::min<int64_t>(most, (threads + 255) / 256)));
+}
+
+// Fewest parts per row (column) that give every SM a few work items: a part streams only its share
+// of the weights but all the activations, so more parts than needed cost activation traffic.
+int parts_for(const int (&units)[4], int64_t tiles, int num_sm) {
+  int f = 0;
+  while (f < 3 && units[f] * tiles < 3 * int64_t(num_sm)) ++f;
+  return f;
+}
+
+template <int MODE>
+vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s) {
+  if (k.units == 0) return VBSR_OK;
+  const int64_t most = MODE == kWeightGrad ? tiles : std::max<int64_t>(1, (int64_t(1) << 30) / k.units);
+  for (int64_t t0 = 0; t0 < tiles; t0 += most) {
+    k.tile0 = int(t0);
+    k.tiles = int(std::min(most, tiles - t0));
+    const int64_t items = MODE == kWeightGrad ? k.units : int64_t(k.units) * k.tiles;
+    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, pair_smem<MODE>(), s>>>(k);
+    VBSR_CUDA(cudaGetLastError());
   }
+  return VBSR_OK;
 }
 
-__global__ void gated_dact_kernel(const float* G, const float* U, const float* dH, long long n,
-                                  int act, float* dG, float* dU) {
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n;
-       i += (long long)gridDim.x * blockDim.x) {
-    float a, da;
-    act_both(act, G[i], a, da);
-    dG[i] = dH[i] * U[i] * da;
-    dU[i] = dH[i] * a;
-  }
+PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char* ws) {
+  PairParams k{};
+  k.entries = p->entries;
+  k.group_col = p->group_col;
+  k.R = g.R;
+  k.act = p->act;
+  k.tokens = tokens;
+  k.M = p->M;
+  k.K = p->K;
+  k.x = ws + g.x_at;
+  k.dy = ws + g.dy_at;
+  k.w = p->w;
+  k.exps = reinterpret_cast<const int*>(ws + 2 * kPartialBytes);
+  k.w_exp = p->w_exp;
+  k.status = p->d_status;
+  return k;
 }
 
-// One CTA per block column and kTok tokens: dB = A_gate^T dG + A_up^T dU.
-__global__ void gated_dinput_kernel(vbsr_device_matrix ga, vbsr_device_matrix ua, const float* gv,
-                                    const float* uv, const int32_t* col_ptr, const int32_t* col_blk,
-                                    const int32_t* col_row, const float* dG, const float* dU,
-                                    long long tokens, float* dB) {
-  const int col = blockIdx.x, w = ga.col_size[col];
-  const long long M = ga.scalar_rows, K = ga.scalar_cols, t0 = (long long)blockIdx.y * kTok;
-  for (int i = threadIdx.x; i < w * kTok; i += blockDim.x) {
-    const int c = i % w;
-    const long long t = t0 + i / w;
-    if (t >= tokens) continue;
-    float sum = 0.0f;
-    for (int which = 0; which < 2; ++which) {
-      const vbsr_device_matrix& a = which ? ua : ga;
-      const float* v = which ? uv : gv;
-      const float* dy = (which ? dU : dG) + t * M;
-      for (int e = col_ptr[2 * col + which]; e < col_ptr[2 * col + which + 1]; ++e) {
-        const int row = col_row[e], h = a.row_size[row];
-        const float* av = v + a.value_off[col_blk[e]] + (long long)c * h;
-        const float* d = dy + a.row_scalar_off[row];
-        float part = 0.0f;
-        for (int r = 0; r < h; ++r) part = fmaf(av[r], d[r], part);
-        sum += part;
-      }
-    }
-    dB[t * K + ga.col_scalar_off[col] + c] = sum;
-  }
+// A panel in pairs: its largest magnitude, then the pairs. which: 0 the activations, 1 the gradients.
+template <class Source>
+vbsr_status make_panel(const Source& src, const Panels& g, int64_t tokens, char* ws, int which,
+                       cudaStream_t s) {
+  float* partial = reinterpret_cast<float*>(ws + which * kPartialBytes);
+  int* exponent = reinterpret_cast<int*>(ws + 2 * kPartialBytes) + which;
+  const int64_t groups = src.features / 8;
+  const int n = ctas_for(groups * tokens, kAmaxCtas);
+  panel_amax_kernel<<<n, 256, 0, s>>>(src, tokens, partial);
+  panel_pair_kernel<<<ctas_for(groups * g.tiles * g.R, 148 * 16), 256, 0, s>>>(
+      src, tokens, g.R, int(g.tiles), partial, n,
+      reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at)), exponent);
+  VBSR_CUDA(cudaGetLastError());
+  return VBSR_OK;
 }
 
-// One CTA per block: dA = dY B^T at its h x w elements.
-__global__ void gated_dweight_kernel(vbsr_device_matrix a, const float* B, const float* dY,
-                                     long long tokens, float* out) {
-  const int b = blockIdx.x, row = row_of_block(a.row_ptr, a.block_rows, b), c = a.block_col[b];
-  const int h = a.row_size[row], w = a.col_size[c];
-  for (int i = threadIdx.x; i < h * w; i += blockDim.x) {
-    const float* d = dY + a.row_scalar_off[row] + i % h;
-    const float* x = B + a.col_scalar_off[c] + i / h;
-    float sum = 0.0f;
-    for (long long t = 0; t < tokens; ++t) sum = fmaf(d[t * a.scalar_rows], x[t * a.scalar_cols], sum);
-    out[a.value_off[b] + i] = sum;
-  }
+template <class... P>
+int aligned16(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
 }
 
-int64_t dact_bytes(const vbsr_gated* p, int64_t tokens) { return align256(4 * p->M * tokens); }
+template <bool DEVICE>
+vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cudaStream_t s) {
+  const int64_t ng = p->gate->d.nvalues, nu = p->up->d.nvalues;
+  const int n = ctas_for((ng + nu) / 8, kAmaxCtas);
+  values_amax_kernel<<<n, 256, 0, s>>>(gate, ng, up, nu, p->w_partial);
+  pack_kernel<DEVICE><<<p->pack_rows, 256, 0, s>>>(p->pack, gate, up, p->up_byte, p->w_partial, n, p->w,
+                                                   p->w_exp);
+  VBSR_CUDA(cudaGetLastError());
+  return VBSR_OK;
+}
+
+template <class T>
+cudaError_t upload_units(T** dst, int* count, const std::vector<T>& v) {
+  *count = int(v.size());
+  return upload_array(dst, v);
+}
 
 vbsr_status build_gated(vbsr_gated* p) {
   const MatrixData* m[2] = {&p->gate->d, &p->up->d};
-  const int S = p->block_cols;
-  std::vector<int32_t> ptr(size_t(2) * S + 1, 0);
-  for (int which = 0; which < 2; ++which)
-    for (int32_t c : m[which]->h_block_col) ++ptr[2 * size_t(c) + which + 1];
-  for (size_t i = 1; i < ptr.size(); ++i) ptr[i] += ptr[i - 1];
-  std::vector<int32_t> blk(std::max(1, ptr.back())), row(blk.size()), at(ptr.begin(), ptr.end() - 1);
-  for (int which = 0; which < 2; ++which)
-    for (int i = 0; i < m[which]->block_rows; ++i)
-      for (int b = m[which]->h_row_ptr[i]; b < m[which]->h_row_ptr[i + 1]; ++b) {
-        const int e = at[2 * size_t(m[which]->h_block_col[b]) + which]++;
-        blk[e] = b;
-        row[e] = i;
+  const int R = m[0]->block_rows, S = m[0]->block_cols;
+  VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
+  for (const void* k : {reinterpret_cast<const void*>(pair_kernel<kForward>),
+                        reinterpret_cast<const void*>(pair_kernel<kInputGrad>),
+                        reinterpret_cast<const void*>(pair_kernel<kWeightGrad>)})
+    VBSR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   std::max(pair_smem<kForward>(), pair_smem<kInputGrad>())));
+  p->up_byte = align256(4 * m[0]->nvalues);
+
+  // group lists, block rows of both matrices
+  std::vector<uint32_t> group_col;
+  std::vector<uint32_t> g0[2], ng[2];
+  std::vector<PackRow> pack;
+  for (int which = 0; which < 2; ++which) {
+    const MatrixData& d = *m[which];
+    for (int i = 0; i < R; ++i) {
+      g0[which].push_back(uint32_t(group_col.size()));
+      for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
+        const uint32_t col8 = d.h_blk_desc[b] >> 3, n = (d.h_blk_desc[b] & 7u) + 1u;
+        for (uint32_t c = 0; c < n; ++c) group_col.push_back(col8 + c);
       }
-  VBSR_CUDA(upload_array(&p->d_col_ptr, ptr));
-  VBSR_CUDA(upload_array(&p->d_col_blk, blk));
-  VBSR_CUDA(upload_array(&p->d_col_row, row));
+      ng[which].push_back(uint32_t(group_col.size()) - g0[which].back());
+      if (ng[which][i] > 0)
+        pack.push_back({uint64_t(d.h_val_off_row[i]), ng[which][i],
+                        uint32_t(d.h_row_size[i]) | uint32_t(which) << 8});
+    }
+  }
+  if (group_col.size() >= (size_t(1) << 31))
+    return set_error(VBSR_INVALID_ARGUMENT, "matrices exceed the plan's index range");
+  VBSR_CUDA(upload_array(&p->group_col, group_col));
+  p->pack_rows = int(std::max<size_t>(1, pack.size()));
+  if (pack.empty()) pack.push_back({0, 0, 8});
+  VBSR_CUDA(upload_array(&p->pack, pack));
+
+  // units, the largest first: the grid strides over them, which evens out the SMs' shares
+  for (int f = 0; f < 4; ++f) {
+    std::vector<RowUnit> rows;
+    for (int i = 0; i < R; ++i) {
+      const int h = m[0]->h_row_size[i], hp = std::max(8, (h / 8 + (1 << f) - 1) / (1 << f) * 8);
+      for (int r0 = 0; r0 < h; r0 += hp) {
+        RowUnit u{};
+        u.row0 = uint32_t(m[0]->h_row_off[i] + r0);
+        u.shape = uint32_t(h) | uint32_t(std::min(hp, h - r0)) << 8 | uint32_t(r0) << 16;
+        for (int which = 0; which < 2; ++which) {
+          u.g0[which] = g0[which][i];
+          u.ng[which] = ng[which][i];
+          u.w0[which] = uint64_t(4 * m[which]->h_val_off_row[i] + (which ? p->up_byte : 0));
+        }
+        rows.push_back(u);
+      }
+    }
+    std::stable_sort(rows.begin(), rows.end(), [](const RowUnit& a, const RowUnit& b) {
+      auto cost = [](const RowUnit& u) {
+        return uint64_t(u.ng[0] + u.ng[1]) * (32 + ((u.shape >> 8) & 255u));
+      };
+      return cost(a) > cost(b);
+    });
+    VBSR_CUDA(upload_units(&p->rows[f], &p->row_units[f], rows));
+  }
+
+  // blocks by block column, gate then up, in stages of at most 64 rows
+  std::vector<std::vector<ColEntry>> by_col(S);
+  for (int which = 0; which < 2; ++which) {
+    const MatrixData& d = *m[which];
+    for (int i = 0; i < R; ++i) {
+      int64_t val = d.h_val_off_row[i];
+      for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
+        const int h = d.h_row_size[i], c = d.h_block_col[b];
+        by_col[c].push_back({uint32_t((which ? p->M / 8 : 0) + d.h_row_off[i] / 8), uint32_t(h / 8),
+                             uint64_t(4 * val + (which ? p->up_byte : 0))});
+        val += int64_t(h) * d.h_col_size[c];
+      }
+    }
+  }
+  std::vector<ColEntry> entries;
+  std::vector<ColUnit> whole(S);
+  std::vector<int64_t> col_rows(S, 0);
+  int64_t col0 = 0;
+  for (int c = 0; c < S; ++c) {
+    ColUnit& u = whole[c];
+    u.col0 = uint32_t(col0);
+    u.w = uint32_t(m[0]->h_col_size[c]);
+    u.s0 = uint32_t(entries.size() / kColEntries);
+    col0 += u.w;
+    uint32_t in_stage = 0, groups = 0;
+    for (const ColEntry& e : by_col[c]) {
+      if (in_stage == 0 || in_stage == kColEntries || groups + e.h8 > 8) {
+        entries.resize((entries.size() + kColEntries - 1) / kColEntries * kColEntries);
+        in_stage = groups = 0;
+        ++u.ns;
+      }
+      entries.push_back(e);
+      ++in_stage;
+      groups += e.h8;
+      col_rows[c] += 8 * e.h8;
+    }
+    entries.resize((entries.size() + kColEntries - 1) / kColEntries * kColEntries);
+  }
+  VBSR_CUDA(upload_array(&p->entries, entries));
+  for (int f = 0; f < 4; ++f) {
+    std::vector<std::pair<int64_t, ColUnit>> cols;
+    for (int c = 0; c < S; ++c) {
+      const int w = int(whole[c].w), wp = std::max(8, (w / 8 + (1 << f) - 1) / (1 << f) * 8);
+      for (int c0 = 0; c0 < w; c0 += wp) {
+        ColUnit u = whole[c];
+        u.c0 = uint32_t(c0);
+        u.col0 += u.c0;
+        u.w = uint32_t(std::min(wp, w - c0));
+        cols.push_back({-col_rows[c] * (32 + int64_t(u.w)), u});
+      }
+    }
+    std::stable_sort(cols.begin(), cols.end(),
+                     [](const auto& a, const auto& b) { return a.first < b.first; });
+    std::vector<ColUnit> sorted;
+    for (const auto& c : cols) sorted.push_back(c.second);
+    VBSR_CUDA(upload_units(&p->cols[f], &p->col_units[f], sorted));
+  }
+
+  // weight gradients: 16 groups (128 columns) of a block row at a time
+  std::vector<GradUnit> grads;
+  for (int which = 0; which < 2; ++which)
+    for (int i = 0; i < R; ++i)
+      for (uint32_t g = 0; g < ng[which][i]; g += 16) {
+        const int h = m[which]->h_row_size[i];
+        grads.push_back({g0[which][i] + g, std::min(16u, ng[which][i] - g),
+                         uint32_t((which ? p->M / 8 : 0) + m[which]->h_row_off[i] / 8), uint32_t(h),
+                         uint64_t(m[which]->h_val_off_row[i] + int64_t(g) * 8 * h), uint32_t(which), 0});
+      }
+  std::stable_sort(grads.begin(), grads.end(), [](const GradUnit& a, const GradUnit& b) {
+    return (32 + a.h) * (8 + a.ng) > (32 + b.h) * (8 + b.ng);
+  });
+  VBSR_CUDA(upload_units(&p->grads, &p->grad_units, grads));
+
   VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
   VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
-  for (int which = 0; which < 2; ++which) {
-    VBSR_CUDA(cudaMalloc(&p->values[which], 4 * std::max<int64_t>(1, m[which]->nvalues)));
-    if (m[which]->nnzb > 0)
-      unpack_blocks<<<unsigned(m[which]->nnzb), 256>>>(view_of(*m[which]), p->values[which]);
-  }
-  VBSR_CUDA(cudaGetLastError());
+  VBSR_CUDA(cudaMalloc(&p->w, p->up_byte + std::max<int64_t>(256, 4 * m[1]->nvalues)));
+  VBSR_CUDA(cudaMalloc(&p->w_exp, sizeof(int)));
+  VBSR_CUDA(cudaMalloc(&p->w_partial, kPartialBytes));
+  const vbsr_status st = pack_weights<true>(p, m[0]->d_values, m[1]->d_values, nullptr);
+  if (st != VBSR_OK) return st;
   VBSR_CUDA(cudaStreamSynchronize(nullptr));
   return VBSR_OK;
 }
@@ -160,11 +290,17 @@ vbsr_status build_gated(vbsr_gated* p) {
 void free_gated(vbsr_gated* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
-  cudaFree(p->values[0]);
-  cudaFree(p->values[1]);
-  cudaFree(p->d_col_ptr);
-  cudaFree(p->d_col_blk);
-  cudaFree(p->d_col_row);
+  cudaFree(p->w);
+  cudaFree(p->w_exp);
+  cudaFree(p->w_partial);
+  cudaFree(p->group_col);
+  cudaFree(p->pack);
+  for (int f = 0; f < 4; ++f) {
+    cudaFree(p->rows[f]);
+    cudaFree(p->cols[f]);
+  }
+  cudaFree(p->entries);
+  cudaFree(p->grads);
   cudaFree(p->d_status);
   delete p;
 }
@@ -201,7 +337,6 @@ vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, in
   p->up = up;
   p->device = g.device;
   p->act = activation;
-  p->block_cols = g.block_cols;
   p->M = g.M;
   p->K = g.K;
   DeviceGuard guard(p->device);
@@ -234,11 +369,7 @@ vbsr_status vbsr_gated_set_values(vbsr_gated* p, const float* gate_values, const
     return set_error(VBSR_INVALID_ARGUMENT, "null values");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  VBSR_CUDA(cudaMemcpyAsync(p->values[0], gate_values, 4 * p->gate->d.nvalues,
-                            cudaMemcpyDeviceToDevice, s));
-  VBSR_CUDA(cudaMemcpyAsync(p->values[1], up_values, 4 * p->up->d.nvalues,
-                            cudaMemcpyDeviceToDevice, s));
-  return VBSR_OK;
+  return pack_weights<false>(p, gate_values, up_values, s);
 }
 
 vbsr_status vbsr_gated_workspace_bytes(const vbsr_gated* p, int64_t tokens, int backward,
@@ -248,7 +379,7 @@ vbsr_status vbsr_gated_workspace_bytes(const vbsr_gated* p, int64_t tokens, int 
   if (bytes == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null output");
   if (tokens < 0 || tokens > kMaxTokens)
     return set_error(VBSR_INVALID_ARGUMENT, "tokens must be between 0 and 2^22");
-  *bytes = backward ? 2 * dact_bytes(p, tokens) : 0;
+  *bytes = std::max(panels_of(p, tokens, false).bytes, backward ? panels_of(p, tokens, true).bytes : 0);
   return VBSR_OK;
 }
 
@@ -264,18 +395,19 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
   if (B == nullptr || H == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null B or H");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const MatrixData &g = p->gate->d, &u = p->up->d;
-  const int64_t step = int64_t(kTok) * 65535;  // grid limit in y
-  for (int64_t t0 = 0; t0 < tokens; t0 += step) {
-    const int64_t n = std::min(step, tokens - t0);
-    const dim3 grid(g.block_rows, unsigned((n + kTok - 1) / kTok));
-    gated_forward_kernel<<<grid, 256, 0, s>>>(view_of(g), view_of(u), p->values[0], p->values[1],
-                                              B + t0 * p->K, n, p->act, H + t0 * p->M,
-                                              G ? G + t0 * p->M : nullptr,
-                                              U ? U + t0 * p->M : nullptr);
-    VBSR_CUDA(cudaGetLastError());
-  }
-  return VBSR_OK;
+  char* ws = static_cast<char*>(workspace);
+  const Panels g = panels_of(p, tokens, false);
+  const vbsr_status st2 = make_panel(PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0, s);
+  if (st2 != VBSR_OK) return st2;
+  PairParams k = params_of(p, g, tokens, ws);
+  const int f = parts_for(p->row_units, g.tiles, p->num_sm);
+  k.rows = p->rows[f];
+  k.units = p->row_units[f];
+  k.out0 = H;
+  k.out1 = G;
+  k.out2 = U;
+  k.vec = aligned16(H, G, U);
+  return launch_pair<kForward>(k, g.tiles, p->num_sm, s);
 }
 
 vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float* G,
@@ -300,25 +432,29 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
     }
     return VBSR_OK;
   }
-  float* dG = static_cast<float*>(workspace);
-  float* dU = reinterpret_cast<float*>(static_cast<char*>(workspace) + dact_bytes(p, tokens));
-  gated_dact_kernel<<<1184, 256, 0, s>>>(G, U, dH, p->M * tokens, p->act, dG, dU);
-  VBSR_CUDA(cudaGetLastError());
-  const int64_t step = int64_t(kTok) * 65535;
-  for (int64_t t0 = 0; dB != nullptr && t0 < tokens; t0 += step) {
-    const int64_t n = std::min(step, tokens - t0);
-    const dim3 grid(p->block_cols, unsigned((n + kTok - 1) / kTok));
-    gated_dinput_kernel<<<grid, 256, 0, s>>>(view_of(g), view_of(u), p->values[0], p->values[1],
-                                             p->d_col_ptr, p->d_col_blk, p->d_col_row,
-                                             dG + t0 * p->M, dU + t0 * p->M, n, dB + t0 * p->K);
-    VBSR_CUDA(cudaGetLastError());
+  char* ws = static_cast<char*>(workspace);
+  const Panels n = panels_of(p, tokens, true);
+  vbsr_status st2 = make_panel(GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1, s);
+  if (st2 != VBSR_OK) return st2;
+  PairParams k = params_of(p, n, tokens, ws);
+  if (dB != nullptr) {
+    const int f = parts_for(p->col_units, n.tiles, p->num_sm);
+    k.cols = p->cols[f];
+    k.units = p->col_units[f];
+    k.out0 = dB;
+    k.vec = aligned16(dB);
+    st2 = launch_pair<kInputGrad>(k, n.tiles, p->num_sm, s);
+    if (st2 != VBSR_OK) return st2;
   }
   if (dgate != nullptr) {
-    if (g.nnzb > 0)
-      gated_dweight_kernel<<<unsigned(g.nnzb), 256, 0, s>>>(view_of(g), B, dG, tokens, dgate);
-    if (u.nnzb > 0)
-      gated_dweight_kernel<<<unsigned(u.nnzb), 256, 0, s>>>(view_of(u), B, dU, tokens, dup);
-    VBSR_CUDA(cudaGetLastError());
+    st2 = make_panel(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 0, s);
+    if (st2 != VBSR_OK) return st2;
+    k.grads = p->grads;
+    k.units = p->grad_units;
+    k.out0 = dgate;
+    k.out1 = dup;
+    k.vec = aligned16(dgate, dup);
+    return launch_pair<kWeightGrad>(k, n.tiles, p->num_sm, s);
   }
   return VBSR_OK;
 }
