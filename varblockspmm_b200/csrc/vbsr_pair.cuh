@@ -25,16 +25,27 @@
 // groups, and an odd last one is paired with a tile of zeros (and, on the weights' side, with itself,
 // so that no stale bytes are multiplied).
 //
-// The kernel: one persistent CTA per SM; a producer warp (bulk copies into a ring of slots, and each
-// slot's list of MMA steps), one MMA thread that only works off those lists, four epilogue warps on
-// two accumulator buffers. Tokens are on the M side (64 or 128 rows): with weights there, blocks of
+// Accumulation. The tensor core cuts off (does not round) each step's sum: 36 steps of 16 products
+// into one accumulator were measured 1.1e-6 off (2-norm), against 2e-7 for fp32 arithmetic, and the
+// error grows with the number of steps. So an accumulator takes kChunkSteps steps or a little more
+// and is then added in fp32 registers by the epilogue warps, while the next steps go to another
+// accumulator.
+//
+// The kernel: one persistent CTA per SM. Four producer warps take turns with the stages: each issues
+// a stage's bulk copies into a slot of the ring and writes the slot's list of MMA steps (four, and a
+// stage's list of places fetched while the one before is issued, because that fetch takes about
+// as long as four stages take to stream). One MMA thread only works off those lists. Eight epilogue
+// warps, two per TMEM quadrant, take every second tile of 8 columns each. Tokens are on the M side (64 or 128 rows): with weights there, blocks of
 // 8 to 56 rows would leave most of an MMA empty. What bounds it: the copies into shared memory.
 // A weight group of 32 h bytes needs 32 R bytes of activations, from L2, so few tokens run at the
 // weights' HBM rate and many at the L2-to-shared-memory rate, h / 2 operations per byte.
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "vbsr_kernels_common.cuh"
+#include "vbsr_lm.cuh"
 
 namespace vbsr_b200 {
 
@@ -82,6 +93,7 @@ struct PairParams {
   int R, act;
   long long tokens, M, K;
   const char* x;              // activation panel in pairs (kInt8: in 16-column chunks)
+  long long x_chunks;         // kInt8: chunks per tile of it
   const char* dy;             // gradient panel in pairs
   const char* w;              // weights in pairs (kInt8: int8 chunks)
   const int* exps;            // exponents of x and dy: the call's
@@ -99,7 +111,6 @@ struct PairStep {
   u64 a, b;
 };
 constexpr u64 kStepFresh = 1ull << 60;  // first step into its accumulator: overwrite
-constexpr u64 kStepUp = 1ull << 59;     // second accumulator (up)
 constexpr u64 kStepOdd = 1ull << 58;    // the second K half of A is the tile of zeros
 constexpr u64 kStepMask = (1ull << 56) - 1;
 constexpr int kMaxSteps = 32;
@@ -109,10 +120,16 @@ constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17;
 
 template <int MODE>
 struct PairShape {
-  static constexpr int slots = MODE == kForward || MODE == kInt8 ? 8 : 4;
-  static constexpr int slot_bytes = MODE == kForward || MODE == kInt8 ? 24 * 1024 : 48 * 1024;
+  static constexpr bool rows = MODE == kForward || MODE == kInt8;
+  static constexpr int slots = rows ? 8 : 4;
+  static constexpr int slot_bytes = rows ? 24 * 1024 : 48 * 1024;
+  static constexpr int accs = rows ? 4 : 2;             // accumulators in TMEM
+  static constexpr uint32_t acc_cols = 512 / accs;
 };
-constexpr int kPairThreads = 256;
+constexpr int kProducers = 4;                      // warps 0 .. 3; the MMA thread is in warp 4
+constexpr int kEpilogueWarp = 8, kEpilogueWarps = 8;
+constexpr int kPairThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
+constexpr int kChunkSteps = 8;
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage
@@ -150,7 +167,7 @@ __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, ui
       : "memory");
 }
 
-// 8 accumulator columns each from one, three or four places, loaded and waited for in one statement
+// 8 accumulator columns each from one, two or three places, loaded and waited for in one statement
 // (the registers are not valid before the wait).
 __device__ __forceinline__ void tc_ld8_1(uint32_t a, float (&v)[8]) {
   asm volatile(
@@ -174,20 +191,15 @@ __device__ __forceinline__ void tc_ld8_3(uint32_t a, uint32_t b, uint32_t c, flo
       : "r"(a), "r"(b), "r"(c)
       : "memory");
 }
-__device__ __forceinline__ void tc_ld8_4(uint32_t a, uint32_t b, uint32_t c, uint32_t d,
-                                         float (&v)[8], float (&w)[8], float (&x)[8], float (&y)[8]) {
+__device__ __forceinline__ void tc_ld8_2(uint32_t a, uint32_t b, float (&v)[8], float (&w)[8]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
         "=f"(v[7]), "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]),
-        "=f"(w[6]), "=f"(w[7]), "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]),
-        "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]),
-        "=f"(y[4]), "=f"(y[5]), "=f"(y[6]), "=f"(y[7])
-      : "r"(a), "r"(b), "r"(c), "r"(d)
+        "=f"(w[6]), "=f"(w[7])
+      : "r"(a), "r"(b)
       : "memory");
 }
 
@@ -219,305 +231,351 @@ __device__ __forceinline__ void unscale(int e, float& f1, float& f2) {
   f2 = __int_as_float((b + 127) << 23);
 }
 
+// Stages and accumulation chunks of a row unit: groups per stage, stages per chunk.
+template <int MODE>
+struct RowStages {
+  int cap, per_chunk;
+  __device__ __forceinline__ RowStages(int R, int hp) {
+    const int b = (MODE == kInt8 ? 16 : 32) * (R + hp);
+    cap = PairShape<MODE>::slot_bytes / b;
+    const int most = MODE == kInt8 ? 32 : 2 * kChunkSteps;
+    cap = (cap < most ? cap : most) & ~1;
+    per_chunk = MODE == kInt8 ? 1 << 30 : (2 * kChunkSteps) / cap;
+  }
+  __device__ __forceinline__ int stages(int groups) const { return (groups + cap - 1) / cap; }
+  __device__ __forceinline__ int chunks(int groups) const {
+    return MODE == kInt8 ? (groups > 0) : (stages(groups) + per_chunk - 1) / per_chunk;
+  }
+};
+constexpr int kChunkStages = 2;  // kInputGrad, kWeightGrad: stages (of 4 or so steps) per chunk
+
+// The units of this CTA's work items, 32 at a time in the lanes' registers and the next 32 on their
+// way; get() broadcasts one.
+template <class Unit>
+struct UnitWin {
+  static constexpr int W = sizeof(Unit) / 16;
+  uint4 cur[W], next[W];
+  const Unit* units;
+  int items, tiles, first;
+  __device__ __forceinline__ void load(int k, uint4 (&v)[W]) const {
+    const long long item = blockIdx.x + (long long)k * gridDim.x;
+    if (item < items) {
+      const uint4* q = reinterpret_cast<const uint4*>(units + int(item) / tiles);
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = __ldg(q + i);
+    }
+  }
+  __device__ __forceinline__ void init(const Unit* u, int items_, int tiles_, int lane) {
+    units = u;
+    items = items_;
+    tiles = tiles_;
+    first = 0;
+    load(lane, cur);
+    load(32 + lane, next);
+  }
+  // the CTA's k-th item; k never decreases and grows by at most one
+  __device__ __forceinline__ Unit get(int k, int lane) {
+    if (k - first == 32) {
+      first += 32;
+#pragma unroll
+      for (int i = 0; i < W; ++i) cur[i] = next[i];
+      load(first + 32 + lane, next);
+    }
+    Unit u;
+    uint4* o = reinterpret_cast<uint4*>(&u);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      o[i].x = __shfl_sync(0xffffffffu, cur[i].x, k - first);
+      o[i].y = __shfl_sync(0xffffffffu, cur[i].y, k - first);
+      o[i].z = __shfl_sync(0xffffffffu, cur[i].z, k - first);
+      o[i].w = __shfl_sync(0xffffffffu, cur[i].w, k - first);
+    }
+    return u;
+  }
+};
+
 struct PairBars {
   uint32_t full, empty, acc_full, acc_empty, drain;  // first barrier of each array
 };
 
-// The producer's ring position.
-struct Ring {
-  uint32_t slot = 0, parity = 1;  // parity of the empty barrier to wait for
-  uint32_t filled = 0;            // stages issued
-  template <int SLOTS>
-  __device__ __forceinline__ void next() {
-    ++filled;
-    if (++slot == SLOTS) {
-      slot = 0;
-      parity ^= 1u;
-    }
-  }
-};
-
 struct PairShared {
-  u64 full[8], empty[8], acc_full[2], acc_empty[2], drain;
+  u64 full[8], empty[8], acc_full[4], acc_empty[4], drain;
   PairStep steps[8][kMaxSteps];
   uint32_t header[8];
   uint32_t tmem;
   volatile int abort_flag;
 };
 
-// ---- producer: kForward and kInt8 ----------------------------------------------------------------
+// ---- producers -----------------------------------------------------------------------------------
+//
+// Stage g of the CTA goes to slot g % SLOTS and is issued by warp g % kProducers. A warp fetches its
+// next stage's list before it issues the one in hand.
+
+template <int MODE>
+__device__ __forceinline__ bool wait_slot(const PairParams& p, PairShared& sh, const PairBars& bars,
+                                          uint32_t g) {
+  constexpr uint32_t SLOTS = PairShape<MODE>::slots;
+  return wait_warp(bars.empty + 8 * (g % SLOTS), ((g / SLOTS) & 1u) ^ 1u, p.status, &sh.abort_flag);
+}
+// Announces the slot's list and bytes; the lanes' list entries are written before.
+__device__ __forceinline__ void announce(PairShared& sh, uint32_t slot, uint32_t full, uint32_t header,
+                                         uint32_t bytes, int lane) {
+  if (lane == 0) sh.header[slot] = header;
+  __syncwarp();
+  if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+  __syncwarp();
+}
+// The end marker, a stage without steps, by the warp whose turn it is.
+template <int MODE>
+__device__ __forceinline__ void produce_end(const PairParams& p, PairShared& sh, const PairBars& bars,
+                                            uint32_t g, int warp, int lane) {
+  constexpr uint32_t SLOTS = PairShape<MODE>::slots;
+  if (g % kProducers != uint32_t(warp) || !wait_slot<MODE>(p, sh, bars, g)) return;
+  if (lane == 0) {
+    sh.header[g % SLOTS] = 0u;
+    mbar_arrive(bars.full + 8 * (g % SLOTS));
+  }
+}
 
 template <int MODE>
 __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots, uint32_t zero,
-                             const PairBars& bars, int lane) {
+                             const PairBars& bars, int warp, int lane) {
   constexpr bool I8 = MODE == kInt8;
-  constexpr int SLOTS = PairShape<MODE>::slots, BYTES = PairShape<MODE>::slot_bytes;
+  constexpr uint32_t SLOTS = PairShape<MODE>::slots, BYTES = PairShape<MODE>::slot_bytes;
   const uint32_t xb = (I8 ? 16u : 32u) * uint32_t(p.R);  // panel bytes of a group
   const uint64_t pol_x = policy_evict_last(), pol_w = policy_evict_first();
+  const long long per_tile = I8 ? p.x_chunks : p.K >> 3;
   const int items = p.units * p.tiles;
-  Ring ring;
-  int item = blockIdx.x;
-  // work ahead: the unit of the next item, the group columns of the next stage
-  RowUnit u{};
-  if (item < items) u = p.rows[item / p.tiles];
-  auto seek = [&](int& it, RowUnit& un, int& which) {  // next item with groups
-    while (it < items && un.ng[0] + un.ng[1] == 0) {
-      it += gridDim.x;
-      if (it < items) un = p.rows[it / p.tiles];
-    }
-    which = it < items && un.ng[0] == 0 ? 1 : 0;
+  struct Stage {
+    uint32_t g, shape, flags, col;  // flags: of the header
+    int n, off, which, tile;
+    const char* w;
   };
-  int which = 0, off = 0;
-  seek(item, u, which);
-  int nitem = item + int(gridDim.x);
-  RowUnit nu{};
-  if (nitem < items) nu = p.rows[nitem / p.tiles];
-  auto load_cols = [&](const RowUnit& un, int wh, int of) {
-    return of + lane < int(un.ng[wh]) ? p.group_col[un.g0[wh] + of + lane] : 0u;
-  };
-  uint32_t col = item < items ? load_cols(u, which, 0) : 0u;
-  bool ok = true;
-  while (item < items) {
-    const int h = int(u.shape & 255u), hp = int((u.shape >> 8) & 255u), r0 = int(u.shape >> 16);
-    const uint32_t wb = (I8 ? 16u : 32u) * uint32_t(hp);
-    int cap = BYTES / int(xb + wb);
-    cap = (cap < 32 ? cap : 32) & ~1;
-    const int n = min(cap, int(u.ng[which]) - off);
-    // the next stage
-    int w2 = which, o2 = off + n, it2 = item;
-    RowUnit u2 = u;
-    if (o2 >= int(u.ng[w2])) {
-      o2 = 0;
-      if (w2 == 0 && u.ng[1] > 0) {
-        w2 = 1;
-      } else {
-        it2 = nitem;
-        u2 = nu;
-        seek(it2, u2, w2);
-        nitem = it2 + int(gridDim.x);
-        if (nitem < items) nu = p.rows[nitem / p.tiles];
-      }
-    }
-    const bool last = it2 != item;
-    const uint32_t col2 = it2 < items ? load_cols(u2, w2, o2) : 0u;
-
-    if (!(ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag))) break;
-    const uint32_t base = slots + ring.slot * BYTES, full = bars.full + 8 * ring.slot;
-    const uint32_t wbase = base + uint32_t(n) * xb;
-    const int steps = (n + 1) / 2;
-    if (lane < steps) {
-      const bool pair = 2 * lane + 1 < n;
+  auto issue = [&](const Stage& st) {
+    if (!wait_slot<MODE>(p, sh, bars, st.g)) return false;
+    const int h = int(st.shape & 255u), hp = int((st.shape >> 8) & 255u), r0 = int(st.shape >> 16);
+    const uint32_t wb = (I8 ? 16u : 32u) * uint32_t(hp), n = uint32_t(st.n);
+    const uint32_t slot = st.g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    const uint32_t wbase = base + n * xb, steps = (n + 1) / 2;
+    if (lane < int(steps)) {
+      const bool pair = 2u * lane + 1 < n;
       const uint32_t a = base + 2u * lane * xb, b = wbase + 2u * lane * wb;
-      sh.steps[ring.slot][lane].a = core_desc(a, pair ? xb : zero - a, 128) |
-                                    (lane == 0 && off == 0 ? kStepFresh : 0) |
-                                    (which ? kStepUp : 0) | (pair ? 0 : kStepOdd);
-      sh.steps[ring.slot][lane].b = core_desc(b, pair ? wb : 0u, 128);
+      sh.steps[slot][lane].a = core_desc(a, pair ? xb : zero - a, 128) |
+                               (lane == 0 && (st.flags & kHdrFirst) ? kStepFresh : 0) |
+                               (pair ? 0 : kStepOdd);
+      sh.steps[slot][lane].b = core_desc(b, pair ? wb : 0u, 128);
     }
-    if (lane == 0)
-      sh.header[ring.slot] = uint32_t(steps) | uint32_t(hp) << 5 |
-                             (off == 0 && (which == 0 || u.ng[0] == 0) ? kHdrFirst : 0u) |
-                             (last ? kHdrLast : 0u);
-    __syncwarp();
-    if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(n) * (xb + wb));
-    __syncwarp();
+    announce(sh, slot, full, steps | uint32_t(hp) << 5 | st.flags, n * (xb + wb), lane);
     // weights: one run, or per group the part's rows of hi and of lo'
-    const char* wsrc = p.w + u.w0[which] + (long long)off * (I8 ? 16 : 32) * h;
     if (hp == h) {
       if (lane == 0) {
         if (p.tiles == 1)
-          bulk_g2s(wbase, wsrc, uint32_t(n) * wb, full, pol_w);
+          bulk_g2s(wbase, st.w, n * wb, full, pol_w);
         else
-          bulk_g2s_plain(wbase, wsrc, uint32_t(n) * wb, full);
+          bulk_g2s_plain(wbase, st.w, n * wb, full);
       }
-    } else if (lane < n) {
-      const char* g = wsrc + (long long)lane * (I8 ? 16 : 32) * h + 16 * r0;
+    } else if (lane < st.n) {
+      const char* g = st.w + (long long)lane * (I8 ? 16 : 32) * h + 16 * r0;
       bulk_g2s_plain(wbase + lane * wb, g, 16u * hp, full);
       if (!I8) bulk_g2s_plain(wbase + lane * wb + 16u * hp, g + 16 * h, 16u * hp, full);
     }
     // activations: one copy per run of neighbouring groups
-    const uint32_t before = __shfl_up_sync(0xffffffffu, col, 1);
-    const bool head = lane < n && (lane == 0 || col != before + 1);
+    const uint32_t before = __shfl_up_sync(0xffffffffu, st.col, 1);
+    const bool head = lane < st.n && (lane == 0 || st.col != before + 1);
     const uint32_t heads = __ballot_sync(0xffffffffu, head) | (n < 32 ? 1u << n : 0u);
     if (head) {
       const uint32_t rest = lane < 31 ? heads >> (lane + 1) : 0u;
       const uint32_t run = rest ? uint32_t(__ffs(rest)) : uint32_t(32 - lane);
-      const long long tile = p.tile0 + item % p.tiles;
-      const long long per_tile = I8 ? (p.K >> 3) + 1 : p.K >> 3;  // see panel8_chunks
-      bulk_g2s(base + lane * xb, p.x + (tile * per_tile + col) * xb, run * xb, full, pol_x);
+      bulk_g2s(base + lane * xb, p.x + (st.tile * per_tile + st.col) * xb, run * xb, full, pol_x);
     }
-    ring.next<SLOTS>();
-    item = it2;
-    which = w2;
-    off = o2;
-    u = u2;
-    col = col2;
-  }
-  if (ok) {  // end marker
-    ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag);
-    if (ok && lane == 0) {
-      sh.header[ring.slot] = 0u;
-      mbar_arrive(bars.full + 8 * ring.slot);
+    return true;
+  };
+  UnitWin<RowUnit> win;
+  win.init(p.rows, items, p.tiles, lane);
+  Stage held{};
+  bool have = false;
+  uint32_t g0 = 0;  // stages before this item
+  int k = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
+    const RowUnit u = win.get(k, lane);
+    const RowStages<MODE> rs(p.R, int((u.shape >> 8) & 255u));
+    const int s0 = rs.stages(int(u.ng[0])), total = s0 + rs.stages(int(u.ng[1]));
+    for (int j = int((uint32_t(warp) - g0) % kProducers); j < total; j += kProducers) {
+      Stage st;
+      st.which = j >= s0;
+      const int jj = st.which ? j - s0 : j, ns = st.which ? total - s0 : s0;
+      const int groups = int(st.which ? u.ng[1] : u.ng[0]);
+      st.g = g0 + j;
+      st.shape = u.shape;
+      st.off = jj * rs.cap;
+      st.n = min(rs.cap, groups - st.off);
+      st.tile = p.tile0 + item % p.tiles;
+      st.flags = (jj % rs.per_chunk == 0 ? kHdrFirst : 0u) |
+                 (jj % rs.per_chunk == rs.per_chunk - 1 || jj + 1 == ns ? kHdrLast : 0u);
+      const uint32_t g = (st.which ? u.g0[1] : u.g0[0]) + st.off + lane;
+      st.col = lane < st.n ? __ldg(p.group_col + g) : 0u;
+      st.w = p.w + (st.which ? u.w0[1] : u.w0[0]) +
+             (long long)st.off * (I8 ? 16 : 32) * int(u.shape & 255u);
+      if (have && !issue(held)) return;
+      held = st;
+      have = true;
     }
-    if (ok) ring.next<SLOTS>();
+    g0 += uint32_t(total);
   }
+  if (have && !issue(held)) return;
+  produce_end<MODE>(p, sh, bars, g0, warp, lane);
 }
 
-// ---- producer: kInputGrad ------------------------------------------------------------------------
-
 __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh, uint32_t slots,
-                                             uint32_t zero, const PairBars& bars, int lane) {
-  constexpr int SLOTS = PairShape<kInputGrad>::slots, BYTES = PairShape<kInputGrad>::slot_bytes;
+                                             uint32_t zero, const PairBars& bars, int warp, int lane) {
+  constexpr uint32_t SLOTS = PairShape<kInputGrad>::slots, BYTES = PairShape<kInputGrad>::slot_bytes;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
   const int items = p.units * p.tiles;
   const long long per_tile = 2 * (p.M >> 3);
-  Ring ring;
-  bool ok = true;
-  int item = blockIdx.x;
-  ColUnit nu{};
-  if (item < items) nu = p.cols[item / p.tiles];
-  for (; ok && item < items; item += gridDim.x) {
-    const ColUnit u = nu;
-    if (item + int(gridDim.x) < items) nu = p.cols[(item + gridDim.x) / p.tiles];
-    const char* dy = p.dy + (p.tile0 + item % p.tiles) * per_tile * xb;
-    auto load = [&](uint32_t s) {
-      ColEntry e{};
-      if (lane < kColEntries && s < u.ns) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.entries) +
-                              (long long)(u.s0 + s) * kColEntries + lane);
-        e.dy_group = v.x;
-        e.h8 = v.y;
-        e.w_byte = u64(v.z) | u64(v.w) << 32;
-      }
-      return e;
-    };
-    ColEntry next = load(0);
-    for (uint32_t s = 0; s < u.ns; ++s) {
-      const ColEntry e = next;
-      next = load(s + 1);
-      // places of the entries: groups before this one, and its steps
-      uint32_t g = e.h8, st = (e.h8 + 1) / 2;
+  struct Stage {
+    uint32_t g, flags, w, c0;
+    int tile;
+    ColEntry e;
+  };
+  auto issue = [&](const Stage& st) {
+    const ColEntry& e = st.e;
+    // places of the entries: groups before this one, and its steps
+    uint32_t g = e.h8, steps = (e.h8 + 1) / 2;
 #pragma unroll
-      for (int d = 1; d < kColEntries; d *= 2) {
-        const uint32_t g2 = __shfl_up_sync(0xffffffffu, g, d), s2 = __shfl_up_sync(0xffffffffu, st, d);
-        if (lane >= d) {
-          g += g2;
-          st += s2;
-        }
+    for (int d = 1; d < kColEntries; d *= 2) {
+      const uint32_t g2 = __shfl_up_sync(0xffffffffu, g, d), s2 = __shfl_up_sync(0xffffffffu, steps, d);
+      if (lane >= d) {
+        g += g2;
+        steps += s2;
       }
-      const uint32_t groups = __shfl_sync(0xffffffffu, g, kColEntries - 1);
-      const uint32_t steps = __shfl_sync(0xffffffffu, st, kColEntries - 1);
-      const uint32_t g_before = g - e.h8, s_before = st - (e.h8 + 1) / 2;
-      if (!(ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag))) break;
-      const uint32_t base = slots + ring.slot * BYTES, full = bars.full + 8 * ring.slot;
-      const uint32_t a0 = base + g_before * xb, b0 = base + groups * xb + g_before * 32u * u.w;
-      const uint32_t h = 8u * e.h8;
-      if (lane < kColEntries)
-        for (uint32_t j = 0; 2 * j < e.h8; ++j) {
-          const bool pair = 2 * j + 1 < e.h8;
-          const uint32_t a = a0 + 2 * j * xb;
-          PairStep& out = sh.steps[ring.slot][s_before + j];
-          out.a = core_desc(a, pair ? xb : zero - a, 128) |
-                  (s == 0 && s_before + j == 0 ? kStepFresh : 0) | (pair ? 0 : kStepOdd);
-          // columns 8 apart are 16 h apart (hi and lo' tiles alternate), rows 8 apart 128 bytes
-          out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
-        }
-      if (lane == 0)
-        sh.header[ring.slot] = steps | u.w << 5 | (s == 0 ? kHdrFirst : 0u) |
-                               (s + 1 == u.ns ? kHdrLast : 0u);
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(full, groups * (xb + 32u * u.w));
-      __syncwarp();
-      if (e.h8) {
-        bulk_g2s(a0, dy + (long long)e.dy_group * xb, e.h8 * xb, full, pol_x);
-        bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(u.c0 >> 3) * 32 * h, 4u * h * u.w, full);
+    }
+    const uint32_t groups = __shfl_sync(0xffffffffu, g, kColEntries - 1);
+    const uint32_t all_steps = __shfl_sync(0xffffffffu, steps, kColEntries - 1);
+    const uint32_t g_before = g - e.h8, s_before = steps - (e.h8 + 1) / 2;
+    if (!wait_slot<kInputGrad>(p, sh, bars, st.g)) return false;
+    const uint32_t slot = st.g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    const uint32_t a0 = base + g_before * xb, b0 = base + groups * xb + g_before * 32u * st.w;
+    const uint32_t h = 8u * e.h8;
+    if (lane < kColEntries)
+      for (uint32_t j = 0; 2 * j < e.h8; ++j) {
+        const bool pair = 2 * j + 1 < e.h8;
+        const uint32_t a = a0 + 2 * j * xb;
+        PairStep& out = sh.steps[slot][s_before + j];
+        out.a = core_desc(a, pair ? xb : zero - a, 128) |
+                (s_before + j == 0 && (st.flags & kHdrFirst) ? kStepFresh : 0) | (pair ? 0 : kStepOdd);
+        // columns 8 apart are 16 h apart (hi and lo' tiles alternate), rows 8 apart 128 bytes
+        out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
       }
-      ring.next<SLOTS>();
+    announce(sh, slot, full, all_steps | st.w << 5 | st.flags, groups * (xb + 32u * st.w), lane);
+    if (e.h8) {
+      bulk_g2s(a0, p.dy + (st.tile * per_tile + e.dy_group) * xb, e.h8 * xb, full, pol_x);
+      bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(st.c0 >> 3) * 32 * h, 4u * h * st.w, full);
     }
-  }
-  if (ok) {
-    ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag);
-    if (ok && lane == 0) {
-      sh.header[ring.slot] = 0u;
-      mbar_arrive(bars.full + 8 * ring.slot);
+    return true;
+  };
+  UnitWin<ColUnit> win;
+  win.init(p.cols, items, p.tiles, lane);
+  Stage held{};
+  bool have = false;
+  uint32_t g0 = 0;
+  int k = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
+    const ColUnit u = win.get(k, lane);
+    for (uint32_t j = (uint32_t(warp) - g0) % kProducers; j < u.ns; j += kProducers) {
+      Stage st;
+      st.g = g0 + j;
+      st.w = u.w;
+      st.c0 = u.c0;
+      st.tile = p.tile0 + item % p.tiles;
+      st.flags = (j % kChunkStages == 0 ? kHdrFirst : 0u) |
+                 (j % kChunkStages == kChunkStages - 1 || j + 1 == u.ns ? kHdrLast : 0u);
+      st.e = ColEntry{};
+      if (lane < kColEntries) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.entries) +
+                              (long long)(u.s0 + j) * kColEntries + lane);
+        st.e.dy_group = v.x;
+        st.e.h8 = v.y;
+        st.e.w_byte = u64(v.z) | u64(v.w) << 32;
+      }
+      if (have && !issue(held)) return;
+      held = st;
+      have = true;
     }
+    g0 += u.ns;
   }
+  if (have && !issue(held)) return;
+  produce_end<kInputGrad>(p, sh, bars, g0, warp, lane);
 }
 
-// ---- producer: kWeightGrad -----------------------------------------------------------------------
-
-// A stage is kGradTokens tokens (the last of a tile fewer) of the unit's 16 activation groups and of
-// its h / 8 gradient groups, each group [kGradTokens of hi][kGradTokens of lo'].
+// Token stages of a weight-gradient unit: kGradTokens tokens of a tile (the last of a tile fewer) of
+// the unit's 16 activation groups and h / 8 gradient groups, each group [kGradTokens of hi][of lo'].
+__device__ __forceinline__ int grad_stages(const PairParams& p) {
+  return p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
+}
 __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& sh, uint32_t slots,
-                                              const PairBars& bars, int lane) {
-  constexpr int SLOTS = PairShape<kWeightGrad>::slots, BYTES = PairShape<kWeightGrad>::slot_bytes;
+                                              const PairBars& bars, int warp, int lane) {
+  constexpr uint32_t SLOTS = PairShape<kWeightGrad>::slots, BYTES = PairShape<kWeightGrad>::slot_bytes;
   constexpr uint32_t GB = 32u * kGradTokens;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
-  Ring ring;
-  bool ok = true;
-  int item = blockIdx.x;
+  const int per_tile = (p.R + kGradTokens - 1) / kGradTokens, total = p.tiles * per_tile;
+  UnitWin<GradUnit> win;
+  win.init(p.grads, p.units, 1, lane);
+  uint32_t g0 = 0;
+  int k = 0;
+  uint32_t next_col = 0;
+  auto load_col = [&](const GradUnit& u) {
+    return lane < int(u.ng) ? __ldg(p.group_col + u.g0 + lane) : 0u;
+  };
   GradUnit nu{};
-  uint32_t ncol = 0;
-  if (item < p.units) {
-    nu = p.grads[item];
-    ncol = lane < int(nu.ng) ? p.group_col[nu.g0 + lane] : 0u;
+  if (int(blockIdx.x) < p.units) {
+    nu = win.get(0, lane);
+    next_col = load_col(nu);
   }
-  for (; ok && item < p.units; item += gridDim.x) {
+  for (int item = blockIdx.x; item < p.units; item += gridDim.x) {
     const GradUnit u = nu;
-    const uint32_t col = ncol;
+    const uint32_t col = next_col;
     if (item + int(gridDim.x) < p.units) {
-      nu = p.grads[item + gridDim.x];
-      ncol = lane < int(nu.ng) ? p.group_col[nu.g0 + lane] : 0u;
+      nu = win.get(++k, lane);
+      next_col = load_col(nu);
     }
     const uint32_t h8 = u.h / 8;
-    for (int tile = 0; ok && tile < p.tiles; ++tile) {
-      const char* x = p.x + ((long long)tile * (p.K >> 3) + col) * xb;
-      const char* dy = p.dy + ((long long)tile * 2 * (p.M >> 3) + u.dy_group + lane - 16) * xb;
-      for (int t0 = 0; t0 < p.R; t0 += kGradTokens) {
-        const int nt = min(kGradTokens, p.R - t0);
-        if (!(ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag)))
-          break;
-        const uint32_t base = slots + ring.slot * BYTES, full = bars.full + 8 * ring.slot;
-        const int steps = nt / 16;
-        if (lane < steps) {
-          PairStep& out = sh.steps[ring.slot][lane];
-          out.a = core_desc(base + 256u * lane, 128u, GB) |
-                  (tile == 0 && t0 == 0 && lane == 0 ? kStepFresh : 0);
-          out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
-        }
-        if (lane == 0)
-          sh.header[ring.slot] = uint32_t(steps) | u.h << 5 |
-                                 (tile == 0 && t0 == 0 ? kHdrFirst : 0u) |
-                                 (tile + 1 == p.tiles && t0 + kGradTokens >= p.R ? kHdrLast : 0u);
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(full, (u.ng + h8) * 32u * uint32_t(nt));
-        __syncwarp();
-        const bool is_x = lane < int(u.ng), is_dy = lane >= 16 && lane < 16 + int(h8);
-        if (is_x || is_dy) {
-          const char* src = (is_x ? x : dy) + 16 * t0;
-          const uint32_t dst = base + lane * GB;
-          bulk_g2s(dst, src, 16u * nt, full, pol_x);
-          bulk_g2s(dst + GB / 2, src + 16 * p.R, 16u * nt, full, pol_x);
-        }
-        ring.next<SLOTS>();
+    const bool is_x = lane < int(u.ng), is_dy = lane >= 16 && lane < 16 + int(h8);
+    const char* src0 = is_x ? p.x + (long long)col * xb : p.dy + ((long long)u.dy_group + lane - 16) * xb;
+    const long long tile_step = (is_x ? p.K >> 3 : 2 * (p.M >> 3)) * xb;
+    for (int j = int((uint32_t(warp) - g0) % kProducers); j < total; j += kProducers) {
+      const int tile = j / per_tile, t0 = (j % per_tile) * kGradTokens, nt = min(kGradTokens, p.R - t0);
+      const uint32_t g = g0 + j;
+      if (!wait_slot<kWeightGrad>(p, sh, bars, g)) return;
+      const uint32_t slot = g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
+      const uint32_t steps = uint32_t(nt) / 16;
+      const uint32_t flags = (j % kChunkStages == 0 ? kHdrFirst : 0u) |
+                             (j % kChunkStages == kChunkStages - 1 || j + 1 == total ? kHdrLast : 0u);
+      if (lane < int(steps)) {
+        PairStep& out = sh.steps[slot][lane];
+        out.a = core_desc(base + 256u * lane, 128u, GB) |
+                (lane == 0 && (flags & kHdrFirst) ? kStepFresh : 0);
+        out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
+      }
+      announce(sh, slot, full, steps | u.h << 5 | flags, (u.ng + h8) * 32u * uint32_t(nt), lane);
+      if (is_x || is_dy) {
+        const char* src = src0 + tile * tile_step + 16 * t0;
+        const uint32_t dst = base + lane * GB;
+        bulk_g2s(dst, src, 16u * nt, full, pol_x);
+        bulk_g2s(dst + GB / 2, src + 16 * p.R, 16u * nt, full, pol_x);
       }
     }
+    g0 += uint32_t(total);
   }
-  if (ok) {
-    ok = wait_warp(bars.empty + 8 * ring.slot, ring.parity, p.status, &sh.abort_flag);
-    if (ok && lane == 0) {
-      sh.header[ring.slot] = 0u;
-      mbar_arrive(bars.full + 8 * ring.slot);
-    }
-  }
+  produce_end<kWeightGrad>(p, sh, bars, g0, warp, lane);
 }
 
 // ---- MMA thread ----------------------------------------------------------------------------------
 
 template <int MODE>
 __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& bars) {
-  constexpr int SLOTS = PairShape<MODE>::slots;
+  constexpr uint32_t SLOTS = PairShape<MODE>::slots, ACCS = PairShape<MODE>::accs;
   const int m = MODE == kWeightGrad ? 128 : (p.R > 64 ? 128 : 64);
   // D f32, A and B f16 (kInt8: D s32, A and B s8); transposed (MN-major) operands in bits 15 and 16
   const uint32_t form = (MODE == kInt8 ? (2u << 4) | (1u << 7) | (1u << 10) : (1u << 4)) |
@@ -531,11 +589,11 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     const uint32_t hdr = *reinterpret_cast<volatile uint32_t*>(&sh.header[slot]);
     const int steps = int(hdr & 63u), n = int((hdr >> 8) & 15u) * 8;
     if (steps == 0) break;
-    const uint32_t buf = use & 1u;
+    const uint32_t buf = use % ACCS;
     if (hdr & kHdrFirst)
-      if (!wait_one(bars.acc_empty + 8 * buf, ((use >> 1) & 1u) ^ 1u, p.status, &sh.abort_flag)) return;
+      if (!wait_one(bars.acc_empty + 8 * buf, ((use / ACCS) & 1u) ^ 1u, p.status, &sh.abort_flag)) return;
     tc_fence_after();
-    const uint32_t d0 = sh.tmem + 256u * buf;
+    const uint32_t d = sh.tmem + PairShape<MODE>::acc_cols * buf;
     // N of one tile of n columns: a multiple of 16 for M = 128 (one tile more is read, and its
     // columns are not used)
     const int n1 = m == 128 || MODE == kInt8 ? (n + 15) & ~15 : n;
@@ -544,7 +602,6 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
       const PairStep st = sh.steps[slot][s];
       const u64 a = st.a & kStepMask, b = st.b;
       const uint32_t acc = (st.a & kStepFresh) ? 0u : 1u;
-      const uint32_t d = d0 + ((st.a & kStepUp) ? 128u : 0u);
       if (MODE == kInt8) {
         tc_mma_i8(d, a, b, i1, acc);
         continue;
@@ -584,94 +641,115 @@ __device__ __forceinline__ void store8(float* dst, const float (&v)[8], int vec)
 }
 constexpr float kLoUnit = 1.0f / 2048.0f;  // 2^-11
 
+// Epilogue warp e of a quadrant takes the 8-column tiles c with c % 2 == e.
 template <int MODE>
-__device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, int quad, int lane) {
+__device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, int quad, int e,
+                         int lane) {
+  constexpr uint32_t ACCS = PairShape<MODE>::accs;
   const bool wide = MODE == kWeightGrad || p.R > 64;  // M = 128; M = 64 fills lanes 0..15
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
-  const bool in_tile = wide || lane < 16;
-  const int items = MODE == kWeightGrad ? p.units : p.units * p.tiles;
+  const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
+  const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles;
   float f1 = 1.0f, f2 = 1.0f;
   if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
   if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
   if (MODE == kWeightGrad) unscale(p.exps[0] + p.exps[1], f1, f2);
+  using Unit = typename std::conditional<PairShape<MODE>::rows, RowUnit,
+                  typename std::conditional<MODE == kInputGrad, ColUnit, GradUnit>::type>::type;
+  UnitWin<Unit> win;
+  if constexpr (PairShape<MODE>::rows) win.init(p.rows, items, tiles, lane);
+  else if constexpr (MODE == kInputGrad) win.init(p.cols, items, tiles, lane);
+  else win.init(p.grads, items, tiles, lane);
   uint32_t use = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint32_t buf = use & 1u;
-    const uint32_t d0 = sh.tmem + 256u * buf + (uint32_t(32 * quad) << 16);
-    const long long t = MODE == kWeightGrad ? 0 : (long long)(p.tile0 + item % p.tiles) * p.R + row;
-    bool work = true;
-    int n = 0;
-    bool live = false;
-    RowUnit ru{};
-    ColUnit cu{};
-    GradUnit gu{};
-    if (MODE == kForward || MODE == kInt8) {
-      ru = p.rows[item / p.tiles];
-      n = int((ru.shape >> 8) & 255u);
-      work = ru.ng[0] + ru.ng[1] > 0;
-      live = in_tile && row < p.R && t < p.tokens;
-    } else if (MODE == kInputGrad) {
-      cu = p.cols[item / p.tiles];
-      n = int(cu.w);
-      work = cu.ns > 0;
-      live = in_tile && row < p.R && t < p.tokens;
+  int k = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
+    const Unit u = win.get(k, lane);
+    const long long t = MODE == kWeightGrad ? 0 : (long long)(p.tile0 + item % tiles) * p.R + row;
+    int n, chunks[2] = {0, 0};
+    bool live;
+    if constexpr (PairShape<MODE>::rows) {
+      n = int((u.shape >> 8) & 255u);
+      const RowStages<MODE> rs(p.R, n);
+      chunks[0] = rs.chunks(int(u.ng[0]));
+      chunks[1] = rs.chunks(int(u.ng[1]));
+      live = in_tile && t < p.tokens;
+    } else if constexpr (MODE == kInputGrad) {
+      n = int(u.w);
+      chunks[0] = (int(u.ns) + kChunkStages - 1) / kChunkStages;
+      live = in_tile && t < p.tokens;
     } else {
-      gu = p.grads[item];
-      n = int(gu.h);
-      live = row < int(gu.ng) * 8;
+      n = int(u.h);
+      chunks[0] = (grad_stages(p) + kChunkStages - 1) / kChunkStages;
+      live = row < int(u.ng) * 8;
     }
-    if (work) {
-      if (!wait_warp(bars.acc_full + 8 * buf, (use >> 1) & 1u, p.status, &sh.abort_flag)) return;
-      tc_fence_after();
-    }
-    float rs = 0.0f;
-    if (MODE == kInt8 && live) rs = p.token_scale[t];
-    for (int c = 0; c < n; c += 8) {
-      if (MODE == kForward) {
-        float g[8] = {}, u[8] = {}, gl[8] = {}, ul[8] = {};
-        if (work) tc_ld8_4(d0 + c, d0 + n + c, d0 + 128 + c, d0 + 128 + n + c, g, gl, u, ul);
-        if (live) {
-          float hv[8];
+    float acc[MODE == kForward ? 2 : 1][4][8] = {};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {  // a matrix without blocks here left its columns unwritten
-            g[i] = ru.ng[0] ? fmaf(gl[i], kLoUnit, g[i]) * f1 * f2 : 0.0f;
-            u[i] = ru.ng[1] ? fmaf(ul[i], kLoUnit, u[i]) * f1 * f2 : 0.0f;
-            hv[i] = act_value(p.act, g[i]) * u[i];
+    for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
+      for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
+        const uint32_t buf = use % ACCS;
+        if (!wait_warp(bars.acc_full + 8 * buf, (use / ACCS) & 1u, p.status, &sh.abort_flag)) return;
+        tc_fence_after();
+        const uint32_t d = sh.tmem + PairShape<MODE>::acc_cols * buf + (uint32_t(32 * quad) << 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = 16 * j + 8 * e;
+          if (c >= n) break;
+          float* a = acc[which][j];
+          float v[8], l1[8], l2[8];
+          if (MODE == kInt8) {
+            tc_ld8_1(d + c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = v[i];  // 32-bit integers, carried as they are
+          } else if (MODE == kForward) {
+            tc_ld8_2(d + c, d + n + c, v, l1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] += fmaf(l1[i], kLoUnit, v[i]);
+          } else {
+            tc_ld8_3(d + 2 * c, d + 2 * c + 8, d + 128 + c, v, l1, l2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] += fmaf(l1[i] + l2[i], kLoUnit, v[i]);
           }
-          const long long o = t * p.M + ru.row0 + c;
-          store8(p.out0 + o, hv, p.vec);
-          if (p.out1 != nullptr) {
-            store8(p.out1 + o, g, p.vec);
-            store8(p.out2 + o, u, p.vec);
-          }
         }
-      } else if (MODE == kInt8) {
-        float v[8] = {};
-        if (work) tc_ld8_1(d0 + c, v);
-        if (live) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = float(__float_as_int(v[i])) * (rs * p.row_scale[ru.row0 + c + i]);
-          store8(p.out0 + t * p.M + ru.row0 + c, v, p.vec);
-        }
-      } else {
-        float v[8] = {}, l1[8] = {}, l2[8] = {};
-        if (work) tc_ld8_3(d0 + 2 * c, d0 + 2 * c + 8, d0 + 128 + c, v, l1, l2);
-        if (live) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = fmaf(l1[i] + l2[i], kLoUnit, v[i]) * f1 * f2;
-          float* dst = MODE == kInputGrad
-                           ? p.out0 + t * p.K + cu.col0 + c
-                           : (gu.which ? p.out1 : p.out0) + gu.out + (long long)row * n + c;
-          store8(dst, v, p.vec);
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.acc_empty + 8 * buf);
       }
     }
-    if (work) {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars.acc_empty + 8 * buf);
-      ++use;
+    if (!live) continue;
+    const float ts = MODE == kInt8 ? p.token_scale[t] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = 16 * j + 8 * e;
+      if (c >= n) break;
+      float(&v)[8] = acc[0][j];
+      if constexpr (MODE == kForward) {
+        float(&w)[8] = acc[1][j];
+        float hv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = v[i] * f1 * f2;
+          w[i] = w[i] * f1 * f2;
+          hv[i] = act_value(p.act, v[i]) * w[i];
+        }
+        const long long o = t * p.M + u.row0 + c;
+        store8(p.out0 + o, hv, p.vec);
+        if (p.out1 != nullptr) {
+          store8(p.out1 + o, v, p.vec);
+          store8(p.out2 + o, w, p.vec);
+        }
+      } else if constexpr (MODE == kInt8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = float(__float_as_int(v[i])) * (ts * p.row_scale[u.row0 + c + i]);
+        store8(p.out0 + t * p.M + u.row0 + c, v, p.vec);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * f1 * f2;
+        if constexpr (MODE == kInputGrad)
+          store8(p.out0 + t * p.K + u.col0 + c, v, p.vec);
+        else
+          store8((u.which ? p.out1 : p.out0) + u.out + (long long)row * n + c, v, p.vec);
+      }
     }
   }
 }
@@ -693,9 +771,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
       mbar_init(bars.full + 8 * s, 1);
       mbar_init(bars.empty + 8 * s, 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < PairShape<MODE>::accs; ++b) {
       mbar_init(bars.acc_full + 8 * b, 1);
-      mbar_init(bars.acc_empty + 8 * b, 4);
+      mbar_init(bars.acc_empty + 8 * b, kEpilogueWarps);
     }
     mbar_init(bars.drain, 1);
     sh.abort_flag = 0;
@@ -704,7 +782,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   for (int i = threadIdx.x; i < kZeroBytes / 16; i += kPairThreads)
     reinterpret_cast<uint4*>(zero_ptr)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
-  if (warp == 1) {
+  if (warp == kProducers) {
     tc_alloc(smem_addr(&sh.tmem), 512);
     tc_relinquish();
   }
@@ -712,18 +790,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   __syncthreads();
   tc_fence_after();
 
-  if (warp == 0) {
-    if (MODE == kForward || MODE == kInt8)
-      produce_rows<MODE>(p, sh, slots, zero, bars, lane);
-    else if (MODE == kInputGrad)
-      produce_cols(p, sh, slots, zero, bars, lane);
+  if (warp < kProducers) {
+    if constexpr (PairShape<MODE>::rows)
+      produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
+    else if constexpr (MODE == kInputGrad)
+      produce_cols(p, sh, slots, zero, bars, warp, lane);
     else
-      produce_grads(p, sh, slots, bars, lane);
-  } else if (warp == 1) {
+      produce_grads(p, sh, slots, bars, warp, lane);
+  } else if (warp == kProducers) {
     if (lane == 0) issue_mmas<MODE>(p, sh, bars);
     __syncwarp();
-  } else if (warp >= 4) {
-    epilogue<MODE>(p, sh, bars, warp - 4, lane);
+  } else if (warp >= kEpilogueWarp) {
+    epilogue<MODE>(p, sh, bars, (warp - kEpilogueWarp) & 3, (warp - kEpilogueWarp) >> 2, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -734,7 +812,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
     __syncthreads();
   }
   tc_fence_after();
-  if (warp == 1) tc_dealloc(sh.tmem, 512);
+  if (warp == kProducers) tc_dealloc(sh.tmem, 512);
 }
 
 }  // namespace vbsr_b200
