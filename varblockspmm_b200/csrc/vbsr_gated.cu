@@ -45,12 +45,13 @@ struct Panels {
 };
 constexpr int64_t kPartialBytes = 4 * kAmaxCtas + (256 - 4 * kAmaxCtas % 256) % 256;
 
-// Tiles of at most 128 tokens, as even as their step allows: 8 tokens (core matrices), or 16 where
-// the tokens are summed over (K = 16).
+// Tiles of at most 128 tokens, evenly sized; multiples of 16 where the tokens are summed over (K = 16).
+// In the forward direction any number goes: an MMA's rows behind the last token hold other bytes, and
+// a row's result depends on that row alone.
 Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
   Panels g;
   if (tokens == 0) return g;
-  const int64_t step = backward ? 16 : 8;
+  const int64_t step = backward ? 16 : 1;
   g.tiles = (tokens + 127) / 128;
   g.R = int(((tokens + g.tiles - 1) / g.tiles + step - 1) / step * step);
   g.x_at = 2 * kPartialBytes + 256;  // largest magnitudes of both panels, exponents

@@ -19,7 +19,7 @@
 // MN-major operand (weight gradients, summed over tokens):
 //   weights: block row by block row, 8-column group by group, [h rows of hi][h rows of lo'];
 //            the group at packed value offset o starts at byte 4 o.
-//   panels:  per tile of R tokens (a multiple of 8, at most 128) and 8-feature group,
+//   panels:  per tile of R tokens (at most 128; a multiple of 16 for the gradients) and 8-feature group,
 //            [R tokens of hi][R tokens of lo'], zeros behind the last token.
 // Block widths are multiples of 8, so any block is a whole number of groups; K = 16 steps take two
 // groups, and an odd last one is paired with a tile of zeros (and, on the weights' side, with itself,
@@ -31,14 +31,17 @@
 // and is then added in fp32 registers by the epilogue warps, while the next steps go to another
 // accumulator.
 //
-// The kernel: one persistent CTA per SM. Four producer warps take turns with the stages: each issues
-// a stage's bulk copies into a slot of the ring and writes the slot's list of MMA steps (four, and a
-// stage's list of places fetched while the one before is issued, because that fetch takes about
-// as long as four stages take to stream). One MMA thread only works off those lists. Eight epilogue
-// warps, two per TMEM quadrant, take every second tile of 8 columns each. Tokens are on the M side (64 or 128 rows): with weights there, blocks of
-// 8 to 56 rows would leave most of an MMA empty. What bounds it: the copies into shared memory.
-// A weight group of 32 h bytes needs 32 R bytes of activations, from L2, so few tokens run at the
-// weights' HBM rate and many at the L2-to-shared-memory rate, h / 2 operations per byte.
+// The kernel: one persistent CTA per SM with four pipelines, each a producer warp, a ring of slots, an
+// MMA thread and an accumulator; they take the accumulation chunks in turn. A producer issues a
+// stage's bulk copies into a slot and writes the slot's list of MMA steps; the MMA thread only works
+// off that list. Four, because both halves are latency: fetching a stage's list of places takes as
+// long as several stages take to stream, and a single MMA thread, which reads two descriptors
+// from shared memory per step, was measured at 400 clocks a step where the operands need about 140.
+// Eight epilogue warps, two per TMEM quadrant, take every second tile of 8 columns each. Tokens are
+// on the M side (64 or 128 rows): with weights there, blocks of 8 to 56 rows would leave most of an
+// MMA empty. What bounds it: the copies into shared memory. A weight group of 32 h bytes needs 32 R
+// bytes of activations, from L2, so few tokens run at the weights' HBM rate and many at the
+// L2-to-shared-memory rate, h / 2 operations per byte.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -121,12 +124,11 @@ constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17;
 template <int MODE>
 struct PairShape {
   static constexpr bool rows = MODE == kForward || MODE == kInt8;
-  static constexpr int slots = rows ? 8 : 4;
-  static constexpr int slot_bytes = rows ? 24 * 1024 : 48 * 1024;
-  static constexpr int accs = rows ? 4 : 2;             // accumulators in TMEM
-  static constexpr uint32_t acc_cols = 512 / accs;
+  static constexpr uint32_t ring = rows ? 2 : 1;  // slots per pipeline
+  static constexpr uint32_t slot_bytes = rows ? 24 * 1024 : 48 * 1024;
 };
-constexpr int kProducers = 4;                      // warps 0 .. 3; the MMA thread is in warp 4
+constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA threads in warps 4 .. 7
+constexpr uint32_t kAccCols = 128;  // TMEM columns of an accumulator: hi sums, then lo sums
 constexpr int kEpilogueWarp = 8, kEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr int kChunkSteps = 8;
@@ -135,7 +137,7 @@ constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's o
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage
 template <int MODE>
 constexpr int pair_smem() {
-  return PairShape<MODE>::slots * PairShape<MODE>::slot_bytes + kZeroBytes + kTailBytes + 1024;
+  return kPipes * PairShape<MODE>::ring * PairShape<MODE>::slot_bytes + kZeroBytes + kTailBytes + 1024;
 }
 
 __device__ __forceinline__ u64 core_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -167,7 +169,7 @@ __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, ui
       : "memory");
 }
 
-// 8 accumulator columns each from one, two or three places, loaded and waited for in one statement
+// 8 accumulator columns each from one or two places, loaded and waited for in one statement
 // (the registers are not valid before the wait).
 __device__ __forceinline__ void tc_ld8_1(uint32_t a, float (&v)[8]) {
   asm volatile(
@@ -175,20 +177,6 @@ __device__ __forceinline__ void tc_ld8_1(uint32_t a, float (&v)[8]) {
       "tcgen05.wait::ld.sync.aligned;"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
       : "r"(a)
-      : "memory");
-}
-__device__ __forceinline__ void tc_ld8_3(uint32_t a, uint32_t b, uint32_t c, float (&v)[8],
-                                         float (&w)[8], float (&x)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-        "=f"(v[7]), "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]),
-        "=f"(w[6]), "=f"(w[7]), "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]),
-        "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
-      : "r"(a), "r"(b), "r"(c)
       : "memory");
 }
 __device__ __forceinline__ void tc_ld8_2(uint32_t a, uint32_t b, float (&v)[8], float (&w)[8]) {
@@ -240,14 +228,14 @@ struct RowStages {
     cap = PairShape<MODE>::slot_bytes / b;
     const int most = MODE == kInt8 ? 32 : 2 * kChunkSteps;
     cap = (cap < most ? cap : most) & ~1;
-    per_chunk = MODE == kInt8 ? 1 << 30 : (2 * kChunkSteps) / cap;
+    per_chunk = MODE == kInt8 ? 1 << 20 : (2 * kChunkSteps) / cap;
   }
   __device__ __forceinline__ int stages(int groups) const { return (groups + cap - 1) / cap; }
   __device__ __forceinline__ int chunks(int groups) const {
     return MODE == kInt8 ? (groups > 0) : (stages(groups) + per_chunk - 1) / per_chunk;
   }
 };
-constexpr int kChunkStages = 2;  // kInputGrad, kWeightGrad: stages (of 4 or so steps) per chunk
+// kInputGrad, kWeightGrad: a stage (of at most 8 and 4 steps) is a chunk.
 
 // The units of this CTA's work items, 32 at a time in the lanes' registers and the next 32 on their
 // way; get() broadcasts one.
@@ -299,7 +287,7 @@ struct PairBars {
 };
 
 struct PairShared {
-  u64 full[8], empty[8], acc_full[4], acc_empty[4], drain;
+  u64 full[8], empty[8], acc_full[4], acc_empty[4], drain[4];
   PairStep steps[8][kMaxSteps];
   uint32_t header[8];
   uint32_t tmem;
@@ -308,14 +296,22 @@ struct PairShared {
 
 // ---- producers -----------------------------------------------------------------------------------
 //
-// Stage g of the CTA goes to slot g % SLOTS and is issued by warp g % kProducers. A warp fetches its
-// next stage's list before it issues the one in hand.
+// Pipeline q takes the CTA's accumulation chunks c with c % kPipes == q. A producer fetches its next
+// stage's list before it issues the one in hand.
 
+// A pipeline's slots: stage i of the pipeline is in slot i % ring.
+template <int MODE>
+struct Pipe {
+  static constexpr uint32_t RING = PairShape<MODE>::ring;
+  uint32_t first;  // first slot
+  uint32_t i = 0;
+  __device__ __forceinline__ uint32_t slot() const { return first + i % RING; }
+  __device__ __forceinline__ uint32_t parity() const { return (i / RING) & 1u; }
+};
 template <int MODE>
 __device__ __forceinline__ bool wait_slot(const PairParams& p, PairShared& sh, const PairBars& bars,
-                                          uint32_t g) {
-  constexpr uint32_t SLOTS = PairShape<MODE>::slots;
-  return wait_warp(bars.empty + 8 * (g % SLOTS), ((g / SLOTS) & 1u) ^ 1u, p.status, &sh.abort_flag);
+                                          const Pipe<MODE>& pipe) {
+  return wait_warp(bars.empty + 8 * pipe.slot(), pipe.parity() ^ 1u, p.status, &sh.abort_flag);
 }
 // Announces the slot's list and bytes; the lanes' list entries are written before.
 __device__ __forceinline__ void announce(PairShared& sh, uint32_t slot, uint32_t full, uint32_t header,
@@ -325,15 +321,14 @@ __device__ __forceinline__ void announce(PairShared& sh, uint32_t slot, uint32_t
   if (lane == 0) mbar_arrive_expect_tx(full, bytes);
   __syncwarp();
 }
-// The end marker, a stage without steps, by the warp whose turn it is.
+// The end marker, a stage without steps.
 template <int MODE>
 __device__ __forceinline__ void produce_end(const PairParams& p, PairShared& sh, const PairBars& bars,
-                                            uint32_t g, int warp, int lane) {
-  constexpr uint32_t SLOTS = PairShape<MODE>::slots;
-  if (g % kProducers != uint32_t(warp) || !wait_slot<MODE>(p, sh, bars, g)) return;
+                                            const Pipe<MODE>& pipe, int lane) {
+  if (!wait_slot<MODE>(p, sh, bars, pipe)) return;
   if (lane == 0) {
-    sh.header[g % SLOTS] = 0u;
-    mbar_arrive(bars.full + 8 * (g % SLOTS));
+    sh.header[pipe.slot()] = 0u;
+    mbar_arrive(bars.full + 8 * pipe.slot());
   }
 }
 
@@ -341,25 +336,26 @@ template <int MODE>
 __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots, uint32_t zero,
                              const PairBars& bars, int warp, int lane) {
   constexpr bool I8 = MODE == kInt8;
-  constexpr uint32_t SLOTS = PairShape<MODE>::slots, BYTES = PairShape<MODE>::slot_bytes;
+  constexpr uint32_t BYTES = PairShape<MODE>::slot_bytes;
   const uint32_t xb = (I8 ? 16u : 32u) * uint32_t(p.R);  // panel bytes of a group
   const uint64_t pol_x = policy_evict_last(), pol_w = policy_evict_first();
   const long long per_tile = I8 ? p.x_chunks : p.K >> 3;
   const int items = p.units * p.tiles;
   struct Stage {
-    uint32_t g, shape, flags, col;  // flags: of the header
-    int n, off, which, tile;
+    uint32_t shape, flags, col;  // flags: of the header
+    int n, tile;
     const char* w;
   };
+  Pipe<MODE> pipe{uint32_t(warp) * PairShape<MODE>::ring};
   auto issue = [&](const Stage& st) {
-    if (!wait_slot<MODE>(p, sh, bars, st.g)) return false;
+    if (!wait_slot<MODE>(p, sh, bars, pipe)) return false;
     const int h = int(st.shape & 255u), hp = int((st.shape >> 8) & 255u), r0 = int(st.shape >> 16);
     const uint32_t wb = (I8 ? 16u : 32u) * uint32_t(hp), n = uint32_t(st.n);
-    const uint32_t slot = st.g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
-    const uint32_t wbase = base + n * xb, steps = (n + 1) / 2;
+    const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    const uint32_t xbase = base + n * wb, steps = (n + 1) / 2;  // weights first: 128-byte aligned
     if (lane < int(steps)) {
       const bool pair = 2u * lane + 1 < n;
-      const uint32_t a = base + 2u * lane * xb, b = wbase + 2u * lane * wb;
+      const uint32_t a = xbase + 2u * lane * xb, b = base + 2u * lane * wb;
       sh.steps[slot][lane].a = core_desc(a, pair ? xb : zero - a, 128) |
                                (lane == 0 && (st.flags & kHdrFirst) ? kStepFresh : 0) |
                                (pair ? 0 : kStepOdd);
@@ -370,14 +366,14 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
     if (hp == h) {
       if (lane == 0) {
         if (p.tiles == 1)
-          bulk_g2s(wbase, st.w, n * wb, full, pol_w);
+          bulk_g2s(base, st.w, n * wb, full, pol_w);
         else
-          bulk_g2s_plain(wbase, st.w, n * wb, full);
+          bulk_g2s_plain(base, st.w, n * wb, full);
       }
     } else if (lane < st.n) {
       const char* g = st.w + (long long)lane * (I8 ? 16 : 32) * h + 16 * r0;
-      bulk_g2s_plain(wbase + lane * wb, g, 16u * hp, full);
-      if (!I8) bulk_g2s_plain(wbase + lane * wb + 16u * hp, g + 16 * h, 16u * hp, full);
+      bulk_g2s_plain(base + lane * wb, g, 16u * hp, full);
+      if (!I8) bulk_g2s_plain(base + lane * wb + 16u * hp, g + 16 * h, 16u * hp, full);
     }
     // activations: one copy per run of neighbouring groups
     const uint32_t before = __shfl_up_sync(0xffffffffu, st.col, 1);
@@ -386,58 +382,58 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
     if (head) {
       const uint32_t rest = lane < 31 ? heads >> (lane + 1) : 0u;
       const uint32_t run = rest ? uint32_t(__ffs(rest)) : uint32_t(32 - lane);
-      bulk_g2s(base + lane * xb, p.x + (st.tile * per_tile + st.col) * xb, run * xb, full, pol_x);
+      bulk_g2s(xbase + lane * xb, p.x + (st.tile * per_tile + st.col) * xb, run * xb, full, pol_x);
     }
+    ++pipe.i;
     return true;
   };
   UnitWin<RowUnit> win;
   win.init(p.rows, items, p.tiles, lane);
   Stage held{};
   bool have = false;
-  uint32_t g0 = 0;  // stages before this item
+  uint32_t c0 = 0;  // chunks before this item
   int k = 0;
   for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
     const RowUnit u = win.get(k, lane);
     const RowStages<MODE> rs(p.R, int((u.shape >> 8) & 255u));
-    const int s0 = rs.stages(int(u.ng[0])), total = s0 + rs.stages(int(u.ng[1]));
-    for (int j = int((uint32_t(warp) - g0) % kProducers); j < total; j += kProducers) {
-      Stage st;
-      st.which = j >= s0;
-      const int jj = st.which ? j - s0 : j, ns = st.which ? total - s0 : s0;
-      const int groups = int(st.which ? u.ng[1] : u.ng[0]);
-      st.g = g0 + j;
-      st.shape = u.shape;
-      st.off = jj * rs.cap;
-      st.n = min(rs.cap, groups - st.off);
-      st.tile = p.tile0 + item % p.tiles;
-      st.flags = (jj % rs.per_chunk == 0 ? kHdrFirst : 0u) |
-                 (jj % rs.per_chunk == rs.per_chunk - 1 || jj + 1 == ns ? kHdrLast : 0u);
-      const uint32_t g = (st.which ? u.g0[1] : u.g0[0]) + st.off + lane;
-      st.col = lane < st.n ? __ldg(p.group_col + g) : 0u;
-      st.w = p.w + (st.which ? u.w0[1] : u.w0[0]) +
-             (long long)st.off * (I8 ? 16 : 32) * int(u.shape & 255u);
-      if (have && !issue(held)) return;
-      held = st;
-      have = true;
+    const int n0 = rs.chunks(int(u.ng[0])), total = n0 + rs.chunks(int(u.ng[1]));
+    for (int ch = int((uint32_t(warp) - c0) % kPipes); ch < total; ch += kPipes) {
+      const bool up = ch >= n0;
+      const int groups = int(up ? u.ng[1] : u.ng[0]), ns = rs.stages(groups);
+      const int j0 = (up ? ch - n0 : ch) * rs.per_chunk, j1 = min(ns, j0 + rs.per_chunk);
+      for (int j = j0; j < j1; ++j) {
+        const int off = j * rs.cap;
+        Stage st;
+        st.shape = u.shape;
+        st.n = min(rs.cap, groups - off);
+        st.tile = p.tile0 + item % p.tiles;
+        st.flags = (j == j0 ? kHdrFirst : 0u) | (j + 1 == j1 ? kHdrLast : 0u);
+        st.col = lane < st.n ? __ldg(p.group_col + (up ? u.g0[1] : u.g0[0]) + off + lane) : 0u;
+        st.w = p.w + (up ? u.w0[1] : u.w0[0]) + (long long)off * (I8 ? 16 : 32) * int(u.shape & 255u);
+        if (have && !issue(held)) return;
+        held = st;
+        have = true;
+      }
     }
-    g0 += uint32_t(total);
+    c0 += uint32_t(total);
   }
   if (have && !issue(held)) return;
-  produce_end<MODE>(p, sh, bars, g0, warp, lane);
+  produce_end<MODE>(p, sh, bars, pipe, lane);
 }
 
 __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh, uint32_t slots,
                                              uint32_t zero, const PairBars& bars, int warp, int lane) {
-  constexpr uint32_t SLOTS = PairShape<kInputGrad>::slots, BYTES = PairShape<kInputGrad>::slot_bytes;
+  constexpr uint32_t BYTES = PairShape<kInputGrad>::slot_bytes;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
   const int items = p.units * p.tiles;
   const long long per_tile = 2 * (p.M >> 3);
   struct Stage {
-    uint32_t g, flags, w, c0;
+    uint32_t w, c0;
     int tile;
     ColEntry e;
   };
+  Pipe<kInputGrad> pipe{uint32_t(warp) * PairShape<kInputGrad>::ring};
   auto issue = [&](const Stage& st) {
     const ColEntry& e = st.e;
     // places of the entries: groups before this one, and its steps
@@ -453,8 +449,8 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
     const uint32_t groups = __shfl_sync(0xffffffffu, g, kColEntries - 1);
     const uint32_t all_steps = __shfl_sync(0xffffffffu, steps, kColEntries - 1);
     const uint32_t g_before = g - e.h8, s_before = steps - (e.h8 + 1) / 2;
-    if (!wait_slot<kInputGrad>(p, sh, bars, st.g)) return false;
-    const uint32_t slot = st.g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    if (!wait_slot<kInputGrad>(p, sh, bars, pipe)) return false;
+    const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
     const uint32_t a0 = base + g_before * xb, b0 = base + groups * xb + g_before * 32u * st.w;
     const uint32_t h = 8u * e.h8;
     if (lane < kColEntries)
@@ -463,33 +459,31 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
         const uint32_t a = a0 + 2 * j * xb;
         PairStep& out = sh.steps[slot][s_before + j];
         out.a = core_desc(a, pair ? xb : zero - a, 128) |
-                (s_before + j == 0 && (st.flags & kHdrFirst) ? kStepFresh : 0) | (pair ? 0 : kStepOdd);
+                (s_before + j == 0 ? kStepFresh : 0) | (pair ? 0 : kStepOdd);
         // columns 8 apart are 16 h apart (hi and lo' tiles alternate), rows 8 apart 128 bytes
         out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
       }
-    announce(sh, slot, full, all_steps | st.w << 5 | st.flags, groups * (xb + 32u * st.w), lane);
+    announce(sh, slot, full, all_steps | st.w << 5 | kHdrFirst | kHdrLast, groups * (xb + 32u * st.w), lane);
     if (e.h8) {
       bulk_g2s(a0, p.dy + (st.tile * per_tile + e.dy_group) * xb, e.h8 * xb, full, pol_x);
       bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(st.c0 >> 3) * 32 * h, 4u * h * st.w, full);
     }
+    ++pipe.i;
     return true;
   };
   UnitWin<ColUnit> win;
   win.init(p.cols, items, p.tiles, lane);
   Stage held{};
   bool have = false;
-  uint32_t g0 = 0;
+  uint32_t c0 = 0;
   int k = 0;
   for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
     const ColUnit u = win.get(k, lane);
-    for (uint32_t j = (uint32_t(warp) - g0) % kProducers; j < u.ns; j += kProducers) {
+    for (uint32_t j = (uint32_t(warp) - c0) % kPipes; j < u.ns; j += kPipes) {
       Stage st;
-      st.g = g0 + j;
       st.w = u.w;
       st.c0 = u.c0;
       st.tile = p.tile0 + item % p.tiles;
-      st.flags = (j % kChunkStages == 0 ? kHdrFirst : 0u) |
-                 (j % kChunkStages == kChunkStages - 1 || j + 1 == u.ns ? kHdrLast : 0u);
       st.e = ColEntry{};
       if (lane < kColEntries) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.entries) +
@@ -502,29 +496,26 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
       held = st;
       have = true;
     }
-    g0 += u.ns;
+    c0 += u.ns;
   }
   if (have && !issue(held)) return;
-  produce_end<kInputGrad>(p, sh, bars, g0, warp, lane);
+  produce_end<kInputGrad>(p, sh, bars, pipe, lane);
 }
 
 // Token stages of a weight-gradient unit: kGradTokens tokens of a tile (the last of a tile fewer) of
 // the unit's 16 activation groups and h / 8 gradient groups, each group [kGradTokens of hi][of lo'].
-__device__ __forceinline__ int grad_stages(const PairParams& p) {
-  return p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
-}
 __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& sh, uint32_t slots,
                                               const PairBars& bars, int warp, int lane) {
-  constexpr uint32_t SLOTS = PairShape<kWeightGrad>::slots, BYTES = PairShape<kWeightGrad>::slot_bytes;
+  constexpr uint32_t BYTES = PairShape<kWeightGrad>::slot_bytes;
   constexpr uint32_t GB = 32u * kGradTokens;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
   const int per_tile = (p.R + kGradTokens - 1) / kGradTokens, total = p.tiles * per_tile;
   UnitWin<GradUnit> win;
   win.init(p.grads, p.units, 1, lane);
-  uint32_t g0 = 0;
+  Pipe<kWeightGrad> pipe{uint32_t(warp) * PairShape<kWeightGrad>::ring};
+  uint32_t c0 = 0, next_col = 0;
   int k = 0;
-  uint32_t next_col = 0;
   auto load_col = [&](const GradUnit& u) {
     return lane < int(u.ng) ? __ldg(p.group_col + u.g0 + lane) : 0u;
   };
@@ -544,21 +535,18 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
     const bool is_x = lane < int(u.ng), is_dy = lane >= 16 && lane < 16 + int(h8);
     const char* src0 = is_x ? p.x + (long long)col * xb : p.dy + ((long long)u.dy_group + lane - 16) * xb;
     const long long tile_step = (is_x ? p.K >> 3 : 2 * (p.M >> 3)) * xb;
-    for (int j = int((uint32_t(warp) - g0) % kProducers); j < total; j += kProducers) {
+    for (int j = int((uint32_t(warp) - c0) % kPipes); j < total; j += kPipes, ++pipe.i) {
       const int tile = j / per_tile, t0 = (j % per_tile) * kGradTokens, nt = min(kGradTokens, p.R - t0);
-      const uint32_t g = g0 + j;
-      if (!wait_slot<kWeightGrad>(p, sh, bars, g)) return;
-      const uint32_t slot = g % SLOTS, base = slots + slot * BYTES, full = bars.full + 8 * slot;
+      if (!wait_slot<kWeightGrad>(p, sh, bars, pipe)) return;
+      const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
       const uint32_t steps = uint32_t(nt) / 16;
-      const uint32_t flags = (j % kChunkStages == 0 ? kHdrFirst : 0u) |
-                             (j % kChunkStages == kChunkStages - 1 || j + 1 == total ? kHdrLast : 0u);
       if (lane < int(steps)) {
         PairStep& out = sh.steps[slot][lane];
         out.a = core_desc(base + 256u * lane, 128u, GB) |
-                (lane == 0 && (flags & kHdrFirst) ? kStepFresh : 0);
+                (lane == 0 ? kStepFresh : 0);
         out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
       }
-      announce(sh, slot, full, steps | u.h << 5 | flags, (u.ng + h8) * 32u * uint32_t(nt), lane);
+      announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast, (u.ng + h8) * 32u * uint32_t(nt), lane);
       if (is_x || is_dy) {
         const char* src = src0 + tile * tile_step + 16 * t0;
         const uint32_t dst = base + lane * GB;
@@ -566,16 +554,15 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
         bulk_g2s(dst + GB / 2, src + 16 * p.R, 16u * nt, full, pol_x);
       }
     }
-    g0 += uint32_t(total);
+    c0 += uint32_t(total);
   }
-  produce_end<kWeightGrad>(p, sh, bars, g0, warp, lane);
+  produce_end<kWeightGrad>(p, sh, bars, pipe, lane);
 }
 
-// ---- MMA thread ----------------------------------------------------------------------------------
+// ---- MMA threads ---------------------------------------------------------------------------------
 
 template <int MODE>
-__device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& bars) {
-  constexpr uint32_t SLOTS = PairShape<MODE>::slots, ACCS = PairShape<MODE>::accs;
+__device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& bars, int q) {
   const int m = MODE == kWeightGrad ? 128 : (p.R > 64 ? 128 : 64);
   // D f32, A and B f16 (kInt8: D s32, A and B s8); transposed (MN-major) operands in bits 15 and 16
   const uint32_t form = (MODE == kInt8 ? (2u << 4) | (1u << 7) | (1u << 10) : (1u << 4)) |
@@ -583,49 +570,50 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
                         (MODE == kWeightGrad || MODE == kInputGrad ? 1u << 16 : 0u) |
                         (uint32_t(m >> 4) << 24);
   const u64 lo = MODE == kWeightGrad ? kGradTokens : u64(p.R);  // hi to lo' tile of A, in 16 bytes
-  uint32_t slot = 0, parity = 0, use = 0;
-  while (true) {
-    if (!wait_one(bars.full + 8 * slot, parity, p.status, &sh.abort_flag)) return;
+  const uint32_t d = sh.tmem + kAccCols * uint32_t(q);
+  Pipe<MODE> pipe{uint32_t(q) * PairShape<MODE>::ring};
+  uint32_t free_parity = 1;  // of the accumulator
+  for (;; ++pipe.i) {
+    const uint32_t slot = pipe.slot();
+    if (!wait_one(bars.full + 8 * slot, pipe.parity(), p.status, &sh.abort_flag)) return;
     const uint32_t hdr = *reinterpret_cast<volatile uint32_t*>(&sh.header[slot]);
     const int steps = int(hdr & 63u), n = int((hdr >> 8) & 15u) * 8;
     if (steps == 0) break;
-    const uint32_t buf = use % ACCS;
-    if (hdr & kHdrFirst)
-      if (!wait_one(bars.acc_empty + 8 * buf, ((use / ACCS) & 1u) ^ 1u, p.status, &sh.abort_flag)) return;
+    PairStep next = sh.steps[slot][0];
+    if (hdr & kHdrFirst) {
+      if (!wait_one(bars.acc_empty + 8 * q, free_parity, p.status, &sh.abort_flag)) return;
+      free_parity ^= 1u;
+    }
     tc_fence_after();
-    const uint32_t d = sh.tmem + PairShape<MODE>::acc_cols * buf;
     // N of one tile of n columns: a multiple of 16 for M = 128 (one tile more is read, and its
     // columns are not used)
     const int n1 = m == 128 || MODE == kInt8 ? (n + 15) & ~15 : n;
     const uint32_t i1 = form | (uint32_t(n1 >> 3) << 17), i2 = form | (uint32_t(2 * n >> 3) << 17);
     for (int s = 0; s < steps; ++s) {
-      const PairStep st = sh.steps[slot][s];
+      const PairStep st = next;
+      if (s + 1 < steps) next = sh.steps[slot][s + 1];
       const u64 a = st.a & kStepMask, b = st.b;
       const uint32_t acc = (st.a & kStepFresh) ? 0u : 1u;
       if (MODE == kInt8) {
         tc_mma_i8(d, a, b, i1, acc);
         continue;
       }
-      // hi x [hi; lo'] and lo' x hi
       const u64 a2 = a + lo - ((st.a & kStepOdd) ? lo << 16 : 0ull);
-      tc_mma_f16(d, a, b, i2, acc);
-      if (MODE == kForward)  // columns [n, 2n) hold hi lo'; lo' hi joins them
+      if (MODE == kForward) {  // hi x [hi; lo'], then lo' x hi into the columns of hi lo'
+        tc_mma_f16(d, a, b, i2, acc);
         tc_mma_f16(d + n, a2, b, i1, 1u);
-      else  // hi and lo' columns alternate by 8: every second tile, into columns of its own
-        tc_mma_f16(d + 128u, a2, b + (b & (0x3FFFull << 32)), i1, acc);
+      } else {  // B's hi and lo' tiles alternate: every second one
+        const u64 sbo = (b >> 32) & 0x3FFFull, bh = b + (sbo << 32);
+        tc_mma_f16(d, a, bh, i1, acc);
+        tc_mma_f16(d + 64u, a, bh + sbo, i1, acc);
+        tc_mma_f16(d + 64u, a2, bh, i1, 1u);
+      }
     }
     tc_commit(bars.empty + 8 * slot);
-    if (hdr & kHdrLast) {
-      tc_commit(bars.acc_full + 8 * buf);
-      ++use;
-    }
-    if (++slot == SLOTS) {
-      slot = 0;
-      parity ^= 1u;
-    }
+    if (hdr & kHdrLast) tc_commit(bars.acc_full + 8 * q);
   }
-  tc_commit(bars.drain);  // nothing may arrive on a barrier of a CTA that has gone
-  wait_one(bars.drain, 0, p.status, &sh.abort_flag);
+  tc_commit(bars.drain + 8 * q);  // nothing may arrive on a barrier of a CTA that has gone
+  wait_one(bars.drain + 8 * q, 0, p.status, &sh.abort_flag);
 }
 
 // ---- epilogue ------------------------------------------------------------------------------------
@@ -645,7 +633,6 @@ constexpr float kLoUnit = 1.0f / 2048.0f;  // 2^-11
 template <int MODE>
 __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, int quad, int e,
                          int lane) {
-  constexpr uint32_t ACCS = PairShape<MODE>::accs;
   const bool wide = MODE == kWeightGrad || p.R > 64;  // M = 128; M = 64 fills lanes 0..15
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
   const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
@@ -675,39 +662,35 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       live = in_tile && t < p.tokens;
     } else if constexpr (MODE == kInputGrad) {
       n = int(u.w);
-      chunks[0] = (int(u.ns) + kChunkStages - 1) / kChunkStages;
+      chunks[0] = int(u.ns);
       live = in_tile && t < p.tokens;
     } else {
       n = int(u.h);
-      chunks[0] = (grad_stages(p) + kChunkStages - 1) / kChunkStages;
+      chunks[0] = p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
       live = row < int(u.ng) * 8;
     }
     float acc[MODE == kForward ? 2 : 1][4][8] = {};
 #pragma unroll
     for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
       for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
-        const uint32_t buf = use % ACCS;
-        if (!wait_warp(bars.acc_full + 8 * buf, (use / ACCS) & 1u, p.status, &sh.abort_flag)) return;
+        const uint32_t buf = use % kPipes;
+        if (!wait_warp(bars.acc_full + 8 * buf, (use / kPipes) & 1u, p.status, &sh.abort_flag)) return;
         tc_fence_after();
-        const uint32_t d = sh.tmem + PairShape<MODE>::acc_cols * buf + (uint32_t(32 * quad) << 16);
+        const uint32_t d = sh.tmem + kAccCols * buf + (uint32_t(32 * quad) << 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 16 * j + 8 * e;
           if (c >= n) break;
           float* a = acc[which][j];
-          float v[8], l1[8], l2[8];
+          float v[8], l1[8];
           if (MODE == kInt8) {
             tc_ld8_1(d + c, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[i] = v[i];  // 32-bit integers, carried as they are
-          } else if (MODE == kForward) {
-            tc_ld8_2(d + c, d + n + c, v, l1);
+          } else {
+            tc_ld8_2(d + c, d + (MODE == kForward ? n : 64) + c, v, l1);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[i] += fmaf(l1[i], kLoUnit, v[i]);
-          } else {
-            tc_ld8_3(d + 2 * c, d + 2 * c + 8, d + 128 + c, v, l1, l2);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] += fmaf(l1[i] + l2[i], kLoUnit, v[i]);
           }
         }
         tc_fence_before();
@@ -758,31 +741,31 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
 
 template <int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
-  constexpr int SLOTS = PairShape<MODE>::slots, BYTES = PairShape<MODE>::slot_bytes;
+  constexpr int SLOTS = kPipes * PairShape<MODE>::ring, BYTES = PairShape<MODE>::slot_bytes;
   extern __shared__ char dyn[];
   __shared__ PairShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t slots = (smem_addr(dyn) + 1023u) & ~1023u, zero = slots + SLOTS * BYTES;
   char* zero_ptr = dyn + (zero - smem_addr(dyn));
   const PairBars bars{smem_addr(sh.full), smem_addr(sh.empty), smem_addr(sh.acc_full),
-                      smem_addr(sh.acc_empty), smem_addr(&sh.drain)};
+                      smem_addr(sh.acc_empty), smem_addr(sh.drain)};
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(bars.full + 8 * s, 1);
       mbar_init(bars.empty + 8 * s, 1);
     }
-    for (int b = 0; b < PairShape<MODE>::accs; ++b) {
+    for (int b = 0; b < kPipes; ++b) {
       mbar_init(bars.acc_full + 8 * b, 1);
       mbar_init(bars.acc_empty + 8 * b, kEpilogueWarps);
+      mbar_init(bars.drain + 8 * b, 1);
     }
-    mbar_init(bars.drain, 1);
     sh.abort_flag = 0;
     mbar_fence_init();
   }
   for (int i = threadIdx.x; i < kZeroBytes / 16; i += kPairThreads)
     reinterpret_cast<uint4*>(zero_ptr)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
-  if (warp == kProducers) {
+  if (warp == kPipes) {
     tc_alloc(smem_addr(&sh.tmem), 512);
     tc_relinquish();
   }
@@ -790,15 +773,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   __syncthreads();
   tc_fence_after();
 
-  if (warp < kProducers) {
+  if (warp < kPipes) {
     if constexpr (PairShape<MODE>::rows)
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)
       produce_cols(p, sh, slots, zero, bars, warp, lane);
     else
       produce_grads(p, sh, slots, bars, warp, lane);
-  } else if (warp == kProducers) {
-    if (lane == 0) issue_mmas<MODE>(p, sh, bars);
+  } else if (warp < 2 * kPipes) {
+    if (lane == 0) issue_mmas<MODE>(p, sh, bars, warp - kPipes);
     __syncwarp();
   } else if (warp >= kEpilogueWarp) {
     epilogue<MODE>(p, sh, bars, (warp - kEpilogueWarp) & 3, (warp - kEpilogueWarp) >> 2, lane);
@@ -812,7 +795,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
     __syncthreads();
   }
   tc_fence_after();
-  if (warp == kProducers) tc_dealloc(sh.tmem, 512);
+  if (warp == kPipes) tc_dealloc(sh.tmem, 512);
 }
 
 }  // namespace vbsr_b200
