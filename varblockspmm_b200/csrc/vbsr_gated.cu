@@ -8,10 +8,61 @@
 
 #include "vbsr_internal.h"
 #include "vbsr_lm.cuh"
-#include "vbsr_pair.cuh"
+#include "vbsr_pair_host.cuh"
 #include "vbsr_panels.cuh"
 
 using namespace vbsr_b200;
+
+namespace vbsr_b200 {
+// ---- weights -------------------------------------------------------------------------------------
+
+static __global__ void __launch_bounds__(256) values_amax_kernel(const float* a, long long na, const float* b,
+                                                          long long nb, float* partial) {
+  float m = 0.0f;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < na + nb; i += gridDim.x * 256ll)
+    m = fmaxf(m, finite_abs(i < na ? a[i] : b[i - na]));
+  m = cta_max(m);
+  if (threadIdx.x == 0) partial[blockIdx.x] = m;
+}
+
+// A block row of a packed array in pairs; `row_val` is its first value, `groups` its 8-column groups.
+// DEVICE: from the engine's device format (vbsr_tiles.h), else from the packed reference layout; a row
+// is a sequence of groups of 8 h values in both.
+template <bool DEVICE>
+__device__ __forceinline__ void pack_row(const float* values, long long row_val, int h, long long groups,
+                                         float s, char* out) {
+  for (long long i = threadIdx.x; i < groups * h; i += blockDim.x) {
+    const long long g = i / h;
+    const int r = int(i % h);
+    const float* src = values + row_val + g * 8 * h;
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      v[c] = DEVICE ? src[r * 8 + (((c >> 2) ^ ((r >> 2) & 1)) * 4) + (c & 3)] : src[(long long)c * h + r];
+    uint4 hi, lo;
+    to_pair8(v, s, hi, lo);
+    char* o = out + 4 * row_val + g * 32 * h + 16 * r;
+    *reinterpret_cast<uint4*>(o) = hi;
+    *reinterpret_cast<uint4*>(o + 16 * h) = lo;
+  }
+}
+struct PackRow {
+  uint64_t val;     // first value, in the array of its matrix
+  uint32_t groups;  // 8-column groups
+  uint32_t h_which; // h | which << 8
+};
+template <bool DEVICE>
+__global__ void __launch_bounds__(256) pack_kernel(const PackRow* rows, const float* gate, const float* up,
+                                                   long long up_byte, const float* partial, int count,
+                                                   char* out, int* exponent) {
+  const int e = partial_exponent(partial, count);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
+  const PackRow r = rows[blockIdx.x];
+  const int which = int(r.h_which >> 8);
+  pack_row<DEVICE>(which ? up : gate, (long long)r.val, int(r.h_which & 255u), r.groups, pow2(e),
+                   out + (which ? up_byte : 0));
+}
+}  // namespace vbsr_b200
 
 struct vbsr_gated {
   const vbsr_matrix *gate = nullptr, *up = nullptr;
@@ -60,32 +111,6 @@ Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
   return g;
 }
 
-int ctas_for(int64_t threads, int most) {
-  return int(std::max<int64_t>(1, std::min<int64_t>(most, (threads + 255) / 256)));
-}
-
-// Fewest parts per row (column) that give every SM a few work items: a part streams only its share
-// of the weights but all the activations, so more parts than needed cost activation traffic.
-int parts_for(const int (&units)[4], int64_t tiles, int num_sm) {
-  int f = 0;
-  while (f < 3 && units[f] * tiles < 3 * int64_t(num_sm)) ++f;
-  return f;
-}
-
-template <int MODE>
-vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s) {
-  if (k.units == 0) return VBSR_OK;
-  const int64_t most = MODE == kWeightGrad ? tiles : std::max<int64_t>(1, (int64_t(1) << 30) / k.units);
-  for (int64_t t0 = 0; t0 < tiles; t0 += most) {
-    k.tile0 = int(t0);
-    k.tiles = int(std::min(most, tiles - t0));
-    const int64_t items = MODE == kWeightGrad ? k.units : int64_t(k.units) * k.tiles;
-    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, pair_smem<MODE>(), s>>>(k);
-    VBSR_CUDA(cudaGetLastError());
-  }
-  return VBSR_OK;
-}
-
 PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char* ws) {
   PairParams k{};
   k.entries = p->entries;
@@ -120,11 +145,6 @@ vbsr_status make_panel(const Source& src, const Panels& g, int64_t tokens, char*
   return VBSR_OK;
 }
 
-template <class... P>
-int aligned16(const P*... p) {
-  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
-}
-
 template <bool DEVICE>
 vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cudaStream_t s) {
   const int64_t ng = p->gate->d.nvalues, nu = p->up->d.nvalues;
@@ -134,12 +154,6 @@ vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cuda
                                                    p->w_exp);
   VBSR_CUDA(cudaGetLastError());
   return VBSR_OK;
-}
-
-template <class T>
-cudaError_t upload_units(T** dst, int* count, const std::vector<T>& v) {
-  *count = int(v.size());
-  return upload_array(dst, v);
 }
 
 vbsr_status build_gated(vbsr_gated* p) {
@@ -178,31 +192,18 @@ vbsr_status build_gated(vbsr_gated* p) {
   if (pack.empty()) pack.push_back({0, 0, 8});
   VBSR_CUDA(upload_array(&p->pack, pack));
 
-  // units, the largest first: the grid strides over them, which evens out the SMs' shares
-  for (int f = 0; f < 4; ++f) {
-    std::vector<RowUnit> rows;
-    for (int i = 0; i < R; ++i) {
-      const int h = m[0]->h_row_size[i], hp = std::max(8, (h / 8 + (1 << f) - 1) / (1 << f) * 8);
-      for (int r0 = 0; r0 < h; r0 += hp) {
-        RowUnit u{};
-        u.row0 = uint32_t(m[0]->h_row_off[i] + r0);
-        u.shape = uint32_t(h) | uint32_t(std::min(hp, h - r0)) << 8 | uint32_t(r0) << 16;
-        for (int which = 0; which < 2; ++which) {
-          u.g0[which] = g0[which][i];
-          u.ng[which] = ng[which][i];
-          u.w0[which] = uint64_t(4 * m[which]->h_val_off_row[i] + (which ? p->up_byte : 0));
-        }
-        rows.push_back(u);
-      }
+  std::vector<RowUnit> whole_rows(R);
+  for (int i = 0; i < R; ++i) {
+    whole_rows[i].row0 = uint32_t(m[0]->h_row_off[i]);
+    whole_rows[i].shape = uint32_t(m[0]->h_row_size[i]);
+    for (int which = 0; which < 2; ++which) {
+      whole_rows[i].g0[which] = g0[which][i];
+      whole_rows[i].ng[which] = ng[which][i];
+      whole_rows[i].w0[which] = uint64_t(4 * m[which]->h_val_off_row[i] + (which ? p->up_byte : 0));
     }
-    std::stable_sort(rows.begin(), rows.end(), [](const RowUnit& a, const RowUnit& b) {
-      auto cost = [](const RowUnit& u) {
-        return uint64_t(u.ng[0] + u.ng[1]) * (32 + ((u.shape >> 8) & 255u));
-      };
-      return cost(a) > cost(b);
-    });
-    VBSR_CUDA(upload_units(&p->rows[f], &p->row_units[f], rows));
   }
+  const vbsr_status su = upload_row_units(whole_rows, p->rows, p->row_units);
+  if (su != VBSR_OK) return su;
 
   // blocks by block column, gate then up, in stages of at most 64 rows
   std::vector<std::vector<ColEntry>> by_col(S);

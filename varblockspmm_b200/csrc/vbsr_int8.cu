@@ -3,25 +3,30 @@
 
 #include <algorithm>
 #include <new>
+#include <vector>
 
 #include "vbsr_internal.h"
 #include "vbsr_lm.cuh"
+#include "vbsr_pair_host.cuh"
+#include "vbsr_panels.cuh"
 #include "vbsr_tiles.h"
 
 using namespace vbsr_b200;
 
 struct vbsr_int8 {
   const vbsr_matrix* m = nullptr;
-  int device = 0;
+  int device = 0, num_sm = 148;
   int64_t M = 0, K = 0;
-  int8_t* values = nullptr;  // packed
+  char* w = nullptr;  // weights in 16-column chunks
+  uint32_t* chunk_col = nullptr;
+  RowUnit* rows[4] = {};
+  int row_units[4] = {};
   float* row_scale = nullptr;
   int* d_status = nullptr;
 };
 
 namespace {
 
-constexpr int kTok = 8;                     // tokens per CTA
 constexpr int64_t kMaxRowWidth = 131072;    // 127 * 127 * width stays below 2^31
 
 // The integer nearest to x / s, ties to even, as of the exact quotient (s > 0, |x| <= 127.5 s up to
@@ -102,24 +107,119 @@ __global__ void quantize_rows_kernel(vbsr_device_matrix a, int8_t* values, float
   }
 }
 
-// One CTA per block row and kTok tokens; a thread sums one (row, token).
-__global__ void int8_kernel(vbsr_device_matrix a, const int8_t* v, const float* row_scale,
-                            const int8_t* Q, const float* token_scale, long long tokens, float* C) {
-  const int row = blockIdx.x, h = a.row_size[row];
-  const long long t0 = (long long)blockIdx.y * kTok;
-  for (int i = threadIdx.x; i < h * kTok; i += blockDim.x) {
-    const int r = i % h;
-    const long long t = t0 + i / h;
-    if (t >= tokens) continue;
-    int sum = 0;
-    for (int b = a.row_ptr[row]; b < a.row_ptr[row + 1]; ++b) {
-      const int c = a.block_col[b], w = a.col_size[c];
-      const int8_t* x = Q + t * a.scalar_cols + a.col_scalar_off[c];
-      const int8_t* av = v + a.value_off[b] + r;
-      for (int k = 0; k < w; ++k) sum += int(av[(long long)k * h]) * int(x[k]);
+// ---- operands of the tensor-core product (pair_kernel<kInt8>, vbsr_pair.cuh) ----------------------
+//
+// An MMA step takes K = 32, two chunks of 16 columns. A block of width w is cut into chunks from its
+// first column; the last chunk of a width that is 8 mod 16 is filled with zero weights (11% more bytes
+// over the eight widths). Blocks start at multiples of 8, so the panel holds a 16-column chunk from
+// every multiple of 8 on, each column twice: the even ones first, then the odd ones, so that the chunks
+// of a block are neighbours and arrive with one copy. Per tile of R tokens, a chunk is R rows of 16
+// bytes.
+__host__ __device__ constexpr int64_t chunk_place(int64_t col8, int64_t K) {
+  return (col8 & 1) * ((K / 8 + 1) / 2) + (col8 >> 1);
+}
+
+// Block row's weights from the packed layout: [chunk][h rows][16].
+struct LayRow {
+  uint64_t val, out;  // first packed value, first byte
+  uint32_t b0, b1, h, pad;
+};
+__global__ void __launch_bounds__(256) lay_weights_kernel(const LayRow* rows, const uint32_t* blk_desc,
+                                                          const int8_t* values, char* out) {
+  const LayRow r = rows[blockIdx.x];
+  const int8_t* v = values + r.val;
+  char* o = out + r.out;
+  for (uint32_t b = r.b0; b < r.b1; ++b) {
+    const int w = int((blk_desc[b] & 7u) + 1u) * 8, chunks = (w + 15) / 16, h = int(r.h);
+    for (int i = threadIdx.x; i < chunks * h; i += blockDim.x) {
+      const int c = i / h, row = i % h;
+      union {
+        int8_t q[16];
+        uint4 u;
+      } x;
+      for (int k = 0; k < 16; ++k) x.q[k] = 16 * c + k < w ? v[(16 * c + k) * h + row] : int8_t(0);
+      *reinterpret_cast<uint4*>(o + 16 * i) = x.u;
     }
-    const long long o = a.row_scalar_off[row] + r;
-    C[t * a.scalar_rows + o] = float(sum) * (token_scale[t] * row_scale[o]);
+    v += h * w;
+    o += 16 * chunks * h;
+  }
+}
+
+// Largest magnitude of each of `splits` equal parts of every token, or NaN: grid (splits, tokens).
+__global__ void __launch_bounds__(256) token_amax_kernel(const float* B, long long K, int vec,
+                                                         float* partial) {
+  const float* x = B + (long long)blockIdx.y * K;
+  const long long g0 = (K / 8) * blockIdx.x / gridDim.x, g1 = (K / 8) * (blockIdx.x + 1) / gridDim.x;
+  float m = 0.0f;
+  bool finite = true;
+  for (long long g = g0 + threadIdx.x; g < g1; g += blockDim.x) {
+    float v[8];
+    load8(x + 8 * g, vec, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m = fmaxf(m, fabsf(v[i]));
+      finite = finite && isfinite(v[i]);
+    }
+  }
+  m = block_amax(m, finite);
+  if (threadIdx.x == 0)
+    partial[(long long)blockIdx.y * gridDim.x + blockIdx.x] = finite ? m : __int_as_float(0x7fc00000);
+}
+
+// The panel's chunks of one tile per grid row. FLOAT: from fp32 values (partial maxima given, scales
+// written), else from int8 ones. A thread takes 8 columns of a token: the first half of their own
+// chunk and the second half of the one before.
+template <bool FLOAT>
+__global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long long tokens, long long K,
+                                                          int R, int vec, const float* partial, int splits,
+                                                          float* token_scale, char* out) {
+  __shared__ float scale[128];
+  const long long t0 = (long long)blockIdx.y * R, groups = K / 8;
+  if (FLOAT) {
+    for (int r = threadIdx.x; r < R && t0 + r < tokens; r += blockDim.x) {
+      float m = 0.0f;
+      bool finite = true;
+      for (int i = 0; i < splits; ++i) {
+        const float x = partial[(t0 + r) * splits + i];
+        finite = finite && x == x;
+        m = fmaxf(m, x);
+      }
+      scale[r] = scale_of(m, finite);
+      if (blockIdx.x == 0) token_scale[t0 + r] = scale[r];
+    }
+    __syncthreads();
+  }
+  char* tile = out + t0 * groups * 16;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < groups * R; i += gridDim.x * 256ll) {
+    const int r = int(i % R);
+    const long long g = i / R, t = t0 + r;
+    union {
+      int8_t q[8];
+      uint2 u;
+    } x;
+    x.u = make_uint2(0, 0);
+    if (t < tokens) {
+      if (FLOAT) {
+        const float s = scale[r];
+        if (s > 0.0f) {
+          float v[8];
+          load8(static_cast<const float*>(src) + t * K + 8 * g, vec, v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x.q[k] = int8_t(quantize_exact(v[k], s));
+        }
+      } else {
+        const int8_t* q = static_cast<const int8_t*>(src) + t * K + 8 * g;
+        if (vec) {
+          x.u = *reinterpret_cast<const uint2*>(q);
+        } else {
+          for (int k = 0; k < 8; ++k) x.q[k] = q[k];
+        }
+      }
+    }
+    *reinterpret_cast<uint2*>(tile + (chunk_place(g, K) * R + r) * 16) = x.u;
+    if (g > 0) *reinterpret_cast<uint2*>(tile + (chunk_place(g - 1, K) * R + r) * 16 + 8) = x.u;
+    if (g + 1 == groups)
+      *reinterpret_cast<uint2*>(tile + (chunk_place(g, K) * R + r) * 16 + 8) = make_uint2(0, 0);
   }
 }
 
@@ -130,26 +230,67 @@ vbsr_status launch_quantize(const float* B, int64_t K, int64_t tokens, int8_t* Q
   return VBSR_OK;
 }
 
-vbsr_status launch_int8(const vbsr_int8* p, const int8_t* Q, const float* scale, int64_t tokens,
-                        float* C, cudaStream_t s) {
-  const MatrixData& d = p->m->d;
-  const int64_t step = int64_t(kTok) * 65535;  // grid limit in y
-  for (int64_t t0 = 0; t0 < tokens; t0 += step) {
-    const int64_t n = std::min(step, tokens - t0);
-    const dim3 grid(d.block_rows, unsigned((n + kTok - 1) / kTok));
-    int8_kernel<<<grid, 256, 0, s>>>(view_of(d), p->values, p->row_scale, Q + t0 * p->K, scale + t0,
-                                     n, C + t0 * p->M);
-    VBSR_CUDA(cudaGetLastError());
-  }
-  return VBSR_OK;
+// Geometry of a call: even tiles of at most 128 tokens; few tokens are searched for their largest
+// magnitude by several CTAs each.
+struct Geometry {
+  int R = 0, splits = 1;
+  int64_t tiles = 0, scale_at = 0, panel_at = 0, bytes = 0;
+};
+Geometry geometry_of(const vbsr_int8* p, int64_t tokens) {
+  Geometry g;
+  if (tokens == 0) return g;
+  g.tiles = (tokens + 127) / 128;
+  g.R = int((tokens + g.tiles - 1) / g.tiles);
+  g.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(64, p->K / 1024), 296 / tokens)));
+  g.scale_at = align256(4 * tokens * g.splits);
+  g.panel_at = g.scale_at + align256(4 * tokens);
+  g.bytes = g.panel_at + align256(g.tiles * g.R * (p->K / 8) * 16);
+  return g;
 }
 
-int64_t q_bytes(const vbsr_int8* p, int64_t tokens) { return align256(p->K * tokens); }
+vbsr_status launch_int8(const vbsr_int8* p, const Geometry& g, const float* scale, int64_t tokens,
+                        const char* panel, float* C, cudaStream_t s) {
+  PairParams k{};
+  const int f = parts_for(p->row_units, g.tiles, p->num_sm);
+  k.rows = p->rows[f];
+  k.units = p->row_units[f];
+  k.group_col = p->chunk_col;
+  k.R = g.R;
+  k.tokens = tokens;
+  k.M = p->M;
+  k.K = p->K;
+  k.x = panel;
+  k.x_chunks = p->K / 8;
+  k.w = p->w;
+  k.row_scale = p->row_scale;
+  k.token_scale = scale;
+  k.out0 = C;
+  k.vec = aligned16(C);
+  k.status = p->d_status;
+  return launch_pair<kInt8>(k, g.tiles, p->num_sm, s);
+}
+
+template <bool FLOAT>
+vbsr_status launch_chunks(const vbsr_int8* p, const Geometry& g, const void* src, int vec, int64_t tokens,
+                          char* ws, cudaStream_t s) {
+  // one grid row per tile (at most 32768, see kMaxTokens)
+  const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(ctas_for(p->K / 8 * g.R, 592),
+                                                                 (2368 + g.tiles - 1) / g.tiles))),
+                  unsigned(g.tiles));
+  chunk_panel_kernel<FLOAT><<<grid, 256, 0, s>>>(src, tokens, p->K, g.R, vec,
+                                                 reinterpret_cast<const float*>(ws), g.splits,
+                                                 reinterpret_cast<float*>(ws + g.scale_at),
+                                                 ws + g.panel_at);
+  VBSR_CUDA(cudaGetLastError());
+  return VBSR_OK;
+}
 
 void free_int8(vbsr_int8* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
-  cudaFree(p->values);
+  cudaFree(p->w);
+  cudaFree(p->chunk_col);
+  for (RowUnit* r : p->rows) cudaFree(r);
   cudaFree(p->row_scale);
   cudaFree(p->d_status);
   delete p;
@@ -157,13 +298,45 @@ void free_int8(vbsr_int8* p) {
 
 vbsr_status build_int8(vbsr_int8* p, const int8_t* values, const float* row_scale) {
   const MatrixData& d = p->m->d;
-  VBSR_CUDA(cudaMalloc(&p->values, std::max<int64_t>(1, d.nvalues)));
+  VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
+  VBSR_CUDA(cudaFuncSetAttribute(pair_kernel<kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 pair_smem<kInt8>()));
+  std::vector<uint32_t> cols;
+  std::vector<LayRow> lay;
+  std::vector<RowUnit> whole(d.block_rows);
+  uint64_t at = 0;
+  for (int i = 0; i < d.block_rows; ++i) {
+    RowUnit& u = whole[i];
+    u.row0 = uint32_t(d.h_row_off[i]);
+    u.shape = uint32_t(d.h_row_size[i]);
+    u.g0[0] = uint32_t(cols.size());
+    u.w0[0] = at;
+    for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
+      const int64_t col8 = d.h_blk_desc[b] >> 3, w8 = (d.h_blk_desc[b] & 7u) + 1u;
+      for (int64_t c = 0; c < w8; c += 2) cols.push_back(uint32_t(chunk_place(col8 + c, p->K)));
+    }
+    u.ng[0] = uint32_t(cols.size()) - u.g0[0];
+    lay.push_back({uint64_t(d.h_val_off_row[i]), at, uint32_t(d.h_row_ptr[i]),
+                   uint32_t(d.h_row_ptr[i + 1]), uint32_t(d.h_row_size[i]), 0});
+    at += uint64_t(16) * d.h_row_size[i] * u.ng[0];
+  }
+  VBSR_CUDA(upload_array(&p->chunk_col, cols));
+  const vbsr_status st = upload_row_units(whole, p->rows, p->row_units);
+  if (st != VBSR_OK) return st;
+  VBSR_CUDA(cudaMalloc(&p->w, std::max<uint64_t>(256, at)));
   VBSR_CUDA(cudaMalloc(&p->row_scale, 4 * d.M));
   VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
   VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMemcpy(p->values, values, d.nvalues, cudaMemcpyDeviceToDevice));
   VBSR_CUDA(cudaMemcpy(p->row_scale, row_scale, 4 * d.M, cudaMemcpyDeviceToDevice));
-  VBSR_CUDA(cudaStreamSynchronize(nullptr));
+  LayRow* d_lay = nullptr;
+  cudaError_t e = upload_array(&d_lay, lay);
+  if (e == cudaSuccess) {
+    lay_weights_kernel<<<unsigned(d.block_rows), 256>>>(d_lay, d.d_blk_desc, values, p->w);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+  cudaFree(d_lay);
+  VBSR_CUDA(e);
   return VBSR_OK;
 }
 
@@ -216,7 +389,7 @@ vbsr_status vbsr_int8_workspace_bytes(const vbsr_int8* p, int64_t tokens, int64_
   if (bytes == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null output");
   if (tokens < 0 || tokens > kMaxTokens)
     return set_error(VBSR_INVALID_ARGUMENT, "tokens must be between 0 and 2^22");
-  *bytes = q_bytes(p, tokens) + align256(4 * tokens);
+  *bytes = geometry_of(p, tokens).bytes;
   return VBSR_OK;
 }
 
@@ -231,7 +404,12 @@ vbsr_status vbsr_int8_execute(const vbsr_int8* p, const int8_t* Q, const float* 
   if (Q == nullptr || token_scale == nullptr || C == nullptr)
     return set_error(VBSR_INVALID_ARGUMENT, "null Q, token_scale or C");
   DeviceGuard guard(p->device);
-  return launch_int8(p, Q, token_scale, tokens, C, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const Geometry g = geometry_of(p, tokens);
+  st = launch_chunks<false>(p, g, Q, (reinterpret_cast<uintptr_t>(Q) & 7u) == 0, tokens, ws, s);
+  if (st != VBSR_OK) return st;
+  return launch_int8(p, g, token_scale, tokens, ws + g.panel_at, C, s);
 }
 
 vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t tokens, float* C,
@@ -245,11 +423,18 @@ vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t 
   if (B == nullptr || C == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null B or C");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int8_t* Q = static_cast<int8_t*>(workspace);
-  float* scale = reinterpret_cast<float*>(Q + q_bytes(p, tokens));
-  st = launch_quantize(B, p->K, tokens, Q, scale, s);
+  char* ws = static_cast<char*>(workspace);
+  const Geometry g = geometry_of(p, tokens);
+  const int vec = aligned16(B);
+  for (int64_t t0 = 0; t0 < tokens; t0 += 65535) {  // grid limit in y
+    const int64_t n = std::min<int64_t>(65535, tokens - t0);
+    token_amax_kernel<<<dim3(unsigned(g.splits), unsigned(n)), 256, 0, s>>>(
+        B + t0 * p->K, p->K, vec, reinterpret_cast<float*>(ws) + t0 * g.splits);
+  }
+  VBSR_CUDA(cudaGetLastError());
+  st = launch_chunks<true>(p, g, B, vec, tokens, ws, s);
   if (st != VBSR_OK) return st;
-  return launch_int8(p, Q, scale, tokens, C, s);
+  return launch_int8(p, g, reinterpret_cast<const float*>(ws + g.scale_at), tokens, ws + g.panel_at, C, s);
 }
 
 vbsr_status vbsr_int8_check_status(const vbsr_int8* p, vbsr_stream_t stream) {

@@ -708,12 +708,16 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       if constexpr (MODE == kForward) {
         float(&w)[8] = acc[1][j];
         float hv[8];
+        with_act(p.act, [&](auto kind) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = v[i] * f1 * f2;
-          w[i] = w[i] * f1 * f2;
-          hv[i] = act_value(p.act, v[i]) * w[i];
-        }
+          for (int i = 0; i < 8; ++i) {
+            v[i] = v[i] * f1 * f2;
+            w[i] = w[i] * f1 * f2;
+            float a, da;
+            act_both<decltype(kind)::value>(v[i], a, da);
+            hv[i] = a * w[i];
+          }
+        });
         const long long o = t * p.M + u.row0 + c;
         store8(p.out0 + o, hv, p.vec);
         if (p.out1 != nullptr) {

@@ -1,0 +1,76 @@
+// vbsr_pair_host.cuh — host side shared by the operators on pair_kernel: launches, work units.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "vbsr_lm.cuh"
+#include "vbsr_pair.cuh"
+
+namespace vbsr_b200 {
+
+inline int ctas_for(int64_t threads, int most) {
+  return int(std::max<int64_t>(1, std::min<int64_t>(most, (threads + 255) / 256)));
+}
+
+// Fewest parts per row (column) that give every SM a few work items: a part streams only its share
+// of the weights but all the activations, so more parts than needed cost activation traffic.
+inline int parts_for(const int (&units)[4], int64_t tiles, int num_sm) {
+  int f = 0;
+  while (f < 3 && units[f] * tiles < 3 * int64_t(num_sm)) ++f;
+  return f;
+}
+
+template <int MODE>
+vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s) {
+  if (k.units == 0) return VBSR_OK;
+  const int64_t most = MODE == kWeightGrad ? tiles : std::max<int64_t>(1, (int64_t(1) << 30) / k.units);
+  for (int64_t t0 = 0; t0 < tiles; t0 += most) {
+    k.tile0 = int(t0);
+    k.tiles = int(std::min(most, tiles - t0));
+    const int64_t items = MODE == kWeightGrad ? k.units : int64_t(k.units) * k.tiles;
+    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, pair_smem<MODE>(), s>>>(k);
+    VBSR_CUDA(cudaGetLastError());
+  }
+  return VBSR_OK;
+}
+
+template <class... P>
+int aligned16(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
+}
+
+template <class T>
+cudaError_t upload_units(T** dst, int* count, const std::vector<T>& v) {
+  *count = int(v.size());
+  return upload_array(dst, v);
+}
+
+// Units of the block rows (given whole, shape = height), cut into 1, 2, 4 and 8 parts where their height
+// allows, the largest first: the grid strides over them, which evens out the SMs' shares. A unit's cost is
+// its weights' bytes and as much as 32 rows' for the activations.
+inline vbsr_status upload_row_units(const std::vector<RowUnit>& whole, RowUnit* (&rows)[4], int (&count)[4]) {
+  for (int f = 0; f < 4; ++f) {
+    std::vector<RowUnit> units;
+    for (const RowUnit& w : whole) {
+      const int h = int(w.shape), hp = std::max(8, (h / 8 + (1 << f) - 1) / (1 << f) * 8);
+      for (int r0 = 0; r0 < h; r0 += hp) {
+        RowUnit u = w;
+        u.row0 += uint32_t(r0);
+        u.shape = uint32_t(h) | uint32_t(std::min(hp, h - r0)) << 8 | uint32_t(r0) << 16;
+        units.push_back(u);
+      }
+    }
+    std::stable_sort(units.begin(), units.end(), [](const RowUnit& a, const RowUnit& b) {
+      auto cost = [](const RowUnit& u) {
+        return uint64_t(u.ng[0] + u.ng[1]) * (32 + ((u.shape >> 8) & 255u));
+      };
+      return cost(a) > cost(b);
+    });
+    VBSR_CUDA(upload_units(&rows[f], &count[f], units));
+  }
+  return VBSR_OK;
+}
+
+}  // namespace vbsr_b200

@@ -1,5 +1,5 @@
-// vbsr_panels.cuh — the pre-passes of the block-sparse layer operators: fp32 panels and weights to
-// operand pairs (layout and reasons in vbsr_pair.cuh).
+// vbsr_panels.cuh — the pre-passes of the block-sparse layer operators: fp32 panels to operand
+// pairs (layout and reasons in vbsr_pair.cuh).
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -91,13 +91,15 @@ struct GateSource {
     load8(G + o, vec, a);
     load8(U + o, vec, u);
     load8(dH + o, vec, d);
+    with_act(act, [&](auto kind) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float val, der;
-      act_both(act, a[i], val, der);
-      v[0][i] = d[i] * u[i] * der;
-      v[1][i] = d[i] * val;
-    }
+      for (int i = 0; i < 8; ++i) {
+        float val, der;
+        act_both<decltype(kind)::value>(a[i], val, der);
+        v[0][i] = d[i] * u[i] * der;
+        v[1][i] = d[i] * val;
+      }
+    });
   }
 };
 
@@ -142,55 +144,6 @@ __global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long t
       o[R] = lo;
     }
   }
-}
-
-// ---- weights -------------------------------------------------------------------------------------
-
-__global__ void __launch_bounds__(256) values_amax_kernel(const float* a, long long na, const float* b,
-                                                          long long nb, float* partial) {
-  float m = 0.0f;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < na + nb; i += gridDim.x * 256ll)
-    m = fmaxf(m, finite_abs(i < na ? a[i] : b[i - na]));
-  m = cta_max(m);
-  if (threadIdx.x == 0) partial[blockIdx.x] = m;
-}
-
-// A block row of a packed array in pairs; `row_val` is its first value, `groups` its 8-column groups.
-// DEVICE: from the engine's device format (vbsr_tiles.h), else from the packed reference layout; a row
-// is a sequence of groups of 8 h values in both.
-template <bool DEVICE>
-__device__ __forceinline__ void pack_row(const float* values, long long row_val, int h, long long groups,
-                                         float s, char* out) {
-  for (long long i = threadIdx.x; i < groups * h; i += blockDim.x) {
-    const long long g = i / h;
-    const int r = int(i % h);
-    const float* src = values + row_val + g * 8 * h;
-    float v[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-      v[c] = DEVICE ? src[r * 8 + (((c >> 2) ^ ((r >> 2) & 1)) * 4) + (c & 3)] : src[(long long)c * h + r];
-    uint4 hi, lo;
-    to_pair8(v, s, hi, lo);
-    char* o = out + 4 * row_val + g * 32 * h + 16 * r;
-    *reinterpret_cast<uint4*>(o) = hi;
-    *reinterpret_cast<uint4*>(o + 16 * h) = lo;
-  }
-}
-struct PackRow {
-  uint64_t val;     // first value, in the array of its matrix
-  uint32_t groups;  // 8-column groups
-  uint32_t h_which; // h | which << 8
-};
-template <bool DEVICE>
-__global__ void __launch_bounds__(256) pack_kernel(const PackRow* rows, const float* gate, const float* up,
-                                                   long long up_byte, const float* partial, int count,
-                                                   char* out, int* exponent) {
-  const int e = partial_exponent(partial, count);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
-  const PackRow r = rows[blockIdx.x];
-  const int which = int(r.h_which >> 8);
-  pack_row<DEVICE>(which ? up : gate, (long long)r.val, int(r.h_which & 255u), r.groups, pow2(e),
-                   out + (which ? up_byte : 0));
 }
 
 }  // namespace vbsr_b200
