@@ -164,7 +164,7 @@ vbsr_status build_gated(vbsr_gated* p) {
                         reinterpret_cast<const void*>(pair_kernel<kInputGrad>),
                         reinterpret_cast<const void*>(pair_kernel<kWeightGrad>)})
     VBSR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   std::max(pair_smem<kForward>(), pair_smem<kInputGrad>())));
+                                   kPairSmem));
   p->up_byte = align256(4 * m[0]->nvalues);
 
   // group lists, block rows of both matrices
@@ -180,6 +180,8 @@ vbsr_status build_gated(vbsr_gated* p) {
         for (uint32_t c = 0; c < n; ++c) group_col.push_back(col8 + c);
       }
       ng[which].push_back(uint32_t(group_col.size()) - g0[which].back());
+      if (ng[which][i] >= (1u << 27))
+        return set_error(VBSR_INVALID_ARGUMENT, "a block row is too long for the plan's index range");
       if (ng[which][i] > 0)
         pack.push_back({uint64_t(d.h_val_off_row[i]), ng[which][i],
                         uint32_t(d.h_row_size[i]) | uint32_t(which) << 8});
@@ -402,13 +404,11 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
   const vbsr_status st2 = make_panel(PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, g, tokens, ws);
-  const int f = parts_for(p->row_units, g.tiles, p->num_sm);
-  k.rows = p->rows[f];
-  k.units = p->row_units[f];
   k.out0 = H;
   k.out1 = G;
   k.out2 = U;
   k.vec = aligned16(H, G, U);
+  choose_rows(k, p->rows, p->row_units, g.tiles, p->num_sm);
   return launch_pair<kForward>(k, g.tiles, p->num_sm, s);
 }
 

@@ -251,9 +251,6 @@ Geometry geometry_of(const vbsr_int8* p, int64_t tokens) {
 vbsr_status launch_int8(const vbsr_int8* p, const Geometry& g, const float* scale, int64_t tokens,
                         const char* panel, float* C, cudaStream_t s) {
   PairParams k{};
-  const int f = parts_for(p->row_units, g.tiles, p->num_sm);
-  k.rows = p->rows[f];
-  k.units = p->row_units[f];
   k.group_col = p->chunk_col;
   k.R = g.R;
   k.tokens = tokens;
@@ -267,6 +264,7 @@ vbsr_status launch_int8(const vbsr_int8* p, const Geometry& g, const float* scal
   k.out0 = C;
   k.vec = aligned16(C);
   k.status = p->d_status;
+  choose_rows(k, p->rows, p->row_units, g.tiles, p->num_sm);
   return launch_pair<kInt8>(k, g.tiles, p->num_sm, s);
 }
 
@@ -300,7 +298,7 @@ vbsr_status build_int8(vbsr_int8* p, const int8_t* values, const float* row_scal
   const MatrixData& d = p->m->d;
   VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
   VBSR_CUDA(cudaFuncSetAttribute(pair_kernel<kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 pair_smem<kInt8>()));
+                                 kPairSmem));
   std::vector<uint32_t> cols;
   std::vector<LayRow> lay;
   std::vector<RowUnit> whole(d.block_rows);

@@ -59,8 +59,8 @@ enum PairMode { kForward = 0, kInputGrad = 1, kWeightGrad = 2, kInt8 = 3 };
 struct alignas(16) RowUnit {
   uint32_t row0;   // first row of C
   uint32_t shape;  // h | hp << 8 | r0 << 16
-  uint32_t g0[2];  // first entry of the group list
   uint32_t ng[2];  // groups (kInt8: 16-column chunks)
+  uint32_t g0[2];  // first entry of the group list
   uint64_t w0[2];  // byte of the first group's weights
   uint64_t pad;
 };
@@ -94,6 +94,7 @@ struct PairParams {
   const uint32_t* group_col;  // per group: scalar column / 8
   int units, tiles, tile0;    // work items are units x tiles from tile0 on (kWeightGrad: units)
   int R, act;
+  int ring_log, acc_log;      // slots and accumulators per pipeline
   long long tokens, M, K;
   const char* x;              // activation panel in pairs (kInt8: in 16-column chunks)
   long long x_chunks;         // kInt8: chunks per tile of it
@@ -116,29 +117,28 @@ struct PairStep {
 constexpr u64 kStepFresh = 1ull << 60;  // first step into its accumulator: overwrite
 constexpr u64 kStepOdd = 1ull << 58;    // the second K half of A is the tile of zeros
 constexpr u64 kStepMask = (1ull << 56) - 1;
-constexpr int kMaxSteps = 32;
+constexpr int kMaxSteps = 16;
 
 // Slot header: steps | N/8 << 8 | flags. No steps: end of the work.
 constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17;
 
-template <int MODE>
-struct PairShape {
-  static constexpr bool rows = MODE == kForward || MODE == kInt8;
-  static constexpr uint32_t ring = rows ? 2 : 1;  // slots per pipeline
-  static constexpr uint32_t slot_bytes = rows ? 24 * 1024 : 48 * 1024;
-};
+__host__ __device__ constexpr bool by_rows(int mode) { return mode == kForward || mode == kInt8; }
 constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA threads in warps 4 .. 7
-constexpr uint32_t kAccCols = 128;  // TMEM columns of an accumulator: hi sums, then lo sums
+// A pipeline's share of shared memory, cut into 2^ring_log slots, and of the 512 TMEM columns, cut into
+// 2^acc_log accumulators of 128 or 64 columns (hi sums, then lo sums).
+constexpr uint32_t kPipeBytes = 48 * 1024;
+constexpr int kMaxSlots = 16, kMaxAccs = 8;
 constexpr int kEpilogueWarp = 8, kEpilogueWarps = 8;
 constexpr int kPairThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr int kChunkSteps = 8;
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage
-template <int MODE>
-constexpr int pair_smem() {
-  return kPipes * PairShape<MODE>::ring * PairShape<MODE>::slot_bytes + kZeroBytes + kTailBytes + 1024;
-}
+// kForward, kInt8: results pass through shared memory, two matrices of R rows and 2^stage_log(R)
+// columns with 4 of padding; two such buffers for up to 16 tokens.
+constexpr int kStageBytes = 2 * 128 * 20 * 4;
+__host__ __device__ constexpr int stage_log(int R) { return R <= 32 ? 6 : (R <= 64 ? 5 : 4); }
+constexpr int kPairSmem = kPipes * kPipeBytes + kZeroBytes + kTailBytes + kStageBytes + 1024;
 
 __device__ __forceinline__ u64 core_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return u64((addr >> 4) & 0x3FFFu) | (u64((lbo >> 4) & 0x3FFFu) << 16) |
@@ -169,25 +169,139 @@ __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, ui
       : "memory");
 }
 
-// 8 accumulator columns each from one or two places, loaded and waited for in one statement
-// (the registers are not valid before the wait).
-__device__ __forceinline__ void tc_ld8_1(uint32_t a, float (&v)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-      : "r"(a)
-      : "memory");
-}
-__device__ __forceinline__ void tc_ld8_2(uint32_t a, uint32_t b, float (&v)[8], float (&w)[8]) {
+// Tiles of 8 accumulator columns, loaded and waited for in one statement (the registers are not valid
+// before the wait): NJ tiles 16 columns apart from `a` on, and as many from `b` on (tc_ld1: from `a` only).
+template <int NJ>
+__device__ __forceinline__ void tc_ld2(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]);
+template <>
+__device__ __forceinline__ void tc_ld2<1>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-        "=f"(v[7]), "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]),
-        "=f"(w[6]), "=f"(w[7])
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]),
+        "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7])
       : "r"(a), "r"(b)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld2<2>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(w[0][0]), "=f"(w[0][1]),
+        "=f"(w[0][2]), "=f"(w[0][3]), "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7]),
+        "=f"(w[1][0]), "=f"(w[1][1]), "=f"(w[1][2]), "=f"(w[1][3]), "=f"(w[1][4]), "=f"(w[1][5]),
+        "=f"(w[1][6]), "=f"(w[1][7])
+      : "r"(a), "r"(a + 16), "r"(b), "r"(b + 16)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld2<3>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%48];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%49];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%50];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%51];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%32, %33, %34, %35, %36, %37, %38, %39}, [%52];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%40, %41, %42, %43, %44, %45, %46, %47}, [%53];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
+        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
+        "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]), "=f"(w[0][4]), "=f"(w[0][5]),
+        "=f"(w[0][6]), "=f"(w[0][7]), "=f"(w[1][0]), "=f"(w[1][1]), "=f"(w[1][2]), "=f"(w[1][3]),
+        "=f"(w[1][4]), "=f"(w[1][5]), "=f"(w[1][6]), "=f"(w[1][7]), "=f"(w[2][0]), "=f"(w[2][1]),
+        "=f"(w[2][2]), "=f"(w[2][3]), "=f"(w[2][4]), "=f"(w[2][5]), "=f"(w[2][6]), "=f"(w[2][7])
+      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(b), "r"(b + 16), "r"(b + 32)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld2<4>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%65];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%66];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%67];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%32, %33, %34, %35, %36, %37, %38, %39}, [%68];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%40, %41, %42, %43, %44, %45, %46, %47}, [%69];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%48, %49, %50, %51, %52, %53, %54, %55}, [%70];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%56, %57, %58, %59, %60, %61, %62, %63}, [%71];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
+        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
+        "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]), "=f"(v[3][4]), "=f"(v[3][5]),
+        "=f"(v[3][6]), "=f"(v[3][7]), "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]),
+        "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7]), "=f"(w[1][0]), "=f"(w[1][1]),
+        "=f"(w[1][2]), "=f"(w[1][3]), "=f"(w[1][4]), "=f"(w[1][5]), "=f"(w[1][6]), "=f"(w[1][7]),
+        "=f"(w[2][0]), "=f"(w[2][1]), "=f"(w[2][2]), "=f"(w[2][3]), "=f"(w[2][4]), "=f"(w[2][5]),
+        "=f"(w[2][6]), "=f"(w[2][7]), "=f"(w[3][0]), "=f"(w[3][1]), "=f"(w[3][2]), "=f"(w[3][3]),
+        "=f"(w[3][4]), "=f"(w[3][5]), "=f"(w[3][6]), "=f"(w[3][7])
+      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(a + 48), "r"(b), "r"(b + 16), "r"(b + 32), "r"(b + 48)
+      : "memory");
+}
+template <int NJ>
+__device__ __forceinline__ void tc_ld1(uint32_t a, float (&v)[4][8]);
+template <>
+__device__ __forceinline__ void tc_ld1<1>(uint32_t a, float (&v)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7])
+      : "r"(a)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld1<2>(uint32_t a, float (&v)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7])
+      : "r"(a), "r"(a + 16)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld1<3>(uint32_t a, float (&v)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
+        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7])
+      : "r"(a), "r"(a + 16), "r"(a + 32)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tc_ld1<4>(uint32_t a, float (&v)[4][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
+        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
+        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
+        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
+        "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]), "=f"(v[3][4]), "=f"(v[3][5]),
+        "=f"(v[3][6]), "=f"(v[3][7])
+      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(a + 48)
       : "memory");
 }
 
@@ -219,20 +333,34 @@ __device__ __forceinline__ void unscale(int e, float& f1, float& f2) {
   f2 = __int_as_float((b + 127) << 23);
 }
 
-// Stages and accumulation chunks of a row unit: groups per stage, stages per chunk.
-template <int MODE>
+// n / d for 0 <= n < 2^27 and 1 <= d <= 32, with m = ceil(2^32 / d) (d = 1: m = 0): n m / 2^32 is off
+// by n (m d - 2^32) / 2^32 < 1 / d.
+__device__ __forceinline__ uint32_t div_magic(uint32_t d) {
+  return d == 1 ? 0u : uint32_t((0x100000000ull + d - 1) / d);
+}
+__device__ __forceinline__ int div_by(int n, uint32_t magic) {
+  return magic ? int(__umulhi(uint32_t(n), magic)) : n;
+}
+
+// Stages and accumulation chunks of the row units of one height: groups per stage, stages per chunk. An
+// integer division takes tens of clocks and every role would do several per work item, so they are
+// worked out once per height.
 struct RowStages {
-  int cap, per_chunk;
-  __device__ __forceinline__ RowStages(int R, int hp) {
-    const int b = (MODE == kInt8 ? 16 : 32) * (R + hp);
-    cap = PairShape<MODE>::slot_bytes / b;
+  int cap, per_chunk;  // kInt8: one chunk, per_chunk = 0
+  uint32_t cap_magic, chunk_magic;
+  template <int MODE>
+  __device__ __forceinline__ void init(const PairParams& p, int hp) {
+    cap = int(kPipeBytes >> p.ring_log) / ((MODE == kInt8 ? 16 : 32) * (p.R + hp));
     const int most = MODE == kInt8 ? 32 : 2 * kChunkSteps;
     cap = (cap < most ? cap : most) & ~1;
-    per_chunk = MODE == kInt8 ? 1 << 20 : (2 * kChunkSteps) / cap;
+    per_chunk = MODE == kInt8 ? 0 : (2 * kChunkSteps) / cap;
+    cap_magic = div_magic(cap);
+    chunk_magic = MODE == kInt8 ? 0u : div_magic(per_chunk);
   }
-  __device__ __forceinline__ int stages(int groups) const { return (groups + cap - 1) / cap; }
+  __device__ __forceinline__ int stages(int groups) const { return div_by(groups + cap - 1, cap_magic); }
   __device__ __forceinline__ int chunks(int groups) const {
-    return MODE == kInt8 ? (groups > 0) : (stages(groups) + per_chunk - 1) / per_chunk;
+    if (per_chunk == 0) return groups > 0;
+    return div_by(stages(groups) + per_chunk - 1, chunk_magic);
   }
 };
 // kInputGrad, kWeightGrad: a stage (of at most 8 and 4 steps) is a chunk.
@@ -282,14 +410,26 @@ struct UnitWin {
   }
 };
 
+// Token tile of the CTA's items, item = unit x tiles + tile, kept without divisions.
+struct TileWalk {
+  int tile, step, tiles;
+  __device__ __forceinline__ TileWalk(int tiles_)
+      : tile(int(blockIdx.x) % tiles_), step(int(gridDim.x) % tiles_), tiles(tiles_) {}
+  __device__ __forceinline__ void next() {
+    tile += step;
+    if (tile >= tiles) tile -= tiles;
+  }
+};
+
 struct PairBars {
   uint32_t full, empty, acc_full, acc_empty, drain;  // first barrier of each array
 };
 
 struct PairShared {
-  u64 full[8], empty[8], acc_full[4], acc_empty[4], drain[4];
-  PairStep steps[8][kMaxSteps];
-  uint32_t header[8];
+  RowStages stages[8];  // by height / 8 - 1
+  u64 full[kMaxSlots], empty[kMaxSlots], acc_full[kMaxAccs], acc_empty[kMaxAccs], drain[kPipes];
+  PairStep steps[kMaxSlots][kMaxSteps];
+  uint32_t header[kMaxSlots];
   uint32_t tmem;
   volatile int abort_flag;
 };
@@ -299,18 +439,21 @@ struct PairShared {
 // Pipeline q takes the CTA's accumulation chunks c with c % kPipes == q. A producer fetches its next
 // stage's list before it issues the one in hand.
 
-// A pipeline's slots: stage i of the pipeline is in slot i % ring.
-template <int MODE>
+// A pipeline's slots: its stage i is in slot i % ring.
 struct Pipe {
-  static constexpr uint32_t RING = PairShape<MODE>::ring;
-  uint32_t first;  // first slot
+  int q, log;
   uint32_t i = 0;
-  __device__ __forceinline__ uint32_t slot() const { return first + i % RING; }
-  __device__ __forceinline__ uint32_t parity() const { return (i / RING) & 1u; }
+  __device__ __forceinline__ Pipe(const PairParams& p, int q_) : q(q_), log(p.ring_log) {}
+  __device__ __forceinline__ uint32_t slot() const {
+    return (uint32_t(q) << log) + (i & ((1u << log) - 1u));
+  }
+  __device__ __forceinline__ uint32_t parity() const { return (i >> log) & 1u; }
+  __device__ __forceinline__ uint32_t base(uint32_t slots) const {
+    return slots + slot() * (kPipeBytes >> log);
+  }
 };
-template <int MODE>
 __device__ __forceinline__ bool wait_slot(const PairParams& p, PairShared& sh, const PairBars& bars,
-                                          const Pipe<MODE>& pipe) {
+                                          const Pipe& pipe) {
   return wait_warp(bars.empty + 8 * pipe.slot(), pipe.parity() ^ 1u, p.status, &sh.abort_flag);
 }
 // Announces the slot's list and bytes; the lanes' list entries are written before.
@@ -322,10 +465,9 @@ __device__ __forceinline__ void announce(PairShared& sh, uint32_t slot, uint32_t
   __syncwarp();
 }
 // The end marker, a stage without steps.
-template <int MODE>
 __device__ __forceinline__ void produce_end(const PairParams& p, PairShared& sh, const PairBars& bars,
-                                            const Pipe<MODE>& pipe, int lane) {
-  if (!wait_slot<MODE>(p, sh, bars, pipe)) return;
+                                            const Pipe& pipe, int lane) {
+  if (!wait_slot(p, sh, bars, pipe)) return;
   if (lane == 0) {
     sh.header[pipe.slot()] = 0u;
     mbar_arrive(bars.full + 8 * pipe.slot());
@@ -336,7 +478,6 @@ template <int MODE>
 __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots, uint32_t zero,
                              const PairBars& bars, int warp, int lane) {
   constexpr bool I8 = MODE == kInt8;
-  constexpr uint32_t BYTES = PairShape<MODE>::slot_bytes;
   const uint32_t xb = (I8 ? 16u : 32u) * uint32_t(p.R);  // panel bytes of a group
   const uint64_t pol_x = policy_evict_last(), pol_w = policy_evict_first();
   const long long per_tile = I8 ? p.x_chunks : p.K >> 3;
@@ -346,12 +487,12 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
     int n, tile;
     const char* w;
   };
-  Pipe<MODE> pipe{uint32_t(warp) * PairShape<MODE>::ring};
+  Pipe pipe(p, warp);
   auto issue = [&](const Stage& st) {
-    if (!wait_slot<MODE>(p, sh, bars, pipe)) return false;
+    if (!wait_slot(p, sh, bars, pipe)) return false;
     const int h = int(st.shape & 255u), hp = int((st.shape >> 8) & 255u), r0 = int(st.shape >> 16);
     const uint32_t wb = (I8 ? 16u : 32u) * uint32_t(hp), n = uint32_t(st.n);
-    const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    const uint32_t slot = pipe.slot(), base = pipe.base(slots), full = bars.full + 8 * slot;
     const uint32_t xbase = base + n * wb, steps = (n + 1) / 2;  // weights first: 128-byte aligned
     if (lane < int(steps)) {
       const bool pair = 2u * lane + 1 < n;
@@ -393,20 +534,21 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
   bool have = false;
   uint32_t c0 = 0;  // chunks before this item
   int k = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
+  TileWalk walk(p.tiles);
+  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k, walk.next()) {
     const RowUnit u = win.get(k, lane);
-    const RowStages<MODE> rs(p.R, int((u.shape >> 8) & 255u));
+    const RowStages rs = sh.stages[((u.shape >> 11) & 31u) - 1u];
     const int n0 = rs.chunks(int(u.ng[0])), total = n0 + rs.chunks(int(u.ng[1]));
     for (int ch = int((uint32_t(warp) - c0) % kPipes); ch < total; ch += kPipes) {
       const bool up = ch >= n0;
       const int groups = int(up ? u.ng[1] : u.ng[0]), ns = rs.stages(groups);
-      const int j0 = (up ? ch - n0 : ch) * rs.per_chunk, j1 = min(ns, j0 + rs.per_chunk);
+      const int j0 = (up ? ch - n0 : ch) * rs.per_chunk, j1 = I8 ? ns : min(ns, j0 + rs.per_chunk);
       for (int j = j0; j < j1; ++j) {
         const int off = j * rs.cap;
         Stage st;
         st.shape = u.shape;
         st.n = min(rs.cap, groups - off);
-        st.tile = p.tile0 + item % p.tiles;
+        st.tile = p.tile0 + walk.tile;
         st.flags = (j == j0 ? kHdrFirst : 0u) | (j + 1 == j1 ? kHdrLast : 0u);
         st.col = lane < st.n ? __ldg(p.group_col + (up ? u.g0[1] : u.g0[0]) + off + lane) : 0u;
         st.w = p.w + (up ? u.w0[1] : u.w0[0]) + (long long)off * (I8 ? 16 : 32) * int(u.shape & 255u);
@@ -418,12 +560,11 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
     c0 += uint32_t(total);
   }
   if (have && !issue(held)) return;
-  produce_end<MODE>(p, sh, bars, pipe, lane);
+  produce_end(p, sh, bars, pipe, lane);
 }
 
 __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh, uint32_t slots,
                                              uint32_t zero, const PairBars& bars, int warp, int lane) {
-  constexpr uint32_t BYTES = PairShape<kInputGrad>::slot_bytes;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
   const int items = p.units * p.tiles;
@@ -433,7 +574,7 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
     int tile;
     ColEntry e;
   };
-  Pipe<kInputGrad> pipe{uint32_t(warp) * PairShape<kInputGrad>::ring};
+  Pipe pipe(p, warp);
   auto issue = [&](const Stage& st) {
     const ColEntry& e = st.e;
     // places of the entries: groups before this one, and its steps
@@ -449,8 +590,8 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
     const uint32_t groups = __shfl_sync(0xffffffffu, g, kColEntries - 1);
     const uint32_t all_steps = __shfl_sync(0xffffffffu, steps, kColEntries - 1);
     const uint32_t g_before = g - e.h8, s_before = steps - (e.h8 + 1) / 2;
-    if (!wait_slot<kInputGrad>(p, sh, bars, pipe)) return false;
-    const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
+    if (!wait_slot(p, sh, bars, pipe)) return false;
+    const uint32_t slot = pipe.slot(), base = pipe.base(slots), full = bars.full + 8 * slot;
     const uint32_t a0 = base + g_before * xb, b0 = base + groups * xb + g_before * 32u * st.w;
     const uint32_t h = 8u * e.h8;
     if (lane < kColEntries)
@@ -477,13 +618,14 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
   bool have = false;
   uint32_t c0 = 0;
   int k = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
+  TileWalk walk(p.tiles);
+  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k, walk.next()) {
     const ColUnit u = win.get(k, lane);
     for (uint32_t j = (uint32_t(warp) - c0) % kPipes; j < u.ns; j += kPipes) {
       Stage st;
       st.w = u.w;
       st.c0 = u.c0;
-      st.tile = p.tile0 + item % p.tiles;
+      st.tile = p.tile0 + walk.tile;
       st.e = ColEntry{};
       if (lane < kColEntries) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.entries) +
@@ -499,21 +641,20 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
     c0 += u.ns;
   }
   if (have && !issue(held)) return;
-  produce_end<kInputGrad>(p, sh, bars, pipe, lane);
+  produce_end(p, sh, bars, pipe, lane);
 }
 
 // Token stages of a weight-gradient unit: kGradTokens tokens of a tile (the last of a tile fewer) of
 // the unit's 16 activation groups and h / 8 gradient groups, each group [kGradTokens of hi][of lo'].
 __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& sh, uint32_t slots,
                                               const PairBars& bars, int warp, int lane) {
-  constexpr uint32_t BYTES = PairShape<kWeightGrad>::slot_bytes;
   constexpr uint32_t GB = 32u * kGradTokens;
   const uint32_t xb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
   const int per_tile = (p.R + kGradTokens - 1) / kGradTokens, total = p.tiles * per_tile;
   UnitWin<GradUnit> win;
   win.init(p.grads, p.units, 1, lane);
-  Pipe<kWeightGrad> pipe{uint32_t(warp) * PairShape<kWeightGrad>::ring};
+  Pipe pipe(p, warp);
   uint32_t c0 = 0, next_col = 0;
   int k = 0;
   auto load_col = [&](const GradUnit& u) {
@@ -537,8 +678,8 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
     const long long tile_step = (is_x ? p.K >> 3 : 2 * (p.M >> 3)) * xb;
     for (int j = int((uint32_t(warp) - c0) % kPipes); j < total; j += kPipes, ++pipe.i) {
       const int tile = j / per_tile, t0 = (j % per_tile) * kGradTokens, nt = min(kGradTokens, p.R - t0);
-      if (!wait_slot<kWeightGrad>(p, sh, bars, pipe)) return;
-      const uint32_t slot = pipe.slot(), base = slots + slot * BYTES, full = bars.full + 8 * slot;
+      if (!wait_slot(p, sh, bars, pipe)) return;
+      const uint32_t slot = pipe.slot(), base = pipe.base(slots), full = bars.full + 8 * slot;
       const uint32_t steps = uint32_t(nt) / 16;
       if (lane < int(steps)) {
         PairStep& out = sh.steps[slot][lane];
@@ -556,8 +697,14 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
     }
     c0 += uint32_t(total);
   }
-  produce_end<kWeightGrad>(p, sh, bars, pipe, lane);
+  produce_end(p, sh, bars, pipe, lane);
 }
+
+// Accumulator of a pipeline's chunk, and the TMEM columns of one.
+__device__ __forceinline__ uint32_t acc_of(const PairParams& p, uint32_t q, uint32_t chunk) {
+  return q + kPipes * (chunk & ((1u << p.acc_log) - 1u));
+}
+__device__ __forceinline__ uint32_t acc_cols(const PairParams& p) { return 128u >> p.acc_log; }
 
 // ---- MMA threads ---------------------------------------------------------------------------------
 
@@ -570,9 +717,8 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
                         (MODE == kWeightGrad || MODE == kInputGrad ? 1u << 16 : 0u) |
                         (uint32_t(m >> 4) << 24);
   const u64 lo = MODE == kWeightGrad ? kGradTokens : u64(p.R);  // hi to lo' tile of A, in 16 bytes
-  const uint32_t d = sh.tmem + kAccCols * uint32_t(q);
-  Pipe<MODE> pipe{uint32_t(q) * PairShape<MODE>::ring};
-  uint32_t free_parity = 1;  // of the accumulator
+  Pipe pipe(p, q);
+  uint32_t chunk = 0;  // of this pipeline: accumulator q + kPipes (chunk % accumulators)
   for (;; ++pipe.i) {
     const uint32_t slot = pipe.slot();
     if (!wait_one(bars.full + 8 * slot, pipe.parity(), p.status, &sh.abort_flag)) return;
@@ -580,10 +726,10 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     const int steps = int(hdr & 63u), n = int((hdr >> 8) & 15u) * 8;
     if (steps == 0) break;
     PairStep next = sh.steps[slot][0];
-    if (hdr & kHdrFirst) {
-      if (!wait_one(bars.acc_empty + 8 * q, free_parity, p.status, &sh.abort_flag)) return;
-      free_parity ^= 1u;
-    }
+    const uint32_t acc_no = acc_of(p, q, chunk), d = sh.tmem + acc_no * acc_cols(p);
+    if (hdr & kHdrFirst)
+      if (!wait_one(bars.acc_empty + 8 * acc_no, ((chunk >> p.acc_log) & 1u) ^ 1u, p.status, &sh.abort_flag))
+        return;
     tc_fence_after();
     // N of one tile of n columns: a multiple of 16 for M = 128 (one tile more is read, and its
     // columns are not used)
@@ -610,7 +756,10 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
       }
     }
     tc_commit(bars.empty + 8 * slot);
-    if (hdr & kHdrLast) tc_commit(bars.acc_full + 8 * q);
+    if (hdr & kHdrLast) {
+      tc_commit(bars.acc_full + 8 * acc_no);
+      ++chunk;
+    }
   }
   tc_commit(bars.drain + 8 * q);  // nothing may arrive on a barrier of a CTA that has gone
   wait_one(bars.drain + 8 * q, 0, p.status, &sh.abort_flag);
@@ -627,12 +776,89 @@ __device__ __forceinline__ void store8(float* dst, const float (&v)[8], int vec)
     for (int i = 0; i < 8; ++i) dst[i] = v[i];
   }
 }
+__device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vec) {
+  if (vec) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = v[i];
+  }
+}
+__device__ __forceinline__ void epilogue_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+}
 constexpr float kLoUnit = 1.0f / 2048.0f;  // 2^-11
+
+// Adds NJ tiles of an accumulation chunk: hi sums at column `hi`, lo sums at `lo` (kInt8: the integers at
+// `hi`, carried as they are).
+template <int MODE, int NJ>
+__device__ __forceinline__ void add_chunk(float (&acc)[4][8], uint32_t hi, uint32_t lo) {
+  if constexpr (MODE == kInt8) {
+    tc_ld1<NJ>(hi, acc);
+  } else {
+    float v[4][8], w[4][8];
+    tc_ld2<NJ>(hi, lo, v, w);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[j][i] += fmaf(w[j][i], kLoUnit, v[j][i]);
+  }
+}
+
+// Output of a row unit's tile from the staged sums: a thread takes four neighbouring elements of a row, so
+// that few tokens' activations are shared out too and whole lines are stored.
+template <int MODE>
+__device__ __forceinline__ void write_staged(const PairParams& p, const float* st, const float* st_up, int ld,
+                                             int log4, int n, uint32_t row0, long long t0, int thread,
+                                             float f1, float f2, const float (&rs)[4], float ts) {
+  const int sc = 4 * (thread & ((1 << log4) - 1));
+  if (sc >= n) return;
+  for (int r = thread >> log4; r < p.R; r += 256 >> log4) {
+    const long long t = t0 + r;
+    if (t >= p.tokens) break;
+    const long long o = t * p.M + row0 + sc;
+    float v[4], hv[4];
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(st + r * ld + sc);
+    if constexpr (MODE == kForward) {
+      float w[4];
+      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(st_up + r * ld + sc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = v[i] * f1 * f2;
+        w[i] = w[i] * f1 * f2;
+      }
+      with_act(p.act, [&](auto kind) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float a, da;
+          act_both<decltype(kind)::value>(v[i], a, da);
+          hv[i] = a * w[i];
+        }
+      });
+      if (p.out1 != nullptr) {
+        store4(p.out1 + o, v, p.vec);
+        store4(p.out2 + o, w, p.vec);
+      }
+    } else {
+      const float s = r < (256 >> log4) ? ts : __ldg(p.token_scale + t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hv[i] = float(__float_as_int(v[i])) * (s * rs[i]);
+    }
+    store4(p.out0 + o, hv, p.vec);
+  }
+}
+
+// The part of a unit that the epilogue reads, 16 bytes.
+template <int MODE>
+__device__ __forceinline__ uint4 unit_head(const PairParams& p, int unit) {
+  if constexpr (by_rows(MODE)) return __ldg(reinterpret_cast<const uint4*>(p.rows + unit));
+  else return __ldg(reinterpret_cast<const uint4*>(p.cols + unit));
+}
 
 // Epilogue warp e of a quadrant takes the 8-column tiles c with c % 2 == e.
 template <int MODE>
-__device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, int quad, int e,
-                         int lane) {
+__device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, float* stage, int quad,
+                         int e, int lane) {
   const bool wide = MODE == kWeightGrad || p.R > 64;  // M = 128; M = 64 fills lanes 0..15
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
   const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
@@ -641,101 +867,112 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
   if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
   if (MODE == kWeightGrad) unscale(p.exps[0] + p.exps[1], f1, f2);
-  using Unit = typename std::conditional<PairShape<MODE>::rows, RowUnit,
-                  typename std::conditional<MODE == kInputGrad, ColUnit, GradUnit>::type>::type;
-  UnitWin<Unit> win;
-  if constexpr (PairShape<MODE>::rows) win.init(p.rows, items, tiles, lane);
-  else if constexpr (MODE == kInputGrad) win.init(p.cols, items, tiles, lane);
-  else win.init(p.grads, items, tiles, lane);
+  const int thread = 128 * e + 32 * quad + lane, slog = stage_log(p.R), ld = (1 << slog) + 4;
   uint32_t use = 0;
+  bool ok = true;
+  TileWalk walk(tiles);
+  // the next item's unit is fetched while this one's sums are waited for
+  const int units_step = int(gridDim.x) / tiles;
+  int unit = int(blockIdx.x) / tiles;
+  uint4 next = make_uint4(0, 0, 0, 0), next2 = next;
+  auto fetch = [&](int un) {
+    if constexpr (MODE == kWeightGrad) {
+      next = __ldg(reinterpret_cast<const uint4*>(p.grads + un));
+      next2 = __ldg(reinterpret_cast<const uint4*>(p.grads + un) + 1);
+    } else {
+      next = unit_head<MODE>(p, un);
+    }
+  };
+  if (int(blockIdx.x) < items) fetch(unit);
   int k = 0;
   for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
-    const Unit u = win.get(k, lane);
-    const long long t = MODE == kWeightGrad ? 0 : (long long)(p.tile0 + item % tiles) * p.R + row;
+    const uint4 u = next, u2 = next2;
+    const int tile = walk.tile;
+    unit += units_step + (tile + walk.step >= tiles ? 1 : 0);
+    walk.next();
+    if (item + int(gridDim.x) < items) fetch(unit);
+    const long long t0 = (long long)(p.tile0 + tile) * p.R;
     int n, chunks[2] = {0, 0};
-    bool live;
-    if constexpr (PairShape<MODE>::rows) {
-      n = int((u.shape >> 8) & 255u);
-      const RowStages<MODE> rs(p.R, n);
-      chunks[0] = rs.chunks(int(u.ng[0]));
-      chunks[1] = rs.chunks(int(u.ng[1]));
-      live = in_tile && t < p.tokens;
+    if constexpr (by_rows(MODE)) {
+      n = int((u.y >> 8) & 255u);
+      const RowStages rs = sh.stages[n / 8 - 1];
+      chunks[0] = rs.chunks(int(u.z));
+      chunks[1] = rs.chunks(int(u.w));
     } else if constexpr (MODE == kInputGrad) {
-      n = int(u.w);
-      chunks[0] = int(u.ns);
-      live = in_tile && t < p.tokens;
+      n = int(u.y);
+      chunks[0] = int(u.w);
     } else {
-      n = int(u.h);
+      n = int(u.w);
       chunks[0] = p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
-      live = row < int(u.ng) * 8;
     }
+    // scales of the elements that this thread writes, fetched before the sums are waited for
+    float ts = 0.0f, rs[4] = {};
+    const int log4 = slog - 2;
+    if constexpr (MODE == kInt8) {
+      const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;
+      if (sr < p.R && t0 + sr < p.tokens) ts = __ldg(p.token_scale + t0 + sr);
+      if (sc < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + sc + i);
+      }
+    }
+    const int nj = (n / 8 + 1 - e) / 2;  // this warp's tiles
     float acc[MODE == kForward ? 2 : 1][4][8] = {};
 #pragma unroll
     for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
       for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
-        const uint32_t buf = use % kPipes;
-        if (!wait_warp(bars.acc_full + 8 * buf, (use / kPipes) & 1u, p.status, &sh.abort_flag)) return;
+        const uint32_t chunk = use / kPipes, buf = acc_of(p, use % kPipes, chunk);
+        // after an abort nothing is waited for, but the warps stay together (epilogue_sync)
+        if (ok) ok = wait_warp(bars.acc_full + 8 * buf, (chunk >> p.acc_log) & 1u, p.status, &sh.abort_flag);
         tc_fence_after();
-        const uint32_t d = sh.tmem + kAccCols * buf + (uint32_t(32 * quad) << 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = 16 * j + 8 * e;
-          if (c >= n) break;
-          float* a = acc[which][j];
-          float v[8], l1[8];
-          if (MODE == kInt8) {
-            tc_ld8_1(d + c, v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = v[i];  // 32-bit integers, carried as they are
-          } else {
-            tc_ld8_2(d + c, d + (MODE == kForward ? n : 64) + c, v, l1);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] += fmaf(l1[i], kLoUnit, v[i]);
-          }
+        const uint32_t d = sh.tmem + acc_cols(p) * buf + (uint32_t(32 * quad) << 16) + 8u * e;
+        const uint32_t lo = d + (MODE == kForward ? n : 64);
+        switch (nj) {
+          case 1: add_chunk<MODE, 1>(acc[which], d, lo); break;
+          case 2: add_chunk<MODE, 2>(acc[which], d, lo); break;
+          case 3: add_chunk<MODE, 3>(acc[which], d, lo); break;
+          case 4: add_chunk<MODE, 4>(acc[which], d, lo); break;
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.acc_empty + 8 * buf);
       }
     }
-    if (!live) continue;
-    const float ts = MODE == kInt8 ? p.token_scale[t] : 0.0f;
+    if constexpr (by_rows(MODE)) {
+      const bool two = p.R <= 16;  // two buffers: the next item's barrier parts readers and writers
+      float* st = stage + (two ? (k & 1) * (2 * p.R * ld) : 0);
+      float* st_up = st + p.R * ld;
+      for (int c0 = 0; c0 < n; c0 += 1 << slog) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = 16 * j + 8 * e;
-      if (c >= n) break;
-      float(&v)[8] = acc[0][j];
-      if constexpr (MODE == kForward) {
-        float(&w)[8] = acc[1][j];
-        float hv[8];
-        with_act(p.act, [&](auto kind) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = v[i] * f1 * f2;
-            w[i] = w[i] * f1 * f2;
-            float a, da;
-            act_both<decltype(kind)::value>(v[i], a, da);
-            hv[i] = a * w[i];
-          }
-        });
-        const long long o = t * p.M + u.row0 + c;
-        store8(p.out0 + o, hv, p.vec);
-        if (p.out1 != nullptr) {
-          store8(p.out1 + o, v, p.vec);
-          store8(p.out2 + o, w, p.vec);
+        for (int j = 0; j < 4; ++j) {
+          const int c = 16 * j + 8 * e - c0;
+          if (!in_tile || c < 0 || c >= (1 << slog) || j >= nj) continue;
+          store8(st + row * ld + c, acc[0][j], 1);
+          if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j], 1);
         }
-      } else if constexpr (MODE == kInt8) {
+        epilogue_sync();
+        if (MODE == kInt8 && c0 > 0) {
+          const int sc = c0 + 4 * (thread & ((1 << log4) - 1));
+          if (sc < n) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = float(__float_as_int(v[i])) * (ts * p.row_scale[u.row0 + c + i]);
-        store8(p.out0 + t * p.M + u.row0 + c, v, p.vec);
-      } else {
+            for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + sc + i);
+          }
+        }
+        write_staged<MODE>(p, st, st_up, ld, log4, n - c0, u.x + c0, t0, thread, f1, f2, rs, ts);
+        if (!two) epilogue_sync();
+      }
+    } else {
+      const bool live = MODE == kWeightGrad ? row < int(u.y) * 8 : in_tile && t0 + row < p.tokens;
+      if (!live) continue;
+      float* dst = MODE == kInputGrad
+                       ? p.out0 + (t0 + row) * p.K + u.x
+                       : ((u2.z & 1u) ? p.out1 : p.out0) + (u64(u2.x) | u64(u2.y) << 32) + (long long)row * n;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * f1 * f2;
-        if constexpr (MODE == kInputGrad)
-          store8(p.out0 + t * p.K + u.col0 + c, v, p.vec);
-        else
-          store8((u.which ? p.out1 : p.out0) + u.out + (long long)row * n + c, v, p.vec);
+      for (int j = 0; j < 4; ++j) {
+        if (j >= nj) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[0][j][i] = acc[0][j][i] * f1 * f2;
+        store8(dst + 16 * j + 8 * e, acc[0][j], p.vec);
       }
     }
   }
@@ -745,29 +982,29 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
 
 template <int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
-  constexpr int SLOTS = kPipes * PairShape<MODE>::ring, BYTES = PairShape<MODE>::slot_bytes;
   extern __shared__ char dyn[];
   __shared__ PairShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t slots = (smem_addr(dyn) + 1023u) & ~1023u, zero = slots + SLOTS * BYTES;
+  const uint32_t slots = (smem_addr(dyn) + 1023u) & ~1023u, zero = slots + kPipes * kPipeBytes;
   char* zero_ptr = dyn + (zero - smem_addr(dyn));
   const PairBars bars{smem_addr(sh.full), smem_addr(sh.empty), smem_addr(sh.acc_full),
                       smem_addr(sh.acc_empty), smem_addr(sh.drain)};
   if (threadIdx.x == 0) {
-    for (int s = 0; s < SLOTS; ++s) {
+    for (int s = 0; s < kMaxSlots; ++s) {
       mbar_init(bars.full + 8 * s, 1);
       mbar_init(bars.empty + 8 * s, 1);
     }
-    for (int b = 0; b < kPipes; ++b) {
+    for (int b = 0; b < kMaxAccs; ++b) {
       mbar_init(bars.acc_full + 8 * b, 1);
       mbar_init(bars.acc_empty + 8 * b, kEpilogueWarps);
-      mbar_init(bars.drain + 8 * b, 1);
     }
+    for (int b = 0; b < kPipes; ++b) mbar_init(bars.drain + 8 * b, 1);
     sh.abort_flag = 0;
     mbar_fence_init();
   }
   for (int i = threadIdx.x; i < kZeroBytes / 16; i += kPairThreads)
     reinterpret_cast<uint4*>(zero_ptr)[i] = make_uint4(0, 0, 0, 0);
+  if (by_rows(MODE) && warp == 1 && lane < 8) sh.stages[lane].template init<MODE>(p, 8 * (lane + 1));
   fence_proxy_async_smem();
   if (warp == kPipes) {
     tc_alloc(smem_addr(&sh.tmem), 512);
@@ -778,7 +1015,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   tc_fence_after();
 
   if (warp < kPipes) {
-    if constexpr (PairShape<MODE>::rows)
+    if constexpr (by_rows(MODE))
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)
       produce_cols(p, sh, slots, zero, bars, warp, lane);
@@ -788,7 +1025,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
     if (lane == 0) issue_mmas<MODE>(p, sh, bars, warp - kPipes);
     __syncwarp();
   } else if (warp >= kEpilogueWarp) {
-    epilogue<MODE>(p, sh, bars, (warp - kEpilogueWarp) & 3, (warp - kEpilogueWarp) >> 2, lane);
+    float* stage = reinterpret_cast<float*>(zero_ptr + kZeroBytes + kTailBytes);
+    epilogue<MODE>(p, sh, bars, stage, (warp - kEpilogueWarp) & 3, (warp - kEpilogueWarp) >> 2, lane);
   }
   tc_fence_before();
   __syncthreads();

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <vector>
 
 #include "vbsr_lm.cuh"
@@ -22,6 +23,19 @@ inline int parts_for(const int (&units)[4], int64_t tiles, int num_sm) {
   return f;
 }
 
+// Row units for a call, and how a pipeline's memory is cut.
+inline void choose_rows(PairParams& k, RowUnit* const (&rows)[4], const int (&units)[4], int64_t tiles,
+                        int num_sm) {
+  static const int kMinF = getenv("VF") ? atoi(getenv("VF")) : 0, kR = getenv("VR") ? atoi(getenv("VR")) : 32, kRing = getenv("VRING") ? atoi(getenv("VRING")) : 1;
+  int f = parts_for(units, tiles, num_sm);
+  const bool small = k.R <= kR;
+  if (small) f = std::max(f, kMinF);
+  k.rows = rows[f];
+  k.units = units[f];
+  k.ring_log = small ? kRing : 1;
+  k.acc_log = f >= 1 ? 1 : 0;
+}
+
 template <int MODE>
 vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s) {
   if (k.units == 0) return VBSR_OK;
@@ -30,7 +44,7 @@ vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s)
     k.tile0 = int(t0);
     k.tiles = int(std::min(most, tiles - t0));
     const int64_t items = MODE == kWeightGrad ? k.units : int64_t(k.units) * k.tiles;
-    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, pair_smem<MODE>(), s>>>(k);
+    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, kPairSmem, s>>>(k);
     VBSR_CUDA(cudaGetLastError());
   }
   return VBSR_OK;
