@@ -135,6 +135,43 @@ def test_gated_structures(cuda, name, kind):
     check_backward(cuda, plan, gate, up, kind, X)
 
 
+@pytest.mark.parametrize("tokens", [1, 40, 130])
+def test_many_work_items_per_sm(cuda, tokens):
+    """Matrices with far more block rows and columns than the GPU has SMs, short rows and empty ones."""
+    torch = cuda
+    rng = np.random.default_rng(6)
+    rows, cols = 2500, 60
+    rs = rng.choice((8, 16, 24, 64), rows, p=(0.5, 0.3, 0.1, 0.1))
+    cs = rng.choice((8, 16, 40), cols)
+    empty = tuple(np.flatnonzero(rng.random(rows) < 0.2))
+    gate = ref.matrix(rows, cols, 5, 61, row_size=rs, col_size=cs, empty=empty)
+    up = ref.matrix(rows, cols, 30, 62, row_size=rs, col_size=cs, empty=empty[::2])
+    X = activations(tokens, gate.scalar_cols(), tokens)
+    plan = vb.GatedPlan(vb.Matrix(gate), vb.Matrix(up))
+    want = Gated(gate, up, vb.Activation.SiLU, X)
+    for _ in range(3):
+        _, (H, G, U) = run_forward(torch, plan, X, gate.scalar_rows())
+        close(G, want.G, want.tol[0], "G")
+        close(U, want.U, want.tol[1], "U")
+        close(H, want.H, want.H_tol, "H")
+    check_backward(torch, plan, gate, up, vb.Activation.SiLU, X)
+    tall = ref.matrix(cols, rows, 300, 63, row_size=cs, col_size=rs)  # many block columns
+    wide = ref.matrix(cols, rows, 200, 64, row_size=cs, col_size=rs)
+    X2 = activations(tokens, tall.scalar_cols(), 3)
+    check_backward(torch, vb.GatedPlan(vb.Matrix(tall), vb.Matrix(wide)), tall, wide,
+                   vb.Activation.SiLU, X2)
+    q, sc = int8_weights(up, 7)
+    C = torch.empty(tokens, up.scalar_rows(), device="cuda")
+    i8 = vb.Int8Plan(vb.Matrix(up), torch.from_numpy(q).cuda(), torch.from_numpy(sc).cuda())
+    Q, ts = quantized(X)
+    want8 = (Q @ ref.dense(up, q).T) * ts[:, None].astype(np.float64) * sc
+    for _ in range(3):
+        C.fill_(float("nan"))
+        i8.execute_panel(torch.from_numpy(X).cuda(), C)
+        i8.check_status()
+        close(C, want8, 4 * ref.U * np.abs(want8), "C")
+
+
 @pytest.mark.parametrize("size", SIZES)
 def test_gated_every_block_height_and_width(cuda, size):
     for rows, cols in (((size,), SIZES), (SIZES, (size,))):

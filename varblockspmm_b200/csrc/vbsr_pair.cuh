@@ -37,8 +37,8 @@
 // off that list. Four, because both halves are latency: fetching a stage's list of places takes as
 // long as several stages take to stream, and a single MMA thread, which reads two descriptors
 // from shared memory per step, was measured at 400 clocks a step where the operands need about 140.
-// Eight epilogue warps, two per TMEM quadrant, take every second tile of 8 columns each. Tokens are
-// on the M side (64 or 128 rows): with weights there, blocks of 8 to 56 rows would leave most of an
+// Two epilogue groups of four warps, one warp per TMEM quadrant, take every second work item each. Tokens
+// are on the M side (64 or 128 rows): with weights there, blocks of 8 to 56 rows would leave most of an
 // MMA empty. What bounds it: the copies into shared memory. A weight group of 32 h bytes needs 32 R
 // bytes of activations, from L2, so few tokens run at the weights' HBM rate and many at the
 // L2-to-shared-memory rate, h / 2 operations per byte.
@@ -120,7 +120,8 @@ constexpr u64 kStepMask = (1ull << 56) - 1;
 constexpr int kMaxSteps = 16;
 
 // Slot header: steps | N/8 << 8 | flags. No steps: end of the work.
-constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17;
+constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17, kHdrOdd = 1u << 18;
+constexpr uint32_t kHdrGroup = 1u << 19;  // the item's epilogue group
 
 __host__ __device__ constexpr bool by_rows(int mode) { return mode == kForward || mode == kInt8; }
 constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA threads in warps 4 .. 7
@@ -128,17 +129,24 @@ constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA threads in warps 4 .. 7
 // 2^acc_log accumulators of 128 or 64 columns (hi sums, then lo sums).
 constexpr uint32_t kPipeBytes = 48 * 1024;
 constexpr int kMaxSlots = 16, kMaxAccs = 8;
-constexpr int kEpilogueWarp = 8, kEpilogueWarps = 8;
-constexpr int kPairThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
+constexpr int kEpilogueWarp = 8, kEpilogueGroups = 2;
+constexpr int kPairThreads = 32 * (kEpilogueWarp + 4 * kEpilogueGroups);
+// The 128 registers per thread that the kernel is launched with, shared out again over its four
+// warpgroups: producers, MMA threads, and two of the epilogue.
+constexpr int kProducerRegs = 88, kMmaRegs = 40, kEpilogueRegs = 192;
+static_assert(kPairThreads == 512 && kProducerRegs + kMmaRegs + 2 * kEpilogueRegs <= 4 * 128, "registers");
 constexpr int kChunkSteps = 8;
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage
-// kForward, kInt8: results pass through shared memory, two matrices of R rows and 2^stage_log(R)
-// columns with 4 of padding; two such buffers for up to 16 tokens.
-constexpr int kStageBytes = 2 * 128 * 20 * 4;
-__host__ __device__ constexpr int stage_log(int R) { return R <= 32 ? 6 : (R <= 64 ? 5 : 4); }
-constexpr int kPairSmem = kPipes * kPipeBytes + kZeroBytes + kTailBytes + kStageBytes + 1024;
+// kForward, kInt8: results pass through shared memory, R rows and 2^stage_log columns (rows padded by 16
+// bytes, except rows of 32) of two matrices or one; a buffer for each of the two epilogue groups.
+constexpr int kStageBytes = 10 * 1024 + 256;
+__host__ __device__ constexpr int stage_log(int mode, int R) {
+  return (R <= 16 ? 6 : (R <= 32 ? 5 : (R <= 64 ? 4 : 3))) + (mode == kInt8 && R > 16 ? 1 : 0);
+}
+__host__ __device__ constexpr int stage_ld(int log) { return log == 3 ? 8 : (1 << log) + 4; }
+constexpr int kPairSmem = kPipes * kPipeBytes + kZeroBytes + kTailBytes + 2 * kStageBytes + 1024;
 
 __device__ __forceinline__ u64 core_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return u64((addr >> 4) & 0x3FFFu) | (u64((lbo >> 4) & 0x3FFFu) << 16) |
@@ -169,139 +177,32 @@ __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, ui
       : "memory");
 }
 
-// Tiles of 8 accumulator columns, loaded and waited for in one statement (the registers are not valid
-// before the wait): NJ tiles 16 columns apart from `a` on, and as many from `b` on (tc_ld1: from `a` only).
-template <int NJ>
-__device__ __forceinline__ void tc_ld2(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]);
-template <>
-__device__ __forceinline__ void tc_ld2<1>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
+// 16 accumulator columns from one or two places, loaded and waited for in one statement (the registers are
+// not valid before the wait).
+__device__ __forceinline__ void tc_ld16(uint32_t a, float (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, "
+      "%8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]),
-        "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7])
-      : "r"(a), "r"(b)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tc_ld2<2>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(w[0][0]), "=f"(w[0][1]),
-        "=f"(w[0][2]), "=f"(w[0][3]), "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7]),
-        "=f"(w[1][0]), "=f"(w[1][1]), "=f"(w[1][2]), "=f"(w[1][3]), "=f"(w[1][4]), "=f"(w[1][5]),
-        "=f"(w[1][6]), "=f"(w[1][7])
-      : "r"(a), "r"(a + 16), "r"(b), "r"(b + 16)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tc_ld2<3>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%48];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%49];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%50];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%51];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%32, %33, %34, %35, %36, %37, %38, %39}, [%52];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%40, %41, %42, %43, %44, %45, %46, %47}, [%53];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
-        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
-        "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]), "=f"(w[0][4]), "=f"(w[0][5]),
-        "=f"(w[0][6]), "=f"(w[0][7]), "=f"(w[1][0]), "=f"(w[1][1]), "=f"(w[1][2]), "=f"(w[1][3]),
-        "=f"(w[1][4]), "=f"(w[1][5]), "=f"(w[1][6]), "=f"(w[1][7]), "=f"(w[2][0]), "=f"(w[2][1]),
-        "=f"(w[2][2]), "=f"(w[2][3]), "=f"(w[2][4]), "=f"(w[2][5]), "=f"(w[2][6]), "=f"(w[2][7])
-      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(b), "r"(b + 16), "r"(b + 32)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tc_ld2<4>(uint32_t a, uint32_t b, float (&v)[4][8], float (&w)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%64];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%65];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%66];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%67];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%32, %33, %34, %35, %36, %37, %38, %39}, [%68];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%40, %41, %42, %43, %44, %45, %46, %47}, [%69];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%48, %49, %50, %51, %52, %53, %54, %55}, [%70];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%56, %57, %58, %59, %60, %61, %62, %63}, [%71];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
-        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
-        "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]), "=f"(v[3][4]), "=f"(v[3][5]),
-        "=f"(v[3][6]), "=f"(v[3][7]), "=f"(w[0][0]), "=f"(w[0][1]), "=f"(w[0][2]), "=f"(w[0][3]),
-        "=f"(w[0][4]), "=f"(w[0][5]), "=f"(w[0][6]), "=f"(w[0][7]), "=f"(w[1][0]), "=f"(w[1][1]),
-        "=f"(w[1][2]), "=f"(w[1][3]), "=f"(w[1][4]), "=f"(w[1][5]), "=f"(w[1][6]), "=f"(w[1][7]),
-        "=f"(w[2][0]), "=f"(w[2][1]), "=f"(w[2][2]), "=f"(w[2][3]), "=f"(w[2][4]), "=f"(w[2][5]),
-        "=f"(w[2][6]), "=f"(w[2][7]), "=f"(w[3][0]), "=f"(w[3][1]), "=f"(w[3][2]), "=f"(w[3][3]),
-        "=f"(w[3][4]), "=f"(w[3][5]), "=f"(w[3][6]), "=f"(w[3][7])
-      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(a + 48), "r"(b), "r"(b + 16), "r"(b + 32), "r"(b + 48)
-      : "memory");
-}
-template <int NJ>
-__device__ __forceinline__ void tc_ld1(uint32_t a, float (&v)[4][8]);
-template <>
-__device__ __forceinline__ void tc_ld1<1>(uint32_t a, float (&v)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+        "=f"(v[15])
       : "r"(a)
       : "memory");
 }
-template <>
-__device__ __forceinline__ void tc_ld1<2>(uint32_t a, float (&v)[4][8]) {
+__device__ __forceinline__ void tc_ld16(uint32_t a, uint32_t b, float (&v)[16], float (&w)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, "
+      "%8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, "
+      "%24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7])
-      : "r"(a), "r"(a + 16)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tc_ld1<3>(uint32_t a, float (&v)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
-        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7])
-      : "r"(a), "r"(a + 16), "r"(a + 32)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tc_ld1<4>(uint32_t a, float (&v)[4][8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%32];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%33];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%34];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24, %25, %26, %27, %28, %29, %30, %31}, [%35];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]),
-        "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]),
-        "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[2][0]), "=f"(v[2][1]),
-        "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[2][4]), "=f"(v[2][5]), "=f"(v[2][6]), "=f"(v[2][7]),
-        "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]), "=f"(v[3][4]), "=f"(v[3][5]),
-        "=f"(v[3][6]), "=f"(v[3][7])
-      : "r"(a), "r"(a + 16), "r"(a + 32), "r"(a + 48)
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+        "=f"(v[15]), "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3]), "=f"(w[4]), "=f"(w[5]), "=f"(w[6]),
+        "=f"(w[7]), "=f"(w[8]), "=f"(w[9]), "=f"(w[10]), "=f"(w[11]), "=f"(w[12]), "=f"(w[13]),
+        "=f"(w[14]), "=f"(w[15])
+      : "r"(a), "r"(b)
       : "memory");
 }
 
@@ -427,7 +328,7 @@ struct PairBars {
 
 struct PairShared {
   RowStages stages[8];  // by height / 8 - 1
-  u64 full[kMaxSlots], empty[kMaxSlots], acc_full[kMaxAccs], acc_empty[kMaxAccs], drain[kPipes];
+  u64 full[kMaxSlots], empty[kMaxSlots], acc_full[2 * kMaxAccs], acc_empty[kMaxAccs], drain[kPipes];
   PairStep steps[kMaxSlots][kMaxSteps];
   uint32_t header[kMaxSlots];
   uint32_t tmem;
@@ -494,15 +395,14 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
     const uint32_t wb = (I8 ? 16u : 32u) * uint32_t(hp), n = uint32_t(st.n);
     const uint32_t slot = pipe.slot(), base = pipe.base(slots), full = bars.full + 8 * slot;
     const uint32_t xbase = base + n * wb, steps = (n + 1) / 2;  // weights first: 128-byte aligned
-    if (lane < int(steps)) {
-      const bool pair = 2u * lane + 1 < n;
-      const uint32_t a = xbase + 2u * lane * xb, b = base + 2u * lane * wb;
-      sh.steps[slot][lane].a = core_desc(a, pair ? xb : zero - a, 128) |
-                               (lane == 0 && (st.flags & kHdrFirst) ? kStepFresh : 0) |
-                               (pair ? 0 : kStepOdd);
-      sh.steps[slot][lane].b = core_desc(b, pair ? wb : 0u, 128);
+    // the steps are evenly spaced: the list holds the first and, if the number of groups is odd, the last
+    if (lane == 0) {
+      sh.steps[slot][0] = {core_desc(xbase, xb, 128), core_desc(base, wb, 128)};
+      const uint32_t a = xbase + (n - 1) * xb;
+      if (n & 1u) sh.steps[slot][1] = {core_desc(a, zero - a, 128), core_desc(base + (n - 1) * wb, 0u, 128)};
     }
-    announce(sh, slot, full, steps | uint32_t(hp) << 5 | st.flags, n * (xb + wb), lane);
+    announce(sh, slot, full, steps | uint32_t(hp) << 5 | st.flags | (n & 1u ? kHdrOdd : 0u), n * (xb + wb),
+             lane);
     // weights: one run, or per group the part's rows of hi and of lo'
     if (hp == h) {
       if (lane == 0) {
@@ -549,7 +449,7 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
         st.shape = u.shape;
         st.n = min(rs.cap, groups - off);
         st.tile = p.tile0 + walk.tile;
-        st.flags = (j == j0 ? kHdrFirst : 0u) | (j + 1 == j1 ? kHdrLast : 0u);
+        st.flags = (j == j0 ? kHdrFirst : 0u) | (j + 1 == j1 ? kHdrLast : 0u) | (k & 1 ? kHdrGroup : 0u);
         st.col = lane < st.n ? __ldg(p.group_col + (up ? u.g0[1] : u.g0[0]) + off + lane) : 0u;
         st.w = p.w + (up ? u.w0[1] : u.w0[0]) + (long long)off * (I8 ? 16 : 32) * int(u.shape & 255u);
         if (have && !issue(held)) return;
@@ -570,7 +470,7 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
   const int items = p.units * p.tiles;
   const long long per_tile = 2 * (p.M >> 3);
   struct Stage {
-    uint32_t w, c0;
+    uint32_t w, c0, flags;
     int tile;
     ColEntry e;
   };
@@ -604,7 +504,7 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
         // columns 8 apart are 16 h apart (hi and lo' tiles alternate), rows 8 apart 128 bytes
         out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
       }
-    announce(sh, slot, full, all_steps | st.w << 5 | kHdrFirst | kHdrLast, groups * (xb + 32u * st.w), lane);
+    announce(sh, slot, full, all_steps | st.w << 5 | st.flags, groups * (xb + 32u * st.w), lane);
     if (e.h8) {
       bulk_g2s(a0, p.dy + (st.tile * per_tile + e.dy_group) * xb, e.h8 * xb, full, pol_x);
       bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(st.c0 >> 3) * 32 * h, 4u * h * st.w, full);
@@ -625,6 +525,7 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
       Stage st;
       st.w = u.w;
       st.c0 = u.c0;
+      st.flags = kHdrFirst | kHdrLast | (k & 1 ? kHdrGroup : 0u);
       st.tile = p.tile0 + walk.tile;
       st.e = ColEntry{};
       if (lane < kColEntries) {
@@ -665,7 +566,8 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
     nu = win.get(0, lane);
     next_col = load_col(nu);
   }
-  for (int item = blockIdx.x; item < p.units; item += gridDim.x) {
+  uint32_t group = 0;
+  for (int item = blockIdx.x; item < p.units; item += gridDim.x, group ^= kHdrGroup) {
     const GradUnit u = nu;
     const uint32_t col = next_col;
     if (item + int(gridDim.x) < p.units) {
@@ -687,7 +589,7 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
                 (lane == 0 ? kStepFresh : 0);
         out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
       }
-      announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast, (u.ng + h8) * 32u * uint32_t(nt), lane);
+      announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast | group, (u.ng + h8) * 32u * uint32_t(nt), lane);
       if (is_x || is_dy) {
         const char* src = src0 + tile * tile_step + 16 * t0;
         const uint32_t dst = base + lane * GB;
@@ -716,6 +618,7 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
                         (MODE == kWeightGrad ? 1u << 15 : 0u) |
                         (MODE == kWeightGrad || MODE == kInputGrad ? 1u << 16 : 0u) |
                         (uint32_t(m >> 4) << 24);
+  const uint32_t xb16 = (MODE == kInt8 ? 1u : 2u) * uint32_t(p.R);  // panel group, in 16 bytes
   const u64 lo = MODE == kWeightGrad ? kGradTokens : u64(p.R);  // hi to lo' tile of A, in 16 bytes
   Pipe pipe(p, q);
   uint32_t chunk = 0;  // of this pipeline: accumulator q + kPipes (chunk % accumulators)
@@ -734,30 +637,44 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     // N of one tile of n columns: a multiple of 16 for M = 128 (one tile more is read, and its
     // columns are not used)
     const int n1 = m == 128 || MODE == kInt8 ? (n + 15) & ~15 : n;
-    const uint32_t i1 = form | (uint32_t(n1 >> 3) << 17), i2 = form | (uint32_t(2 * n >> 3) << 17);
+    const uint32_t i1 = form | (uint32_t(n1 >> 3) << 17);
+    [[maybe_unused]] const uint32_t i2 = form | (uint32_t(2 * n >> 3) << 17);
+    if constexpr (by_rows(MODE)) {
+      const u64 da = (2u * xb16), db = (MODE == kInt8 ? 2u : 4u) * uint32_t(n);  // two groups, in 16 bytes
+      const int even = steps - ((hdr & kHdrOdd) ? 1 : 0);
+      u64 a = next.a, b = next.b;
+      uint32_t acc = (hdr & kHdrFirst) ? 0u : 1u;
+      auto step = [&](u64 a1, u64 a2, u64 b1) {
+        if (MODE == kInt8) {
+          tc_mma_i8(d, a1, b1, i1, acc);
+        } else {  // hi x [hi; lo'], then lo' x hi into the columns of hi lo'
+          tc_mma_f16(d, a1, b1, i2, acc);
+          tc_mma_f16(d + n, a2, b1, i1, 1u);
+        }
+        acc = 1u;
+      };
+#pragma unroll 2
+      for (int s = 0; s < even; ++s, a += da, b += db) step(a, a + lo, b);
+      if (hdr & kHdrOdd) {
+        const PairStep st = sh.steps[slot][1];
+        step(st.a, st.a + lo - (lo << 16), st.b);
+      }
+    } else
     for (int s = 0; s < steps; ++s) {
       const PairStep st = next;
       if (s + 1 < steps) next = sh.steps[slot][s + 1];
       const u64 a = st.a & kStepMask, b = st.b;
       const uint32_t acc = (st.a & kStepFresh) ? 0u : 1u;
-      if (MODE == kInt8) {
-        tc_mma_i8(d, a, b, i1, acc);
-        continue;
-      }
       const u64 a2 = a + lo - ((st.a & kStepOdd) ? lo << 16 : 0ull);
-      if (MODE == kForward) {  // hi x [hi; lo'], then lo' x hi into the columns of hi lo'
-        tc_mma_f16(d, a, b, i2, acc);
-        tc_mma_f16(d + n, a2, b, i1, 1u);
-      } else {  // B's hi and lo' tiles alternate: every second one
-        const u64 sbo = (b >> 32) & 0x3FFFull, bh = b + (sbo << 32);
-        tc_mma_f16(d, a, bh, i1, acc);
-        tc_mma_f16(d + 64u, a, bh + sbo, i1, acc);
-        tc_mma_f16(d + 64u, a2, bh, i1, 1u);
-      }
+      // B's hi and lo' tiles alternate: every second one
+      const u64 sbo = (b >> 32) & 0x3FFFull, bh = b + (sbo << 32);
+      tc_mma_f16(d, a, bh, i1, acc);
+      tc_mma_f16(d + 64u, a, bh + sbo, i1, acc);
+      tc_mma_f16(d + 64u, a2, bh, i1, 1u);
     }
     tc_commit(bars.empty + 8 * slot);
     if (hdr & kHdrLast) {
-      tc_commit(bars.acc_full + 8 * acc_no);
+      tc_commit(bars.acc_full + 8 * (acc_no + ((hdr & kHdrGroup) ? kMaxAccs : 0)));
       ++chunk;
     }
   }
@@ -767,14 +684,9 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
 
 // ---- epilogue ------------------------------------------------------------------------------------
 
-__device__ __forceinline__ void store8(float* dst, const float (&v)[8], int vec) {
-  if (vec) {
-    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = v[i];
-  }
+__device__ __forceinline__ void store8(float* dst, const float* v) {
+  reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vec) {
   if (vec) {
@@ -784,24 +696,22 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vec)
     for (int i = 0; i < 4; ++i) dst[i] = v[i];
   }
 }
-__device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+__device__ __forceinline__ void group_sync(int e) {
+  asm volatile("bar.sync %0, 128;" ::"r"(e + 1) : "memory");
 }
 constexpr float kLoUnit = 1.0f / 2048.0f;  // 2^-11
 
-// Adds NJ tiles of an accumulation chunk: hi sums at column `hi`, lo sums at `lo` (kInt8: the integers at
-// `hi`, carried as they are).
-template <int MODE, int NJ>
-__device__ __forceinline__ void add_chunk(float (&acc)[4][8], uint32_t hi, uint32_t lo) {
+// Adds a 16-column tile of an accumulation chunk: hi sums at column `hi`, lo sums at `lo` (kInt8: the
+// integers at `hi`, carried as they are).
+template <int MODE>
+__device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t lo) {
   if constexpr (MODE == kInt8) {
-    tc_ld1<NJ>(hi, acc);
+    tc_ld16(hi, acc);
   } else {
-    float v[4][8], w[4][8];
-    tc_ld2<NJ>(hi, lo, v, w);
+    float v[16], w[16];
+    tc_ld16(hi, lo, v, w);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[j][i] += fmaf(w[j][i], kLoUnit, v[j][i]);
+    for (int i = 0; i < 16; ++i) acc[i] += fmaf(w[i], kLoUnit, v[i]);
   }
 }
 
@@ -813,7 +723,7 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
                                              float f1, float f2, const float (&rs)[4], float ts) {
   const int sc = 4 * (thread & ((1 << log4) - 1));
   if (sc >= n) return;
-  for (int r = thread >> log4; r < p.R; r += 256 >> log4) {
+  for (int r = thread >> log4; r < p.R; r += 128 >> log4) {
     const long long t = t0 + r;
     if (t >= p.tokens) break;
     const long long o = t * p.M + row0 + sc;
@@ -840,7 +750,7 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
         store4(p.out2 + o, w, p.vec);
       }
     } else {
-      const float s = r < (256 >> log4) ? ts : __ldg(p.token_scale + t);
+      const float s = r < (128 >> log4) ? ts : __ldg(p.token_scale + t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) hv[i] = float(__float_as_int(v[i])) * (s * rs[i]);
     }
@@ -848,50 +758,57 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
   }
 }
 
+// TMEM quadrants that hold tokens: M = 64 puts 16 rows in a quadrant, M = 128 32.
+template <int MODE>
+__device__ __forceinline__ int live_quads(const PairParams& p) {
+  if (MODE == kWeightGrad) return 4;
+  return p.R > 64 ? (p.R + 31) / 32 : (p.R + 15) / 16;
+}
+
 // The part of a unit that the epilogue reads, 16 bytes.
 template <int MODE>
 __device__ __forceinline__ uint4 unit_head(const PairParams& p, int unit) {
   if constexpr (by_rows(MODE)) return __ldg(reinterpret_cast<const uint4*>(p.rows + unit));
-  else return __ldg(reinterpret_cast<const uint4*>(p.cols + unit));
+  else if constexpr (MODE == kInputGrad) return __ldg(reinterpret_cast<const uint4*>(p.cols + unit));
+  else return __ldg(reinterpret_cast<const uint4*>(p.grads + unit));
 }
 
-// Epilogue warp e of a quadrant takes the 8-column tiles c with c % 2 == e.
+// Epilogue group e (four warps, one per TMEM quadrant) takes every second of the CTA's work items, so that
+// one item's sums are added while the other's output is worked out.
 template <int MODE>
 __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& bars, float* stage, int quad,
                          int e, int lane) {
   const bool wide = MODE == kWeightGrad || p.R > 64;  // M = 128; M = 64 fills lanes 0..15
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
   const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
-  const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles;
+  const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles, grid = int(gridDim.x);
   float f1 = 1.0f, f2 = 1.0f;
   if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
   if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
   if (MODE == kWeightGrad) unscale(p.exps[0] + p.exps[1], f1, f2);
-  const int thread = 128 * e + 32 * quad + lane, slog = stage_log(p.R), ld = (1 << slog) + 4;
-  uint32_t use = 0;
+  const int quads = live_quads<MODE>(p);
+  const int thread = 32 * quad + lane, slog = stage_log(MODE, p.R), ld = stage_ld(slog), log4 = slog - 2;
+  const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;  // staged output: column, first row
+  uint32_t use = 0, phases = 0;  // chunks of the CTA so far; parity of this group's phase per accumulator
   bool ok = true;
-  TileWalk walk(tiles);
-  // the next item's unit is fetched while this one's sums are waited for
-  const int units_step = int(gridDim.x) / tiles;
+  // units are fetched two items ahead: the other group's are only counted
+  const int units_step = grid / tiles;
   int unit = int(blockIdx.x) / tiles;
-  uint4 next = make_uint4(0, 0, 0, 0), next2 = next;
-  auto fetch = [&](int un) {
-    if constexpr (MODE == kWeightGrad) {
-      next = __ldg(reinterpret_cast<const uint4*>(p.grads + un));
-      next2 = __ldg(reinterpret_cast<const uint4*>(p.grads + un) + 1);
-    } else {
-      next = unit_head<MODE>(p, un);
-    }
+  TileWalk walk(tiles), ahead(tiles);
+  int item_ahead = blockIdx.x;
+  auto fetch = [&]() {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (item_ahead < items) v = unit_head<MODE>(p, unit);
+    unit += units_step + (ahead.tile + ahead.step >= tiles ? 1 : 0);
+    ahead.next();
+    item_ahead += grid;
+    return v;
   };
-  if (int(blockIdx.x) < items) fetch(unit);
-  int k = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x, ++k) {
-    const uint4 u = next, u2 = next2;
-    const int tile = walk.tile;
-    unit += units_step + (tile + walk.step >= tiles ? 1 : 0);
-    walk.next();
-    if (item + int(gridDim.x) < items) fetch(unit);
-    const long long t0 = (long long)(p.tile0 + tile) * p.R;
+  uint4 h1 = fetch(), h2 = fetch();
+  for (int item = blockIdx.x, k = 0; item < items; item += grid, ++k, walk.next()) {
+    const uint4 u = h1;
+    h1 = h2;
+    h2 = fetch();
     int n, chunks[2] = {0, 0};
     if constexpr (by_rows(MODE)) {
       n = int((u.y >> 8) & 255u);
@@ -905,74 +822,86 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       n = int(u.w);
       chunks[0] = p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
     }
+    if ((k & 1) != e) {
+      use += uint32_t(chunks[0] + chunks[1]);
+      continue;
+    }
+    const long long t0 = (long long)(p.tile0 + walk.tile) * p.R;
+    uint4 g2 = make_uint4(0, 0, 0, 0);
+    if constexpr (MODE == kWeightGrad) g2 = __ldg(reinterpret_cast<const uint4*>(p.grads + item) + 1);
     // scales of the elements that this thread writes, fetched before the sums are waited for
     float ts = 0.0f, rs[4] = {};
-    const int log4 = slog - 2;
-    if constexpr (MODE == kInt8) {
-      const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;
-      if (sr < p.R && t0 + sr < p.tokens) ts = __ldg(p.token_scale + t0 + sr);
-      if (sc < n) {
+    auto load_rs = [&](int c0) {
+      if constexpr (MODE == kInt8) {
+        if (c0 + sc < n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + sc + i);
-      }
-    }
-    const int nj = (n / 8 + 1 - e) / 2;  // this warp's tiles
-    float acc[MODE == kForward ? 2 : 1][4][8] = {};
-#pragma unroll
-    for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
-      for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
-        const uint32_t chunk = use / kPipes, buf = acc_of(p, use % kPipes, chunk);
-        // after an abort nothing is waited for, but the warps stay together (epilogue_sync)
-        if (ok) ok = wait_warp(bars.acc_full + 8 * buf, (chunk >> p.acc_log) & 1u, p.status, &sh.abort_flag);
-        tc_fence_after();
-        const uint32_t d = sh.tmem + acc_cols(p) * buf + (uint32_t(32 * quad) << 16) + 8u * e;
-        const uint32_t lo = d + (MODE == kForward ? n : 64);
-        switch (nj) {
-          case 1: add_chunk<MODE, 1>(acc[which], d, lo); break;
-          case 2: add_chunk<MODE, 2>(acc[which], d, lo); break;
-          case 3: add_chunk<MODE, 3>(acc[which], d, lo); break;
-          case 4: add_chunk<MODE, 4>(acc[which], d, lo); break;
+          for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + c0 + sc + i);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars.acc_empty + 8 * buf);
       }
+    };
+    if constexpr (MODE == kInt8) {
+      if (sr < p.R && t0 + sr < p.tokens) ts = __ldg(p.token_scale + t0 + sr);
+      load_rs(0);
+    }
+    float acc[MODE == kForward ? 2 : 1][4][16] = {};
+    if (quad < quads) {
+#pragma unroll
+      for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
+        for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
+          const uint32_t buf = acc_of(p, use % kPipes, use / kPipes);
+          // after an abort nothing is waited for, but the warps stay together (group_sync)
+          if (ok)
+            ok = wait_warp(bars.acc_full + 8 * (buf + kMaxAccs * e), (phases >> buf) & 1u, p.status, &sh.abort_flag);
+          phases ^= 1u << buf;
+          tc_fence_after();
+          const uint32_t d = sh.tmem + acc_cols(p) * buf + (uint32_t(32 * quad) << 16);
+          const uint32_t lo = d + (MODE == kForward ? n : 64);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (16 * j >= n) break;  // an odd last tile of 8 reads 8 columns more of its accumulator
+            add_tile<MODE>(acc[which][j], d + 16 * j, lo + 16 * j);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.acc_empty + 8 * buf);
+        }
+      }
+    } else {
+      use += uint32_t(chunks[0] + chunks[1]);
     }
     if constexpr (by_rows(MODE)) {
-      const bool two = p.R <= 16;  // two buffers: the next item's barrier parts readers and writers
-      float* st = stage + (two ? (k & 1) * (2 * p.R * ld) : 0);
-      float* st_up = st + p.R * ld;
+      float* st_up = stage + p.R * ld;
       for (int c0 = 0; c0 < n; c0 += 1 << slog) {
+        group_sync(e);  // the buffer has been read
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = 16 * j + 8 * e - c0;
-          if (!in_tile || c < 0 || c >= (1 << slog) || j >= nj) continue;
-          store8(st + row * ld + c, acc[0][j], 1);
-          if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j], 1);
+        for (int j = 0; j < 8; ++j) {
+          const int c = 8 * j - c0;
+          if (!in_tile || c < 0 || c >= (1 << slog) || 8 * j >= n) continue;
+          store8(stage + row * ld + c, acc[0][j / 2] + 8 * (j & 1));
+          if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j / 2] + 8 * (j & 1));
         }
-        epilogue_sync();
-        if (MODE == kInt8 && c0 > 0) {
-          const int sc = c0 + 4 * (thread & ((1 << log4) - 1));
-          if (sc < n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + sc + i);
-          }
-        }
-        write_staged<MODE>(p, st, st_up, ld, log4, n - c0, u.x + c0, t0, thread, f1, f2, rs, ts);
-        if (!two) epilogue_sync();
+        group_sync(e);
+        write_staged<MODE>(p, stage, st_up, ld, log4, n - c0, u.x + c0, t0, thread, f1, f2, rs, ts);
+        load_rs(c0 + (1 << slog));
       }
     } else {
       const bool live = MODE == kWeightGrad ? row < int(u.y) * 8 : in_tile && t0 + row < p.tokens;
       if (!live) continue;
       float* dst = MODE == kInputGrad
                        ? p.out0 + (t0 + row) * p.K + u.x
-                       : ((u2.z & 1u) ? p.out1 : p.out0) + (u64(u2.x) | u64(u2.y) << 32) + (long long)row * n;
+                       : ((g2.z & 1u) ? p.out1 : p.out0) + (u64(g2.x) | u64(g2.y) << 32) + (long long)row * n;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= nj) break;
+      for (int j = 0; j < 8; ++j) {
+        if (8 * j >= n) break;
+        float* a = acc[0][j / 2] + 8 * (j & 1);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[0][j][i] = acc[0][j][i] * f1 * f2;
-        store8(dst + 16 * j + 8 * e, acc[0][j], p.vec);
+        for (int i = 0; i < 8; ++i) a[i] = a[i] * f1 * f2;
+        if (p.vec) {
+          store8(dst + 8 * j, a);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[8 * j + i] = a[i];
+        }
       }
     }
   }
@@ -995,8 +924,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
       mbar_init(bars.empty + 8 * s, 1);
     }
     for (int b = 0; b < kMaxAccs; ++b) {
-      mbar_init(bars.acc_full + 8 * b, 1);
-      mbar_init(bars.acc_empty + 8 * b, kEpilogueWarps);
+      mbar_init(bars.acc_full + 8 * b, 1);  // one for each epilogue group, which see only their own phases
+      mbar_init(bars.acc_full + 8 * (kMaxAccs + b), 1);
+      mbar_init(bars.acc_empty + 8 * b, live_quads<MODE>(p));
     }
     for (int b = 0; b < kPipes; ++b) mbar_init(bars.drain + 8 * b, 1);
     sh.abort_flag = 0;
@@ -1015,6 +945,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   tc_fence_after();
 
   if (warp < kPipes) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     if constexpr (by_rows(MODE))
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)
@@ -1022,11 +953,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
     else
       produce_grads(p, sh, slots, bars, warp, lane);
   } else if (warp < 2 * kPipes) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
     if (lane == 0) issue_mmas<MODE>(p, sh, bars, warp - kPipes);
     __syncwarp();
   } else if (warp >= kEpilogueWarp) {
-    float* stage = reinterpret_cast<float*>(zero_ptr + kZeroBytes + kTailBytes);
-    epilogue<MODE>(p, sh, bars, stage, (warp - kEpilogueWarp) & 3, (warp - kEpilogueWarp) >> 2, lane);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
+    const int group = (warp - kEpilogueWarp) >> 2;
+    float* stage = reinterpret_cast<float*>(zero_ptr + kZeroBytes + kTailBytes + group * kStageBytes);
+    epilogue<MODE>(p, sh, bars, stage, (warp - kEpilogueWarp) & 3, group, lane);
   }
   tc_fence_before();
   __syncthreads();
