@@ -136,12 +136,17 @@ vbsr_status make_panel(const Source& src, const Panels& g, int64_t tokens, char*
   float* partial = reinterpret_cast<float*>(ws + which * kPartialBytes);
   int* exponent = reinterpret_cast<int*>(ws + 2 * kPartialBytes) + which;
   const int64_t groups = src.features / 8;
+  uint4* out = reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at));
+  if (groups * tokens * Source::parts <= kSmallGroups) {
+    panel_small_kernel<<<kSmallCtas, kSmallThreads, 0, s>>>(src, tokens, g.R, int(g.tiles), out, exponent);
+    VBSR_CUDA(cudaGetLastError());
+    return VBSR_OK;
+  }
   const int n = ctas_for(groups * tokens, kAmaxCtas);
   panel_amax_kernel<<<n, 256, 0, s>>>(src, tokens, partial);
-  panel_pair_kernel<<<ctas_for(groups * g.tiles * g.R, 148 * 16), 256, 0, s>>>(
-      src, tokens, g.R, int(g.tiles), partial, n,
-      reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at)), exponent);
   VBSR_CUDA(cudaGetLastError());
+  VBSR_CUDA(launch_after(panel_pair_kernel<Source>, dim3(ctas_for(groups * g.tiles * g.R, 148 * 16)), 256, 0, s,
+                         src, tokens, g.R, int(g.tiles), partial, n, out, exponent));
   return VBSR_OK;
 }
 

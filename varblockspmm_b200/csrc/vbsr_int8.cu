@@ -29,16 +29,29 @@ namespace {
 
 constexpr int64_t kMaxRowWidth = 131072;    // 127 * 127 * width stays below 2^31
 
-// The integer nearest to x / s, ties to even, as of the exact quotient (s > 0, |x| <= 127.5 s up to
-// rounding). The fp32 quotient can round onto or across a half; the residual x - q s is exact in
-// fma (|q| <= 128 and the difference is at most about s), and its comparison with s / 2 decides.
-__device__ __forceinline__ int quantize_exact(float x, float s) {
-  float q = rintf(x / s);
-  const float r = fmaf(-q, s, x), half = 0.5f * s;
-  if (r > half || (r == half && (int(q) & 1))) q += 1.0f;
-  if (r < -half || (r == -half && (int(q) & 1))) q -= 1.0f;
-  return max(-127, min(127, int(q)));
-}
+// A scale ready for use: s is a normal number far from the smallest (tiny scales and the values that go
+// with them are multiplied by 2^120, exactly); s = 0 stands for a scale that is 0 or NaN.
+struct Quantizer {
+  float s, inv, up;
+  __device__ __forceinline__ explicit Quantizer(float scale) {
+    up = scale < 1e-30f ? __int_as_float((120 + 127) << 23) : 1.0f;
+    s = scale > 0.0f ? scale * up : 0.0f;
+    inv = 1.0f / s;
+  }
+  // The integer nearest to x / s, ties to even, as of the exact quotient (|x| <= 127.5 s up to rounding).
+  // x inv is off by less than 2^-15, which can take q across a half but not further; the residual x - q s
+  // is exact in fma (|q| <= 128 and the difference is at most about s), and its comparison with s / 2
+  // decides.
+  __device__ __forceinline__ int operator()(float x) const {
+    if (s == 0.0f) return 0;
+    x *= up;
+    float q = rintf(x * inv);
+    const float r = fmaf(-q, s, x), half = 0.5f * s;
+    if (r > half || (r == half && (int(q) & 1))) q += 1.0f;
+    if (r < -half || (r == -half && (int(q) & 1))) q -= 1.0f;
+    return max(-127, min(127, int(q)));
+  }
+};
 
 // Largest magnitude of a CTA's values; NaN or infinity give NaN.
 __device__ __forceinline__ float scale_of(float amax, bool finite) {
@@ -73,9 +86,10 @@ __global__ void quantize_panel_kernel(const float* B, long long K, int8_t* Q, fl
   }
   m = block_amax(m, finite);
   const float s = scale_of(m, finite);
+  const Quantizer quant(s);
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
   for (long long i = threadIdx.x; i < K; i += blockDim.x)
-    q[i] = int8_t(s > 0.0f ? quantize_exact(x[i], s) : 0);
+    q[i] = int8_t(quant(x[i]));
 }
 
 // One warp per scalar row of a block row; one CTA per block row.
@@ -94,7 +108,7 @@ __global__ void quantize_rows_kernel(vbsr_device_matrix a, int8_t* values, float
             m = fmaxf(m, fabsf(x));
             finite = finite && isfinite(x);
           } else {
-            values[vo + r + (long long)k * h] = int8_t(s > 0.0f ? quantize_exact(x, s) : 0);
+            values[vo + r + (long long)k * h] = int8_t(Quantizer(s)(x));
           }
         }
       }
@@ -148,6 +162,7 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const LayRow* rows, co
 // Largest magnitude of each of `splits` equal parts of every token, or NaN: grid (splits, tokens).
 __global__ void __launch_bounds__(256) token_amax_kernel(const float* B, long long K, int vec,
                                                          float* partial) {
+  griddep_launch_dependents();
   const float* x = B + (long long)blockIdx.y * K;
   const long long g0 = (K / 8) * blockIdx.x / gridDim.x, g1 = (K / 8) * (blockIdx.x + 1) / gridDim.x;
   float m = 0.0f;
@@ -174,6 +189,8 @@ __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long 
                                                           int R, int vec, const float* partial, int splits,
                                                           float* token_scale, char* out) {
   __shared__ float scale[128];
+  griddep_launch_dependents();
+  griddep_wait();
   const long long t0 = (long long)blockIdx.y * R, groups = K / 8;
   if (FLOAT) {
     for (int r = threadIdx.x; r < R && t0 + r < tokens; r += blockDim.x) {
@@ -200,12 +217,12 @@ __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long 
     x.u = make_uint2(0, 0);
     if (t < tokens) {
       if (FLOAT) {
-        const float s = scale[r];
-        if (s > 0.0f) {
+        const Quantizer quant(scale[r]);
+        if (quant.s > 0.0f) {
           float v[8];
           load8(static_cast<const float*>(src) + t * K + 8 * g, vec, v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x.q[k] = int8_t(quantize_exact(v[k], s));
+          for (int k = 0; k < 8; ++k) x.q[k] = int8_t(quant(v[k]));
         }
       } else {
         const int8_t* q = static_cast<const int8_t*>(src) + t * K + 8 * g;
@@ -275,11 +292,16 @@ vbsr_status launch_chunks(const vbsr_int8* p, const Geometry& g, const void* src
   const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(ctas_for(p->K / 8 * g.R, 592),
                                                                  (2368 + g.tiles - 1) / g.tiles))),
                   unsigned(g.tiles));
-  chunk_panel_kernel<FLOAT><<<grid, 256, 0, s>>>(src, tokens, p->K, g.R, vec,
-                                                 reinterpret_cast<const float*>(ws), g.splits,
-                                                 reinterpret_cast<float*>(ws + g.scale_at),
-                                                 ws + g.panel_at);
-  VBSR_CUDA(cudaGetLastError());
+  const float* partial = reinterpret_cast<const float*>(ws);
+  float* scale = reinterpret_cast<float*>(ws + g.scale_at);
+  if (FLOAT) {
+    VBSR_CUDA(launch_after(chunk_panel_kernel<FLOAT>, grid, 256, 0, s, src, tokens, p->K, g.R, vec, partial,
+                           g.splits, scale, ws + g.panel_at));
+  } else {  // the first kernel of its call: after everything before it
+    chunk_panel_kernel<FLOAT><<<grid, 256, 0, s>>>(src, tokens, p->K, g.R, vec, partial, g.splits, scale,
+                                                   ws + g.panel_at);
+    VBSR_CUDA(cudaGetLastError());
+  }
   return VBSR_OK;
 }
 

@@ -782,6 +782,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
   const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
   const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles, grid = int(gridDim.x);
+  griddep_wait();
   float f1 = 1.0f, f2 = 1.0f;
   if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
   if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
@@ -946,6 +947,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
 
   if (warp < kPipes) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    griddep_wait();
     if constexpr (by_rows(MODE))
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)

@@ -36,6 +36,23 @@ inline void choose_rows(PairParams& k, RowUnit* const (&rows)[4], const int (&un
   k.acc_log = f >= 1 ? 1 : 0;
 }
 
+// Launches a kernel that itself waits (griddep_wait) for the one before it on the stream: it may be set up
+// while that one still runs.
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 template <int MODE>
 vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s) {
   if (k.units == 0) return VBSR_OK;
@@ -44,8 +61,8 @@ vbsr_status launch_pair(PairParams k, int64_t tiles, int num_sm, cudaStream_t s)
     k.tile0 = int(t0);
     k.tiles = int(std::min(most, tiles - t0));
     const int64_t items = MODE == kWeightGrad ? k.units : int64_t(k.units) * k.tiles;
-    pair_kernel<MODE><<<unsigned(std::min<int64_t>(num_sm, items)), kPairThreads, kPairSmem, s>>>(k);
-    VBSR_CUDA(cudaGetLastError());
+    VBSR_CUDA(launch_after(pair_kernel<MODE>, dim3(unsigned(std::min<int64_t>(num_sm, items))), kPairThreads,
+                           kPairSmem, s, k));
   }
   return VBSR_OK;
 }

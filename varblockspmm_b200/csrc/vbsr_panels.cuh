@@ -1,10 +1,12 @@
 // vbsr_panels.cuh — the pre-passes of the block-sparse layer operators: fp32 panels to operand
 // pairs (layout and reasons in vbsr_pair.cuh).
 #pragma once
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "vbsr_lm.cuh"
+#include "vbsr_ptx.cuh"
 
 namespace vbsr_b200 {
 
@@ -103,11 +105,12 @@ struct GateSource {
   }
 };
 
+// The largest finite magnitude of a thread's groups.
 template <class Source>
-__global__ void __launch_bounds__(256) panel_amax_kernel(Source src, long long tokens, float* partial) {
+__device__ __forceinline__ float largest(const Source& src, long long tokens, long long first, long long step) {
   const long long groups = src.features >> 3, n = tokens * groups;
   float m = 0.0f;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+  for (long long i = first; i < n; i += step) {
     float v[Source::parts][8];
     src.load(i / groups, i % groups, v);
 #pragma unroll
@@ -115,22 +118,17 @@ __global__ void __launch_bounds__(256) panel_amax_kernel(Source src, long long t
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[q][j]));
   }
-  m = cta_max(m);
-  if (threadIdx.x == 0) partial[blockIdx.x] = m;
+  return m;
 }
 
-// The panel in pairs: per tile of R tokens, part and 8-feature group, [R of hi][R of lo'] rows of 16
-// bytes. Neighbouring threads take neighbouring tokens (512 contiguous bytes written per warp; each
-// reads one whole 32-byte sector).
+// A thread's share of the panel in pairs: per tile of R tokens, part and 8-feature group, [R of hi]
+// [R of lo'] rows of 16 bytes. Neighbouring threads take neighbouring tokens (512 contiguous bytes written
+// per warp; each reads one whole 32-byte sector).
 template <class Source>
-__global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long tokens, int R, int tiles,
-                                                         const float* partial, int count, uint4* out,
-                                                         int* exponent) {
-  const int e = partial_exponent(partial, count);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
-  const float s = pow2(e);
+__device__ __forceinline__ void write_pairs(const Source& src, long long tokens, int R, int tiles, float s,
+                                            uint4* out, long long first, long long step) {
   const long long groups = src.features >> 3, n = groups * tiles * R;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+  for (long long i = first; i < n; i += step) {
     const int r = int(i % R);
     const long long g = (i / R) % groups, tile = i / R / groups, t = tile * R + r;
     float v[Source::parts][8] = {};
@@ -144,6 +142,48 @@ __global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long t
       o[R] = lo;
     }
   }
+}
+
+template <class Source>
+__global__ void __launch_bounds__(256) panel_amax_kernel(Source src, long long tokens, float* partial) {
+  griddep_launch_dependents();
+  const float m = cta_max(largest(src, tokens, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll));
+  if (threadIdx.x == 0) partial[blockIdx.x] = m;
+}
+
+template <class Source>
+__global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long tokens, int R, int tiles,
+                                                         const float* partial, int count, uint4* out,
+                                                         int* exponent) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int e = partial_exponent(partial, count);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
+  write_pairs(src, tokens, R, tiles, pow2(e), out, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+}
+
+// Both in one launch for a small panel: one cluster of kSmallCtas CTAs, which exchange their largest
+// magnitudes through distributed shared memory and read their values a second time from the caches. Against
+// the two kernels it saves a launch; above kSmallGroups 8-value groups its few SMs cost more than that.
+constexpr int kSmallCtas = 8, kSmallThreads = 512;
+constexpr int64_t kSmallGroups = 32768;
+template <class Source>
+__global__ void __cluster_dims__(kSmallCtas) __launch_bounds__(kSmallThreads)
+    panel_small_kernel(Source src, long long tokens, int R, int tiles, uint4* out, int* exponent) {
+  __shared__ float maxima[kSmallCtas];
+  griddep_launch_dependents();
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const long long first = blockIdx.x * (long long)kSmallThreads + threadIdx.x;
+  const long long step = (long long)kSmallCtas * kSmallThreads;
+  float m = cta_max(largest(src, tokens, first, step));
+  if (threadIdx.x < kSmallCtas) *cluster.map_shared_rank(&maxima[blockIdx.x], threadIdx.x) = m;
+  cluster.sync();
+#pragma unroll
+  for (int i = 0; i < kSmallCtas; ++i) m = fmaxf(m, maxima[i]);
+  const int e = pair_exponent(m);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
+  write_pairs(src, tokens, R, tiles, pow2(e), out, first, step);
 }
 
 }  // namespace vbsr_b200
