@@ -145,7 +145,7 @@ vbsr_status make_panel(const Source& src, const Panels& g, int64_t tokens, char*
   const int n = ctas_for(groups * tokens, kAmaxCtas);
   panel_amax_kernel<<<n, 256, 0, s>>>(src, tokens, partial);
   VBSR_CUDA(cudaGetLastError());
-  VBSR_CUDA(launch_after(panel_pair_kernel<Source>, dim3(ctas_for(groups * g.tiles * g.R, 148 * 16)), 256, 0, s,
+  VBSR_CUDA(launch_after(panel_pair_kernel<Source>, dim3(ctas_for(groups * g.tiles * g.R / 4, 148 * 7)), 256, 0, s,
                          src, tokens, g.R, int(g.tiles), partial, n, out, exponent));
   return VBSR_OK;
 }

@@ -33,23 +33,22 @@ constexpr int64_t kMaxRowWidth = 131072;    // 127 * 127 * width stays below 2^3
 // with them are multiplied by 2^120, exactly); s = 0 stands for a scale that is 0 or NaN.
 struct Quantizer {
   float s, inv, up;
+  Quantizer() = default;
   __device__ __forceinline__ explicit Quantizer(float scale) {
     up = scale < 1e-30f ? __int_as_float((120 + 127) << 23) : 1.0f;
     s = scale > 0.0f ? scale * up : 0.0f;
-    inv = 1.0f / s;
+    inv = s > 0.0f ? 1.0f / s : 0.0f;
   }
   // The integer nearest to x / s, ties to even, as of the exact quotient (|x| <= 127.5 s up to rounding).
   // x inv is off by less than 2^-15, which can take q across a half but not further; the residual x - q s
   // is exact in fma (|q| <= 128 and the difference is at most about s), and its comparison with s / 2
   // decides.
   __device__ __forceinline__ int operator()(float x) const {
-    if (s == 0.0f) return 0;
     x *= up;
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, s, x), half = 0.5f * s;
-    if (r > half || (r == half && (int(q) & 1))) q += 1.0f;
-    if (r < -half || (r == -half && (int(q) & 1))) q -= 1.0f;
-    return max(-127, min(127, int(q)));
+    int q = __float2int_rn(x * inv);
+    const float r = fmaf(-float(q), s, x), half = 0.5f * s, a = fabsf(r);
+    if (a > half || (a == half && (q & 1))) q += r > 0.0f ? 1 : -1;
+    return s > 0.0f ? max(-127, min(127, q)) : 0;
   }
 };
 
@@ -182,13 +181,14 @@ __global__ void __launch_bounds__(256) token_amax_kernel(const float* B, long lo
 }
 
 // The panel's chunks of one tile per grid row. FLOAT: from fp32 values (partial maxima given, scales
-// written), else from int8 ones. A thread takes 8 columns of a token: the first half of their own
-// chunk and the second half of the one before.
-template <bool FLOAT>
+// written), else from int8 ones. Blocks of tokens x groups (UNITS of 8 columns) go through shared memory, as
+// panel_pair_kernel's; the group behind a block is read too, for the second half of its last chunk.
+template <bool FLOAT, int UNITS>
 __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long long tokens, long long K,
                                                           int R, int vec, const float* partial, int splits,
                                                           float* token_scale, char* out) {
-  __shared__ float scale[128];
+  __shared__ Quantizer quant[128];
+  __shared__ uint2 q8[UNITS + 32];
   griddep_launch_dependents();
   griddep_wait();
   const long long t0 = (long long)blockIdx.y * R, groups = K / 8;
@@ -201,42 +201,54 @@ __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long 
         finite = finite && x == x;
         m = fmaxf(m, x);
       }
-      scale[r] = scale_of(m, finite);
-      if (blockIdx.x == 0) token_scale[t0 + r] = scale[r];
+      const float s = scale_of(m, finite);
+      quant[r] = Quantizer(s);
+      if (blockIdx.x == 0) token_scale[t0 + r] = s;
     }
-    __syncthreads();
   }
   char* tile = out + t0 * groups * 16;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < groups * R; i += gridDim.x * 256ll) {
-    const int r = int(i % R);
-    const long long g = i / R, t = t0 + r;
-    union {
-      int8_t q[8];
-      uint2 u;
-    } x;
-    x.u = make_uint2(0, 0);
-    if (t < tokens) {
+  const PanelBlocks b(R, 1, groups, UNITS);
+  union Octet {
+    int8_t q[8];
+    uint2 u;
+  };
+  for (long long item = blockIdx.x; item < b.items; item += gridDim.x) {
+    const PanelBlocks::Place at = b.place(item);
+    auto live = [&](int r, int g) { return at.r + r < R && t0 + at.r + r < tokens && at.g + g < groups; };
+    auto place = [&](int r, int g) { return (t0 + at.r + r) * K + 8 * (at.g + g); };
+    auto octet = [&](int r, int g) {  // 8 columns as they are, or quantised
+      Octet x;
+      x.u = make_uint2(0, 0);
+      if (!live(r, g)) return x.u;
       if (FLOAT) {
-        const Quantizer quant(scale[r]);
-        if (quant.s > 0.0f) {
-          float v[8];
-          load8(static_cast<const float*>(src) + t * K + 8 * g, vec, v);
+        float v[8];
+        load8(static_cast<const float*>(src) + place(r, g), vec, v);
+        const Quantizer q = quant[at.r + r];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x.q[k] = int8_t(quant(v[k]));
-        }
+        for (int k = 0; k < 8; ++k) x.q[k] = int8_t(q(v[k]));
+      } else if (vec) {
+        x.u = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(src) + place(r, g));
       } else {
-        const int8_t* q = static_cast<const int8_t*>(src) + t * K + 8 * g;
-        if (vec) {
-          x.u = *reinterpret_cast<const uint2*>(q);
-        } else {
-          for (int k = 0; k < 8; ++k) x.q[k] = q[k];
-        }
+        for (int k = 0; k < 8; ++k) x.q[k] = static_cast<const int8_t*>(src)[place(r, g) + k];
       }
+      return x.u;
+    };
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < UNITS / 256; ++k) {
+      const int u = threadIdx.x + 256 * k, r = u >> b.gg_log, g = u & (b.gg - 1);
+      q8[b.slot(r, g)] = octet(r, g);
     }
-    *reinterpret_cast<uint2*>(tile + (chunk_place(g, K) * R + r) * 16) = x.u;
-    if (g > 0) *reinterpret_cast<uint2*>(tile + (chunk_place(g - 1, K) * R + r) * 16 + 8) = x.u;
-    if (g + 1 == groups)
-      *reinterpret_cast<uint2*>(tile + (chunk_place(g, K) * R + r) * 16 + 8) = make_uint2(0, 0);
+    if (int(threadIdx.x) < b.tt) q8[b.slot(threadIdx.x, b.gg)] = octet(threadIdx.x, b.gg);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < UNITS / 256; ++k) {
+      const int u = threadIdx.x + 256 * k, r = u & (b.tt - 1), g = u >> b.tt_log;
+      if (at.r + r >= R || at.g + g >= groups) continue;
+      const uint2 first = q8[b.slot(r, g)], second = q8[b.slot(r, g + 1)];
+      *reinterpret_cast<uint4*>(tile + (chunk_place(at.g + g, K) * R + at.r + r) * 16) =
+          make_uint4(first.x, first.y, second.x, second.y);
+    }
   }
 }
 
@@ -288,18 +300,19 @@ vbsr_status launch_int8(const vbsr_int8* p, const Geometry& g, const float* scal
 template <bool FLOAT>
 vbsr_status launch_chunks(const vbsr_int8* p, const Geometry& g, const void* src, int vec, int64_t tokens,
                           char* ws, cudaStream_t s) {
-  // one grid row per tile (at most 32768, see kMaxTokens)
-  const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>(ctas_for(p->K / 8 * g.R, 592),
-                                                                 (2368 + g.tiles - 1) / g.tiles))),
-                  unsigned(g.tiles));
   const float* partial = reinterpret_cast<const float*>(ws);
   float* scale = reinterpret_cast<float*>(ws + g.scale_at);
+  // few values: small blocks, so that there are enough of them
+  const bool small = p->K / 8 * g.R * g.tiles < 592 * 1024;
+  const int64_t blocks = (p->K / 8 * g.R + (small ? 255 : 1023)) / (small ? 256 : 1024);
+  // one grid row per tile (at most 32768, see kMaxTokens)
+  const dim3 grid(unsigned(std::max<int64_t>(1, std::min(blocks, 1184 / g.tiles))), unsigned(g.tiles));
+  const auto kernel = small ? chunk_panel_kernel<FLOAT, 256> : chunk_panel_kernel<FLOAT, 1024>;
   if (FLOAT) {
-    VBSR_CUDA(launch_after(chunk_panel_kernel<FLOAT>, grid, 256, 0, s, src, tokens, p->K, g.R, vec, partial,
-                           g.splits, scale, ws + g.panel_at));
+    VBSR_CUDA(launch_after(kernel, grid, 256, 0, s, src, tokens, p->K, g.R, vec, partial, g.splits, scale,
+                           ws + g.panel_at));
   } else {  // the first kernel of its call: after everything before it
-    chunk_panel_kernel<FLOAT><<<grid, 256, 0, s>>>(src, tokens, p->K, g.R, vec, partial, g.splits, scale,
-                                                   ws + g.panel_at);
+    kernel<<<grid, 256, 0, s>>>(src, tokens, p->K, g.R, vec, partial, g.splits, scale, ws + g.panel_at);
     VBSR_CUDA(cudaGetLastError());
   }
   return VBSR_OK;

@@ -71,15 +71,14 @@ __device__ __forceinline__ void load8(const float* p, int vec, float (&v)[8]) {
   }
 }
 
-// Sources of a panel's values: 8 features from 8 g of token t.
+// Sources of a panel's values, 8 at a time: the i-th 8 values of the [tokens, features] array (features is
+// a multiple of 8).
 struct PlainSource {
   const float* x;
-  long long features;  // multiple of 8
+  long long features;
   int vec;             // x is 16-byte aligned
   static constexpr int parts = 1;
-  __device__ __forceinline__ void load(long long t, long long g, float (&v)[1][8]) const {
-    load8(x + t * features + 8 * g, vec, v[0]);
-  }
+  __device__ __forceinline__ void load(long long i, float (&v)[1][8]) const { load8(x + 8 * i, vec, v[0]); }
 };
 // dG = dH U act'(G) and dU = dH act(G); two panels one behind the other.
 struct GateSource {
@@ -87,8 +86,8 @@ struct GateSource {
   long long features;
   int vec, act;
   static constexpr int parts = 2;
-  __device__ __forceinline__ void load(long long t, long long g, float (&v)[2][8]) const {
-    const long long o = t * features + 8 * g;
+  __device__ __forceinline__ void load(long long i, float (&v)[2][8]) const {
+    const long long o = 8 * i;
     float a[8], u[8], d[8];
     load8(G + o, vec, a);
     load8(U + o, vec, u);
@@ -105,14 +104,69 @@ struct GateSource {
   }
 };
 
+// Place i = (tile groups + g) R + r of a panel, i going up by `step`: divisions only at the start.
+struct PanelWalk {
+  long long g, tile, step_g, step_tile, groups;
+  int r, step_r, R;
+  __device__ __forceinline__ PanelWalk(long long first, long long step, int R_, long long groups_)
+      : groups(groups_), R(R_) {
+    const long long q = first / R, sq = step / R;
+    r = int(first - q * R);
+    step_r = int(step - sq * R);
+    tile = q / groups;
+    g = q - tile * groups;
+    step_tile = sq / groups;
+    step_g = sq - step_tile * groups;
+  }
+  __device__ __forceinline__ void next() {
+    r += step_r;
+    g += step_g;
+    tile += step_tile;
+    if (r >= R) {
+      r -= R;
+      ++g;
+    }
+    if (g >= groups) {
+      g -= groups;
+      ++tile;
+    }
+  }
+};
+
+// A panel cut into blocks of tt tokens (a power of two up to 32) x gg groups, tt gg = units.
+struct PanelBlocks {
+  int tt, tt_log, gg, gg_log, r_blocks, R;
+  long long groups, g_blocks, items;
+  struct Place {
+    long long tile, g;
+    int r;
+  };
+  __device__ __forceinline__ PanelBlocks(int R_, int tiles, long long groups_, int units) : R(R_), groups(groups_) {
+    tt_log = R <= 1 ? 0 : min(5, 32 - __clz(R - 1));
+    tt = 1 << tt_log;
+    gg = units >> tt_log;
+    gg_log = 31 - __clz(gg);
+    r_blocks = (R + tt - 1) >> tt_log;
+    g_blocks = (groups + gg - 1) >> gg_log;
+    items = g_blocks * r_blocks * tiles;
+  }
+  __device__ __forceinline__ Place place(long long item) const {
+    const long long q = item / g_blocks;
+    return {q / r_blocks, (item - q * g_blocks) << gg_log, int(q % r_blocks) << tt_log};
+  }
+  // place of (token, group) in shared memory: tokens neighbouring, shifted by the group so that both the
+  // writing along groups and the reading along tokens spread over the banks
+  __device__ __forceinline__ int slot(int t, int g) const { return (g << tt_log) + ((t + g) & (tt - 1)); }
+};
+
 // The largest finite magnitude of a thread's groups.
 template <class Source>
 __device__ __forceinline__ float largest(const Source& src, long long tokens, long long first, long long step) {
-  const long long groups = src.features >> 3, n = tokens * groups;
+  const long long n = tokens * (src.features >> 3);
   float m = 0.0f;
   for (long long i = first; i < n; i += step) {
     float v[Source::parts][8];
-    src.load(i / groups, i % groups, v);
+    src.load(i, v);
 #pragma unroll
     for (int q = 0; q < Source::parts; ++q)
 #pragma unroll
@@ -127,12 +181,12 @@ __device__ __forceinline__ float largest(const Source& src, long long tokens, lo
 template <class Source>
 __device__ __forceinline__ void write_pairs(const Source& src, long long tokens, int R, int tiles, float s,
                                             uint4* out, long long first, long long step) {
-  const long long groups = src.features >> 3, n = groups * tiles * R;
-  for (long long i = first; i < n; i += step) {
-    const int r = int(i % R);
-    const long long g = (i / R) % groups, tile = i / R / groups, t = tile * R + r;
+  const long long groups = src.features >> 3;
+  for (PanelWalk w(first, step, R, groups); w.tile < tiles; w.next()) {
+    const int r = w.r;
+    const long long g = w.g, tile = w.tile, t = tile * R + r;
     float v[Source::parts][8] = {};
-    if (t < tokens) src.load(t, g, v);
+    if (t < tokens) src.load(t * groups + g, v);
 #pragma unroll
     for (int q = 0; q < Source::parts; ++q) {
       uint4 hi, lo;
@@ -155,11 +209,41 @@ template <class Source>
 __global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long tokens, int R, int tiles,
                                                          const float* partial, int count, uint4* out,
                                                          int* exponent) {
+  // a block of TT tokens (a power of two) x GG groups goes through shared memory: read along the features,
+  // written along the tokens, whole lines both ways
+  constexpr int P = Source::parts, UNITS = 1024 / P;
+  __shared__ uint4 hi[P][UNITS], lo[P][UNITS];
   griddep_launch_dependents();
   griddep_wait();
   const int e = partial_exponent(partial, count);
   if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
-  write_pairs(src, tokens, R, tiles, pow2(e), out, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+  const float s = pow2(e);
+  const PanelBlocks b(R, tiles, src.features >> 3, UNITS);
+  for (long long item = blockIdx.x; item < b.items; item += gridDim.x) {
+    const PanelBlocks::Place at = b.place(item);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < UNITS / 256; ++k) {
+      const int u = threadIdx.x + 256 * k, t = u >> b.gg_log, g = u & (b.gg - 1);
+      const long long token = at.tile * R + at.r + t;
+      float v[P][8] = {};
+      if (at.r + t < R && token < tokens && at.g + g < b.groups) src.load(token * b.groups + at.g + g, v);
+#pragma unroll
+      for (int q = 0; q < P; ++q) to_pair8(v[q], s, hi[q][b.slot(t, g)], lo[q][b.slot(t, g)]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < UNITS / 256; ++k) {
+      const int u = threadIdx.x + 256 * k, t = u & (b.tt - 1), g = u >> b.tt_log;
+      if (at.r + t >= R || at.g + g >= b.groups) continue;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        uint4* o = out + ((at.tile * P + q) * b.groups + at.g + g) * 2 * R + at.r + t;
+        o[0] = hi[q][b.slot(t, g)];
+        o[R] = lo[q][b.slot(t, g)];
+      }
+    }
+  }
 }
 
 // Both in one launch for a small panel: one cluster of kSmallCtas CTAs, which exchange their largest
