@@ -114,7 +114,6 @@ struct PairParams {
 struct PairStep {
   u64 a, b;
 };
-constexpr u64 kStepFresh = 1ull << 60;  // first step into its accumulator: overwrite
 constexpr u64 kStepOdd = 1ull << 58;    // the second K half of A is the tile of zeros
 constexpr u64 kStepMask = (1ull << 56) - 1;
 constexpr int kMaxSteps = 16;
@@ -153,20 +152,37 @@ __device__ __forceinline__ u64 core_desc(uint32_t addr, uint32_t lbo, uint32_t s
          (u64((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
 }
 
-__device__ __forceinline__ void tc_mma_f16(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t acc) {
+// MMAs and commits are issued by the lane with leader != 0; the whole warp runs the code around them, so that
+// descriptors stay in uniform registers (issued from a branch of one lane, each operand is first moved there).
+__device__ __forceinline__ void tc_mma_f16(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t acc,
+                                           uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_i8(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_i8(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t acc,
+                                          uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
+__device__ __forceinline__ void tc_commit_by(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+// A value that is the same in all lanes, as a uniform one.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ u64 uniform(u64 x) {
+  return u64(uniform(uint32_t(x))) | u64(uniform(uint32_t(x >> 32))) << 32;
+}
+
 // Bulk copy without an L2 hint (bulk_g2s has one).
 __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, uint32_t bytes,
                                                uint32_t bar) {
@@ -499,8 +515,7 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
         const bool pair = 2 * j + 1 < e.h8;
         const uint32_t a = a0 + 2 * j * xb;
         PairStep& out = sh.steps[slot][s_before + j];
-        out.a = core_desc(a, pair ? xb : zero - a, 128) |
-                (s_before + j == 0 ? kStepFresh : 0) | (pair ? 0 : kStepOdd);
+        out.a = core_desc(a, pair ? xb : zero - a, 128) | (pair ? 0 : kStepOdd);
         // columns 8 apart are 16 h apart (hi and lo' tiles alternate), rows 8 apart 128 bytes
         out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
       }
@@ -585,8 +600,7 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
       const uint32_t steps = uint32_t(nt) / 16;
       if (lane < int(steps)) {
         PairStep& out = sh.steps[slot][lane];
-        out.a = core_desc(base + 256u * lane, 128u, GB) |
-                (lane == 0 ? kStepFresh : 0);
+        out.a = core_desc(base + 256u * lane, 128u, GB);
         out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
       }
       announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast | group, (u.ng + h8) * 32u * uint32_t(nt), lane);
@@ -608,10 +622,11 @@ __device__ __forceinline__ uint32_t acc_of(const PairParams& p, uint32_t q, uint
 }
 __device__ __forceinline__ uint32_t acc_cols(const PairParams& p) { return 128u >> p.acc_log; }
 
-// ---- MMA threads ---------------------------------------------------------------------------------
+// ---- MMA warps -----------------------------------------------------------------------------------
 
 template <int MODE>
-__device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& bars, int q) {
+__device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& bars, int q_, int lane) {
+  const uint32_t q = uniform(uint32_t(q_)), leader = lane == 0;
   const int m = MODE == kWeightGrad ? 128 : (p.R > 64 ? 128 : 64);
   // D f32, A and B f16 (kInt8: D s32, A and B s8); transposed (MN-major) operands in bits 15 and 16
   const uint32_t form = (MODE == kInt8 ? (2u << 4) | (1u << 7) | (1u << 10) : (1u << 4)) |
@@ -620,18 +635,20 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
                         (uint32_t(m >> 4) << 24);
   const uint32_t xb16 = (MODE == kInt8 ? 1u : 2u) * uint32_t(p.R);  // panel group, in 16 bytes
   const u64 lo = MODE == kWeightGrad ? kGradTokens : u64(p.R);  // hi to lo' tile of A, in 16 bytes
-  Pipe pipe(p, q);
+  const uint32_t tmem = uniform(sh.tmem);
+  Pipe pipe(p, int(q));
   uint32_t chunk = 0;  // of this pipeline: accumulator q + kPipes (chunk % accumulators)
   for (;; ++pipe.i) {
     const uint32_t slot = pipe.slot();
-    if (!wait_one(bars.full + 8 * slot, pipe.parity(), p.status, &sh.abort_flag)) return;
-    const uint32_t hdr = *reinterpret_cast<volatile uint32_t*>(&sh.header[slot]);
+    if (!wait_warp(bars.full + 8 * slot, pipe.parity(), p.status, &sh.abort_flag)) return;
+    const uint32_t hdr = uniform(*reinterpret_cast<volatile uint32_t*>(&sh.header[slot]));
     const int steps = int(hdr & 63u), n = int((hdr >> 8) & 15u) * 8;
     if (steps == 0) break;
-    PairStep next = sh.steps[slot][0];
-    const uint32_t acc_no = acc_of(p, q, chunk), d = sh.tmem + acc_no * acc_cols(p);
+    // the list, one step to a lane
+    const PairStep list = sh.steps[slot][lane & (kMaxSteps - 1)];
+    const uint32_t acc_no = acc_of(p, q, chunk), d = tmem + acc_no * acc_cols(p);
     if (hdr & kHdrFirst)
-      if (!wait_one(bars.acc_empty + 8 * acc_no, ((chunk >> p.acc_log) & 1u) ^ 1u, p.status, &sh.abort_flag))
+      if (!wait_warp(bars.acc_empty + 8 * acc_no, ((chunk >> p.acc_log) & 1u) ^ 1u, p.status, &sh.abort_flag))
         return;
     tc_fence_after();
     // N of one tile of n columns: a multiple of 16 for M = 128 (one tile more is read, and its
@@ -639,47 +656,56 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     const int n1 = m == 128 || MODE == kInt8 ? (n + 15) & ~15 : n;
     const uint32_t i1 = form | (uint32_t(n1 >> 3) << 17);
     [[maybe_unused]] const uint32_t i2 = form | (uint32_t(2 * n >> 3) << 17);
-    if constexpr (by_rows(MODE)) {
-      const u64 da = (2u * xb16), db = (MODE == kInt8 ? 2u : 4u) * uint32_t(n);  // two groups, in 16 bytes
+    uint32_t acc = (hdr & kHdrFirst) ? 0u : 1u;
+    if constexpr (MODE == kForward || MODE == kInt8) {
+      const u64 da = 2u * xb16, db = (MODE == kInt8 ? 2u : 4u) * uint32_t(n);  // two groups, in 16 bytes
       const int even = steps - ((hdr & kHdrOdd) ? 1 : 0);
-      u64 a = next.a, b = next.b;
-      uint32_t acc = (hdr & kHdrFirst) ? 0u : 1u;
+      u64 a = uniform(list.a), b = uniform(list.b);
       auto step = [&](u64 a1, u64 a2, u64 b1) {
         if (MODE == kInt8) {
-          tc_mma_i8(d, a1, b1, i1, acc);
+          tc_mma_i8(d, a1, b1, i1, acc, leader);
         } else {  // hi x [hi; lo'], then lo' x hi into the columns of hi lo'
-          tc_mma_f16(d, a1, b1, i2, acc);
-          tc_mma_f16(d + n, a2, b1, i1, 1u);
+          tc_mma_f16(d, a1, b1, i2, acc, leader);
+          tc_mma_f16(d + n, a2, b1, i1, 1u, leader);
         }
         acc = 1u;
       };
-#pragma unroll 2
       for (int s = 0; s < even; ++s, a += da, b += db) step(a, a + lo, b);
-      if (hdr & kHdrOdd) {
-        const PairStep st = sh.steps[slot][1];
-        step(st.a, st.a + lo - (lo << 16), st.b);
+      if (hdr & kHdrOdd) {  // the second K half of A is the tile of zeros, which has no lo' tile behind it
+        const PairStep last = sh.steps[slot][1];
+        const u64 a1 = uniform(last.a);
+        step(a1, a1 + lo - (lo << 16), uniform(last.b));
       }
-    } else
-    for (int s = 0; s < steps; ++s) {
-      const PairStep st = next;
-      if (s + 1 < steps) next = sh.steps[slot][s + 1];
-      const u64 a = st.a & kStepMask, b = st.b;
-      const uint32_t acc = (st.a & kStepFresh) ? 0u : 1u;
-      const u64 a2 = a + lo - ((st.a & kStepOdd) ? lo << 16 : 0ull);
-      // B's hi and lo' tiles alternate: every second one
-      const u64 sbo = (b >> 32) & 0x3FFFull, bh = b + (sbo << 32);
-      tc_mma_f16(d, a, bh, i1, acc);
-      tc_mma_f16(d + 64u, a, bh + sbo, i1, acc);
-      tc_mma_f16(d + 64u, a2, bh, i1, 1u);
+    } else {
+      auto step = [&](u64 a, u64 a2, u64 b) {  // B's hi and lo' tiles alternate: every second one
+        const u64 sbo = (b >> 32) & 0x3FFFull, bh = b + (sbo << 32);
+        tc_mma_f16(d, a, bh, i1, acc, leader);
+        tc_mma_f16(d + 64u, a, bh + sbo, i1, acc, leader);
+        tc_mma_f16(d + 64u, a2, bh, i1, 1u, leader);
+        acc = 1u;
+      };
+      if constexpr (MODE == kWeightGrad) {  // 16 tokens are two core matrices, 256 bytes, further in both
+        u64 a = uniform(list.a), b = uniform(list.b);
+        for (int s = 0; s < steps; ++s, a += 16, b += 16) step(a, a + lo, b);
+      } else {
+        for (int s = 0; s < steps; ++s) {
+          const uint32_t a_lo = __shfl_sync(0xffffffffu, uint32_t(list.a), s);
+          const uint32_t a_hi = __shfl_sync(0xffffffffu, uint32_t(list.a >> 32), s);
+          const uint32_t b_lo = __shfl_sync(0xffffffffu, uint32_t(list.b), s);
+          const uint32_t b_hi = __shfl_sync(0xffffffffu, uint32_t(list.b >> 32), s);
+          const u64 a = (u64(a_hi) << 32 | a_lo) & kStepMask, b = u64(b_hi) << 32 | b_lo;
+          step(a, a + lo - ((a_hi & uint32_t(kStepOdd >> 32)) ? lo << 16 : 0ull), b);
+        }
+      }
     }
-    tc_commit(bars.empty + 8 * slot);
+    tc_commit_by(bars.empty + 8 * slot, leader);
     if (hdr & kHdrLast) {
-      tc_commit(bars.acc_full + 8 * (acc_no + ((hdr & kHdrGroup) ? kMaxAccs : 0)));
+      tc_commit_by(bars.acc_full + 8 * (acc_no + ((hdr & kHdrGroup) ? kMaxAccs : 0)), leader);
       ++chunk;
     }
   }
-  tc_commit(bars.drain + 8 * q);  // nothing may arrive on a barrier of a CTA that has gone
-  wait_one(bars.drain + 8 * q, 0, p.status, &sh.abort_flag);
+  tc_commit_by(bars.drain + 8 * q, leader);  // nothing may arrive on a barrier of a CTA that has gone
+  wait_warp(bars.drain + 8 * q, 0, p.status, &sh.abort_flag);
 }
 
 // ---- epilogue ------------------------------------------------------------------------------------
@@ -716,27 +742,16 @@ __device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t
 }
 
 // Output of a row unit's tile from the staged sums: a thread takes four neighbouring elements of a row, so
-// that few tokens' activations are shared out too and whole lines are stored.
+// that few tokens' activations are shared out too and whole lines are stored. Two rows at a time, because
+// an element is a chain of latencies (shared memory, exponential, quotient).
 template <int MODE>
 __device__ __forceinline__ void write_staged(const PairParams& p, const float* st, const float* st_up, int ld,
-                                             int log4, int n, uint32_t row0, long long t0, int thread,
-                                             float f1, float f2, const float (&rs)[4], float ts) {
-  const int sc = 4 * (thread & ((1 << log4) - 1));
-  if (sc >= n) return;
-  for (int r = thread >> log4; r < p.R; r += 128 >> log4) {
-    const long long t = t0 + r;
-    if (t >= p.tokens) break;
-    const long long o = t * p.M + row0 + sc;
-    float v[4], hv[4];
-    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(st + r * ld + sc);
+                                             int step, int sc, int sr, int rows, long long o, float f1, float f2,
+                                             const float (&rs)[4], float ts, long long t0) {
+  // o: place of (row 0, column sc) in the output
+  auto finish = [&](int r, long long at, float (&v)[4], float (&w)[4]) {
+    float hv[4];
     if constexpr (MODE == kForward) {
-      float w[4];
-      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(st_up + r * ld + sc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = v[i] * f1 * f2;
-        w[i] = w[i] * f1 * f2;
-      }
       with_act(p.act, [&](auto kind) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -746,15 +761,36 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
         }
       });
       if (p.out1 != nullptr) {
-        store4(p.out1 + o, v, p.vec);
-        store4(p.out2 + o, w, p.vec);
+        store4(p.out1 + at, v, p.vec);
+        store4(p.out2 + at, w, p.vec);
       }
     } else {
-      const float s = r < (128 >> log4) ? ts : __ldg(p.token_scale + t);
+      const float s = r == sr ? ts : __ldg(p.token_scale + t0 + r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) hv[i] = float(__float_as_int(v[i])) * (s * rs[i]);
     }
-    store4(p.out0 + o, hv, p.vec);
+    store4(p.out0 + at, hv, p.vec);
+  };
+  auto load = [&](int r, float (&v)[4], float (&w)[4]) {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(st + r * ld + sc);
+    if constexpr (MODE == kForward) {
+      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(st_up + r * ld + sc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = v[i] * f1 * f2;
+        w[i] = w[i] * f1 * f2;
+      }
+    }
+  };
+  const long long hop = step * p.M;
+  o += sr * p.M;
+  for (int r = sr; r < rows; r += 2 * step, o += 2 * hop) {
+    float v[2][4], w[2][4];
+    const bool two = r + step < rows;
+    load(r, v[0], w[0]);
+    load(two ? r + step : r, v[1], w[1]);
+    finish(r, o, v[0], w[0]);
+    if (two) finish(r + step, o + hop, v[1], w[1]);
   }
 }
 
@@ -792,24 +828,25 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;  // staged output: column, first row
   uint32_t use = 0, phases = 0;  // chunks of the CTA so far; parity of this group's phase per accumulator
   bool ok = true;
-  // units are fetched two items ahead: the other group's are only counted
-  const int units_step = grid / tiles;
-  int unit = int(blockIdx.x) / tiles;
-  TileWalk walk(tiles), ahead(tiles);
-  int item_ahead = blockIdx.x;
-  auto fetch = [&]() {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (item_ahead < items) v = unit_head<MODE>(p, unit);
-    unit += units_step + (ahead.tile + ahead.step >= tiles ? 1 : 0);
-    ahead.next();
-    item_ahead += grid;
-    return v;
+  // the units of the next 32 items in the lanes' registers, and the 32 after them on their way
+  TileWalk walk(tiles);
+  uint4 heads, heads2;
+  auto fetch = [&](int k) {
+    const long long item = blockIdx.x + (long long)(k + lane) * grid;
+    return item < items ? unit_head<MODE>(p, int(item) / tiles) : make_uint4(0, 0, 0, 0);
   };
-  uint4 h1 = fetch(), h2 = fetch();
+  heads = fetch(0);
+  heads2 = fetch(32);
   for (int item = blockIdx.x, k = 0; item < items; item += grid, ++k, walk.next()) {
-    const uint4 u = h1;
-    h1 = h2;
-    h2 = fetch();
+    if (k > 0 && (k & 31) == 0) {
+      heads = heads2;
+      heads2 = fetch(k + 32);
+    }
+    uint4 u;
+    u.x = __shfl_sync(0xffffffffu, heads.x, k & 31);
+    u.y = __shfl_sync(0xffffffffu, heads.y, k & 31);
+    u.z = __shfl_sync(0xffffffffu, heads.z, k & 31);
+    u.w = __shfl_sync(0xffffffffu, heads.w, k & 31);
     int n, chunks[2] = {0, 0};
     if constexpr (by_rows(MODE)) {
       n = int((u.y >> 8) & 255u);
@@ -872,6 +909,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     }
     if constexpr (by_rows(MODE)) {
       float* st_up = stage + p.R * ld;
+      const int rows = int(min((long long)p.R, p.tokens - t0));
       for (int c0 = 0; c0 < n; c0 += 1 << slog) {
         group_sync(e);  // the buffer has been read
 #pragma unroll
@@ -882,7 +920,9 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
           if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j / 2] + 8 * (j & 1));
         }
         group_sync(e);
-        write_staged<MODE>(p, stage, st_up, ld, log4, n - c0, u.x + c0, t0, thread, f1, f2, rs, ts);
+        if (c0 + sc < n)
+          write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc, f1, f2, rs,
+                             ts, t0);
         load_rs(c0 + (1 << slog));
       }
     } else {
@@ -956,8 +996,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
       produce_grads(p, sh, slots, bars, warp, lane);
   } else if (warp < 2 * kPipes) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (lane == 0) issue_mmas<MODE>(p, sh, bars, warp - kPipes);
-    __syncwarp();
+    issue_mmas<MODE>(p, sh, bars, warp - kPipes, lane);
   } else if (warp >= kEpilogueWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
     const int group = (warp - kEpilogueWarp) >> 2;
