@@ -367,6 +367,7 @@ vbsr_status vbsr_ortho_create(const vbsr_matrix* m, vbsr_ortho** out);
 vbsr_status vbsr_ortho_destroy(vbsr_ortho* p);
 vbsr_status vbsr_ortho_execute(const vbsr_ortho* p, const float* values, float* out, int steps,
                                float eps, const float* coefficients, vbsr_stream_t stream);
+vbsr_status vbsr_ortho_check_status(const vbsr_ortho* p, vbsr_stream_t stream);
 
 /* ---- Raw launchers kept for source compatibility ------------------------------------------ */
 

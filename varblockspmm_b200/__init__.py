@@ -194,6 +194,7 @@ _sig = {
     "vbsr_matrix_quantize": [_vp, _vp, _vp, _vp],
     "vbsr_ortho_create": [_vp, C.POINTER(_vp)],
     "vbsr_ortho_destroy": [_vp],
+    "vbsr_ortho_check_status": [_vp, _vp],
     "vbsr_ortho_execute": [_vp, _vp, _vp, C.c_int, C.c_float, C.POINTER(C.c_float), _vp],
 }
 for _name, _args in _sig.items():
@@ -896,6 +897,10 @@ class OrthoPlan:
                                        _panel(out, self._values, 1, "out", self._device), int(steps),
                                        float(eps), (C.c_float * 3)(*coefficients),
                                        _stream_ptr(stream)))
+
+    def check_status(self, stream=None):
+        """Synchronises `stream` and raises if a kernel of the plan recorded a timeout."""
+        _check(_lib.vbsr_ortho_check_status(self._h, _stream_ptr(stream)))
 
     def close(self):
         if self._h:

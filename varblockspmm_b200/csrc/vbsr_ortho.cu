@@ -11,13 +11,21 @@
 // accumulator (lo lo is below 2^-22 of it). The iterates of a convergent iteration have entries of at
 // most about one, and P of about 11; 2^10 leaves room up to 64. X itself is carried in fp32 registers.
 //
-// Layout. 16-row strips of X, one per warp, live in registers in the accumulator layout of mma.sync,
-// which is also its A operand's layout, so a strip enters the next product without leaving the
-// registers; the other operand (all of X, or all of A) is read from shared memory, rows padded by 16
-// bytes so that ldmatrix meets no bank conflict. A needs no transposed copy: it is symmetric. mma.sync
-// and not tcgen05, because the products are chained through elementwise steps and of any size from 8
-// to 64: the result of each would go TMEM to registers to shared memory, and M = 64 is mostly
-// empty for the small blocks.
+// Two forms, by the block's shorter side m.
+//
+// m <= 32, mma.sync: 16-row strips of X, one per warp, live in registers in the accumulator layout, which is
+// also the A operand's layout, so a strip enters the next product without leaving the registers; the other
+// operand (all of X, or all of A) is read from shared memory, rows padded by 16 bytes so that ldmatrix meets
+// no bank conflict. A needs no transposed copy: it is symmetric. (M = 64 of a tcgen05 MMA would be mostly
+// empty here.)
+//
+// m > 32, tcgen05: four warps own two blocks, one above the other, a thread one row of X. Operands are core
+// matrices in shared memory, written once per product as pairs; X serves K-major as both operands of X X^T
+// and MN-major as the second of P X. A and A A stay in TMEM, where the threads read their rows. An MMA has
+// M = 128, both blocks' rows, against the columns of both (X X^T, A A; the mixed quarters are not used) or
+// one after the other (P X): with M = 64 the tensor core does the same work, but the accumulator fills
+// 16 lanes of 32, and the conversions, which bound it, took twice the instructions (measured 1353 us for
+// 32768 blocks of 8 to 64, 8192 of them above 48 x 48; mma.sync for all sizes: 701 us).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -27,11 +35,11 @@
 
 #include "vbsr_internal.h"
 #include "vbsr_lm.cuh"
-#include "vbsr_ptx.cuh"
+#include "vbsr_pair_host.cuh"
 
 using namespace vbsr_b200;
 
-// The blocks of a CTA: one of more than 32 rows, two of more than 16, or four (val = -1: none).
+// The blocks of a CTA: two of more than 32 rows or of more than 16, or four (val = -1: none).
 struct alignas(16) OrthoSlot {
   int64_t val;       // first value
   uint32_t shape;    // h | w << 8 | ceil(m / 16) << 16 | ceil(n / 16) << 24
@@ -40,8 +48,9 @@ struct alignas(16) OrthoSlot {
 
 struct vbsr_ortho {
   const vbsr_matrix* m = nullptr;
-  int device = 0, ctas = 0;
+  int device = 0, big_ctas = 0, small_ctas = 0;  // of blocks of more than 32 rows, which come first; others
   OrthoSlot* slots = nullptr;
+  int* d_status = nullptr;
 };
 
 namespace {
@@ -50,7 +59,7 @@ constexpr float kScale = 1024.0f, kUnscale2 = 1.0f / (1024.0f * 1024.0f);
 
 // Barrier of the MT warps of a block, the CTA's `group`-th.
 template <int MT>
-__device__ __forceinline__ void group_sync(int group) {
+__device__ __forceinline__ void strip_sync(int group) {
   if (MT == 1)
     __syncwarp();
   else
@@ -89,6 +98,28 @@ __device__ __forceinline__ void pair2(float x, float y, float s, uint32_t& hi, u
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// |V| as 2^e |V / 2^e| with 2^e about the largest magnitude, so that the squares neither overflow nor vanish;
+// a NaN or infinity makes the sum NaN or infinite, and then the block.
+struct Norm {
+  int e;
+  float down;
+  __device__ __forceinline__ explicit Norm(float amax) {
+    const bool usable = amax > 0.0f && amax < __int_as_float(0x7f800000);
+    e = usable ? max(-125, min(125, ilogbf(amax))) : 0;
+    down = __int_as_float((127 - e) << 23);
+  }
+  __device__ __forceinline__ float add(float sum, float v) const {
+    const float y = v * down;
+    return fmaf(y, y, sum);
+  }
+  // 1 / (|V| + eps) times 2^e, 0 for a block of zeros without eps
+  __device__ __forceinline__ float inverse(float sum, float eps) const {
+    const float norm = sqrtf(sum) + eps * down;
+    return norm == 0.0f ? 0.0f : 1.0f / norm;
+  }
+  __device__ __forceinline__ float apply(float v, float inv) const { return v * down * inv; }
+};
+
 // A strip (T tiles of 8 columns) as pairs: the A operands of its T / 2 k-tiles.
 template <int T>
 struct StripPair {
@@ -125,22 +156,26 @@ __device__ __forceinline__ void strip_product(float (&d)[T][4], const StripPair<
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[j][i] = 0.0f;
   const int r = lane & 7, q = lane >> 3;
+  constexpr int J = T % 4 == 0 ? 4 : 2;  // tiles at a time: independent sums, an MMA waits for its sum's last one
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int j = 0; j < T; j += 2) {
-      // the four 8 x 8 pieces: k halves of tile j, then of tile j + 1
-      const int n = 8 * (j + (q >> 1)), k = 16 * kt + 8 * (q & 1);
-      const uint32_t addr = base + 2u * (TRANS ? (k + r) * LD + n : (n + r) * LD + k);
-      uint32_t bh[4], bl[4];
-      ldsm4<TRANS>(addr, bh);
-      ldsm4<TRANS>(addr + lo_off, bl);
-      mma16816(d[j], a.hi[kt], bl[0], bl[1]);
-      mma16816(d[j + 1], a.hi[kt], bl[2], bl[3]);
-      mma16816(d[j], a.lo[kt], bh[0], bh[1]);
-      mma16816(d[j + 1], a.lo[kt], bh[2], bh[3]);
-      mma16816(d[j], a.hi[kt], bh[0], bh[1]);
-      mma16816(d[j + 1], a.hi[kt], bh[2], bh[3]);
+    for (int j = 0; j < T; j += J) {
+      uint32_t bh[J / 2][4], bl[J / 2][4];
+#pragma unroll
+      for (int i = 0; i < J / 2; ++i) {
+        // the four 8 x 8 pieces: k halves of tile j + 2 i, then of the next
+        const int n = 8 * (j + 2 * i + (q >> 1)), k = 16 * kt + 8 * (q & 1);
+        const uint32_t addr = base + 2u * (TRANS ? (k + r) * LD + n : (n + r) * LD + k);
+        ldsm4<TRANS>(addr, bh[i]);
+        ldsm4<TRANS>(addr + lo_off, bl[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < J; ++i) mma16816(d[j + i], a.hi[kt], bl[i / 2][2 * (i & 1)], bl[i / 2][2 * (i & 1) + 1]);
+#pragma unroll
+      for (int i = 0; i < J; ++i) mma16816(d[j + i], a.lo[kt], bh[i / 2][2 * (i & 1)], bh[i / 2][2 * (i & 1) + 1]);
+#pragma unroll
+      for (int i = 0; i < J; ++i) mma16816(d[j + i], a.hi[kt], bh[i / 2][2 * (i & 1)], bh[i / 2][2 * (i & 1) + 1]);
     }
 }
 
@@ -150,6 +185,7 @@ struct OrthoParams {
   float* out;
   int steps;
   float eps, a, b, c;
+  int* status;
 };
 
 // Shared memory of a block of MT x NT 16-tiles: two buffers of X and one of A, each hi and lo.
@@ -161,8 +197,10 @@ struct OrthoSmem {
   static constexpr int red_at = a_at + 2 * a_lo;
   static constexpr int bytes = red_at + 2 * 16;
 };
-constexpr int kOrthoSmem = OrthoSmem<4, 4>::bytes;
-static_assert(2 * OrthoSmem<2, 4>::bytes <= kOrthoSmem && 4 * OrthoSmem<1, 4>::bytes <= kOrthoSmem, "groups");
+constexpr int kMax2(int a, int b) { return a > b ? a : b; }
+constexpr int kSmallSmem = kMax2(2 * OrthoSmem<2, 4>::bytes, 4 * OrthoSmem<1, 4>::bytes);
+// m > 32: X, A and P of two blocks as pairs, 128 x 64 each.
+constexpr int kTileBytes = 128 * 64 * 2, kBigSmem = 6 * kTileBytes + 1024;
 
 template <int MT, int NT>
 __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoSlot& s, char* sm, int group,
@@ -191,31 +229,23 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
     }
     if (MT == 1) return v;
     if (lane == 0) red[4 * slot + strip] = v;
-    group_sync<MT>(group);
+    strip_sync<MT>(group);
     v = red[4 * slot];
 #pragma unroll
     for (int i = 1; i < MT; ++i) v = largest ? fmaxf(v, red[4 * slot + i]) : v + red[4 * slot + i];
     return v;
   };
-  // |V| as amax |V / amax|, so that the squares neither overflow nor vanish
-  amax = reduce(amax, 0, true);
-  const float scale = amax > 0.0f && amax < __int_as_float(0x7f800000) ? amax : 1.0f;
+  const Norm norm(reduce(amax, 0, true));
   float sum = 0.0f;
 #pragma unroll
   for (int j = 0; j < 2 * NT; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float y = x[j][i] / scale;
-      sum = fmaf(y, y, sum);
-    }
-  sum = reduce(sum, 1, false);
-  const float norm = scale * sqrtf(sum) + p.eps;
-  if (norm != 0.0f) {
+    for (int i = 0; i < 4; ++i) sum = norm.add(sum, x[j][i]);
+  const float inv = norm.inverse(reduce(sum, 1, false), p.eps);
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j)
+  for (int j = 0; j < 2 * NT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[j][i] /= norm;
-  }
+    for (int i = 0; i < 4; ++i) x[j][i] = norm.apply(x[j][i], inv);
 
   for (int step = 0; step < p.steps; ++step) {
     char* xs = sm + (step & 1) * S::x_bytes;  // the other buffer may still be read by another warp
@@ -224,13 +254,13 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
       StripPair<2 * NT> xp;
       xp.set(x, kScale);
       xp.template store<S::LDX>(xs, S::x_lo, strip, lane);
-      group_sync<MT>(group);
+      strip_sync<MT>(group);
       strip_product<2 * MT, NT, S::LDX, false>(acc, xp, smem_addr(xs), S::x_lo, lane);
     }
     StripPair<2 * MT> ap;
     ap.set(acc, 1.0f / kScale);  // acc is 2^20 A
     ap.template store<S::LDA>(sm + S::a_at, S::a_lo, strip, lane);
-    group_sync<MT>(group);
+    strip_sync<MT>(group);
     strip_product<2 * MT, MT, S::LDA, false>(sq, ap, smem_addr(sm + S::a_at), S::a_lo, lane);
 #pragma unroll
     for (int j = 0; j < 2 * MT; ++j)
@@ -254,37 +284,220 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
     }
 }
 
-// Four warps: one block of more than 32 rows (three or four strips), two of more than 16 or four.
-__global__ void __launch_bounds__(128, 3) ortho_kernel(OrthoParams p) {
+// Two to four warps a block: two blocks of more than 16 rows in a CTA, or four.
+__global__ void __launch_bounds__(128, 4) ortho_small_kernel(OrthoParams p) {
   extern __shared__ __align__(16) char sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const OrthoSlot* slots = p.slots + 4ll * blockIdx.x;
   const int mt = int((slots[0].shape >> 16) & 255u);
-  const int per = mt <= 1 ? 1 : (mt == 2 ? 2 : 4), group = warp / per, strip = warp % per;
+  const int group = warp / mt, strip = warp % mt;
   const OrthoSlot s = slots[group];
-  if (s.val < 0 || strip >= mt) return;
-  const int nt = int(s.shape >> 24);
+  if (s.val >= 0) {
+    const int nt = int(s.shape >> 24);
 #define VBSR_ORTHO(M, N)                                                                     \
   case 8 * M + N:                                                                            \
     orthogonalize<M, N>(p, s, sm + group * OrthoSmem<M, N>::bytes, group, strip, lane);      \
     break;
-  switch (8 * mt + nt) {
-    VBSR_ORTHO(1, 1) VBSR_ORTHO(1, 2) VBSR_ORTHO(1, 3) VBSR_ORTHO(1, 4) VBSR_ORTHO(2, 2)
-    VBSR_ORTHO(2, 3) VBSR_ORTHO(2, 4) VBSR_ORTHO(3, 3) VBSR_ORTHO(3, 4) VBSR_ORTHO(4, 4)
-  }
+    switch (8 * mt + nt) {
+      VBSR_ORTHO(1, 1) VBSR_ORTHO(1, 2) VBSR_ORTHO(1, 3) VBSR_ORTHO(1, 4) VBSR_ORTHO(2, 2)
+      VBSR_ORTHO(2, 3) VBSR_ORTHO(2, 4)
+    }
 #undef VBSR_ORTHO
+  }
+  griddep_wait();  // it may have started beside the large blocks' kernel: both are done when this one is
+}
+
+// ---- m > 32 --------------------------------------------------------------------------------------
+//
+// An operand: row r of the CTA's 128 (block r / 64), column group g (8 columns) at byte 2048 g + 16 r; hi, and
+// lo kTileBytes behind.
+
+struct OrthoTcShared {
+  u64 done;
+  uint32_t tmem;
+  volatile int abort_flag;
+  float red[2][4];
+};
+
+// A row's 64 values, times s, as pairs into an operand.
+__device__ __forceinline__ void store_pairs(char* tile, int row, const float (&v)[64], float s) {
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    uint4 hi, lo;
+    pair2(v[8 * g], v[8 * g + 1], s, hi.x, lo.x);
+    pair2(v[8 * g + 2], v[8 * g + 3], s, hi.y, lo.y);
+    pair2(v[8 * g + 4], v[8 * g + 5], s, hi.z, lo.z);
+    pair2(v[8 * g + 6], v[8 * g + 7], s, hi.w, lo.w);
+    char* o = tile + 2048 * g + 16 * row;
+    *reinterpret_cast<uint4*>(o) = hi;
+    *reinterpret_cast<uint4*>(o + kTileBytes) = lo;
+  }
+}
+
+// 64 accumulator columns, loaded and waited for.
+__device__ __forceinline__ void tc_ld64(uint32_t a, float (&v)[64]) {
+#pragma unroll
+  for (int i = 0; i < 64; i += 32) {
+    float x[16], y[16];
+    tc_ld16(a + i, a + i + 16, x, y);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      v[i + j] = x[j];
+      v[i + 16 + j] = y[j];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
+  extern __shared__ char sm[];
+  __shared__ OrthoTcShared sh;
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, block = threadIdx.x >> 6, row = threadIdx.x & 63;
+  const OrthoSlot* slots = p.slots + 4ll * blockIdx.x;
+  const OrthoSlot s = slots[block];
+  const int h = int(s.shape & 255u), w = int((s.shape >> 8) & 255u);
+  const int m = min(h, w), n = max(h, w);
+  // 16-column steps that cover both blocks
+  const int mt = max(int((slots[0].shape >> 16) & 255u), int((slots[1].shape >> 16) & 255u));
+  const int nt = max(int(slots[0].shape >> 24), int(slots[1].shape >> 24));
+  const uint32_t base = (smem_addr(sm) + 1023u) & ~1023u;
+  char* xt = sm + (base - smem_addr(sm));
+  char *at = xt + 2 * kTileBytes, *pt = xt + 4 * kTileBytes;
+  const uint32_t done = smem_addr(&sh.done);
+  if (threadIdx.x == 0) {
+    mbar_init(done, 1);
+    sh.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tc_alloc(smem_addr(&sh.tmem), 256);
+    tc_relinquish();
+  }
+  tc_fence_before();
+  const bool live = s.val >= 0 && row < m;
+  const long long si = h <= w ? 1 : h, sj = h <= w ? h : 1;
+  const float* v = p.values + s.val + row * si;
+  float x[64];
+  float amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 64; ++j) {
+    x[j] = live && j < n ? v[j * sj] : 0.0f;
+    amax = fmaxf(amax, fabsf(x[j]));
+  }
+  auto reduce = [&](float y, int slot, bool largest) {  // over the block's two warps
+    for (int d = 16; d; d >>= 1) {
+      const float z = __shfl_xor_sync(0xffffffffu, y, d);
+      y = largest ? fmaxf(y, z) : y + z;
+    }
+    if (lane == 0) sh.red[slot][warp] = y;
+    __syncthreads();
+    const float a = sh.red[slot][2 * block], b = sh.red[slot][2 * block + 1];
+    return largest ? fmaxf(a, b) : a + b;
+  };
+  const Norm norm(reduce(amax, 0, true));
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 64; ++j) sum = norm.add(sum, x[j]);
+  const float inv = norm.inverse(reduce(sum, 1, false), p.eps);
+#pragma unroll
+  for (int j = 0; j < 64; ++j) x[j] = norm.apply(x[j], inv);
+  tc_fence_after();
+  const uint32_t d1 = uniform(sh.tmem), d2 = d1 + 128;  // A, then P X; A A
+  const uint32_t mine = (uint32_t(32 * warp) << 16) + 64u * block;  // this thread's lane and block's columns
+  const uint32_t form = (1u << 4) | (8u << 24);  // D f32, A and B f16, M = 128
+  const uint32_t leader = lane == 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  constexpr u64 LO = kTileBytes >> 4, STEP = 2 * 2048 >> 4;  // lo behind hi; two column groups
+  auto run = [&](auto issue) {
+    fence_proxy_async_smem();  // the operands were written by ordinary stores
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      tc_fence_after();
+      issue();
+      tc_commit_by(done, leader);
+    }
+    // after an abort nothing is waited for, but the threads stay together (__syncthreads)
+    if (ok) ok = wait_warp(done, parity, p.status, &sh.abort_flag);
+    parity ^= 1u;
+    tc_fence_after();
+  };
+  // D = T T^T for both blocks' rows at once, the small terms first
+  auto gram = [&](uint32_t d, uint32_t tile, int ksteps) {
+    const u64 t = core_desc(tile, 2048, 128);
+    const uint32_t id = form | (16u << 17);  // N = 128
+    for (int k = 0; k < ksteps; ++k) {
+      tc_mma_f16(d, t + STEP * k, t + STEP * k + LO, id, k > 0, leader);
+      tc_mma_f16(d, t + STEP * k + LO, t + STEP * k, id, 1u, leader);
+    }
+    for (int k = 0; k < ksteps; ++k) tc_mma_f16(d, t + STEP * k, t + STEP * k, id, 1u, leader);
+  };
+  // columns 64 b .. of D = P X_b: X MN-major, 16 rows are two core matrices
+  auto times_x = [&](uint32_t d) {
+    const u64 a = core_desc(base + 4 * kTileBytes, 2048, 128);
+    const uint32_t id = form | (1u << 16) | (8u << 17);  // N = 64
+    const u64 b0 = core_desc(base, 128, 2048), b1 = core_desc(base + 1024, 128, 2048);
+    for (int k = 0; k < mt; ++k) {  // the two blocks' sums are independent: one waits while the other runs
+      tc_mma_f16(d, a + STEP * k, b0 + 16 * k + LO, id, k > 0, leader);
+      tc_mma_f16(d + 64, a + STEP * k, b1 + 16 * k + LO, id, k > 0, leader);
+      tc_mma_f16(d, a + STEP * k + LO, b0 + 16 * k, id, 1u, leader);
+      tc_mma_f16(d + 64, a + STEP * k + LO, b1 + 16 * k, id, 1u, leader);
+    }
+    for (int k = 0; k < mt; ++k) {
+      tc_mma_f16(d, a + STEP * k, b0 + 16 * k, id, 1u, leader);
+      tc_mma_f16(d + 64, a + STEP * k, b1 + 16 * k, id, 1u, leader);
+    }
+  };
+  const int r = threadIdx.x;
+  for (int step = 0; step < p.steps; ++step) {
+    store_pairs(xt, r, x, kScale);
+    run([&] { gram(d1, base, nt); });
+    float a[64];
+    tc_ld64(d1 + mine, a);
+    store_pairs(at, r, a, 1.0f / kScale);  // a is 2^20 A
+    run([&] { gram(d2, base + 2 * kTileBytes, mt); });
+    {
+      float q[64];
+      tc_ld64(d2 + mine, q);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) a[i] = fmaf(p.c, q[i], p.b * a[i]);  // 2^20 P
+    }
+    store_pairs(pt, r, a, 1.0f / kScale);
+    run([&] { times_x(d1); });
+    tc_ld64(d1 + mine, a);
+#pragma unroll
+    for (int i = 0; i < 64; ++i) x[i] = fmaf(a[i], kUnscale2, p.a * x[i]);
+  }
+  if (live) {
+    float* o = p.out + s.val + row * si;
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+      if (j < n) o[j * sj] = x[j];
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (sh.abort_flag) {  // a wait gave up: its MMAs may still run; give them time before the memory goes
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  tc_fence_after();
+  if (warp == 0) tc_dealloc(sh.tmem, 256);
 }
 
 void free_ortho(vbsr_ortho* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
   cudaFree(p->slots);
+  cudaFree(p->d_status);
   delete p;
 }
 
 vbsr_status build_ortho(vbsr_ortho* p) {
   const MatrixData& d = p->m->d;
-  VBSR_CUDA(cudaFuncSetAttribute(ortho_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrthoSmem));
+  VBSR_CUDA(cudaFuncSetAttribute(ortho_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem));
+  VBSR_CUDA(cudaFuncSetAttribute(ortho_big_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBigSmem));
   std::vector<OrthoSlot> by_class[5][5];
   for (int i = 0; i < d.block_rows; ++i) {
     int64_t val = d.h_val_off_row[i];
@@ -298,18 +511,24 @@ vbsr_status build_ortho(vbsr_ortho* p) {
   }
   // the largest first
   std::vector<OrthoSlot> slots;
-  for (int mt = 4; mt >= 1; --mt)
-    for (int nt = 4; nt >= mt; --nt) {
-      const int per = mt >= 3 ? 1 : (mt == 2 ? 2 : 4);
-      const std::vector<OrthoSlot>& v = by_class[mt][nt];
-      for (size_t i = 0; i < v.size(); i += per)
-        for (int k = 0; k < 4; ++k) {
-          const bool have = k < per && i + k < v.size();
-          slots.push_back(have ? v[i + k] : OrthoSlot{-1, v[i].shape, 0});
-        }
-    }
-  p->ctas = int(slots.size() / 4);
+  auto pack = [&](const std::vector<OrthoSlot>& v, int per) {
+    for (size_t i = 0; i < v.size(); i += per)
+      for (int k = 0; k < 4; ++k) {
+        const bool have = k < per && i + k < v.size();
+        slots.push_back(have ? v[i + k] : OrthoSlot{-1, v[i].shape, 0});
+      }
+  };
+  std::vector<OrthoSlot> big;
+  for (int mt = 4; mt >= 3; --mt)
+    for (int nt = 4; nt >= mt; --nt) big.insert(big.end(), by_class[mt][nt].begin(), by_class[mt][nt].end());
+  pack(big, 2);
+  p->big_ctas = int(slots.size() / 4);
+  for (int mt = 2; mt >= 1; --mt)
+    for (int nt = 4; nt >= mt; --nt) pack(by_class[mt][nt], mt == 2 ? 2 : 4);
+  p->small_ctas = int(slots.size() / 4) - p->big_ctas;
   VBSR_CUDA(upload_array(&p->slots, slots));
+  VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
+  VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
   return VBSR_OK;
 }
 
@@ -356,14 +575,33 @@ vbsr_status vbsr_ortho_execute(const vbsr_ortho* p, const float* values, float* 
   if (!(eps >= 0.0f) || std::isinf(eps))
     return set_error(VBSR_INVALID_ARGUMENT, "eps must be finite and not negative");
   if (coefficients == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null coefficients");
-  if (p->ctas == 0) return VBSR_OK;
+  if (p->big_ctas + p->small_ctas == 0) return VBSR_OK;
   if (values == nullptr || out == nullptr)
     return set_error(VBSR_INVALID_ARGUMENT, "null values or out");
   DeviceGuard guard(p->device);
-  const OrthoParams k{p->slots, values, out, steps, eps, coefficients[0], coefficients[1], coefficients[2]};
-  ortho_kernel<<<unsigned(p->ctas), 128, kOrthoSmem, reinterpret_cast<cudaStream_t>(stream)>>>(k);
-  VBSR_CUDA(cudaGetLastError());
+  OrthoParams k{p->slots, values, out, steps, eps, coefficients[0], coefficients[1], coefficients[2], p->d_status};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p->big_ctas > 0) {
+    ortho_big_kernel<<<unsigned(p->big_ctas), 128, kBigSmem, st>>>(k);
+    VBSR_CUDA(cudaGetLastError());
+  }
+  if (p->small_ctas > 0) {
+    k.slots += 4ll * p->big_ctas;
+    if (p->big_ctas > 0) {
+      VBSR_CUDA(launch_after(ortho_small_kernel, dim3(unsigned(p->small_ctas)), 128, kSmallSmem, st, k));
+    } else {
+      ortho_small_kernel<<<unsigned(p->small_ctas), 128, kSmallSmem, st>>>(k);
+      VBSR_CUDA(cudaGetLastError());
+    }
+  }
   return VBSR_OK;
+}
+
+vbsr_status vbsr_ortho_check_status(const vbsr_ortho* p, vbsr_stream_t stream) {
+  clear_error();
+  if (p == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null plan");
+  DeviceGuard guard(p->device);
+  return read_status(p->d_status, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
