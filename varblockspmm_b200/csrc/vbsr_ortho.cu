@@ -6,10 +6,12 @@
 // stays on chip from its one read to its one write, so global memory sees 8 bytes per value and the
 // rest is tensor-core work, 4 m m n + 2 m^3 operations a step.
 //
-// Precision. Products are formed from fp16 pairs: x 2^10 = hi + lo, both fp16, so an operand is held
-// to 2^-23 of itself or 2^-35 absolutely, and a product is hi lo + lo hi + hi hi in one fp32
-// accumulator (lo lo is below 2^-22 of it). The iterates of a convergent iteration have entries of at
-// most about one, and P of about 11; 2^10 leaves room up to 64. X itself is carried in fp32 registers.
+// Precision. Products are formed from fp16 pairs: X 2^5, A 2^10 and P 2^10 are hi + lo, both fp16, so an
+// operand is held to 2^-23 of itself or 2^-30 (X) and 2^-35 (A, P) absolutely, and a product is
+// hi lo + lo hi + hi hi in one fp32 accumulator (lo lo is below 2^-22 of it). With these powers of two a
+// product comes out in the scale of the next operand: (2^5 X)(2^5 X)^T = 2^10 A. The iterates of a
+// convergent iteration have entries of at most about one, and P of about 11; the scales leave room up to
+// 2^11 in X and 64 in P. X itself is carried, as 2^5 X, in fp32 registers.
 //
 // Two forms, by the block's shorter side m.
 //
@@ -21,7 +23,7 @@
 //
 // m > 32, tcgen05: four warps own two blocks, one above the other, a thread one row of X. Operands are core
 // matrices in shared memory, written once per product as pairs; X serves K-major as both operands of X X^T
-// and MN-major as the second of P X. A and A A stay in TMEM, where the threads read their rows. An MMA has
+// and MN-major as the second of P X. A product is read from TMEM, a row per thread. An MMA has
 // M = 128, both blocks' rows, against the columns of both (X X^T, A A; the mixed quarters are not used) or
 // one after the other (P X): with M = 64 the tensor core does the same work, but the accumulator fills
 // 16 lanes of 32, and the conversions, which bound it, took twice the instructions (measured 1353 us for
@@ -55,7 +57,8 @@ struct vbsr_ortho {
 
 namespace {
 
-constexpr float kScale = 1024.0f, kUnscale2 = 1.0f / (1024.0f * 1024.0f);
+constexpr float kScale = 32.0f;                // of X
+constexpr float kSquare = 1.0f / 1024.0f;      // (2^10 A)(2^10 A) to 2^10 A A; (2^10 P)(2^5 X) to 2^5 P X
 
 // Barrier of the MT warps of a block, the CTA's `group`-th.
 template <int MT>
@@ -87,10 +90,8 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 
-// Two neighbouring values times s as packed fp16 hi and lo.
-__device__ __forceinline__ void pair2(float x, float y, float s, uint32_t& hi, uint32_t& lo) {
-  x *= s;
-  y *= s;
+// Two neighbouring values as packed fp16 hi and lo.
+__device__ __forceinline__ void pair2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
   const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
@@ -112,10 +113,10 @@ struct Norm {
     const float y = v * down;
     return fmaf(y, y, sum);
   }
-  // 1 / (|V| + eps) times 2^e, 0 for a block of zeros without eps
+  // kScale / (|V| + eps) times 2^e, 0 for a block of zeros without eps
   __device__ __forceinline__ float inverse(float sum, float eps) const {
     const float norm = sqrtf(sum) + eps * down;
-    return norm == 0.0f ? 0.0f : 1.0f / norm;
+    return norm == 0.0f ? 0.0f : kScale / norm;
   }
   __device__ __forceinline__ float apply(float v, float inv) const { return v * down * inv; }
 };
@@ -124,11 +125,11 @@ struct Norm {
 template <int T>
 struct StripPair {
   uint32_t hi[T / 2][4], lo[T / 2][4];
-  __device__ __forceinline__ void set(const float (&x)[T][4], float s) {
+  __device__ __forceinline__ void set(const float (&x)[T][4]) {
 #pragma unroll
     for (int j = 0; j < T; ++j) {
-      pair2(x[j][0], x[j][1], s, hi[j / 2][(j & 1) * 2], lo[j / 2][(j & 1) * 2]);
-      pair2(x[j][2], x[j][3], s, hi[j / 2][(j & 1) * 2 + 1], lo[j / 2][(j & 1) * 2 + 1]);
+      pair2(x[j][0], x[j][1], hi[j / 2][(j & 1) * 2], lo[j / 2][(j & 1) * 2]);
+      pair2(x[j][2], x[j][3], hi[j / 2][(j & 1) * 2 + 1], lo[j / 2][(j & 1) * 2 + 1]);
     }
   }
   // rows [16 strip, + 16) of a row-major matrix of row stride LD halves, lo behind hi at `lo_off` bytes
@@ -199,8 +200,8 @@ struct OrthoSmem {
 };
 constexpr int kMax2(int a, int b) { return a > b ? a : b; }
 constexpr int kSmallSmem = kMax2(2 * OrthoSmem<2, 4>::bytes, 4 * OrthoSmem<1, 4>::bytes);
-// m > 32: X, A and P of two blocks as pairs, 128 x 64 each.
-constexpr int kTileBytes = 128 * 64 * 2, kBigSmem = 6 * kTileBytes + 1024;
+// m > 32: X, and A or P, of two blocks as pairs, 128 x 64 each.
+constexpr int kTileBytes = 128 * 64 * 2, kBigSmem = 4 * kTileBytes + 1024;
 
 template <int MT, int NT>
 __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoSlot& s, char* sm, int group,
@@ -252,27 +253,27 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
     float acc[2 * MT][4], sq[2 * MT][4];
     {
       StripPair<2 * NT> xp;
-      xp.set(x, kScale);
+      xp.set(x);
       xp.template store<S::LDX>(xs, S::x_lo, strip, lane);
       strip_sync<MT>(group);
       strip_product<2 * MT, NT, S::LDX, false>(acc, xp, smem_addr(xs), S::x_lo, lane);
     }
     StripPair<2 * MT> ap;
-    ap.set(acc, 1.0f / kScale);  // acc is 2^20 A
+    ap.set(acc);
     ap.template store<S::LDA>(sm + S::a_at, S::a_lo, strip, lane);
     strip_sync<MT>(group);
     strip_product<2 * MT, MT, S::LDA, false>(sq, ap, smem_addr(sm + S::a_at), S::a_lo, lane);
 #pragma unroll
     for (int j = 0; j < 2 * MT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq[j][i] = fmaf(p.c, sq[j][i], p.b * acc[j][i]);  // 2^20 P
-    ap.set(sq, 1.0f / kScale);
+      for (int i = 0; i < 4; ++i) sq[j][i] = fmaf(p.c * kSquare, sq[j][i], p.b * acc[j][i]);
+    ap.set(sq);
     float px[2 * NT][4];
     strip_product<2 * NT, MT, S::LDX, true>(px, ap, smem_addr(xs), S::x_lo, lane);
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[j][i] = fmaf(px[j][i], kUnscale2, p.a * x[j][i]);
+      for (int i = 0; i < 4; ++i) x[j][i] = fmaf(px[j][i], kSquare, p.a * x[j][i]);
   }
 
 #pragma unroll
@@ -280,7 +281,7 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * strip + g + 8 * (i >> 1), col = 8 * j + 2 * t + (i & 1);
-      if (row < m && col < n) p.out[s.val + row * si + col * sj] = x[j][i];
+      if (row < m && col < n) p.out[s.val + row * si + col * sj] = x[j][i] * (1.0f / kScale);
     }
 }
 
@@ -319,15 +320,15 @@ struct OrthoTcShared {
   float red[2][4];
 };
 
-// A row's 64 values, times s, as pairs into an operand.
-__device__ __forceinline__ void store_pairs(char* tile, int row, const float (&v)[64], float s) {
+// A row's 64 values as pairs into an operand.
+__device__ __forceinline__ void store_pairs(char* tile, int row, const float (&v)[64]) {
 #pragma unroll
   for (int g = 0; g < 8; ++g) {
     uint4 hi, lo;
-    pair2(v[8 * g], v[8 * g + 1], s, hi.x, lo.x);
-    pair2(v[8 * g + 2], v[8 * g + 3], s, hi.y, lo.y);
-    pair2(v[8 * g + 4], v[8 * g + 5], s, hi.z, lo.z);
-    pair2(v[8 * g + 6], v[8 * g + 7], s, hi.w, lo.w);
+    pair2(v[8 * g], v[8 * g + 1], hi.x, lo.x);
+    pair2(v[8 * g + 2], v[8 * g + 3], hi.y, lo.y);
+    pair2(v[8 * g + 4], v[8 * g + 5], hi.z, lo.z);
+    pair2(v[8 * g + 6], v[8 * g + 7], hi.w, lo.w);
     char* o = tile + 2048 * g + 16 * row;
     *reinterpret_cast<uint4*>(o) = hi;
     *reinterpret_cast<uint4*>(o + kTileBytes) = lo;
@@ -348,7 +349,7 @@ __device__ __forceinline__ void tc_ld64(uint32_t a, float (&v)[64]) {
   }
 }
 
-__global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
+__global__ void __launch_bounds__(128, 3) ortho_big_kernel(OrthoParams p) {
   extern __shared__ char sm[];
   __shared__ OrthoTcShared sh;
   griddep_launch_dependents();
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
   const int nt = max(int(slots[0].shape >> 24), int(slots[1].shape >> 24));
   const uint32_t base = (smem_addr(sm) + 1023u) & ~1023u;
   char* xt = sm + (base - smem_addr(sm));
-  char *at = xt + 2 * kTileBytes, *pt = xt + 4 * kTileBytes;
+  char* at = xt + 2 * kTileBytes;  // A, then P
   const uint32_t done = smem_addr(&sh.done);
   if (threadIdx.x == 0) {
     mbar_init(done, 1);
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
     mbar_fence_init();
   }
   if (warp == 0) {
-    tc_alloc(smem_addr(&sh.tmem), 256);
+    tc_alloc(smem_addr(&sh.tmem), 128);
     tc_relinquish();
   }
   tc_fence_before();
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
 #pragma unroll
   for (int j = 0; j < 64; ++j) x[j] = norm.apply(x[j], inv);
   tc_fence_after();
-  const uint32_t d1 = uniform(sh.tmem), d2 = d1 + 128;  // A, then P X; A A
+  const uint32_t d = uniform(sh.tmem);  // A, then A A, then P X
   const uint32_t mine = (uint32_t(32 * warp) << 16) + 64u * block;  // this thread's lane and block's columns
   const uint32_t form = (1u << 4) | (8u << 24);  // D f32, A and B f16, M = 128
   const uint32_t leader = lane == 0;
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
     tc_fence_after();
   };
   // D = T T^T for both blocks' rows at once, the small terms first
-  auto gram = [&](uint32_t d, uint32_t tile, int ksteps) {
+  auto gram = [&](uint32_t tile, int ksteps) {
     const u64 t = core_desc(tile, 2048, 128);
     const uint32_t id = form | (16u << 17);  // N = 128
     for (int k = 0; k < ksteps; ++k) {
@@ -434,8 +435,8 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
     for (int k = 0; k < ksteps; ++k) tc_mma_f16(d, t + STEP * k, t + STEP * k, id, 1u, leader);
   };
   // columns 64 b .. of D = P X_b: X MN-major, 16 rows are two core matrices
-  auto times_x = [&](uint32_t d) {
-    const u64 a = core_desc(base + 4 * kTileBytes, 2048, 128);
+  auto times_x = [&]() {
+    const u64 a = core_desc(base + 2 * kTileBytes, 2048, 128);
     const uint32_t id = form | (1u << 16) | (8u << 17);  // N = 64
     const u64 b0 = core_desc(base, 128, 2048), b1 = core_desc(base + 1024, 128, 2048);
     for (int k = 0; k < mt; ++k) {  // the two blocks' sums are independent: one waits while the other runs
@@ -451,29 +452,34 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
   };
   const int r = threadIdx.x;
   for (int step = 0; step < p.steps; ++step) {
-    store_pairs(xt, r, x, kScale);
-    run([&] { gram(d1, base, nt); });
+    store_pairs(xt, r, x);
+    run([&] { gram(base, nt); });
     float a[64];
-    tc_ld64(d1 + mine, a);
-    store_pairs(at, r, a, 1.0f / kScale);  // a is 2^20 A
-    run([&] { gram(d2, base + 2 * kTileBytes, mt); });
-    {
-      float q[64];
-      tc_ld64(d2 + mine, q);
+    tc_ld64(d + mine, a);
+    store_pairs(at, r, a);
+    run([&] { gram(base + 2 * kTileBytes, mt); });
 #pragma unroll
-      for (int i = 0; i < 64; ++i) a[i] = fmaf(p.c, q[i], p.b * a[i]);  // 2^20 P
+    for (int i = 0; i < 64; i += 16) {
+      float q[16];
+      tc_ld16(d + mine + i, q);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) a[i + j] = fmaf(p.c * kSquare, q[j], p.b * a[i + j]);
     }
-    store_pairs(pt, r, a, 1.0f / kScale);
-    run([&] { times_x(d1); });
-    tc_ld64(d1 + mine, a);
+    store_pairs(at, r, a);
+    run([&] { times_x(); });
 #pragma unroll
-    for (int i = 0; i < 64; ++i) x[i] = fmaf(a[i], kUnscale2, p.a * x[i]);
+    for (int i = 0; i < 64; i += 16) {
+      float q[16];
+      tc_ld16(d + mine + i, q);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[i + j] = fmaf(q[j], kSquare, p.a * x[i + j]);
+    }
   }
   if (live) {
     float* o = p.out + s.val + row * si;
 #pragma unroll
     for (int j = 0; j < 64; ++j)
-      if (j < n) o[j * sj] = x[j];
+      if (j < n) o[j * sj] = x[j] * (1.0f / kScale);
   }
   tc_fence_before();
   __syncthreads();
@@ -483,7 +489,7 @@ __global__ void __launch_bounds__(128, 2) ortho_big_kernel(OrthoParams p) {
     __syncthreads();
   }
   tc_fence_after();
-  if (warp == 0) tc_dealloc(sh.tmem, 256);
+  if (warp == 0) tc_dealloc(sh.tmem, 128);
 }
 
 void free_ortho(vbsr_ortho* p) {
