@@ -189,12 +189,12 @@ struct OrthoParams {
   int* status;
 };
 
-// Shared memory of a block of MT x NT 16-tiles: two buffers of X and one of A, each hi and lo.
+// Shared memory of a block of MT x NT 16-tiles: X and A, each hi and lo.
 template <int MT, int NT>
 struct OrthoSmem {
   static constexpr int LDX = 16 * NT + 8, LDA = 16 * MT + 8;
   static constexpr int x_lo = 16 * MT * LDX * 2, x_bytes = 2 * x_lo;
-  static constexpr int a_lo = 16 * MT * LDA * 2, a_at = 2 * x_bytes;
+  static constexpr int a_lo = 16 * MT * LDA * 2, a_at = x_bytes;
   static constexpr int red_at = a_at + 2 * a_lo;
   static constexpr int bytes = red_at + 2 * 16;
 };
@@ -249,7 +249,8 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
     for (int i = 0; i < 4; ++i) x[j][i] = norm.apply(x[j][i], inv);
 
   for (int step = 0; step < p.steps; ++step) {
-    char* xs = sm + (step & 1) * S::x_bytes;  // the other buffer may still be read by another warp
+    strip_sync<MT>(group);  // X may still be read by another warp
+    char* xs = sm;
     float acc[2 * MT][4], sq[2 * MT][4];
     {
       StripPair<2 * NT> xp;
