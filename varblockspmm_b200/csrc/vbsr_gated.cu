@@ -18,9 +18,20 @@ namespace vbsr_b200 {
 
 static __global__ void __launch_bounds__(256) values_amax_kernel(const float* a, long long na, const float* b,
                                                           long long nb, float* partial) {
+  griddep_launch_dependents();
+  // both lengths are multiples of 64
   float m = 0.0f;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < na + nb; i += gridDim.x * 256ll)
-    m = fmaxf(m, finite_abs(i < na ? a[i] : b[i - na]));
+  auto scan = [&](const float* v, long long n) {
+    const int vec = (reinterpret_cast<uintptr_t>(v) & 15u) == 0;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n / 8; i += gridDim.x * 256ll) {
+      float x[8];
+      load8(v + 8 * i, vec, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(x[k]));
+    }
+  };
+  scan(a, na);
+  scan(b, nb);
   m = cta_max(m);
   if (threadIdx.x == 0) partial[blockIdx.x] = m;
 }
@@ -55,6 +66,8 @@ template <bool DEVICE>
 __global__ void __launch_bounds__(256) pack_kernel(const PackRow* rows, const float* gate, const float* up,
                                                    long long up_byte, const float* partial, int count,
                                                    char* out, int* exponent) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int e = partial_exponent(partial, count);
   if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
   const PackRow r = rows[blockIdx.x];
@@ -91,20 +104,28 @@ namespace {
 // Geometry of a call's panels.
 struct Panels {
   int R = 0;        // tokens per tile
+  int x_rows = 0;   // tokens per tile of the activations: R, or R / 2 (what a weight-gradient stage takes)
   int64_t tiles = 0;
   int64_t x_at = 0, dy_at = 0, bytes = 0;
 };
 constexpr int64_t kPartialBytes = 4 * kAmaxCtas + (256 - 4 * kAmaxCtas % 256) % 256;
 
-// Tiles of at most 128 tokens, evenly sized; multiples of 16 where the tokens are summed over (K = 16).
-// In the forward direction any number goes: an MMA's rows behind the last token hold other bytes, and
-// a row's result depends on that row alone.
+// Tiles of at most 128 tokens, evenly sized. In the forward direction any number goes: an MMA's rows behind
+// the last token hold other bytes, and a row's result depends on that row alone. In the backward direction
+// tokens are summed over, in stages of at most kGradTokens, a multiple of 16 (K = 16): a tile is one or two
+// stages.
 Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
   Panels g;
   if (tokens == 0) return g;
-  const int64_t step = backward ? 16 : 1;
   g.tiles = (tokens + 127) / 128;
-  g.R = int(((tokens + g.tiles - 1) / g.tiles + step - 1) / step * step);
+  if (backward) {
+    const int64_t stages = tokens <= kGradTokens ? 1 : 2 * g.tiles;
+    g.x_rows = int(((tokens + stages - 1) / stages + 15) / 16 * 16);
+    g.R = int(stages / g.tiles) * g.x_rows;
+    g.tiles = (tokens + g.R - 1) / g.R;
+  } else {
+    g.R = g.x_rows = int((tokens + g.tiles - 1) / g.tiles);
+  }
   g.x_at = 2 * kPartialBytes + 256;  // largest magnitudes of both panels, exponents
   g.dy_at = g.x_at + align256(g.tiles * g.R * (p->K / 8) * 32);
   g.bytes = backward ? g.dy_at + align256(g.tiles * g.R * (p->M / 4) * 32) : g.dy_at;
@@ -116,6 +137,7 @@ PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char*
   k.entries = p->entries;
   k.group_col = p->group_col;
   k.R = g.R;
+  k.x_rows = g.x_rows;
   k.act = p->act;
   k.tokens = tokens;
   k.M = p->M;
@@ -129,24 +151,34 @@ PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char*
   return k;
 }
 
-// A panel in pairs: its largest magnitude, then the pairs. which: 0 the activations, 1 the gradients.
+// The job of one panel. which: 0 the activations, 1 the gradients.
 template <class Source>
-vbsr_status make_panel(const Source& src, const Panels& g, int64_t tokens, char* ws, int which,
-                       cudaStream_t s) {
-  float* partial = reinterpret_cast<float*>(ws + which * kPartialBytes);
-  int* exponent = reinterpret_cast<int*>(ws + 2 * kPartialBytes) + which;
+PanelJob<Source> job_of(const Source& src, const Panels& g, int64_t tokens, char* ws, int which) {
+  PanelJob<Source> j{src};
+  j.R = which ? g.R : g.x_rows;
+  j.tiles = int(which ? g.tiles : g.tiles * (g.R / g.x_rows));
   const int64_t groups = src.features / 8;
-  uint4* out = reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at));
-  if (groups * tokens * Source::parts <= kSmallGroups) {
-    panel_small_kernel<<<kSmallCtas, kSmallThreads, 0, s>>>(src, tokens, g.R, int(g.tiles), out, exponent);
+  j.amax_ctas = ctas_for(groups * tokens, kAmaxCtas);
+  j.pair_ctas = ctas_for(groups * g.tiles * g.R * Source::parts / 4, 148 * 7);
+  j.partial = reinterpret_cast<float*>(ws + which * kPartialBytes);
+  j.exponent = reinterpret_cast<int*>(ws + 2 * kPartialBytes) + which;
+  j.out = reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at));
+  return j;
+}
+
+// Makes one panel, or two (`both`).
+template <class A, class C>
+vbsr_status make_panels(const PanelJob<A>& a, const PanelJob<C>& c, bool both, int64_t tokens, cudaStream_t s) {
+  auto small = [&](int64_t features, int parts) { return features / 8 * tokens * parts <= kSmallGroups; };
+  if (small(a.src.features, A::parts) && (!both || small(c.src.features, C::parts))) {
+    panel_small_kernel<<<both ? 2 * kSmallCtas : kSmallCtas, kSmallThreads, 0, s>>>(a, c, tokens);
     VBSR_CUDA(cudaGetLastError());
     return VBSR_OK;
   }
-  const int n = ctas_for(groups * tokens, kAmaxCtas);
-  panel_amax_kernel<<<n, 256, 0, s>>>(src, tokens, partial);
+  panel_amax_kernel<<<a.amax_ctas + (both ? c.amax_ctas : 0), 256, 0, s>>>(a, c, tokens);
   VBSR_CUDA(cudaGetLastError());
-  VBSR_CUDA(launch_after(panel_pair_kernel<Source>, dim3(ctas_for(groups * g.tiles * g.R / 4, 148 * 7)), 256, 0, s,
-                         src, tokens, g.R, int(g.tiles), partial, n, out, exponent));
+  VBSR_CUDA(launch_after(panel_pair_kernel<A, C>, dim3(unsigned(a.pair_ctas + (both ? c.pair_ctas : 0))), 256, 0, s,
+                         a, c, tokens));
   return VBSR_OK;
 }
 
@@ -155,9 +187,9 @@ vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cuda
   const int64_t ng = p->gate->d.nvalues, nu = p->up->d.nvalues;
   const int n = ctas_for((ng + nu) / 8, kAmaxCtas);
   values_amax_kernel<<<n, 256, 0, s>>>(gate, ng, up, nu, p->w_partial);
-  pack_kernel<DEVICE><<<p->pack_rows, 256, 0, s>>>(p->pack, gate, up, p->up_byte, p->w_partial, n, p->w,
-                                                   p->w_exp);
   VBSR_CUDA(cudaGetLastError());
+  VBSR_CUDA(launch_after(pack_kernel<DEVICE>, dim3(unsigned(p->pack_rows)), 256, 0, s, p->pack, gate, up,
+                         p->up_byte, p->w_partial, n, p->w, p->w_exp));
   return VBSR_OK;
 }
 
@@ -406,7 +438,8 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   const Panels g = panels_of(p, tokens, false);
-  const vbsr_status st2 = make_panel(PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0, s);
+  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0);
+  const vbsr_status st2 = make_panels(x, x, false, tokens, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, g, tokens, ws);
   k.out0 = H;
@@ -441,7 +474,9 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
   }
   char* ws = static_cast<char*>(workspace);
   const Panels n = panels_of(p, tokens, true);
-  vbsr_status st2 = make_panel(GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1, s);
+  const auto dy = job_of(GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1);
+  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 0);
+  vbsr_status st2 = make_panels(dy, x, dgate != nullptr, tokens, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, n, tokens, ws);
   if (dB != nullptr) {
@@ -452,10 +487,9 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
     k.vec = aligned16(dB);
     st2 = launch_pair<kInputGrad>(k, n.tiles, p->num_sm, s);
     if (st2 != VBSR_OK) return st2;
+    k.beside = 1;  // the weight gradients need the panels only, which are complete
   }
   if (dgate != nullptr) {
-    st2 = make_panel(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 0, s);
-    if (st2 != VBSR_OK) return st2;
     k.grads = p->grads;
     k.units = p->grad_units;
     k.out0 = dgate;

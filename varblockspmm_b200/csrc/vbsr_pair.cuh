@@ -94,6 +94,8 @@ struct PairParams {
   const uint32_t* group_col;  // per group: scalar column / 8
   int units, tiles, tile0;    // work items are units x tiles from tile0 on (kWeightGrad: units)
   int R, act;
+  int x_rows;                 // kWeightGrad: tokens per tile of x, R or R / 2, and per stage
+  int beside;                 // kWeightGrad: may run beside the launch before it (kInputGrad)
   int ring_log, acc_log;      // slots and accumulators per pipeline
   long long tokens, M, K;
   const char* x;              // activation panel in pairs (kInt8: in 16-column chunks)
@@ -137,7 +139,7 @@ static_assert(kPairThreads == 512 && kProducerRegs + kMmaRegs + 2 * kEpilogueReg
 constexpr int kChunkSteps = 12;  // 8: error 3.0e-7, 1 token 49.8 us; 12: 4.6e-7, 42.9 us; 16: 6.1e-7, 42.3 us
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
-constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage
+constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage, at most
 // kForward, kInt8: results pass through shared memory, R rows and 2^stage_log columns (rows padded by 16
 // bytes, except rows of 32) of two matrices or one; a buffer for each of the two epilogue groups.
 constexpr int kStageBytes = 10 * 1024 + 256;
@@ -560,14 +562,13 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
   produce_end(p, sh, bars, pipe, lane);
 }
 
-// Token stages of a weight-gradient unit: kGradTokens tokens of a tile (the last of a tile fewer) of
-// the unit's 16 activation groups and h / 8 gradient groups, each group [kGradTokens of hi][of lo'].
+// Token stages of a weight-gradient unit: x_rows tokens of the unit's 16 activation groups, a copy each, and
+// of its h / 8 gradient groups, which are R tokens long, a copy for hi and one for lo'.
 __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& sh, uint32_t slots,
                                               const PairBars& bars, int warp, int lane) {
-  constexpr uint32_t GB = 32u * kGradTokens;
-  const uint32_t xb = 32u * uint32_t(p.R);
+  const uint32_t nt = uint32_t(p.x_rows), GB = 32u * nt, dyb = 32u * uint32_t(p.R);
   const uint64_t pol_x = policy_evict_last();
-  const int per_tile = (p.R + kGradTokens - 1) / kGradTokens, total = p.tiles * per_tile;
+  const int per_tile = p.R / p.x_rows, total = p.tiles * per_tile;
   UnitWin<GradUnit> win;
   win.init(p.grads, p.units, 1, lane);
   Pipe pipe(p, warp);
@@ -591,24 +592,24 @@ __device__ __forceinline__ void produce_grads(const PairParams& p, PairShared& s
     }
     const uint32_t h8 = u.h / 8;
     const bool is_x = lane < int(u.ng), is_dy = lane >= 16 && lane < 16 + int(h8);
-    const char* src0 = is_x ? p.x + (long long)col * xb : p.dy + ((long long)u.dy_group + lane - 16) * xb;
-    const long long tile_step = (is_x ? p.K >> 3 : 2 * (p.M >> 3)) * xb;
+    const char* src0 = is_x ? p.x + (long long)col * GB : p.dy + ((long long)u.dy_group + lane - 16) * dyb;
     for (int j = int((uint32_t(warp) - c0) % kPipes); j < total; j += kPipes, ++pipe.i) {
-      const int tile = j / per_tile, t0 = (j % per_tile) * kGradTokens, nt = min(kGradTokens, p.R - t0);
       if (!wait_slot(p, sh, bars, pipe)) return;
       const uint32_t slot = pipe.slot(), base = pipe.base(slots), full = bars.full + 8 * slot;
-      const uint32_t steps = uint32_t(nt) / 16;
+      const uint32_t steps = nt / 16;
       if (lane < int(steps)) {
         PairStep& out = sh.steps[slot][lane];
         out.a = core_desc(base + 256u * lane, 128u, GB);
         out.b = core_desc(base + 16u * GB + 256u * lane, 128u, GB / 2);
       }
-      announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast | group, (u.ng + h8) * 32u * uint32_t(nt), lane);
-      if (is_x || is_dy) {
-        const char* src = src0 + tile * tile_step + 16 * t0;
-        const uint32_t dst = base + lane * GB;
-        bulk_g2s(dst, src, 16u * nt, full, pol_x);
-        bulk_g2s(dst + GB / 2, src + 16 * p.R, 16u * nt, full, pol_x);
+      announce(sh, slot, full, steps | u.h << 5 | kHdrFirst | kHdrLast | group, (u.ng + h8) * GB, lane);
+      const uint32_t dst = base + lane * GB;
+      if (is_x) {
+        bulk_g2s(dst, src0 + (long long)j * (p.K >> 3) * GB, GB, full, pol_x);
+      } else if (is_dy) {
+        const char* src = src0 + (long long)(j / per_tile) * 2 * (p.M >> 3) * dyb + 16 * nt * (j % per_tile);
+        bulk_g2s(dst, src, GB / 2, full, pol_x);
+        bulk_g2s(dst + GB / 2, src + 16 * p.R, GB / 2, full, pol_x);
       }
     }
     c0 += uint32_t(total);
@@ -634,7 +635,7 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
                         (MODE == kWeightGrad || MODE == kInputGrad ? 1u << 16 : 0u) |
                         (uint32_t(m >> 4) << 24);
   const uint32_t xb16 = (MODE == kInt8 ? 1u : 2u) * uint32_t(p.R);  // panel group, in 16 bytes
-  const u64 lo = MODE == kWeightGrad ? kGradTokens : u64(p.R);  // hi to lo' tile of A, in 16 bytes
+  const u64 lo = MODE == kWeightGrad ? u64(p.x_rows) : u64(p.R);  // hi to lo' tile of A, in 16 bytes
   const uint32_t tmem = uniform(sh.tmem);
   Pipe pipe(p, int(q));
   uint32_t chunk = 0;  // of this pipeline: accumulator q + kPipes (chunk % accumulators)
@@ -818,7 +819,8 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   const int row = wide ? 32 * quad + lane : 16 * quad + lane;
   const bool in_tile = (wide || lane < 16) && (MODE == kWeightGrad || row < p.R);
   const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles, grid = int(gridDim.x);
-  griddep_wait();
+  if (MODE != kWeightGrad || !p.beside) griddep_wait();
+  if (MODE == kInputGrad) griddep_launch_dependents();
   float f1 = 1.0f, f2 = 1.0f;
   if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
   if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
@@ -858,7 +860,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       chunks[0] = int(u.w);
     } else {
       n = int(u.w);
-      chunks[0] = p.tiles * ((p.R + kGradTokens - 1) / kGradTokens);
+      chunks[0] = p.tiles * (p.R / p.x_rows);
     }
     if ((k & 1) != e) {
       use += uint32_t(chunks[0] + chunks[1]);
@@ -987,7 +989,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
 
   if (warp < kPipes) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    griddep_wait();
+    if (MODE != kWeightGrad || !p.beside) griddep_wait();
     if constexpr (by_rows(MODE))
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)
@@ -1013,6 +1015,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
   }
   tc_fence_after();
   if (warp == kPipes) tc_dealloc(sh.tmem, 512);
+  if (MODE == kWeightGrad && p.beside) griddep_wait();  // the launch beside it is done when this one is
 }
 
 }  // namespace vbsr_b200

@@ -198,28 +198,35 @@ __device__ __forceinline__ void write_pairs(const Source& src, long long tokens,
   }
 }
 
+// One panel to make: tiles of R tokens, largest magnitudes, pairs and exponent.
 template <class Source>
-__global__ void __launch_bounds__(256) panel_amax_kernel(Source src, long long tokens, float* partial) {
-  griddep_launch_dependents();
-  const float m = cta_max(largest(src, tokens, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll));
-  if (threadIdx.x == 0) partial[blockIdx.x] = m;
-}
+struct PanelJob {
+  Source src;
+  int R, tiles;
+  int amax_ctas, pair_ctas;
+  float* partial;
+  uint4* out;
+  int* exponent;
+};
 
 template <class Source>
-__global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long tokens, int R, int tiles,
-                                                         const float* partial, int count, uint4* out,
-                                                         int* exponent) {
-  // a block of TT tokens (a power of two) x GG groups goes through shared memory: read along the features,
-  // written along the tokens, whole lines both ways
-  constexpr int P = Source::parts, UNITS = 1024 / P;
-  __shared__ uint4 hi[P][UNITS], lo[P][UNITS];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int e = partial_exponent(partial, count);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
+__device__ __forceinline__ void panel_amax(const PanelJob<Source>& j, long long tokens, int cta) {
+  const float m = cta_max(largest(j.src, tokens, cta * 256ll + threadIdx.x, j.amax_ctas * 256ll));
+  if (threadIdx.x == 0) j.partial[cta] = m;
+}
+
+// A block of TT tokens (a power of two) x GG groups at a time goes through shared memory: read along the
+// features, written along the tokens, whole lines both ways.
+constexpr int kPanelUnits = 1024;  // 8-value pieces of all parts
+template <class Source>
+__device__ __forceinline__ void panel_pairs(const PanelJob<Source>& j, long long tokens, int cta,
+                                            uint4 (&buf)[2 * kPanelUnits]) {
+  constexpr int P = Source::parts, UNITS = kPanelUnits / P;
+  const int e = partial_exponent(j.partial, j.amax_ctas), R = j.R;
+  if (cta == 0 && threadIdx.x == 0) *j.exponent = e;
   const float s = pow2(e);
-  const PanelBlocks b(R, tiles, src.features >> 3, UNITS);
-  for (long long item = blockIdx.x; item < b.items; item += gridDim.x) {
+  const PanelBlocks b(R, j.tiles, j.src.features >> 3, UNITS);
+  for (long long item = cta; item < b.items; item += j.pair_ctas) {
     const PanelBlocks::Place at = b.place(item);
     __syncthreads();
 #pragma unroll
@@ -227,9 +234,12 @@ __global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long t
       const int u = threadIdx.x + 256 * k, t = u >> b.gg_log, g = u & (b.gg - 1);
       const long long token = at.tile * R + at.r + t;
       float v[P][8] = {};
-      if (at.r + t < R && token < tokens && at.g + g < b.groups) src.load(token * b.groups + at.g + g, v);
+      if (at.r + t < R && token < tokens && at.g + g < b.groups) j.src.load(token * b.groups + at.g + g, v);
 #pragma unroll
-      for (int q = 0; q < P; ++q) to_pair8(v[q], s, hi[q][b.slot(t, g)], lo[q][b.slot(t, g)]);
+      for (int q = 0; q < P; ++q) {
+        uint4* place = buf + 2 * q * UNITS + b.slot(t, g);
+        to_pair8(v[q], s, place[0], place[UNITS]);
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -238,36 +248,61 @@ __global__ void __launch_bounds__(256) panel_pair_kernel(Source src, long long t
       if (at.r + t >= R || at.g + g >= b.groups) continue;
 #pragma unroll
       for (int q = 0; q < P; ++q) {
-        uint4* o = out + ((at.tile * P + q) * b.groups + at.g + g) * 2 * R + at.r + t;
-        o[0] = hi[q][b.slot(t, g)];
-        o[R] = lo[q][b.slot(t, g)];
+        const uint4* place = buf + 2 * q * UNITS + b.slot(t, g);
+        uint4* o = j.out + ((at.tile * P + q) * b.groups + at.g + g) * 2 * R + at.r + t;
+        o[0] = place[0];
+        o[R] = place[UNITS];
       }
     }
   }
 }
 
-// Both in one launch for a small panel: one cluster of kSmallCtas CTAs, which exchange their largest
-// magnitudes through distributed shared memory and read their values a second time from the caches. Against
-// the two kernels it saves a launch; above kSmallGroups 8-value groups its few SMs cost more than that.
+// One panel, or two at once (the CTAs behind the first's), in two launches: largest magnitudes, then pairs.
+template <class A, class C>
+__global__ void __launch_bounds__(256) panel_amax_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
+  griddep_launch_dependents();
+  const int cta = blockIdx.x;
+  if (cta < a.amax_ctas) panel_amax(a, tokens, cta);
+  else panel_amax(c, tokens, cta - a.amax_ctas);
+}
+template <class A, class C>
+__global__ void __launch_bounds__(256) panel_pair_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
+  __shared__ uint4 buf[2 * kPanelUnits];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int cta = blockIdx.x;
+  if (cta < a.pair_ctas) panel_pairs(a, tokens, cta, buf);
+  else panel_pairs(c, tokens, cta - a.pair_ctas, buf);
+}
+
+// Small panels in one launch: a cluster of kSmallCtas CTAs for each, which exchange their largest magnitudes
+// through distributed shared memory and read their values a second time from the caches. Against the two
+// kernels it saves a launch; above kSmallGroups 8-value groups its few SMs cost more than that.
 constexpr int kSmallCtas = 8, kSmallThreads = 512;
 constexpr int64_t kSmallGroups = 32768;
 template <class Source>
-__global__ void __cluster_dims__(kSmallCtas) __launch_bounds__(kSmallThreads)
-    panel_small_kernel(Source src, long long tokens, int R, int tiles, uint4* out, int* exponent) {
-  __shared__ float maxima[kSmallCtas];
-  griddep_launch_dependents();
+__device__ __forceinline__ void panel_small(const PanelJob<Source>& j, long long tokens, float* maxima) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  const long long first = blockIdx.x * (long long)kSmallThreads + threadIdx.x;
+  const int cta = int(blockIdx.x % kSmallCtas);
+  const long long first = cta * (long long)kSmallThreads + threadIdx.x;
   const long long step = (long long)kSmallCtas * kSmallThreads;
-  float m = cta_max(largest(src, tokens, first, step));
-  if (threadIdx.x < kSmallCtas) *cluster.map_shared_rank(&maxima[blockIdx.x], threadIdx.x) = m;
+  float m = cta_max(largest(j.src, tokens, first, step));
+  if (threadIdx.x < kSmallCtas) *cluster.map_shared_rank(&maxima[cta], threadIdx.x) = m;
   cluster.sync();
 #pragma unroll
   for (int i = 0; i < kSmallCtas; ++i) m = fmaxf(m, maxima[i]);
   const int e = pair_exponent(m);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *exponent = e;
-  write_pairs(src, tokens, R, tiles, pow2(e), out, first, step);
+  if (cta == 0 && threadIdx.x == 0) *j.exponent = e;
+  write_pairs(j.src, tokens, j.R, j.tiles, pow2(e), j.out, first, step);
+}
+template <class A, class C>
+__global__ void __cluster_dims__(kSmallCtas) __launch_bounds__(kSmallThreads)
+    panel_small_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
+  __shared__ float maxima[kSmallCtas];
+  griddep_launch_dependents();
+  if (blockIdx.x < kSmallCtas) panel_small(a, tokens, maxima);
+  else panel_small(c, tokens, maxima);
 }
 
 }  // namespace vbsr_b200
