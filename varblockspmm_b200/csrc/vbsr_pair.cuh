@@ -142,7 +142,8 @@ constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's o
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage, at most
 // kForward, kInt8: results pass through shared memory, R rows and 2^stage_log columns (rows padded by 16
 // bytes, except rows of 32) of two matrices or one; a buffer for each of the two epilogue groups.
-constexpr int kStageBytes = 10 * 1024 + 256;
+constexpr int kScaleAhead = 3, kScaleBytes = 4 * 256;  // kInt8: ring of row scales, behind the rows
+constexpr int kStageBytes = 10 * 1024 + 256 + kScaleBytes;
 __host__ __device__ constexpr int stage_log(int mode, int R) {
   return (R <= 16 ? 6 : (R <= 32 ? 5 : (R <= 64 ? 4 : 3))) + (mode == kInt8 && R > 16 ? 1 : 0);
 }
@@ -647,6 +648,7 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     if (steps == 0) break;
     // the list, one step to a lane
     const PairStep list = sh.steps[slot][lane & (kMaxSteps - 1)];
+    const u64 a0 = uniform(list.a), b0 = uniform(list.b);
     const uint32_t acc_no = acc_of(p, q, chunk), d = tmem + acc_no * acc_cols(p);
     if (hdr & kHdrFirst)
       if (!wait_warp(bars.acc_empty + 8 * acc_no, ((chunk >> p.acc_log) & 1u) ^ 1u, p.status, &sh.abort_flag))
@@ -661,7 +663,7 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
     if constexpr (MODE == kForward || MODE == kInt8) {
       const u64 da = 2u * xb16, db = (MODE == kInt8 ? 2u : 4u) * uint32_t(n);  // two groups, in 16 bytes
       const int even = steps - ((hdr & kHdrOdd) ? 1 : 0);
-      u64 a = uniform(list.a), b = uniform(list.b);
+      u64 a = a0, b = b0;
       auto step = [&](u64 a1, u64 a2, u64 b1) {
         if (MODE == kInt8) {
           tc_mma_i8(d, a1, b1, i1, acc, leader);
@@ -686,7 +688,7 @@ __device__ void issue_mmas(const PairParams& p, PairShared& sh, const PairBars& 
         acc = 1u;
       };
       if constexpr (MODE == kWeightGrad) {  // 16 tokens are two core matrices, 256 bytes, further in both
-        u64 a = uniform(list.a), b = uniform(list.b);
+        u64 a = a0, b = b0;
         for (int s = 0; s < steps; ++s, a += 16, b += 16) step(a, a + lo, b);
       } else {
         for (int s = 0; s < steps; ++s) {
@@ -748,9 +750,10 @@ __device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t
 template <int MODE>
 __device__ __forceinline__ void write_staged(const PairParams& p, const float* st, const float* st_up, int ld,
                                              int step, int sc, int sr, int rows, long long o, float f1, float f2,
-                                             const float (&rs)[4], float ts, long long t0) {
+                                             const float* rs, const float* tokens) {
   // o: place of (row 0, column sc) in the output
-  auto finish = [&](int r, long long at, float (&v)[4], float (&w)[4]) {
+  // tokens: the tile's token scales (few, and read again by every unit: they stay in L1)
+  auto finish = [&](long long at, float (&v)[4], float (&w)[4], float ts) {
     float hv[4];
     if constexpr (MODE == kForward) {
       with_act(p.act, [&](auto kind) {
@@ -766,9 +769,8 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
         store4(p.out2 + at, w, p.vec);
       }
     } else {
-      const float s = r == sr ? ts : __ldg(p.token_scale + t0 + r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) hv[i] = float(__float_as_int(v[i])) * (s * rs[i]);
+      for (int i = 0; i < 4; ++i) hv[i] = float(__float_as_int(v[i])) * (ts * rs[i]);
     }
     store4(p.out0 + at, hv, p.vec);
   };
@@ -786,12 +788,16 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
   const long long hop = step * p.M;
   o += sr * p.M;
   for (int r = sr; r < rows; r += 2 * step, o += 2 * hop) {
-    float v[2][4], w[2][4];
+    float v[2][4], w[2][4], ts[2] = {};
     const bool two = r + step < rows;
+    if constexpr (MODE == kInt8) {
+      ts[0] = __ldg(tokens + r);
+      ts[1] = __ldg(tokens + (two ? r + step : r));
+    }
     load(r, v[0], w[0]);
     load(two ? r + step : r, v[1], w[1]);
-    finish(r, o, v[0], w[0]);
-    if (two) finish(r + step, o + hop, v[1], w[1]);
+    finish(o, v[0], w[0], ts[0]);
+    if (two) finish(o + hop, v[1], w[1], ts[1]);
   }
 }
 
@@ -833,16 +839,35 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   // the units of the next 32 items in the lanes' registers, and the 32 after them on their way
   TileWalk walk(tiles);
   uint4 heads, heads2;
+  int head0 = 0;
   auto fetch = [&](int k) {
     const long long item = blockIdx.x + (long long)(k + lane) * grid;
     return item < items ? unit_head<MODE>(p, int(item) / tiles) : make_uint4(0, 0, 0, 0);
   };
   heads = fetch(0);
   heads2 = fetch(32);
+  // kInt8: row scales come through a ring in shared memory, kScaleAhead of the group's items ahead: a load of
+  // the epilogue waits behind the bulk copies in flight, longer than a small item takes
+  float* row_scales = stage + (kStageBytes - kScaleBytes) / 4;
+  auto fetch_scales = [&](int k) {  // of the CTA's item k
+    if constexpr (MODE == kInt8) {
+      const uint32_t x1 = __shfl_sync(0xffffffffu, heads.x, k & 31), x2 = __shfl_sync(0xffffffffu, heads2.x, k & 31);
+      const uint32_t y1 = __shfl_sync(0xffffffffu, heads.y, k & 31), y2 = __shfl_sync(0xffffffffu, heads2.y, k & 31);
+      const bool near = k < head0 + 32;
+      const int n = int(((near ? y1 : y2) >> 8) & 255u);
+      if (quad == 0) {
+        if (blockIdx.x + (long long)k * grid < items && 4 * lane < n)
+          cp_async16(smem_addr(row_scales + 64 * ((k >> 1) & 3) + 4 * lane), p.row_scale + (near ? x1 : x2) + 4 * lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    }
+  };
+  for (int i = 0; i < kScaleAhead; ++i) fetch_scales(e + 2 * i);
   for (int item = blockIdx.x, k = 0; item < items; item += grid, ++k, walk.next()) {
     if (k > 0 && (k & 31) == 0) {
       heads = heads2;
       heads2 = fetch(k + 32);
+      head0 = k;
     }
     uint4 u;
     u.x = __shfl_sync(0xffffffffu, heads.x, k & 31);
@@ -869,20 +894,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     const long long t0 = (long long)(p.tile0 + walk.tile) * p.R;
     uint4 g2 = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == kWeightGrad) g2 = __ldg(reinterpret_cast<const uint4*>(p.grads + item) + 1);
-    // scales of the elements that this thread writes, fetched before the sums are waited for
-    float ts = 0.0f, rs[4] = {};
-    auto load_rs = [&](int c0) {
-      if constexpr (MODE == kInt8) {
-        if (c0 + sc < n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rs[i] = __ldg(p.row_scale + u.x + c0 + sc + i);
-        }
-      }
-    };
-    if constexpr (MODE == kInt8) {
-      if (sr < p.R && t0 + sr < p.tokens) ts = __ldg(p.token_scale + t0 + sr);
-      load_rs(0);
-    }
+    if constexpr (MODE == kInt8) fetch_scales(k + 2 * kScaleAhead);
     float acc[MODE == kForward ? 2 : 1][4][16] = {};
     if (quad < quads) {
 #pragma unroll
@@ -911,21 +923,23 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     }
     if constexpr (by_rows(MODE)) {
       float* st_up = stage + p.R * ld;
+      const float* row_scale = row_scales + 64 * ((k >> 1) & 3);
       const int rows = int(min((long long)p.R, p.tokens - t0));
       for (int c0 = 0; c0 < n; c0 += 1 << slog) {
         group_sync(e);  // the buffer has been read
+        if (MODE == kInt8 && quad == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead) : "memory");
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int c = 8 * j - c0;
           if (!in_tile || c < 0 || c >= (1 << slog) || 8 * j >= n) continue;
-          store8(stage + row * ld + c, acc[0][j / 2] + 8 * (j & 1));
+          float* v = acc[0][j / 2] + 8 * (j & 1);
+          store8(stage + row * ld + c, v);
           if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j / 2] + 8 * (j & 1));
         }
         group_sync(e);
         if (c0 + sc < n)
-          write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc, f1, f2, rs,
-                             ts, t0);
-        load_rs(c0 + (1 << slog));
+          write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc, f1, f2,
+                             row_scale + c0 + sc, p.token_scale + t0);
       }
     } else {
       const bool live = MODE == kWeightGrad ? row < int(u.y) * 8 : in_tile && t0 + row < p.tokens;
