@@ -91,6 +91,7 @@ struct vbsr_gated {
   // work units with every block row (column) whole, and cut into 2, 4 and 8 parts
   RowUnit* rows[4] = {};
   int row_units[4] = {};
+  int max_height = 64;
   ColUnit* cols[4] = {};
   int col_units[4] = {};
   ColEntry* entries = nullptr;
@@ -196,6 +197,7 @@ vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cuda
 vbsr_status build_gated(vbsr_gated* p) {
   const MatrixData* m[2] = {&p->gate->d, &p->up->d};
   const int R = m[0]->block_rows, S = m[0]->block_cols;
+  p->max_height = *std::max_element(p->gate->d.h_row_size.begin(), p->gate->d.h_row_size.end());
   VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
   for (const void* k : {reinterpret_cast<const void*>(pair_kernel<kForward>),
                         reinterpret_cast<const void*>(pair_kernel<kInputGrad>),
@@ -446,7 +448,7 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
   k.out1 = G;
   k.out2 = U;
   k.vec = aligned16(H, G, U);
-  choose_rows(k, p->rows, p->row_units, g.tiles, p->num_sm);
+  choose_rows(k, p->rows, p->row_units, g.tiles, p->num_sm, p->max_height);
   return launch_pair<kForward>(k, g.tiles, p->num_sm, s);
 }
 

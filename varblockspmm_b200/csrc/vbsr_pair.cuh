@@ -435,6 +435,7 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
       bulk_g2s_plain(base + lane * wb, g, 16u * hp, full);
       if (!I8) bulk_g2s_plain(base + lane * wb + 16u * hp, g + 16 * h, 16u * hp, full);
     }
+    if (pipe.i == 0) griddep_wait();
     // activations: one copy per run of neighbouring groups
     const uint32_t before = __shfl_up_sync(0xffffffffu, st.col, 1);
     const bool head = lane < st.n && (lane == 0 || st.col != before + 1);
@@ -523,10 +524,9 @@ __device__ __forceinline__ void produce_cols(const PairParams& p, PairShared& sh
         out.b = core_desc(b0 + 256u * j, pair ? 128u : 0u, 16u * h);
       }
     announce(sh, slot, full, all_steps | st.w << 5 | st.flags, groups * (xb + 32u * st.w), lane);
-    if (e.h8) {
-      bulk_g2s(a0, p.dy + (st.tile * per_tile + e.dy_group) * xb, e.h8 * xb, full, pol_x);
-      bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(st.c0 >> 3) * 32 * h, 4u * h * st.w, full);
-    }
+    if (e.h8) bulk_g2s_plain(b0, p.w + e.w_byte + (long long)(st.c0 >> 3) * 32 * h, 4u * h * st.w, full);
+    if (pipe.i == 0) griddep_wait();
+    if (e.h8) bulk_g2s(a0, p.dy + (st.tile * per_tile + e.dy_group) * xb, e.h8 * xb, full, pol_x);
     ++pipe.i;
     return true;
   };
@@ -1003,7 +1003,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_kernel(PairParams p) {
 
   if (warp < kPipes) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    if (MODE != kWeightGrad || !p.beside) griddep_wait();
+    // the launch before makes the panel; by rows and columns the first weights are fetched meanwhile
+    if (MODE == kWeightGrad && !p.beside) griddep_wait();
     if constexpr (by_rows(MODE))
       produce_rows<MODE>(p, sh, slots, zero, bars, warp, lane);
     else if constexpr (MODE == kInputGrad)
