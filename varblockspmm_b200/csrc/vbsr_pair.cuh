@@ -717,6 +717,14 @@ __device__ __forceinline__ void store8(float* dst, const float* v) {
   reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
+__device__ __forceinline__ void put8(float* dst, const float* v, int vec) {
+  if (vec) {
+    store8(dst, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = v[i];
+  }
+}
 __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vec) {
   if (vec) {
     *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
@@ -921,7 +929,46 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     } else {
       use += uint32_t(chunks[0] + chunks[1]);
     }
-    if constexpr (by_rows(MODE)) {
+    if (MODE == kForward && p.R > 64 && p.out1 == nullptr) {
+      // Every lane has a token, one output: straight from the registers, a 32-byte sector of a row at a time.
+      // (1436 block rows, 765 tokens: 172 us, and 237 us through shared memory as below, whose barriers and
+      // copies, 8 columns at a time for lack of room, cost more than whole lines save. With three outputs the
+      // scattered stores cost more: a training step of 1000 tokens 1195 us, and 1168 us as below.)
+      if (in_tile && t0 + row < p.tokens) {
+        float* o = p.out0 + (t0 + row) * p.M + u.x;
+#pragma unroll 1
+        for (int j = 0; 8 * j < n; ++j, o += 8) {
+          float v[8], w[8], hv[8];
+          auto pick = [&](auto c) {  // registers cannot be indexed by j
+            constexpr int J = decltype(c)::value;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v[i] = acc[0][J / 2][8 * (J & 1) + i] * f1 * f2;
+              w[i] = acc[MODE == kForward ? 1 : 0][J / 2][8 * (J & 1) + i] * f1 * f2;
+            }
+          };
+          switch (j) {
+            case 0: pick(std::integral_constant<int, 0>()); break;
+            case 1: pick(std::integral_constant<int, 1>()); break;
+            case 2: pick(std::integral_constant<int, 2>()); break;
+            case 3: pick(std::integral_constant<int, 3>()); break;
+            case 4: pick(std::integral_constant<int, 4>()); break;
+            case 5: pick(std::integral_constant<int, 5>()); break;
+            case 6: pick(std::integral_constant<int, 6>()); break;
+            default: pick(std::integral_constant<int, 7>()); break;
+          }
+          with_act(p.act, [&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a, da;
+              act_both<decltype(kind)::value>(v[i], a, da);
+              hv[i] = a * w[i];
+            }
+          });
+          put8(o, hv, p.vec);
+        }
+      }
+    } else if constexpr (by_rows(MODE)) {
       float* st_up = stage + p.R * ld;
       const float* row_scale = row_scales + 64 * ((k >> 1) & 3);
       const int rows = int(min((long long)p.R, p.tokens - t0));
@@ -953,12 +1000,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
         float* a = acc[0][j / 2] + 8 * (j & 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = a[i] * f1 * f2;
-        if (p.vec) {
-          store8(dst + 8 * j, a);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dst[8 * j + i] = a[i];
-        }
+        put8(dst + 8 * j, a, p.vec);
       }
     }
   }
