@@ -902,7 +902,6 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     const long long t0 = (long long)(p.tile0 + walk.tile) * p.R;
     uint4 g2 = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == kWeightGrad) g2 = __ldg(reinterpret_cast<const uint4*>(p.grads + item) + 1);
-    if constexpr (MODE == kInt8) fetch_scales(k + 2 * kScaleAhead);
     float acc[MODE == kForward ? 2 : 1][4][16] = {};
     if (quad < quads) {
 #pragma unroll
@@ -929,13 +928,22 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
     } else {
       use += uint32_t(chunks[0] + chunks[1]);
     }
-    if (MODE == kForward && p.R > 64 && p.out1 == nullptr) {
+    [[maybe_unused]] const float* row_scale = row_scales + 64 * ((k >> 1) & 3);
+    if constexpr (MODE == kInt8) {
+      group_sync(e);  // the group's last item, whose place in the ring is filled again, has been written
+      fetch_scales(k + 2 * kScaleAhead);
+      if (quad == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead) : "memory");
+      group_sync(e);
+    }
+    if (by_rows(MODE) && p.R > 64 && p.out1 == nullptr) {
       // Every lane has a token, one output: straight from the registers, a 32-byte sector of a row at a time.
       // (1436 block rows, 765 tokens: 172 us, and 237 us through shared memory as below, whose barriers and
       // copies, 8 columns at a time for lack of room, cost more than whole lines save. With three outputs the
       // scattered stores cost more: a training step of 1000 tokens 1195 us, and 1168 us as below.)
       if (in_tile && t0 + row < p.tokens) {
         float* o = p.out0 + (t0 + row) * p.M + u.x;
+        [[maybe_unused]] float ts = 0.0f;
+        if constexpr (MODE == kInt8) ts = __ldg(p.token_scale + t0 + row);
 #pragma unroll 1
         for (int j = 0; 8 * j < n; ++j, o += 8) {
           float v[8], w[8], hv[8];
@@ -943,8 +951,11 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
             constexpr int J = decltype(c)::value;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              v[i] = acc[0][J / 2][8 * (J & 1) + i] * f1 * f2;
-              w[i] = acc[MODE == kForward ? 1 : 0][J / 2][8 * (J & 1) + i] * f1 * f2;
+              v[i] = acc[0][J / 2][8 * (J & 1) + i];
+              if constexpr (MODE == kForward) {
+                v[i] = v[i] * f1 * f2;
+                w[i] = acc[1][J / 2][8 * (J & 1) + i] * f1 * f2;
+              }
             }
           };
           switch (j) {
@@ -957,24 +968,27 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
             case 6: pick(std::integral_constant<int, 6>()); break;
             default: pick(std::integral_constant<int, 7>()); break;
           }
-          with_act(p.act, [&](auto kind) {
+          if constexpr (MODE == kForward) {
+            with_act(p.act, [&](auto kind) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float a, da;
-              act_both<decltype(kind)::value>(v[i], a, da);
-              hv[i] = a * w[i];
-            }
-          });
+              for (int i = 0; i < 8; ++i) {
+                float a, da;
+                act_both<decltype(kind)::value>(v[i], a, da);
+                hv[i] = a * w[i];
+              }
+            });
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hv[i] = float(__float_as_int(v[i])) * (ts * row_scale[8 * j + i]);
+          }
           put8(o, hv, p.vec);
         }
       }
     } else if constexpr (by_rows(MODE)) {
       float* st_up = stage + p.R * ld;
-      const float* row_scale = row_scales + 64 * ((k >> 1) & 3);
       const int rows = int(min((long long)p.R, p.tokens - t0));
       for (int c0 = 0; c0 < n; c0 += 1 << slog) {
         group_sync(e);  // the buffer has been read
-        if (MODE == kInt8 && quad == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead) : "memory");
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int c = 8 * j - c0;
