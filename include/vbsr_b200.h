@@ -360,8 +360,11 @@ vbsr_status vbsr_matrix_quantize(const vbsr_matrix* m, int8_t* values, float* ro
 /* Orthogonalised block update: every h x w block V of a packed value array (a gradient or momentum
  * of the matrix's values) is replaced by `steps` Newton-Schulz steps
  *   X = V / (|V|_F + eps); then X <- a X + (b A + c A A) X with A = X X^T
- * with (a, b, c) = coefficients[0..2]. `out` may be `values` itself. A block of zeros gives zeros.
- * steps in [0, 64]; `m` gives the structure and must outlive the plan. */
+ * with (a, b, c) = coefficients[0..2]. `out` may be `values` itself. A block of zeros gives zeros; one that
+ * holds a NaN or an infinity gives NaN, the others are not touched by it. The products are at FP32
+ * accuracy as long as the iterates' entries stay below 2^10 in magnitude and those of b A + c A A below
+ * 2^5, as they do by far for coefficients that keep singular values near one; larger ones give
+ * infinities or NaN. steps in [0, 64]; `m` gives the structure and must outlive the plan. */
 typedef struct vbsr_ortho vbsr_ortho;
 vbsr_status vbsr_ortho_create(const vbsr_matrix* m, vbsr_ortho** out);
 vbsr_status vbsr_ortho_destroy(vbsr_ortho* p);

@@ -105,7 +105,7 @@ def check_backward(torch, plan, gate, up, kind, X, seed=5):
               ref.sampled(m, t.T @ np.abs(X64) + ref.product_tolerance(T, mag)), name)
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 16, 33, 64, 65, 128, 129, 300])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 16, 33, 64, 65, 128, 129, 300, 1000])
 @pytest.mark.parametrize("name", ["mixed", "one_long_row"])
 def test_gated_lengths(cuda, name, tokens):
     gate, up = pair(name)
@@ -400,6 +400,53 @@ def test_int8_product(cuda, name, tokens):
     assert torch.equal(C, C2)
 
 
+@pytest.mark.parametrize("tokens", [9, 70, 140])
+@pytest.mark.parametrize("offset", [1, 2])
+def test_int8_unaligned_panels_and_rows_behind(cuda, offset, tokens):
+    torch = cuda
+    m = ref.matrix(5, 220, 30, 41)  # long enough rows for every way of quantising a panel
+    M, K = m.scalar_rows(), m.scalar_cols()
+    q, rs = int8_weights(m, 3)
+    plan = vb.Int8Plan(vb.Matrix(m), torch.from_numpy(q).cuda(), torch.from_numpy(rs).cuda())
+    X = activations(tokens, K, 4)
+    Q, ts = quantized(X)
+    want = (Q @ ref.dense(m, q).T) * ts[:, None].astype(np.float64) * rs
+    xb = torch.zeros(tokens * K + 8, device="cuda")
+    x = xb[offset:offset + tokens * K]
+    x.copy_(torch.from_numpy(X).cuda().reshape(-1))
+    qb = torch.zeros(tokens * K + 8, dtype=torch.int8, device="cuda")
+    qx = qb[offset:offset + tokens * K]
+    qx.copy_(torch.from_numpy(Q.astype(np.int8)).cuda().reshape(-1))
+    for call in (lambda c: plan.execute_panel(x, c),
+                 lambda c: plan.execute(qx, torch.from_numpy(ts).cuda(), c)):
+        out = torch.full((tokens * M + 64,), 7.0, device="cuda")
+        c = out[offset:offset + tokens * M]
+        call(c)
+        plan.check_status()
+        close(c, want, 4 * ref.U * np.abs(want), "C")
+        assert (out[:offset] == 7).all() and (out[offset + tokens * M:] == 7).all()
+
+
+@pytest.mark.parametrize("tokens", [130, 257])
+def test_int8_long_tokens(cuda, tokens):
+    """Tokens long and many enough to be quantised by clusters; one holds an infinity, one zeros."""
+    torch = cuda
+    m = ref.matrix(40, 260, 12, 42)
+    q, rs = int8_weights(m, 5)
+    plan = vb.Int8Plan(vb.Matrix(m), torch.from_numpy(q).cuda(), torch.from_numpy(rs).cuda())
+    assert m.scalar_cols() >= 8192
+    X = activations(tokens, m.scalar_cols(), 9)
+    X[7, 11] = -np.inf
+    Q, ts = quantized(X)
+    want = (Q @ ref.dense(m, q).T) * ts[:, None].astype(np.float64) * rs
+    C = torch.full((tokens, m.scalar_rows()), 7.0, device="cuda")
+    plan.execute_panel(torch.from_numpy(X).cuda(), C)
+    plan.check_status()
+    assert torch.isnan(C[7]).all()
+    keep = np.arange(tokens) != 7
+    close(C[torch.from_numpy(keep).cuda()], want[keep], 4 * ref.U * np.abs(want[keep]), "C")
+
+
 @pytest.mark.parametrize("K", [1, 7, 8, 100, 4096, 40009])
 def test_quantize_panel(cuda, K):
     torch = cuda
@@ -495,6 +542,20 @@ def test_ortho_all_block_sizes(cuda, steps, scale):
     norm = m.values.astype(np.float64) / np.float64(scale)
     check_ortho(m, (norm if eps == 0.0 else m.values.astype(np.float64)), out.cpu().numpy(), steps,
                 eps)
+
+
+@pytest.mark.parametrize("count", [1, 2, 3, 700])
+def test_ortho_counts(cuda, count):
+    """One block, an odd number, and many of one size, large and small."""
+    torch = cuda
+    for h, w in ((64, 40), (48, 56), (24, 64), (8, 16)):
+        m = ref.matrix(count, 3, 1, count, row_size=[h] * count, col_size=[w] * 3)
+        plan = vb.OrthoPlan(vb.Matrix(m))
+        v = torch.from_numpy(m.values).cuda()
+        out = torch.full_like(v, float("nan"))
+        plan.execute(v, out, stream=torch.cuda.current_stream())
+        plan.check_status()
+        check_ortho(m, m.values, out.cpu().numpy())
 
 
 def test_ortho_rank_one_zero_and_not_finite_blocks(cuda):

@@ -349,7 +349,6 @@ vbsr_status launch_int8(const vbsr_int8* p, const Geometry& g, const float* scal
   k.M = p->M;
   k.K = p->K;
   k.x = panel;
-  k.x_chunks = p->K / 8;
   k.w = p->w;
   k.row_scale = p->row_scale;
   k.token_scale = scale;

@@ -32,16 +32,16 @@
 // accumulator.
 //
 // The kernel: one persistent CTA per SM with four pipelines, each a producer warp, a ring of slots, an
-// MMA thread and an accumulator; they take the accumulation chunks in turn. A producer issues a
-// stage's bulk copies into a slot and writes the slot's list of MMA steps; the MMA thread only works
-// off that list. Four, because both halves are latency: fetching a stage's list of places takes as
-// long as several stages take to stream, and a single MMA thread, which reads two descriptors
-// from shared memory per step, was measured at 400 clocks a step where the operands need about 140.
+// MMA warp and its accumulators; they take the accumulation chunks in turn. A producer issues a
+// stage's bulk copies into a slot and writes down where its MMA steps begin; the MMA warp only works
+// off that. Four, because both halves are latency: fetching a stage's list of places takes as
+// long as several stages take to stream, and one warp that issued all MMAs was measured at 400 clocks
+// a step where the operands need about 140 (517 tokens: 701 us with one pipeline, 384 us with four).
 // Two epilogue groups of four warps, one warp per TMEM quadrant, take every second work item each. Tokens
 // are on the M side (64 or 128 rows): with weights there, blocks of 8 to 56 rows would leave most of an
 // MMA empty. What bounds it: the copies into shared memory. A weight group of 32 h bytes needs 32 R
 // bytes of activations, from L2, so few tokens run at the weights' HBM rate and many at the
-// L2-to-shared-memory rate, h / 2 operations per byte.
+// L2-to-shared-memory rate, h / 2 operations per byte (517 tokens, 3.3 GB into shared memory: 11.8 TB/s).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -98,8 +98,7 @@ struct PairParams {
   int beside;                 // kWeightGrad: may run beside the launch before it (kInputGrad)
   int ring_log, acc_log;      // slots and accumulators per pipeline
   long long tokens, M, K;
-  const char* x;              // activation panel in pairs (kInt8: in 16-column chunks)
-  long long x_chunks;         // kInt8: chunks per tile of it
+  const char* x;              // activation panel in pairs (kInt8: in 16-column chunks), K / 8 a tile
   const char* dy;             // gradient panel in pairs
   const char* w;              // weights in pairs (kInt8: int8 chunks)
   const int* exps;            // exponents of x and dy: the call's
@@ -111,8 +110,8 @@ struct PairParams {
   int* status;
 };
 
-// One K step: two MMAs (kInt8: one). a and b are shared-memory descriptors; their unused top bits
-// carry flags.
+// One K step: two MMAs (kInt8: one; gradients: three). a and b are shared-memory descriptors; a flag is in
+// the unused top bits of a.
 struct PairStep {
   u64 a, b;
 };
@@ -120,28 +119,30 @@ constexpr u64 kStepOdd = 1ull << 58;    // the second K half of A is the tile of
 constexpr u64 kStepMask = (1ull << 56) - 1;
 constexpr int kMaxSteps = 16;
 
-// Slot header: steps | N/8 << 8 | flags. No steps: end of the work.
+// Slot header: steps | N/8 << 8 | flags. No steps: end of the work. First, last stage of an accumulation
+// chunk; odd: the last step has one group (kForward, kInt8).
 constexpr uint32_t kHdrFirst = 1u << 16, kHdrLast = 1u << 17, kHdrOdd = 1u << 18;
 constexpr uint32_t kHdrGroup = 1u << 19;  // the item's epilogue group
 
 __host__ __device__ constexpr bool by_rows(int mode) { return mode == kForward || mode == kInt8; }
-constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA threads in warps 4 .. 7
+constexpr int kPipes = 4;  // producer warps 0 .. 3, MMA warps 4 .. 7
 // A pipeline's share of shared memory, cut into 2^ring_log slots, and of the 512 TMEM columns, cut into
 // 2^acc_log accumulators of 128 or 64 columns (hi sums, then lo sums).
 constexpr uint32_t kPipeBytes = 48 * 1024;
-constexpr int kMaxSlots = 16, kMaxAccs = 8;
+constexpr int kMaxSlots = 8, kMaxAccs = 8;
 constexpr int kEpilogueWarp = 8, kEpilogueGroups = 2;
 constexpr int kPairThreads = 32 * (kEpilogueWarp + 4 * kEpilogueGroups);
 // The 128 registers per thread that the kernel is launched with, shared out again over its four
-// warpgroups: producers, MMA threads, and two of the epilogue.
+// warpgroups: producers, MMA warps, and two of the epilogue.
 constexpr int kProducerRegs = 88, kMmaRegs = 40, kEpilogueRegs = 192;
 static_assert(kPairThreads == 512 && kProducerRegs + kMmaRegs + 2 * kEpilogueRegs <= 4 * 128, "registers");
 constexpr int kChunkSteps = 12;  // 8: error 3.0e-7, 1 token 49.8 us; 12: 4.6e-7, 42.9 us; 16: 6.1e-7, 42.3 us
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage, at most
-// kForward, kInt8: results pass through shared memory, R rows and 2^stage_log columns (rows padded by 16
-// bytes, except rows of 32) of two matrices or one; a buffer for each of the two epilogue groups.
+// kForward, kInt8: results pass through shared memory (but see the epilogue), R rows and 2^stage_log columns
+// (rows padded by 16 bytes, except rows of 32) of two matrices or one; a buffer for each of the two epilogue
+// groups.
 constexpr int kScaleAhead = 3, kScaleBytes = 4 * 256;  // kInt8: ring of row scales, behind the rows
 constexpr int kStageBytes = 10 * 1024 + 256 + kScaleBytes;
 __host__ __device__ constexpr int stage_log(int mode, int R) {
@@ -400,7 +401,7 @@ __device__ void produce_rows(const PairParams& p, PairShared& sh, uint32_t slots
   constexpr bool I8 = MODE == kInt8;
   const uint32_t xb = (I8 ? 16u : 32u) * uint32_t(p.R);  // panel bytes of a group
   const uint64_t pol_x = policy_evict_last(), pol_w = policy_evict_first();
-  const long long per_tile = I8 ? p.x_chunks : p.K >> 3;
+  const long long per_tile = p.K >> 3;
   const int items = p.units * p.tiles;
   struct Stage {
     uint32_t shape, flags, col;  // flags: of the header
