@@ -345,7 +345,7 @@ vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t 
                                     vbsr_stream_t stream);
 vbsr_status vbsr_int8_check_status(const vbsr_int8* p, vbsr_stream_t stream);
 /* Symmetric quantisation of a K x tokens panel, one scale per token:
- *   token_scale[t] = max_k |B[k, t]| / 127 (fp32 division);
+ *   token_scale[t] = max_k |B[k, t]| * r, r the fp32 number nearest to 1/127 (fp32 product);
  *   Q[k, t] = B[k, t] / token_scale[t] rounded to the nearest integer, ties to even, as of the exact
  *   quotient, and clamped to [-127, 127]; a token whose scale is 0 has Q = 0.
  * A token that holds a NaN or an infinity has scale NaN and Q = 0, so its products are NaN. Runs on

@@ -366,7 +366,7 @@ def test_gated_streams_and_graphs(cuda):
 def quantized(x, axis=1):
     """(integers, float32 scales) of the definition, the quotient in 64 bits."""
     with np.errstate(all="ignore"):
-        s = (np.abs(x).max(axis=axis, initial=0) / np.float32(127)).astype(np.float32)
+        s = np.abs(x).max(axis=axis, initial=0).astype(np.float32) * (np.float32(1) / np.float32(127))
         q = np.rint(x.astype(np.float64) / np.expand_dims(s.astype(np.float64), axis))
     return np.clip(np.where(np.expand_dims(s, axis) > 0, q, 0), -127, 127), s
 

@@ -54,9 +54,10 @@ struct Quantizer {
   }
 };
 
-// Largest magnitude of a CTA's values; NaN or infinity give NaN.
+// The scale for a largest magnitude: times the fp32 number nearest to 1 / 127, one rounding; NaN where there
+// is a NaN or an infinity.
 __device__ __forceinline__ float scale_of(float amax, bool finite) {
-  return finite ? amax / 127.0f : __int_as_float(0x7fc00000);
+  return finite ? amax * (1.0f / 127.0f) : __int_as_float(0x7fc00000);
 }
 
 __device__ float block_amax(float v, bool& finite) {
