@@ -294,7 +294,10 @@ enum {
  * Both matrices have the same block-row and block-column partition and device; their block patterns
  * may differ. The plan keeps its own copy of both weights, taken from the matrices at creation and
  * replaced by vbsr_gated_set_values; the matrices must outlive the plan (it reads their structure).
- * Products are formed at FP32 accuracy. */
+ * Products are formed at FP32 accuracy, each token's whatever the others hold; weights below 2^-28 of the
+ * largest of both matrices, or activations below 2^-28 of their token's largest, are held to 2^-51 of
+ * that. A token that holds a NaN or an infinity has results that are not finite in the rows that read it;
+ * the other tokens are not touched by it (the weight gradients sum over tokens and are). */
 typedef struct vbsr_gated vbsr_gated;
 vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, int activation,
                               vbsr_gated** out);

@@ -77,11 +77,12 @@ def run_forward(torch, plan, X, M, keep=True):
     return dX, out
 
 
-def check_backward(torch, plan, gate, up, kind, X, seed=5):
+def check_backward(torch, plan, gate, up, kind, X, seed=5, padded=()):
     M, K, T = gate.scalar_rows(), gate.scalar_cols(), len(X)
     dX_in, (H, G, U) = run_forward(torch, plan, X, M)
     rng = np.random.default_rng(seed)
     dH = (1e-3 * rng.standard_normal((T, M))).astype(np.float32)
+    dH[list(padded)] = 0.0
     dB = torch.full((T, K), float("nan"), device="cuda")
     dw = [torch.full((len(m.values),), float("nan"), device="cuda") for m in (gate, up)]
     plan.backward(dX_in, G, U, torch.from_numpy(dH).cuda(), dB, *dw, stream=torch.cuda.current_stream())
@@ -288,6 +289,26 @@ def test_gated_scales(cuda):
         close(G, want.G, want.tol[0], "G")
         close(H, want.H, want.H_tol, "H")
         check_backward(torch, plan, g, u, vb.Activation.ReLU, x)
+
+
+@pytest.mark.parametrize("name,tokens", [("mixed", 9), ("mixed", 70), ("mixed", 300), ("one_long_row", 3),
+                                         ("one_long_row", 200), ("largest_blocks", 129)])
+def test_gated_tokens_of_unlike_size(cuda, name, tokens):
+    """A token 2^50 times the others (a padded place, whose dH is zero) and one 2^60 below them: every
+    token has its own accuracy, forward and backward, and the padded one takes no accuracy from the
+    weight gradients."""
+    torch = cuda
+    gate, up = pair(name)
+    kind = vb.Activation.SiLU
+    X = activations(tokens, gate.scalar_cols(), 31)
+    X[1] *= np.float32(2.0 ** 50)
+    X[tokens - 1] *= np.float32(2.0 ** -60)
+    plan = vb.GatedPlan(vb.Matrix(gate), vb.Matrix(up), kind)
+    want = Gated(gate, up, kind, X)
+    _, (H, G, U) = run_forward(torch, plan, X, gate.scalar_rows())
+    close(G, want.G, want.tol[0], "G")
+    close(U, want.U, want.tol[1], "U")
+    check_backward(torch, plan, gate, up, kind, X, padded=(1,))
 
 
 def test_gated_not_finite_stays_in_its_token(cuda):

@@ -107,8 +107,16 @@ struct Panels {
   int R = 0;        // tokens per tile
   int x_rows = 0;   // tokens per tile of the activations: R, or R / 2 (what a weight-gradient stage takes)
   int64_t tiles = 0;
-  int64_t x_at = 0, dy_at = 0, bytes = 0;
+  int x_splits = 0, dy_splits = 0;  // parts of a token for its largest magnitude
+  int64_t dy_partial_at = 0, exp_at = 0, stage_at = 0, x_at = 0, dy_at = 0, bytes = 0;
 };
+
+// Parts of at least 64 groups, and no more of all tokens than the warps of one grid.
+int splits_of(int64_t features, int64_t tokens) {
+  const int64_t most = std::min<int64_t>(64, features / 8 / 64);
+  return int(std::max<int64_t>(1, std::min<int64_t>(most, 8 * kAmaxCtas / tokens)));
+}
+
 constexpr int64_t kPartialBytes = 4 * kAmaxCtas + (256 - 4 * kAmaxCtas % 256) % 256;
 
 // Tiles of at most 128 tokens, evenly sized. In the forward direction any number goes: an MMA's rows behind
@@ -127,7 +135,12 @@ Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
   } else {
     g.R = g.x_rows = int((tokens + g.tiles - 1) / g.tiles);
   }
-  g.x_at = 2 * kPartialBytes + 256;  // largest magnitudes of both panels, exponents
+  g.x_splits = splits_of(p->K, tokens);
+  g.dy_splits = splits_of(p->M, tokens);
+  g.dy_partial_at = align256(4 * tokens * g.x_splits);
+  g.exp_at = g.dy_partial_at + (backward ? align256(4 * tokens * g.dy_splits) : 0);  // of the tokens
+  g.stage_at = g.exp_at + align256(4 * tokens);                                      // of the stages
+  g.x_at = g.stage_at + (backward ? align256(4 * g.tiles * (g.R / g.x_rows)) : 0);
   g.dy_at = g.x_at + align256(g.tiles * g.R * (p->K / 8) * 32);
   g.bytes = backward ? g.dy_at + align256(g.tiles * g.R * (p->M / 4) * 32) : g.dy_at;
   return g;
@@ -146,33 +159,39 @@ PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char*
   k.x = ws + g.x_at;
   k.dy = ws + g.dy_at;
   k.w = p->w;
-  k.exps = reinterpret_cast<const int*>(ws + 2 * kPartialBytes);
+  k.token_exp = reinterpret_cast<const int*>(ws + g.exp_at);
+  k.stage_exp = reinterpret_cast<const int*>(ws + g.stage_at);
   k.w_exp = p->w_exp;
   k.status = p->d_status;
   return k;
 }
 
-// The job of one panel. which: 0 the activations, 1 the gradients.
+// The job of one panel. which: 0 the activations, 1 the gradients, 2 the activations of the backward pass.
 template <class Source>
 PanelJob<Source> job_of(const Source& src, const Panels& g, int64_t tokens, char* ws, int which) {
+  const bool dy = which == 1;
   PanelJob<Source> j{src};
-  j.R = which ? g.R : g.x_rows;
-  j.tiles = int(which ? g.tiles : g.tiles * (g.R / g.x_rows));
-  const int64_t groups = src.features / 8;
-  j.amax_ctas = ctas_for(groups * tokens, kAmaxCtas);
-  j.pair_ctas = ctas_for(groups * g.tiles * g.R * Source::parts / 4, 148 * 7);
-  j.partial = reinterpret_cast<float*>(ws + which * kPartialBytes);
-  j.exponent = reinterpret_cast<int*>(ws + 2 * kPartialBytes) + which;
-  j.out = reinterpret_cast<uint4*>(ws + (which ? g.dy_at : g.x_at));
+  j.R = dy ? g.R : g.x_rows;
+  j.tiles = int(dy ? g.tiles : g.tiles * (g.R / g.x_rows));
+  j.splits = dy ? g.dy_splits : g.x_splits;
+  j.amax_ctas = ctas_for(32 * tokens * j.splits, kAmaxCtas);
+  j.pair_ctas = ctas_for(src.features / 8 * g.tiles * g.R * Source::parts / 4, 148 * 7);
+  j.partial = reinterpret_cast<float*>(ws + (dy ? g.dy_partial_at : 0));
+  j.exponent = reinterpret_cast<int*>(ws + (which == 2 ? g.stage_at : g.exp_at));
+  j.out = reinterpret_cast<uint4*>(ws + (dy ? g.dy_at : g.x_at));
+  if (which == 2) {
+    j.dy_partial = reinterpret_cast<const float*>(ws + g.dy_partial_at);
+    j.dy_splits = g.dy_splits;
+  }
   return j;
 }
 
-// Makes one panel, or two (`both`).
+// Makes one panel, or two (`both`; the second may be summed over with the first).
 template <class A, class C>
 vbsr_status make_panels(const PanelJob<A>& a, const PanelJob<C>& c, bool both, int64_t tokens, cudaStream_t s) {
   auto small = [&](int64_t features, int parts) { return features / 8 * tokens * parts <= kSmallGroups; };
-  if (small(a.src.features, A::parts) && (!both || small(c.src.features, C::parts))) {
-    panel_small_kernel<<<both ? 2 * kSmallCtas : kSmallCtas, kSmallThreads, 0, s>>>(a, c, tokens);
+  if (tokens <= kSmallTokens && small(a.src.features, A::parts) && (!both || small(c.src.features, C::parts))) {
+    panel_small_kernel<<<both ? 2 * kSmallCtas : kSmallCtas, kSmallThreads, 0, s>>>(a, c, int(tokens));
     VBSR_CUDA(cudaGetLastError());
     return VBSR_OK;
   }
@@ -477,7 +496,7 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
   char* ws = static_cast<char*>(workspace);
   const Panels n = panels_of(p, tokens, true);
   const auto dy = job_of(GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1);
-  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 0);
+  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 2);
   vbsr_status st2 = make_panels(dy, x, dgate != nullptr, tokens, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, n, tokens, ws);

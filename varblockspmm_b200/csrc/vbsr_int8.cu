@@ -269,6 +269,7 @@ __global__ void __cluster_dims__(kTokenCtas) __launch_bounds__(kTokenThreads)
   griddep_launch_dependents();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();  // its CTAs have started, before any writes to another
   const int cta = int(blockIdx.x % kTokenCtas);
   const long long t = blockIdx.x / kTokenCtas, groups = K / 8;  // a tile's rows behind the last token too
   const float* x = B + t * K;
@@ -286,6 +287,7 @@ __global__ void __cluster_dims__(kTokenCtas) __launch_bounds__(kTokenThreads)
     }
   m = block_amax(m, finite);
   if (!finite) m = __int_as_float(0x7fc00000);
+  cluster.barrier_wait();
   if (threadIdx.x < kTokenCtas) *cluster.map_shared_rank(&maxima[cta], threadIdx.x) = m;
   cluster.sync();
   m = 0.0f;

@@ -1,11 +1,13 @@
 // vbsr_pair.cuh — the tensor-core engine of the block-sparse layer operators (tcgen05, TMEM).
 //
 // FP32 accuracy from 16-bit tensor-core products. Every fp32 operand x is held as a pair of fp16
-// numbers: with a power of two 2^e that brings the operand's largest magnitude into [2^14, 2^15),
+// numbers: with a power of two 2^e that brings the largest magnitude (of the weights, or of a token's
+// activations or gradients) into [2^14, 2^15),
 //   hi = fp16(x 2^e),  lo = fp16((x 2^e - hi) 2^11),   x 2^e = hi + lo 2^-11 (1 + d), |d| <= 2^-12,
 // so the pair holds x to 2^-23 of itself (fp32 itself: 2^-24) for every |x| within 2^-28 of the
 // largest, and to 2^-51 of the largest below that. The factor 2^11 keeps lo out of fp16's
-// subnormals. A product of two operands is hi hi + 2^-11 (hi lo + lo hi); lo lo is below 2^-22 of it
+// subnormals. A token has its own e because the tokens of a call may differ by any factor (padded places,
+// outliers); where tokens are summed over, see PanelJob (vbsr_panels.cuh). A product of two operands is hi hi + 2^-11 (hi lo + lo hi); lo lo is below 2^-22 of it
 // and left out. The two sums go to accumulators of their own (fp32, in TMEM) and are joined, and
 // the powers of two taken back, in the epilogue. A pair is four bytes, as the fp32 number is: the
 // weights are laid out as pairs once (4 bytes per value streamed, no conversion in the kernel), the
@@ -101,7 +103,8 @@ struct PairParams {
   const char* x;              // activation panel in pairs (kInt8: in 16-column chunks), K / 8 a tile
   const char* dy;             // gradient panel in pairs
   const char* w;              // weights in pairs (kInt8: int8 chunks)
-  const int* exps;            // exponents of x and dy: the call's
+  const int* token_exp;       // exponents of the tokens of x, or (gradients) dy
+  const int* stage_exp;       // kWeightGrad: sums of the exponents of x and dy, per stage
   const int* w_exp;           // exponent of the weights: the plan's
   const float* row_scale;     // kInt8
   const float* token_scale;
@@ -740,16 +743,19 @@ __device__ __forceinline__ void group_sync(int e) {
 constexpr float kLoUnit = 1.0f / 2048.0f;  // 2^-11
 
 // Adds a 16-column tile of an accumulation chunk: hi sums at column `hi`, lo sums at `lo` (kInt8: the
-// integers at `hi`, carried as they are).
+// integers at `hi`, carried as they are; kWeightGrad: times the stage's power of two f).
 template <int MODE>
-__device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t lo) {
+__device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t lo, float f) {
   if constexpr (MODE == kInt8) {
     tc_ld16(hi, acc);
   } else {
     float v[16], w[16];
     tc_ld16(hi, lo, v, w);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] += fmaf(w[i], kLoUnit, v[i]);
+    for (int i = 0; i < 16; ++i) {
+      const float sum = fmaf(w[i], kLoUnit, v[i]);
+      acc[i] = MODE == kWeightGrad ? fmaf(sum, f, acc[i]) : acc[i] + sum;
+    }
   }
 }
 
@@ -758,8 +764,8 @@ __device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t
 // an element is a chain of latencies (shared memory, exponential, quotient).
 template <int MODE>
 __device__ __forceinline__ void write_staged(const PairParams& p, const float* st, const float* st_up, int ld,
-                                             int step, int sc, int sr, int rows, long long o, float f1, float f2,
-                                             const float* rs, const float* tokens) {
+                                             int step, int sc, int sr, int rows, long long o, const float* rs,
+                                             const float* tokens) {
   // o: place of (row 0, column sc) in the output
   // tokens: the tile's token scales (few, and read again by every unit: they stay in L1)
   auto finish = [&](long long at, float (&v)[4], float (&w)[4], float ts) {
@@ -785,14 +791,8 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
   };
   auto load = [&](int r, float (&v)[4], float (&w)[4]) {
     *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(st + r * ld + sc);
-    if constexpr (MODE == kForward) {
+    if constexpr (MODE == kForward)
       *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(st_up + r * ld + sc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = v[i] * f1 * f2;
-        w[i] = w[i] * f1 * f2;
-      }
-    }
   };
   const long long hop = step * p.M;
   o += sr * p.M;
@@ -800,8 +800,8 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
     float v[2][4], w[2][4], ts[2] = {};
     const bool two = r + step < rows;
     if constexpr (MODE == kInt8) {
-      ts[0] = __ldg(tokens + r);
-      ts[1] = __ldg(tokens + (two ? r + step : r));
+      ts[0] = tokens[r];
+      ts[1] = tokens[two ? r + step : r];
     }
     load(r, v[0], w[0]);
     load(two ? r + step : r, v[1], w[1]);
@@ -836,10 +836,9 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   const int tiles = MODE == kWeightGrad ? 1 : p.tiles, items = p.units * tiles, grid = int(gridDim.x);
   if (MODE != kWeightGrad || !p.beside) griddep_wait();
   if (MODE == kInputGrad) griddep_launch_dependents();
-  float f1 = 1.0f, f2 = 1.0f;
-  if (MODE == kForward) unscale(p.exps[0] + *p.w_exp, f1, f2);
-  if (MODE == kInputGrad) unscale(p.exps[1] + *p.w_exp, f1, f2);
-  if (MODE == kWeightGrad) unscale(p.exps[0] + p.exps[1], f1, f2);
+  constexpr bool per_token = MODE == kForward || MODE == kInputGrad;
+  int exponent = 0, tile_of_exponent = -1;  // of this lane's token and the weights
+  int stage_exp = 0;  // kWeightGrad: of 32 stages, one to a lane
   const int quads = live_quads<MODE>(p);
   const int thread = 32 * quad + lane, slog = stage_log(MODE, p.R), ld = stage_ld(slog), log4 = slog - 2;
   const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;  // staged output: column, first row
@@ -901,6 +900,10 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       continue;
     }
     const long long t0 = (long long)(p.tile0 + walk.tile) * p.R;
+    if (per_token && walk.tile != tile_of_exponent) {
+      tile_of_exponent = walk.tile;
+      exponent = *p.w_exp + (in_tile && t0 + row < p.tokens ? p.token_exp[t0 + row] : 0);
+    }
     uint4 g2 = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == kWeightGrad) g2 = __ldg(reinterpret_cast<const uint4*>(p.grads + item) + 1);
     float acc[MODE == kForward ? 2 : 1][4][16] = {};
@@ -908,6 +911,12 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
 #pragma unroll
       for (int which = 0; which < (MODE == kForward ? 2 : 1); ++which) {
         for (int ch = 0; ch < chunks[which]; ++ch, ++use) {
+          [[maybe_unused]] float f = 1.0f;
+          if constexpr (MODE == kWeightGrad) {
+            if ((ch & 31) == 0 && (ch > 0 || k == e || chunks[0] > 32))
+              stage_exp = ch + lane < chunks[0] ? p.stage_exp[ch + lane] : 0;
+            f = __int_as_float((127 - __shfl_sync(0xffffffffu, stage_exp, ch & 31)) << 23);
+          }
           const uint32_t buf = acc_of(p, use % kPipes, use / kPipes);
           // after an abort nothing is waited for, but the warps stay together (group_sync)
           if (ok)
@@ -919,7 +928,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (16 * j >= n) break;  // an odd last tile of 8 reads 8 columns more of its accumulator
-            add_tile<MODE>(acc[which][j], d + 16 * j, lo + 16 * j);
+            add_tile<MODE>(acc[which][j], d + 16 * j, lo + 16 * j, f);
           }
           tc_fence_before();
           __syncwarp();
@@ -936,6 +945,8 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       if (quad == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead) : "memory");
       group_sync(e);
     }
+    float f1 = 1.0f, f2 = 1.0f;
+    if constexpr (per_token) unscale(exponent, f1, f2);
     if (by_rows(MODE) && p.R > 64 && p.out1 == nullptr) {
       // Every lane has a token, one output: straight from the registers, a 32-byte sector of a row at a time.
       // (1436 block rows, 765 tokens: 172 us, and 237 us through shared memory as below, whose barriers and
@@ -944,7 +955,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       if (in_tile && t0 + row < p.tokens) {
         float* o = p.out0 + (t0 + row) * p.M + u.x;
         [[maybe_unused]] float ts = 0.0f;
-        if constexpr (MODE == kInt8) ts = __ldg(p.token_scale + t0 + row);
+        if constexpr (MODE == kInt8) ts = p.token_scale[t0 + row];
 #pragma unroll 1
         for (int j = 0; 8 * j < n; ++j, o += 8) {
           float v[8], w[8], hv[8];
@@ -995,12 +1006,20 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
           const int c = 8 * j - c0;
           if (!in_tile || c < 0 || c >= (1 << slog) || 8 * j >= n) continue;
           float* v = acc[0][j / 2] + 8 * (j & 1);
+          if constexpr (MODE == kForward) {
+            float* w = acc[1][j / 2] + 8 * (j & 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v[i] = v[i] * f1 * f2;
+              w[i] = w[i] * f1 * f2;
+            }
+            store8(st_up + row * ld + c, w);
+          }
           store8(stage + row * ld + c, v);
-          if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j / 2] + 8 * (j & 1));
         }
         group_sync(e);
         if (c0 + sc < n)
-          write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc, f1, f2,
+          write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc,
                              row_scale + c0 + sc, p.token_scale + t0);
       }
     } else {
@@ -1013,8 +1032,10 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       for (int j = 0; j < 8; ++j) {
         if (8 * j >= n) break;
         float* a = acc[0][j / 2] + 8 * (j & 1);
+        if constexpr (MODE == kInputGrad) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = a[i] * f1 * f2;
+          for (int i = 0; i < 8; ++i) a[i] = a[i] * f1 * f2;
+        }
         put8(dst + 8 * j, a, p.vec);
       }
     }

@@ -10,8 +10,9 @@
 
 namespace vbsr_b200 {
 
-// Largest finite magnitudes are found by a grid of kAmaxCtas CTAs, one partial result each; every CTA
-// of the following kernel takes the maximum of them. No atomics and nothing to clear.
+// Largest finite magnitudes are found by a grid of kAmaxCtas CTAs in partial results (of the weights one
+// per CTA, of a token one per part), and the following kernel takes the maximum of them. No atomics and
+// nothing to clear.
 constexpr int kAmaxCtas = 592;  // four per SM
 
 // Exponent that brings a largest magnitude into [2^14, 2^15); between -113 and 126, so that 2^e is a
@@ -159,82 +160,117 @@ struct PanelBlocks {
   __device__ __forceinline__ int slot(int t, int g) const { return (g << tt_log) + ((t + g) & (tt - 1)); }
 };
 
-// The largest finite magnitude of a thread's groups.
+// The largest finite magnitude of groups first, first + step, ... of a token, over the lanes of a warp.
 template <class Source>
-__device__ __forceinline__ float largest(const Source& src, long long tokens, long long first, long long step) {
-  const long long n = tokens * (src.features >> 3);
+__device__ __forceinline__ float largest(const Source& src, long long token, long long first, long long end,
+                                         int step) {
+  const long long row = token * (src.features >> 3);
   float m = 0.0f;
-  for (long long i = first; i < n; i += step) {
+#pragma unroll 4
+  for (long long g = first; g < end; g += step) {
     float v[Source::parts][8];
-    src.load(i, v);
+    src.load(row + g, v);
 #pragma unroll
     for (int q = 0; q < Source::parts; ++q)
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[q][j]));
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
 
-// A thread's share of the panel in pairs: per tile of R tokens, part and 8-feature group, [R of hi]
-// [R of lo'] rows of 16 bytes. Neighbouring threads take neighbouring tokens (512 contiguous bytes written
-// per warp; each reads one whole 32-byte sector).
-template <class Source>
-__device__ __forceinline__ void write_pairs(const Source& src, long long tokens, int R, int tiles, float s,
-                                            uint4* out, long long first, long long step) {
-  const long long groups = src.features >> 3;
-  for (PanelWalk w(first, step, R, groups); w.tile < tiles; w.next()) {
-    const int r = w.r;
-    const long long g = w.g, tile = w.tile, t = tile * R + r;
-    float v[Source::parts][8] = {};
-    if (t < tokens) src.load(t * groups + g, v);
-#pragma unroll
-    for (int q = 0; q < Source::parts; ++q) {
-      uint4 hi, lo;
-      to_pair8(v[q], s, hi, lo);
-      uint4* o = out + ((tile * Source::parts + q) * groups + g) * 2 * R + r;
-      o[0] = hi;
-      o[R] = lo;
-    }
-  }
-}
-
-// One panel to make: tiles of R tokens, largest magnitudes, pairs and exponent.
+// One panel to make. A token's exponent e brings its largest magnitude into [2^14, 2^15), so a token's
+// accuracy does not depend on the others'. Where tokens are summed over (the activations of the weight
+// gradients, against gradients dY with exponents f) one exponent c has to serve all tokens of a stage: they
+// are written with c - f, and c is the largest for which that is at most e for every token with a gradient.
+// So a token with a small gradient takes no bits from the others, however large it is; without a gradient
+// it has its own e.
 template <class Source>
 struct PanelJob {
   Source src;
-  int R, tiles;
-  int amax_ctas, pair_ctas;
-  float* partial;
+  int R, tiles;  // tiles of R tokens
+  int splits, amax_ctas, pair_ctas;
+  float* partial;  // largest magnitudes of `splits` parts of every token
   uint4* out;
-  int* exponent;
+  int* exponent;   // of every token, or (summed) c of every tile
+  const float* dy_partial;  // summed: the gradients' largest magnitudes, else null
+  int dy_splits;
 };
+
+__device__ __forceinline__ float scale_for(int e) { return e < -126 ? 0.0f : pow2(e); }  // below: less than 1
+// Summed: the bound on c from a token with largest magnitudes x and dy, and the token's exponent.
+__device__ __forceinline__ int sum_bound(float x, float dy) {
+  return x > 0.0f && dy > 0.0f ? min(126, max(-126, pair_exponent(x) + pair_exponent(dy))) : 126;
+}
+__device__ __forceinline__ int sum_exponent(float x, float dy, int c) {
+  return min(c - pair_exponent(dy), pair_exponent(x));
+}
 
 template <class Source>
 __device__ __forceinline__ void panel_amax(const PanelJob<Source>& j, long long tokens, int cta) {
-  const float m = cta_max(largest(j.src, tokens, cta * 256ll + threadIdx.x, j.amax_ctas * 256ll));
-  if (threadIdx.x == 0) j.partial[cta] = m;
+  const long long groups = j.src.features >> 3, parts = tokens * j.splits;
+  const int lane = threadIdx.x & 31;
+  for (long long i = cta * 8ll + (threadIdx.x >> 5); i < parts; i += j.amax_ctas * 8ll) {  // a warp each
+    const long long t = i / j.splits, k = i - t * j.splits;
+    const float m = largest(j.src, t, groups * k / j.splits + lane, groups * (k + 1) / j.splits, 32);
+    if (lane == 0) j.partial[i] = m;
+  }
+}
+
+// Exponents of a tile's tokens into e, several threads to a token; `write`: into the workspace too.
+template <class Source>
+__device__ __forceinline__ void tile_exponents(const PanelJob<Source>& j, long long tokens, long long tile, bool write,
+                                               int (&e)[128]) {
+  const int log = j.R <= 8 ? 5 : __clz(j.R - 1) - 24;  // 32 threads to a token, or 256 / (R rounded up)
+  const int r = threadIdx.x >> log, first = threadIdx.x & ((1 << log) - 1);
+  const long long t = tile * j.R + r;
+  const bool live = r < j.R && t < tokens;
+  float x = 0.0f, dy = 0.0f;
+  if (live) {
+    for (int i = first; i < j.splits; i += 1 << log) x = fmaxf(x, j.partial[t * j.splits + i]);
+    if (j.dy_partial != nullptr)
+      for (int i = first; i < j.dy_splits; i += 1 << log) dy = fmaxf(dy, j.dy_partial[t * j.dy_splits + i]);
+  }
+  for (int o = 1 << log >> 1; o; o >>= 1) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    dy = fmaxf(dy, __shfl_xor_sync(0xffffffffu, dy, o));
+  }
+  if (j.dy_partial != nullptr) {
+    const int c = -int(cta_max(float(-sum_bound(x, dy))));
+    if (first == 0 && r < j.R) e[r] = sum_exponent(x, dy, c);
+    if (write && threadIdx.x == 0) j.exponent[tile] = c;
+  } else if (first == 0 && r < j.R) {
+    e[r] = pair_exponent(x);
+    if (write && live) j.exponent[t] = e[r];
+  }
 }
 
 // A block of TT tokens (a power of two) x GG groups at a time goes through shared memory: read along the
-// features, written along the tokens, whole lines both ways.
+// features, written along the tokens, whole lines both ways. Per tile of R tokens, part and 8-feature group:
+// [R of hi][R of lo'] rows of 16 bytes.
 constexpr int kPanelUnits = 1024;  // 8-value pieces of all parts
 template <class Source>
 __device__ __forceinline__ void panel_pairs(const PanelJob<Source>& j, long long tokens, int cta,
-                                            uint4 (&buf)[2 * kPanelUnits]) {
+                                            uint4 (&buf)[2 * kPanelUnits], int (&e)[128]) {
   constexpr int P = Source::parts, UNITS = kPanelUnits / P;
-  const int e = partial_exponent(j.partial, j.amax_ctas), R = j.R;
-  if (cta == 0 && threadIdx.x == 0) *j.exponent = e;
-  const float s = pow2(e);
+  const int R = j.R;
   const PanelBlocks b(R, j.tiles, j.src.features >> 3, UNITS);
+  long long tile = -1;
   for (long long item = cta; item < b.items; item += j.pair_ctas) {
     const PanelBlocks::Place at = b.place(item);
+    if (at.tile != tile || at.g == 0) tile_exponents(j, tokens, at.tile, at.g == 0, e);
+    tile = at.tile;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < UNITS / 256; ++k) {
       const int u = threadIdx.x + 256 * k, t = u >> b.gg_log, g = u & (b.gg - 1);
       const long long token = at.tile * R + at.r + t;
-      float v[P][8] = {};
-      if (at.r + t < R && token < tokens && at.g + g < b.groups) j.src.load(token * b.groups + at.g + g, v);
+      float v[P][8] = {}, s = 0.0f;
+      if (at.r + t < R && token < tokens && at.g + g < b.groups) {
+        j.src.load(token * b.groups + at.g + g, v);
+        s = scale_for(e[at.r + t]);
+      }
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         uint4* place = buf + 2 * q * UNITS + b.slot(t, g);
@@ -266,43 +302,118 @@ __global__ void __launch_bounds__(256) panel_amax_kernel(PanelJob<A> a, PanelJob
   else panel_amax(c, tokens, cta - a.amax_ctas);
 }
 template <class A, class C>
-__global__ void __launch_bounds__(256) panel_pair_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
+__global__ void __launch_bounds__(256, 4) panel_pair_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
   __shared__ uint4 buf[2 * kPanelUnits];
+  __shared__ int e[128];
   griddep_launch_dependents();
   griddep_wait();
   const int cta = blockIdx.x;
-  if (cta < a.pair_ctas) panel_pairs(a, tokens, cta, buf);
-  else panel_pairs(c, tokens, cta - a.pair_ctas, buf);
+  if (cta < a.pair_ctas) panel_pairs(a, tokens, cta, buf, e);
+  else panel_pairs(c, tokens, cta - a.pair_ctas, buf, e);
 }
 
-// Small panels in one launch: a cluster of kSmallCtas CTAs for each, which exchange their largest magnitudes
-// through distributed shared memory and read their values a second time from the caches. Against the two
-// kernels it saves a launch; above kSmallGroups 8-value groups its few SMs cost more than that.
+// Small panels in one launch: a cluster of kSmallCtas CTAs for each, which exchange their tokens' largest
+// magnitudes through distributed shared memory and read their values a second time from the caches. Against
+// the two kernels it saves a launch; above kSmallGroups 8-value groups its few SMs cost more than that. The
+// cluster of summed activations reads the gradients too, for their exponents.
 constexpr int kSmallCtas = 8, kSmallThreads = 512;
-constexpr int64_t kSmallGroups = 32768;
+constexpr int64_t kSmallGroups = 32768, kSmallTokens = 256;
+struct SmallShared {
+  float x[8 * kSmallTokens], dy[8 * kSmallTokens];  // per token, of the parts of the cluster's warps
+  int e[kSmallTokens], bound[kSmallTokens];
+  float dy_max[kSmallTokens];
+};
+
+// Largest magnitudes of the tokens in every CTA's `table`: 8 << log parts a token, as many warps per token as
+// there are for few tokens. `ready`: waits for the cluster's CTAs to have started (they have arrived) before
+// it writes to them.
 template <class Source>
-__device__ __forceinline__ void panel_small(const PanelJob<Source>& j, long long tokens, float* maxima) {
+__device__ __forceinline__ void small_amax(const Source& src, int tokens, int log, float* table, bool ready) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  const int cta = int(blockIdx.x % kSmallCtas);
-  const long long first = cta * (long long)kSmallThreads + threadIdx.x;
-  const long long step = (long long)kSmallCtas * kSmallThreads;
-  float m = cta_max(largest(j.src, tokens, first, step));
-  if (threadIdx.x < kSmallCtas) *cluster.map_shared_rank(&maxima[cta], threadIdx.x) = m;
-  cluster.sync();
-#pragma unroll
-  for (int i = 0; i < kSmallCtas; ++i) m = fmaxf(m, maxima[i]);
-  const int e = pair_exponent(m);
-  if (cta == 0 && threadIdx.x == 0) *j.exponent = e;
-  write_pairs(j.src, tokens, j.R, j.tiles, pow2(e), j.out, first, step);
+  const int cta = int(blockIdx.x % kSmallCtas), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = cta << log | (warp & ((1 << log) - 1)), parts = kSmallCtas << log;
+  auto of = [&](int t) {
+    return t < tokens ? largest(src, t, 32 * part + lane, src.features >> 3, 32 * parts) : 0.0f;
+  };
+  int t = warp >> log;
+  float m = of(t);
+  if (ready) cluster.barrier_wait();
+  for (; t < tokens; m = of(t)) {
+    if (lane < kSmallCtas) *cluster.map_shared_rank(table + t * parts + part, lane) = m;
+    t += kSmallThreads / 32 >> log;
+  }
 }
+
+template <class A, class C>
+__device__ __forceinline__ void panel_small(const PanelJob<A>& j, const PanelJob<C>& dy, int tokens, SmallShared& sh) {
+  namespace cg = cooperative_groups;
+  const int cta = int(blockIdx.x % kSmallCtas), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool summed = j.dy_partial != nullptr;
+  const int log = tokens > 8 ? 0 : 4 - (tokens > 1 ? 32 - __clz(tokens - 1) : 0), parts = kSmallCtas << log;
+  small_amax(j.src, tokens, log, sh.x, true);
+  if (summed) small_amax(dy.src, tokens, log, sh.dy, false);
+  cg::this_cluster().sync();
+  for (int t = warp; t < tokens; t += kSmallThreads / 32) {
+    float x = 0.0f, d = 0.0f;
+    for (int i = lane; i < parts; i += 32) {
+      x = fmaxf(x, sh.x[t * parts + i]);
+      if (summed) d = fmaxf(d, sh.dy[t * parts + i]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+      d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, o));
+    }
+    if (lane == 0) {
+      sh.e[t] = pair_exponent(x);
+      sh.bound[t] = sum_bound(x, d);
+      sh.dy_max[t] = d;
+      if (!summed && cta == 0) j.exponent[t] = sh.e[t];
+    }
+  }
+  __syncthreads();
+  if (summed) {
+    if (warp < j.tiles) {
+      int c = 126;
+      const int end = min(tokens, (warp + 1) * j.R);
+      for (int t = warp * j.R + lane; t < end; t += 32) c = min(c, sh.bound[t]);
+      c = __reduce_min_sync(0xffffffffu, c);
+      for (int t = warp * j.R + lane; t < end; t += 32) sh.e[t] = min(c - pair_exponent(sh.dy_max[t]), sh.e[t]);
+      if (cta == 0 && lane == 0) j.exponent[warp] = c;
+    }
+    __syncthreads();
+  }
+  // pairs: neighbouring threads take neighbouring tokens (512 contiguous bytes written per warp; each reads
+  // one whole 32-byte sector)
+  const long long groups = j.src.features >> 3;
+  for (PanelWalk w(cta * (long long)kSmallThreads + threadIdx.x, kSmallCtas * (long long)kSmallThreads, j.R, groups);
+       w.tile < j.tiles; w.next()) {
+    const long long t = w.tile * j.R + w.r;
+    float v[A::parts][8] = {}, s = 0.0f;
+    if (t < tokens) {
+      j.src.load(t * groups + w.g, v);
+      s = scale_for(sh.e[t]);
+    }
+#pragma unroll
+    for (int q = 0; q < A::parts; ++q) {
+      uint4 hi, lo;
+      to_pair8(v[q], s, hi, lo);
+      uint4* o = j.out + ((w.tile * A::parts + q) * groups + w.g) * 2 * j.R + w.r;
+      o[0] = hi;
+      o[j.R] = lo;
+    }
+  }
+}
+// The first cluster makes a, a second one c, with a's largest magnitudes where c is summed over.
 template <class A, class C>
 __global__ void __cluster_dims__(kSmallCtas) __launch_bounds__(kSmallThreads)
-    panel_small_kernel(PanelJob<A> a, PanelJob<C> c, long long tokens) {
-  __shared__ float maxima[kSmallCtas];
+    panel_small_kernel(PanelJob<A> a, PanelJob<C> c, int tokens) {
+  __shared__ SmallShared sh;
+  cooperative_groups::this_cluster().barrier_arrive();
   griddep_launch_dependents();
-  if (blockIdx.x < kSmallCtas) panel_small(a, tokens, maxima);
-  else panel_small(c, tokens, maxima);
+  if (blockIdx.x < kSmallCtas) panel_small(a, a, tokens, sh);
+  else panel_small(c, a, tokens, sh);
 }
 
 }  // namespace vbsr_b200
