@@ -108,7 +108,7 @@ struct Panels {
   int x_rows = 0;   // tokens per tile of the activations: R, or R / 2 (what a weight-gradient stage takes)
   int64_t tiles = 0;
   int x_splits = 0, dy_splits = 0;  // parts of a token for its largest magnitude
-  int64_t dy_partial_at = 0, exp_at = 0, stage_at = 0, x_at = 0, dy_at = 0, bytes = 0;
+  int64_t dy_partial_at = 0, token_at = 0, stage_at = 0, x_at = 0, dy_at = 0, bytes = 0;
 };
 
 // Parts of at least 64 groups, and no more of all tokens than the warps of one grid.
@@ -138,8 +138,8 @@ Panels panels_of(const vbsr_gated* p, int64_t tokens, bool backward) {
   g.x_splits = splits_of(p->K, tokens);
   g.dy_splits = splits_of(p->M, tokens);
   g.dy_partial_at = align256(4 * tokens * g.x_splits);
-  g.exp_at = g.dy_partial_at + (backward ? align256(4 * tokens * g.dy_splits) : 0);  // of the tokens
-  g.stage_at = g.exp_at + align256(4 * tokens);                                      // of the stages
+  g.token_at = g.dy_partial_at + (backward ? align256(4 * tokens * g.dy_splits) : 0);  // the tokens' factors
+  g.stage_at = g.token_at + align256(4 * tokens);                                      // the stages'
   g.x_at = g.stage_at + (backward ? align256(4 * g.tiles * (g.R / g.x_rows)) : 0);
   g.dy_at = g.x_at + align256(g.tiles * g.R * (p->K / 8) * 32);
   g.bytes = backward ? g.dy_at + align256(g.tiles * g.R * (p->M / 4) * 32) : g.dy_at;
@@ -159,16 +159,16 @@ PairParams params_of(const vbsr_gated* p, const Panels& g, int64_t tokens, char*
   k.x = ws + g.x_at;
   k.dy = ws + g.dy_at;
   k.w = p->w;
-  k.token_exp = reinterpret_cast<const int*>(ws + g.exp_at);
-  k.stage_exp = reinterpret_cast<const int*>(ws + g.stage_at);
-  k.w_exp = p->w_exp;
+  k.token_factor = reinterpret_cast<const float*>(ws + g.token_at);
+  k.stage_factor = reinterpret_cast<const float*>(ws + g.stage_at);
   k.status = p->d_status;
   return k;
 }
 
 // The job of one panel. which: 0 the activations, 1 the gradients, 2 the activations of the backward pass.
 template <class Source>
-PanelJob<Source> job_of(const Source& src, const Panels& g, int64_t tokens, char* ws, int which) {
+PanelJob<Source> job_of(const vbsr_gated* p, const Source& src, const Panels& g, int64_t tokens, char* ws,
+                        int which) {
   const bool dy = which == 1;
   PanelJob<Source> j{src};
   j.R = dy ? g.R : g.x_rows;
@@ -177,7 +177,8 @@ PanelJob<Source> job_of(const Source& src, const Panels& g, int64_t tokens, char
   j.amax_ctas = ctas_for(32 * tokens * j.splits, kAmaxCtas);
   j.pair_ctas = ctas_for(src.features / 8 * g.tiles * g.R * Source::parts / 4, 148 * 7);
   j.partial = reinterpret_cast<float*>(ws + (dy ? g.dy_partial_at : 0));
-  j.exponent = reinterpret_cast<int*>(ws + (which == 2 ? g.stage_at : g.exp_at));
+  j.w_exp = p->w_exp;
+  j.factor = reinterpret_cast<float*>(ws + (which == 2 ? g.stage_at : g.token_at));
   j.out = reinterpret_cast<uint4*>(ws + (dy ? g.dy_at : g.x_at));
   if (which == 2) {
     j.dy_partial = reinterpret_cast<const float*>(ws + g.dy_partial_at);
@@ -459,7 +460,7 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   const Panels g = panels_of(p, tokens, false);
-  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0);
+  const auto x = job_of(p, PlainSource{B, p->K, aligned16(B)}, g, tokens, ws, 0);
   const vbsr_status st2 = make_panels(x, x, false, tokens, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, g, tokens, ws);
@@ -495,8 +496,8 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
   }
   char* ws = static_cast<char*>(workspace);
   const Panels n = panels_of(p, tokens, true);
-  const auto dy = job_of(GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1);
-  const auto x = job_of(PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 2);
+  const auto dy = job_of(p, GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1);
+  const auto x = job_of(p, PlainSource{B, p->K, aligned16(B)}, n, tokens, ws, 2);
   vbsr_status st2 = make_panels(dy, x, dgate != nullptr, tokens, s);
   if (st2 != VBSR_OK) return st2;
   PairParams k = params_of(p, n, tokens, ws);

@@ -103,9 +103,8 @@ struct PairParams {
   const char* x;              // activation panel in pairs (kInt8: in 16-column chunks), K / 8 a tile
   const char* dy;             // gradient panel in pairs
   const char* w;              // weights in pairs (kInt8: int8 chunks)
-  const int* token_exp;       // exponents of the tokens of x, or (gradients) dy
-  const int* stage_exp;       // kWeightGrad: sums of the exponents of x and dy, per stage
-  const int* w_exp;           // exponent of the weights: the plan's
+  // take back the powers of two of x or dy and the weights, per token; kWeightGrad: of x and dy, per stage
+  const float *token_factor, *stage_factor;
   const float* row_scale;     // kInt8
   const float* token_scale;
   float *out0, *out1, *out2;  // kForward: H, G, U; kInputGrad: dB; kWeightGrad: dgate, dup; kInt8: C
@@ -248,13 +247,6 @@ __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int* sta
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status,
                                           volatile int* abort_flag) {
   return __all_sync(0xffffffffu, wait_one(bar, parity, status, abort_flag)) != 0;
-}
-
-// 2^-e in two factors that neither overflow nor vanish, for |e| <= 252.
-__device__ __forceinline__ void unscale(int e, float& f1, float& f2) {
-  const int a = -e / 2, b = -e - a;
-  f1 = __int_as_float((a + 127) << 23);
-  f2 = __int_as_float((b + 127) << 23);
 }
 
 // n / d for 0 <= n < 2^27 and 1 <= d <= 32, with m = ceil(2^32 / d) (d = 1: m = 0): n m / 2^32 is off
@@ -765,7 +757,7 @@ __device__ __forceinline__ void add_tile(float (&acc)[16], uint32_t hi, uint32_t
 template <int MODE>
 __device__ __forceinline__ void write_staged(const PairParams& p, const float* st, const float* st_up, int ld,
                                              int step, int sc, int sr, int rows, long long o, const float* rs,
-                                             const float* tokens) {
+                                             const float* tokens, const float* factors) {
   // o: place of (row 0, column sc) in the output
   // tokens: the tile's token scales (few, and read again by every unit: they stay in L1)
   auto finish = [&](long long at, float (&v)[4], float (&w)[4], float ts) {
@@ -791,8 +783,15 @@ __device__ __forceinline__ void write_staged(const PairParams& p, const float* s
   };
   auto load = [&](int r, float (&v)[4], float (&w)[4]) {
     *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(st + r * ld + sc);
-    if constexpr (MODE == kForward)
+    if constexpr (MODE == kForward) {
       *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(st_up + r * ld + sc);
+      const float f = factors[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] *= f;
+        w[i] *= f;
+      }
+    }
   };
   const long long hop = step * p.M;
   o += sr * p.M;
@@ -837,8 +836,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   if (MODE != kWeightGrad || !p.beside) griddep_wait();
   if (MODE == kInputGrad) griddep_launch_dependents();
   constexpr bool per_token = MODE == kForward || MODE == kInputGrad;
-  int exponent = 0, tile_of_exponent = -1;  // of this lane's token and the weights
-  int stage_exp = 0;  // kWeightGrad: of 32 stages, one to a lane
+  float stage_factor = 0.0f;  // kWeightGrad: of 32 stages, one to a lane
   const int quads = live_quads<MODE>(p);
   const int thread = 32 * quad + lane, slog = stage_log(MODE, p.R), ld = stage_ld(slog), log4 = slog - 2;
   const int sc = 4 * (thread & ((1 << log4) - 1)), sr = thread >> log4;  // staged output: column, first row
@@ -857,6 +855,8 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
   // kInt8: row scales come through a ring in shared memory, kScaleAhead of the group's items ahead: a load of
   // the epilogue waits behind the bulk copies in flight, longer than a small item takes
   float* row_scales = stage + (kStageBytes - kScaleBytes) / 4;
+  // kForward, kInputGrad: the same place holds the factors of the tile's tokens, two tiles in turn
+  float* token_factors = row_scales;
   auto fetch_scales = [&](int k) {  // of the CTA's item k
     if constexpr (MODE == kInt8) {
       const uint32_t x1 = __shfl_sync(0xffffffffu, heads.x, k & 31), x2 = __shfl_sync(0xffffffffu, heads2.x, k & 31);
@@ -900,10 +900,9 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       continue;
     }
     const long long t0 = (long long)(p.tile0 + walk.tile) * p.R;
-    if (per_token && walk.tile != tile_of_exponent) {
-      tile_of_exponent = walk.tile;
-      exponent = *p.w_exp + (in_tile && t0 + row < p.tokens ? p.token_exp[t0 + row] : 0);
-    }
+    float* factors = token_factors + (tiles > 1 ? 128 * ((k >> 1) & 1) : 0);
+    if (per_token && (tiles > 1 || k == e) && in_tile && t0 + row < p.tokens)
+      cp_async4(smem_addr(factors + row), p.token_factor + t0 + row);
     uint4 g2 = make_uint4(0, 0, 0, 0);
     if constexpr (MODE == kWeightGrad) g2 = __ldg(reinterpret_cast<const uint4*>(p.grads + item) + 1);
     float acc[MODE == kForward ? 2 : 1][4][16] = {};
@@ -914,8 +913,8 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
           [[maybe_unused]] float f = 1.0f;
           if constexpr (MODE == kWeightGrad) {
             if ((ch & 31) == 0 && (ch > 0 || k == e || chunks[0] > 32))
-              stage_exp = ch + lane < chunks[0] ? p.stage_exp[ch + lane] : 0;
-            f = __int_as_float((127 - __shfl_sync(0xffffffffu, stage_exp, ch & 31)) << 23);
+              stage_factor = ch + lane < chunks[0] ? p.stage_factor[ch + lane] : 0.0f;
+            f = __shfl_sync(0xffffffffu, stage_factor, ch & 31);
           }
           const uint32_t buf = acc_of(p, use % kPipes, use / kPipes);
           // after an abort nothing is waited for, but the warps stay together (group_sync)
@@ -945,8 +944,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       if (quad == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead) : "memory");
       group_sync(e);
     }
-    float f1 = 1.0f, f2 = 1.0f;
-    if constexpr (per_token) unscale(exponent, f1, f2);
+    if (per_token) cp_async_wait_all();
     if (by_rows(MODE) && p.R > 64 && p.out1 == nullptr) {
       // Every lane has a token, one output: straight from the registers, a 32-byte sector of a row at a time.
       // (1436 block rows, 765 tokens: 172 us, and 237 us through shared memory as below, whose barriers and
@@ -955,6 +953,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
       if (in_tile && t0 + row < p.tokens) {
         float* o = p.out0 + (t0 + row) * p.M + u.x;
         [[maybe_unused]] float ts = 0.0f;
+        [[maybe_unused]] const float f = factors[row];
         if constexpr (MODE == kInt8) ts = p.token_scale[t0 + row];
 #pragma unroll 1
         for (int j = 0; 8 * j < n; ++j, o += 8) {
@@ -965,8 +964,8 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
             for (int i = 0; i < 8; ++i) {
               v[i] = acc[0][J / 2][8 * (J & 1) + i];
               if constexpr (MODE == kForward) {
-                v[i] = v[i] * f1 * f2;
-                w[i] = acc[1][J / 2][8 * (J & 1) + i] * f1 * f2;
+                v[i] = v[i] * f;
+                w[i] = acc[1][J / 2][8 * (J & 1) + i] * f;
               }
             }
           };
@@ -1006,25 +1005,18 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
           const int c = 8 * j - c0;
           if (!in_tile || c < 0 || c >= (1 << slog) || 8 * j >= n) continue;
           float* v = acc[0][j / 2] + 8 * (j & 1);
-          if constexpr (MODE == kForward) {
-            float* w = acc[1][j / 2] + 8 * (j & 1);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[i] = v[i] * f1 * f2;
-              w[i] = w[i] * f1 * f2;
-            }
-            store8(st_up + row * ld + c, w);
-          }
           store8(stage + row * ld + c, v);
+          if constexpr (MODE == kForward) store8(st_up + row * ld + c, acc[1][j / 2] + 8 * (j & 1));
         }
         group_sync(e);
         if (c0 + sc < n)
           write_staged<MODE>(p, stage, st_up, ld, 128 >> log4, sc, sr, rows, t0 * p.M + u.x + c0 + sc,
-                             row_scale + c0 + sc, p.token_scale + t0);
+                             row_scale + c0 + sc, p.token_scale + t0, factors);
       }
     } else {
       const bool live = MODE == kWeightGrad ? row < int(u.y) * 8 : in_tile && t0 + row < p.tokens;
       if (!live) continue;
+      [[maybe_unused]] const float f = factors[row];
       float* dst = MODE == kInputGrad
                        ? p.out0 + (t0 + row) * p.K + u.x
                        : ((g2.z & 1u) ? p.out1 : p.out0) + (u64(g2.x) | u64(g2.y) << 32) + (long long)row * n;
@@ -1034,7 +1026,7 @@ __device__ void epilogue(const PairParams& p, PairShared& sh, const PairBars& ba
         float* a = acc[0][j / 2] + 8 * (j & 1);
         if constexpr (MODE == kInputGrad) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a[i] = a[i] * f1 * f2;
+          for (int i = 0; i < 8; ++i) a[i] *= f;
         }
         put8(dst + 8 * j, a, p.vec);
       }

@@ -181,7 +181,9 @@ __device__ __forceinline__ float largest(const Source& src, long long token, lon
 }
 
 // One panel to make. A token's exponent e brings its largest magnitude into [2^14, 2^15), so a token's
-// accuracy does not depend on the others'. Where tokens are summed over (the activations of the weight
+// accuracy does not depend on the others'; the output takes 2^e and the weights' power of two back with one
+// factor, so that e is held where that is a normal number (products of largest magnitudes between 2^-98 and
+// 2^154: smaller ones are held to 2^-147, larger ones overflow). Where tokens are summed over (the activations of the weight
 // gradients, against gradients dY with exponents f) one exponent c has to serve all tokens of a stage: they
 // are written with c - f, and c is the largest for which that is at most e for every token with a gradient.
 // So a token with a small gradient takes no bits from the others, however large it is; without a gradient
@@ -193,18 +195,23 @@ struct PanelJob {
   int splits, amax_ctas, pair_ctas;
   float* partial;  // largest magnitudes of `splits` parts of every token
   uint4* out;
-  int* exponent;   // of every token, or (summed) c of every tile
+  const int* w_exp;  // the weights' exponent
+  float* factor;   // for every token's output, or (summed) 2^-c of every tile
   const float* dy_partial;  // summed: the gradients' largest magnitudes, else null
   int dy_splits;
 };
 
 __device__ __forceinline__ float scale_for(int e) { return e < -126 ? 0.0f : pow2(e); }  // below: less than 1
-// Summed: the bound on c from a token with largest magnitudes x and dy, and the token's exponent.
-__device__ __forceinline__ int sum_bound(float x, float dy) {
-  return x > 0.0f && dy > 0.0f ? min(126, max(-126, pair_exponent(x) + pair_exponent(dy))) : 126;
+// A token's exponent, with the weights' exponent w.
+__device__ __forceinline__ int token_exponent(float amax, int w) {
+  return min(126 - w, max(-126 - w, pair_exponent(amax)));
 }
-__device__ __forceinline__ int sum_exponent(float x, float dy, int c) {
-  return min(c - pair_exponent(dy), pair_exponent(x));
+// Summed: the bound on c from a token with largest magnitudes x and dy, and the token's exponent.
+__device__ __forceinline__ int sum_bound(float x, float dy, int w) {
+  return x > 0.0f && dy > 0.0f ? min(126, max(-126, pair_exponent(x) + token_exponent(dy, w))) : 126;
+}
+__device__ __forceinline__ int sum_exponent(float x, float dy, int w, int c) {
+  return min(c - token_exponent(dy, w), pair_exponent(x));
 }
 
 template <class Source>
@@ -226,6 +233,7 @@ __device__ __forceinline__ void tile_exponents(const PanelJob<Source>& j, long l
   const int r = threadIdx.x >> log, first = threadIdx.x & ((1 << log) - 1);
   const long long t = tile * j.R + r;
   const bool live = r < j.R && t < tokens;
+  const int w = *j.w_exp;
   float x = 0.0f, dy = 0.0f;
   if (live) {
     for (int i = first; i < j.splits; i += 1 << log) x = fmaxf(x, j.partial[t * j.splits + i]);
@@ -237,12 +245,12 @@ __device__ __forceinline__ void tile_exponents(const PanelJob<Source>& j, long l
     dy = fmaxf(dy, __shfl_xor_sync(0xffffffffu, dy, o));
   }
   if (j.dy_partial != nullptr) {
-    const int c = -int(cta_max(float(-sum_bound(x, dy))));
-    if (first == 0 && r < j.R) e[r] = sum_exponent(x, dy, c);
-    if (write && threadIdx.x == 0) j.exponent[tile] = c;
+    const int c = -int(cta_max(float(-sum_bound(x, dy, w))));
+    if (first == 0 && r < j.R) e[r] = sum_exponent(x, dy, w, c);
+    if (write && threadIdx.x == 0) j.factor[tile] = pow2(-c);
   } else if (first == 0 && r < j.R) {
-    e[r] = pair_exponent(x);
-    if (write && live) j.exponent[t] = e[r];
+    e[r] = token_exponent(x, w);
+    if (write && live) j.factor[t] = pow2(-e[r] - w);
   }
 }
 
@@ -320,8 +328,7 @@ constexpr int kSmallCtas = 8, kSmallThreads = 512;
 constexpr int64_t kSmallGroups = 32768, kSmallTokens = 256;
 struct SmallShared {
   float x[8 * kSmallTokens], dy[8 * kSmallTokens];  // per token, of the parts of the cluster's warps
-  int e[kSmallTokens], bound[kSmallTokens];
-  float dy_max[kSmallTokens];
+  int e[kSmallTokens], bound[kSmallTokens], dy_e[kSmallTokens];
 };
 
 // Largest magnitudes of the tokens in every CTA's `table`: 8 << log parts a token, as many warps per token as
@@ -350,6 +357,7 @@ __device__ __forceinline__ void panel_small(const PanelJob<A>& j, const PanelJob
   namespace cg = cooperative_groups;
   const int cta = int(blockIdx.x % kSmallCtas), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool summed = j.dy_partial != nullptr;
+  const int w_exp = *j.w_exp;
   const int log = tokens > 8 ? 0 : 4 - (tokens > 1 ? 32 - __clz(tokens - 1) : 0), parts = kSmallCtas << log;
   small_amax(j.src, tokens, log, sh.x, true);
   if (summed) small_amax(dy.src, tokens, log, sh.dy, false);
@@ -366,10 +374,15 @@ __device__ __forceinline__ void panel_small(const PanelJob<A>& j, const PanelJob
       d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, o));
     }
     if (lane == 0) {
-      sh.e[t] = pair_exponent(x);
-      sh.bound[t] = sum_bound(x, d);
-      sh.dy_max[t] = d;
-      if (!summed && cta == 0) j.exponent[t] = sh.e[t];
+      if (summed) {
+        sh.e[t] = pair_exponent(x);
+        sh.bound[t] = sum_bound(x, d, w_exp);
+        sh.dy_e[t] = token_exponent(d, w_exp);
+      } else {
+        const int e = token_exponent(x, w_exp);
+        sh.e[t] = e;
+        if (cta == 0) j.factor[t] = pow2(-e - w_exp);
+      }
     }
   }
   __syncthreads();
@@ -379,8 +392,8 @@ __device__ __forceinline__ void panel_small(const PanelJob<A>& j, const PanelJob
       const int end = min(tokens, (warp + 1) * j.R);
       for (int t = warp * j.R + lane; t < end; t += 32) c = min(c, sh.bound[t]);
       c = __reduce_min_sync(0xffffffffu, c);
-      for (int t = warp * j.R + lane; t < end; t += 32) sh.e[t] = min(c - pair_exponent(sh.dy_max[t]), sh.e[t]);
-      if (cta == 0 && lane == 0) j.exponent[warp] = c;
+      for (int t = warp * j.R + lane; t < end; t += 32) sh.e[t] = min(c - sh.dy_e[t], sh.e[t]);
+      if (cta == 0 && lane == 0) j.factor[warp] = pow2(-c);
     }
     __syncthreads();
   }
