@@ -267,22 +267,24 @@ __device__ __forceinline__ void panel_pairs(const PanelJob<Source>& j, long long
   long long tile = -1;
   for (long long item = cta; item < b.items; item += j.pair_ctas) {
     const PanelBlocks::Place at = b.place(item);
+    float v[UNITS / 256][P][8] = {};  // on their way while the exponents are found
+#pragma unroll
+    for (int k = 0; k < UNITS / 256; ++k) {
+      const int u = threadIdx.x + 256 * k, t = u >> b.gg_log, g = u & (b.gg - 1);
+      const long long token = at.tile * R + at.r + t;
+      if (at.r + t < R && token < tokens && at.g + g < b.groups) j.src.load(token * b.groups + at.g + g, v[k]);
+    }
     if (at.tile != tile || at.g == 0) tile_exponents(j, tokens, at.tile, at.g == 0, e);
     tile = at.tile;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < UNITS / 256; ++k) {
       const int u = threadIdx.x + 256 * k, t = u >> b.gg_log, g = u & (b.gg - 1);
-      const long long token = at.tile * R + at.r + t;
-      float v[P][8] = {}, s = 0.0f;
-      if (at.r + t < R && token < tokens && at.g + g < b.groups) {
-        j.src.load(token * b.groups + at.g + g, v);
-        s = scale_for(e[at.r + t]);
-      }
+      const float s = at.r + t < R ? scale_for(e[at.r + t]) : 0.0f;
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         uint4* place = buf + 2 * q * UNITS + b.slot(t, g);
-        to_pair8(v[q], s, place[0], place[UNITS]);
+        to_pair8(v[k][q], s, place[0], place[UNITS]);
       }
     }
     __syncthreads();
