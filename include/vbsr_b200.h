@@ -329,10 +329,10 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
 vbsr_status vbsr_gated_check_status(const vbsr_gated* p, vbsr_stream_t stream);
 
 /* Product in 8-bit integers, C[r, t] = row_scale[r] * token_scale[t] * sum_k Aq[r, k] Q[k, t]: the
- * sum is exact (32-bit integers), then rounded to fp32 and scaled. Weights are packed int8 device
+ * sum is exact (32-bit integers), then rounded to fp32 and multiplied by the product of the scales. Weights are packed int8 device
  * values with one scale per scalar row (output channel), laid out at creation; `m` gives the
- * structure (its own values are not read) and must outlive the plan. A block row wider than
- * 131072 columns in total could overflow the 32-bit sum and is refused. */
+ * structure (its own values are not read) and must outlive the plan. A block row of
+ * 131072 columns or more in total could overflow the 32-bit sum and is refused. */
 typedef struct vbsr_int8 vbsr_int8;
 vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const float* row_scale,
                              vbsr_int8** out);

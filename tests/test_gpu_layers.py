@@ -248,6 +248,7 @@ def test_gated_set_values_parts_and_zero_tokens(cuda):
     plan.backward(none, empty, empty, empty, none, part[1], part[2])
     torch.cuda.synchronize()
     assert not part[1].any() and not part[2].any()
+    plan.backward(none, empty, empty, empty, none)
 
 
 @pytest.mark.parametrize("offset", [0, 1, 2])
@@ -484,6 +485,26 @@ def test_quantize_panel(cuda, K):
     ok = np.isfinite(X).all(axis=1)
     assert np.array_equal(s[ok], ws[ok]) and np.array_equal(Q[ok], want[ok])
     assert np.isnan(s[~ok]).all() and not Q[~ok].any()
+
+
+def test_int8_widest_row(cuda):
+    """The largest sum that 32 bits have to hold: -128 times -128 over the widest row that is not refused."""
+    torch = cuda
+    m = ref.matrix(1, 2048, 2048, 52, sizes=(64,), row_size=(8,), col_size=(64,) * 2047 + (56,))
+    K, width = m.scalar_cols(), 131064
+    assert K == width
+    low = torch.full((len(m.values),), -128, dtype=torch.int8, device="cuda")
+    plan = vb.Int8Plan(vb.Matrix(m), low, torch.ones(8, device="cuda"))
+    for tokens in (1, 130):
+        C = torch.zeros(tokens, 8, device="cuda")
+        plan.execute(torch.full((tokens, K), -128, dtype=torch.int8, device="cuda"),
+                     torch.ones(tokens, device="cuda"), C)
+        plan.check_status()
+        assert (C.cpu() == np.float32(width * 128 * 128)).all()
+    wide = ref.matrix(1, 2048, 2048, 53, sizes=(64,), row_size=(8,))
+    with pytest.raises(vb.InvalidArgument, match="overflow"):
+        vb.Int8Plan(vb.Matrix(wide), torch.zeros(len(wide.values), dtype=torch.int8, device="cuda"),
+                    torch.ones(8, device="cuda"))
 
 
 def test_quantize_values_and_product(cuda):

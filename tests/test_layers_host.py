@@ -48,3 +48,6 @@ def test_panels_that_are_not_device_tensors():
     import torch
     with pytest.raises(vb.InvalidArgument, match="CUDA"):
         vb.quantize_panel(torch.zeros(2, 8), torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2), 8)
+    for K in (0, -8):
+        with pytest.raises(vb.InvalidArgument, match="positive"):
+            vb.quantize_panel(torch.zeros(2, 8), torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2), K)

@@ -846,6 +846,8 @@ class Int8Plan:
 def quantize_panel(B, Q, token_scale, K: int, tokens=None, stream=None):
     """Symmetric 8-bit quantisation of a K x tokens panel, one scale per token (see
     vbsr_quantize_panel). Tensors decide the device; raw pointers are on the current one."""
+    if K <= 0:
+        raise InvalidArgument("K must be positive")
     T = _tokens(B, K, tokens, "B")
     _dev_ptr(B)  # refuses a tensor that is not on a GPU
     dev = B.device.index if hasattr(B, "device") else -1

@@ -481,7 +481,7 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
   if (st != VBSR_OK) return st;
   if ((dgate == nullptr) != (dup == nullptr))
     return set_error(VBSR_INVALID_ARGUMENT, "dgate and dup are given together or not at all");
-  if (dgate == nullptr && dB == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "no output");
+  if (tokens > 0 && dgate == nullptr && dB == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "no output");
   if (tokens > 0 && (B == nullptr || G == nullptr || U == nullptr || dH == nullptr))
     return set_error(VBSR_INVALID_ARGUMENT, "null B, G, U or dH");
   DeviceGuard guard(p->device);

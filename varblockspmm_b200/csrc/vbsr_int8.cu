@@ -29,7 +29,7 @@ struct vbsr_int8 {
 
 namespace {
 
-constexpr int64_t kMaxRowWidth = 131072;    // 127 * 127 * width stays below 2^31
+constexpr int64_t kMaxRowWidth = 131071;  // 128 * 128 * width stays below 2^31
 
 // A scale ready for use: s is a normal number far from the smallest (tiny scales and the values that go
 // with them are multiplied by 2^120, exactly); s = 0 stands for a scale that is 0 or NaN.
@@ -454,7 +454,7 @@ vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const f
   for (int64_t w : m->d.h_sum_w)
     if (w > kMaxRowWidth)
       return set_error(VBSR_INVALID_ARGUMENT,
-                       "a block row wider than 131072 columns could overflow the 32-bit sum");
+                       "a block row of 131072 columns or more could overflow the 32-bit sum");
   auto* p = new (std::nothrow) vbsr_int8;
   if (p == nullptr) return set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
   p->m = m;
