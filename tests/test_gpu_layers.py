@@ -449,11 +449,11 @@ def test_int8_unaligned_panels_and_rows_behind(cuda, offset, tokens):
         assert (out[:offset] == 7).all() and (out[offset + tokens * M:] == 7).all()
 
 
-@pytest.mark.parametrize("tokens", [130, 257])
-def test_int8_long_tokens(cuda, tokens):
+@pytest.mark.parametrize("tokens,cols", [(130, 260), (257, 260), (260, 240), (129, 1400)])
+def test_int8_long_tokens(cuda, tokens, cols):
     """Tokens long and many enough to be quantised by clusters; one holds an infinity, one zeros."""
     torch = cuda
-    m = ref.matrix(40, 260, 12, 42)
+    m = ref.matrix(40, cols, 12, 42)
     q, rs = int8_weights(m, 5)
     plan = vb.Int8Plan(vb.Matrix(m), torch.from_numpy(q).cuda(), torch.from_numpy(rs).cuda())
     assert m.scalar_cols() >= 8192

@@ -255,67 +255,82 @@ __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long 
   }
 }
 
-// Many long tokens: scales and chunks in one launch, a cluster of kTokenCtas CTAs for each token, which
-// exchange their largest magnitudes through distributed shared memory and read their values a second time
-// from the caches (777 tokens of 36800: 154.8 us a call, against 161.7 us with the two kernels above; 64
-// tokens: the same; 1 token: 33.4 against 32.0). A thread writes its 8 columns to the first half of their
-// own chunk and the second half of the one before.
-constexpr int kTokenCtas = 8, kTokenThreads = 256;
-constexpr int64_t kManyTokens = 128, kLongTokens = 8192;  // at least half of a CTA's threads have values
-__global__ void __cluster_dims__(kTokenCtas) __launch_bounds__(kTokenThreads)
-    token_chunks_kernel(const float* B, long long tokens, long long K, int R, int vec, float* token_scale,
-                        char* out) {
-  __shared__ float maxima[kTokenCtas];
+// Few or long tokens, up to kHeldFeatures: scales and chunks in one launch, a cluster of kTokenCtas CTAs for two
+// tokens. A lane takes 8 columns of one of them, kTokenHeld times, which stay in its registers from their one
+// read until the CTAs have exchanged their largest magnitudes through distributed shared memory. A warp reads
+// 16 neighbouring groups and writes the 15 chunks that begin in the first 15, the second half of a chunk coming
+// from the lane of the next group: 16 bytes of both tokens side by side, a whole sector of 32. Against the two
+// kernels above (whole calls, 64 block rows of 4 blocks): 64 tokens of 8192 9.8 and 12.5 us, 777 of 16384 44 and
+// 48; but 777 of 2048, which fill a quarter of a cluster's lanes, 31 and 22, and 4000 of 16384 199 and 178. One
+// token of 147000, read twice by eight SMs: 39 us, and 32 by the two kernels.
+constexpr int kTokenCtas = 8, kTokenThreads = 256, kTokenWarps = kTokenThreads / 32, kTokenHeld = 5;
+constexpr int64_t kHeldFeatures = 8ll * 15 * kTokenCtas * kTokenWarps * kTokenHeld;  // 38400
+constexpr int64_t kFewTokens = 256, kLongTokens = 16384;
+__global__ void __cluster_dims__(kTokenCtas) __launch_bounds__(kTokenThreads, 4)
+    token_chunks_kernel(const float* B, long long tokens, long long rows, long long K, int R, int vec,
+                        float* token_scale, char* out) {
+  __shared__ float red[kTokenWarps][2], maxima[kTokenCtas][2];
   griddep_launch_dependents();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();  // its CTAs have started, before any writes to another
-  const int cta = int(blockIdx.x % kTokenCtas);
-  const long long t = blockIdx.x / kTokenCtas, groups = K / 8;  // a tile's rows behind the last token too
+  const int cta = int(blockIdx.x % kTokenCtas), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = lane & 1;
+  const long long t = blockIdx.x / kTokenCtas * 2 + which, groups = K / 8;
+  const bool live = t < tokens;  // a tile's rows behind the last token are zeros
   const float* x = B + t * K;
-  float m = 0.0f;
-  bool finite = true;
-  if (t < tokens)
-    for (long long g = cta * kTokenThreads + threadIdx.x; g < groups; g += kTokenCtas * kTokenThreads) {
-      float v[8];
+  const long long warp_g = 15ll * (cta * kTokenWarps + warp), step = 15ll * kTokenCtas * kTokenWarps;
+  auto load = [&](long long base, float (&v)[8]) {
+    const long long g = base + (lane >> 1);
+    if (live && g < groups) {
       load8(x + 8 * g, vec, v);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m = fmaxf(m, fabsf(v[i]));
-        finite = finite && isfinite(v[i]);
-      }
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     }
-  m = block_amax(m, finite);
-  if (!finite) m = __int_as_float(0x7fc00000);
+  };
+  constexpr float kInf = __builtin_huge_valf();  // marks a token that holds a NaN or an infinity
+  float m = 0.0f;
+  float v[kTokenHeld][8];
+#pragma unroll
+  for (int k = 0; k < kTokenHeld; ++k) load(warp_g + k * step, v[k]);
+#pragma unroll
+  for (int k = 0; k < kTokenHeld; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, isfinite(v[k][i]) ? fabsf(v[k][i]) : kInf);
+#pragma unroll
+  for (int o = 16; o > 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane < 2) red[warp][lane] = m;
+  __syncthreads();
   cluster.barrier_wait();
-  if (threadIdx.x < kTokenCtas) *cluster.map_shared_rank(&maxima[cta], threadIdx.x) = m;
+  if (threadIdx.x < 2 * kTokenCtas) {
+    m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTokenWarps; ++i) m = fmaxf(m, red[i][which]);
+    *cluster.map_shared_rank(&maxima[cta][which], threadIdx.x >> 1) = m;
+  }
   cluster.sync();
   m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kTokenCtas; ++i) {
-    finite = finite && maxima[i] == maxima[i];
-    m = fmaxf(m, maxima[i]);
-  }
-  const float s = scale_of(m, finite);
+  for (int i = 0; i < kTokenCtas; ++i) m = fmaxf(m, maxima[i][which]);
+  const float s = scale_of(m, m < kInf);
   const Quantizer quant(s);
-  if (cta == 0 && threadIdx.x == 0 && t < tokens) token_scale[t] = s;
+  if (cta == 0 && threadIdx.x < 2 && live) token_scale[t] = s;
   char* row = out + ((t / R) * R * groups + t % R) * 16;
-  for (long long g = cta * kTokenThreads + threadIdx.x; g < groups; g += kTokenCtas * kTokenThreads) {
+  auto write = [&](long long base, const float (&w)[8]) {
     union {
       int8_t q[8];
       uint2 u;
     } y;
-    y.u = make_uint2(0, 0);
-    if (t < tokens) {
-      float v[8];
-      load8(x + 8 * g, vec, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y.q[i] = int8_t(quant(v[i]));
-    }
-    *reinterpret_cast<uint2*>(row + chunk_place(g, K) * R * 16) = y.u;
-    if (g > 0) *reinterpret_cast<uint2*>(row + chunk_place(g - 1, K) * R * 16 + 8) = y.u;
-    if (g + 1 == groups) *reinterpret_cast<uint2*>(row + chunk_place(g, K) * R * 16 + 8) = make_uint2(0, 0);
-  }
+    for (int i = 0; i < 8; ++i) y.q[i] = int8_t(quant(w[i]));
+    const uint32_t next_x = __shfl_down_sync(0xffffffffu, y.u.x, 2), next_y = __shfl_down_sync(0xffffffffu, y.u.y, 2);
+    const long long g = base + (lane >> 1);
+    if (lane < 30 && t < rows && g < groups)
+      *reinterpret_cast<uint4*>(row + chunk_place(g, K) * R * 16) = make_uint4(y.u.x, y.u.y, next_x, next_y);
+  };
+#pragma unroll
+  for (int k = 0; k < kTokenHeld; ++k)
+    if (warp_g + k * step < groups) write(warp_g + k * step, v[k]);
 }
 
 vbsr_status launch_quantize(const float* B, int64_t K, int64_t tokens, int8_t* Q, float* scale,
@@ -525,9 +540,10 @@ vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t 
   char* ws = static_cast<char*>(workspace);
   const Geometry g = geometry_of(p, tokens);
   const int vec = aligned16(B);
-  if (tokens >= kManyTokens && p->K >= kLongTokens) {
-    token_chunks_kernel<<<unsigned(g.tiles * g.R * kTokenCtas), kTokenThreads, 0, s>>>(
-        B, tokens, p->K, g.R, vec, reinterpret_cast<float*>(ws + g.scale_at), ws + g.panel_at);
+  if (p->K <= kHeldFeatures && (tokens <= kFewTokens || p->K > kLongTokens)) {
+    const int64_t rows = g.tiles * g.R;
+    token_chunks_kernel<<<unsigned((rows + 1) / 2 * kTokenCtas), kTokenThreads, 0, s>>>(
+        B, tokens, rows, p->K, g.R, vec, reinterpret_cast<float*>(ws + g.scale_at), ws + g.panel_at);
     VBSR_CUDA(cudaGetLastError());
     return launch_int8(p, g, reinterpret_cast<const float*>(ws + g.scale_at), tokens, ws + g.panel_at, C, s);
   }
