@@ -134,6 +134,12 @@ vbsr_status vbsr_matrix_create_rows_generated(const vbsr_host_matrix_view* host,
                                               int32_t row_end, uint64_t seed, int device,
                                               vbsr_matrix** out);
 
+/* The structure of `host` alone, for the plans of the block-sparse layers below, which need no values
+ * of a matrix: `host->values` is not read and may be NULL, and no device memory is taken. The engine's
+ * own plans and vbsr_matrix_device_view refuse such a matrix. No reference counterpart. */
+vbsr_status vbsr_matrix_create_structure(const vbsr_host_matrix_view* host, int device,
+                                         vbsr_matrix** out);
+
 vbsr_status vbsr_matrix_destroy(vbsr_matrix* m);
 vbsr_status vbsr_matrix_info_get(const vbsr_matrix* m, vbsr_matrix_info* out);
 vbsr_status vbsr_matrix_device_view(const vbsr_matrix* m, vbsr_device_matrix* out);
@@ -293,7 +299,9 @@ enum {
 /* Gated feed-forward block: with G = A_gate B and U = A_up B, H = act(G) * U (element by element).
  * Both matrices have the same block-row and block-column partition and device; their block patterns
  * may differ. The plan keeps its own copy of both weights, taken from the matrices at creation and
- * replaced by vbsr_gated_set_values; the matrices must outlive the plan (it reads their structure).
+ * replaced by vbsr_gated_set_values; the matrices are not needed after creation. Where one of them holds
+ * its structure only, the plan has no weights until the first vbsr_gated_set_values, and forward and
+ * backward calls (of one token or more) are refused.
  * Products are formed at FP32 accuracy, each token's whatever the others hold; weights below 2^-28 of the
  * largest of both matrices, or activations below 2^-28 of their token's largest, are held to 2^-51 of
  * that. A token that holds a NaN or an infinity has results that are not finite in the rows that read it;
@@ -367,7 +375,7 @@ vbsr_status vbsr_matrix_quantize(const vbsr_matrix* m, int8_t* values, float* ro
  * holds a NaN or an infinity gives NaN, the others are not touched by it. The products are at FP32
  * accuracy as long as the iterates' entries stay below 2^10 in magnitude and those of b A + c A A below
  * 2^5, as they do by far for coefficients that keep singular values near one; larger ones give
- * infinities or NaN. steps in [0, 64]; `m` gives the structure and must outlive the plan. */
+ * infinities or NaN. steps in [0, 64]; `m` gives the structure and is not needed after creation. */
 typedef struct vbsr_ortho vbsr_ortho;
 vbsr_status vbsr_ortho_create(const vbsr_matrix* m, vbsr_ortho** out);
 vbsr_status vbsr_ortho_destroy(vbsr_ortho* p);

@@ -51,3 +51,28 @@ def test_panels_that_are_not_device_tensors():
     for K in (0, -8):
         with pytest.raises(vb.InvalidArgument, match="positive"):
             vb.quantize_panel(torch.zeros(2, 8), torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2), K)
+
+
+def test_matrix_of_structure_only():
+    """A matrix without values needs no GPU and no values; what would read them refuses it."""
+    import lm_reference as ref
+    host = ref.matrix(5, 7, 3, 1)
+    values = len(host.values)
+    host.values = host.values[:0]
+    m = vb.Matrix(host, structure_only=True)
+    info = m.info()
+    assert (info.block_rows, info.block_cols, info.value_count) == (5, 7, values)
+    assert (info.scalar_rows, info.scalar_cols) == (host.scalar_rows(), host.scalar_cols())
+    assert info.device_bytes == 0
+    for call in (m.device_view, lambda: vb.Plan(m, 32)):
+        with pytest.raises(vb.InvalidArgument, match="structure only"):
+            call()
+    refused(_lib.vbsr_matrix_quantize(m._h, None, None, None), "structure only")
+    for kw in (dict(rows=(0, 2)), dict(generated_seed=1)):
+        with pytest.raises(vb.InvalidArgument, match="structure_only"):
+            vb.Matrix(host, structure_only=True, **kw)
+    with pytest.raises(vb.InvalidArgument, match="offsets"):
+        vb.Matrix(host)
+    host.block_col = host.block_col + 7
+    with pytest.raises(vb.InvalidArgument, match="out of range"):
+        vb.Matrix(host, structure_only=True)

@@ -135,6 +135,7 @@ _sig = {
     "vbsr_matrix_create_rows": [C.POINTER(HostView), C.c_int32, C.c_int32, C.c_int, C.POINTER(_vp)],
     "vbsr_matrix_create_rows_generated": [C.POINTER(HostView), C.c_int32, C.c_int32, C.c_uint64,
                                           C.c_int, C.POINTER(_vp)],
+    "vbsr_matrix_create_structure": [C.POINTER(HostView), C.c_int, C.POINTER(_vp)],
     "vbsr_matrix_destroy": [_vp],
     "vbsr_matrix_info_get": [_vp, C.POINTER(MatrixInfo)],
     "vbsr_matrix_device_view": [_vp, C.POINTER(DeviceMatrix)],
@@ -497,13 +498,20 @@ class Matrix:
     Matrix(host) copies all of `host` to the current device. Matrix(host, rows=(r0, r1)) holds
     block rows [r0, r1) only (a multi-GPU shard). generated_seed=s builds the values on the device
     with the counter-based generator instead of copying host values (host.values may be empty).
+    structure_only=True holds the structure without values, on the host (host.values may be empty):
+    enough for GatedPlan, Int8Plan and OrthoPlan, and refused by Plan and device_view().
     """
 
-    def __init__(self, host: HostMatrix, device: int = -1, rows=None, generated_seed=None):
+    def __init__(self, host: HostMatrix, device: int = -1, rows=None, generated_seed=None,
+                 structure_only: bool = False):
         self._h = _vp()
         v = host.view()
         r0, r1 = (0, host.block_rows) if rows is None else rows
-        if generated_seed is not None:
+        if structure_only:
+            if rows is not None or generated_seed is not None:
+                raise InvalidArgument("structure_only goes without rows and generated_seed")
+            _check(_lib.vbsr_matrix_create_structure(C.byref(v), device, C.byref(self._h)))
+        elif generated_seed is not None:
             _check(_lib.vbsr_matrix_create_rows_generated(C.byref(v), r0, r1, generated_seed,
                                                           device, C.byref(self._h)))
         elif rows is None:
@@ -702,12 +710,13 @@ class GatedPlan:
     """Gated feed-forward block on two VBSR weights, H = act(A_gate B) * (A_up B), with its backward
     pass (vbsr_gated_*). No reference counterpart.
 
-        plan = GatedPlan(gate, up, Activation.SiLU)      # two Matrix of one block partition
+        plan = GatedPlan(gate, up, Activation.SiLU)      # two Matrix of one block partition, not kept
         plan.execute(X, H)                               # X [tokens, K], H [tokens, M]
         plan.execute(X, H, G, U)                         # keeps the pre-activations for
         plan.backward(X, G, U, dH, dX, dgate, dup)       # the gradients (dgate, dup packed)
         plan.set_values(gate_values, up_values)          # packed weights after an update
 
+    Where a Matrix holds its structure only, set_values comes before the first execute.
     Panels are K x tokens or M x tokens, column-major (a contiguous [tokens, K] tensor), for any
     number of tokens. Calls are asynchronous on `stream` (None: the legacy default stream). Each
     call's temporary memory is `workspace` (a uint8 CUDA tensor of workspace_bytes(tokens), or a
@@ -715,7 +724,6 @@ class GatedPlan:
     graphs that may run at the same time, need their own."""
 
     def __init__(self, gate: Matrix, up: Matrix, activation: Activation = Activation.SiLU):
-        self._matrices = (gate, up)  # keep them alive
         self._h = _vp()
         _check(_lib.vbsr_gated_create(gate._h, up._h, int(activation), C.byref(self._h)))
         info, self._up_values = gate.info(), up.info().value_count
@@ -876,14 +884,14 @@ def quantize_values(matrix: Matrix, stream=None):
 
 class OrthoPlan:
     """Orthogonalised block updates: `steps` Newton-Schulz steps on every block of a packed value
-    array (a gradient or momentum of the matrix's values; vbsr_ortho_*). No reference counterpart.
+    array (a gradient or momentum of the matrix's values; vbsr_ortho_*). No reference counterpart. The
+    matrix gives the structure and is not kept.
 
         plan = OrthoPlan(matrix)
         plan.execute(dgate, update)                      # update may be dgate itself
     """
 
     def __init__(self, matrix: Matrix):
-        self._matrix = matrix  # keep it alive
         self._h = _vp()
         info = matrix.info()
         self._values, self._device = info.value_count, info.device

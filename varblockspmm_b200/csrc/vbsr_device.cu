@@ -141,22 +141,6 @@ __global__ void rowwise_direct_kernel(vbsr_device_matrix a, const float* __restr
 
 bool valid_rhs(int rhs) { return rhs == 8 || rhs == 16 || rhs == 32 || rhs == 64; }
 
-// A private non-blocking stream for the copies and kernels that build a matrix or a plan. Its work
-// is ordered only by itself, and finish() waits for exactly that work, so creation neither waits
-// for nor stalls other streams of the device (a legacy-stream cudaMemcpy from pageable memory or
-// cudaMemset may still be in flight when it returns, so creation does not use those).
-struct SetupStream {
-  cudaStream_t s = nullptr;
-  cudaError_t init() { return cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking); }
-  cudaError_t finish() { return s ? cudaStreamSynchronize(s) : cudaSuccess; }
-  ~SetupStream() {
-    if (s) {
-      cudaStreamSynchronize(s);
-      cudaStreamDestroy(s);
-    }
-  }
-};
-
 template <class T>
 vbsr_status upload(T** dst, const T* src, size_t n, int64_t* bytes, cudaStream_t s) {
   *dst = nullptr;
@@ -260,7 +244,8 @@ vbsr_status upload_values(MatrixData& d, const float* src, const std::vector<int
   return VBSR_OK;
 }
 
-// Builds the device format of block rows [r0, r1). mode 0: values from host; 1: generated.
+// Builds the device format of block rows [r0, r1). mode 0: values from host; 1: generated; 2: the host copies
+// of the structure alone.
 vbsr_status build_matrix(const vbsr_host_matrix_view* v, int r0, int r1, int mode, uint64_t seed,
                          int device, vbsr_matrix** out) {
   if (out == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null output");
@@ -319,6 +304,17 @@ vbsr_status build_matrix(const vbsr_host_matrix_view* v, int r0, int r1, int mod
       int64_t sw = 0;
       for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) sw += v->col_size[v->block_col[b0 + b]];
       d.h_sum_w[i] = sw;
+    }
+
+    if (mode == 2) {
+      d.structure_only = true;
+      int devices = 0;
+      if (cudaGetDeviceCount(&devices) == cudaSuccess && dev >= devices) {
+        delete m;
+        return set_error(VBSR_INVALID_ARGUMENT, "no such device");
+      }
+      *out = m;
+      return VBSR_OK;
     }
 
     int64_t bytes = 0;
@@ -878,6 +874,13 @@ vbsr_status vbsr_matrix_create_rows_generated(const vbsr_host_matrix_view* host,
   return build_matrix(host, row_begin, row_end, 1, seed, device, out);
 }
 
+vbsr_status vbsr_matrix_create_structure(const vbsr_host_matrix_view* host, int device,
+                                         vbsr_matrix** out) {
+  clear_error();
+  if (host == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null matrix view");
+  return build_matrix(host, 0, host->block_rows, 2, 0, device, out);
+}
+
 vbsr_status vbsr_matrix_destroy(vbsr_matrix* m) {
   clear_error();
   if (m == nullptr) return VBSR_OK;
@@ -910,6 +913,7 @@ vbsr_status vbsr_matrix_device_view(const vbsr_matrix* m, vbsr_device_matrix* o)
   clear_error();
   if (m == nullptr || o == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null argument");
   const MatrixData& d = m->d;
+  if (d.structure_only) return set_error(VBSR_INVALID_ARGUMENT, "the matrix holds its structure only");
   o->block_rows = d.block_rows;
   o->block_cols = d.block_cols;
   o->nnzb = int32_t(d.nnzb);
@@ -939,6 +943,8 @@ vbsr_status vbsr_plan_create_ex(const vbsr_matrix* m, int rhs, int kernel, uint3
                      "GroupedGemmPlan");
   if (kernel != VBSR_KERNEL_AUTO && kernel != VBSR_KERNEL_ROW_OWNED)
     return set_error(VBSR_INVALID_ARGUMENT, "unknown kernel");
+  if (m->d.structure_only)
+    return set_error(VBSR_INVALID_ARGUMENT, "the matrix holds its structure only");
   auto* p = new (std::nothrow) vbsr_plan;
   if (p == nullptr) return set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
   p->m = m;

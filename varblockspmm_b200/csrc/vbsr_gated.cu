@@ -78,9 +78,9 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackRow* rows, const fl
 }  // namespace vbsr_b200
 
 struct vbsr_gated {
-  const vbsr_matrix *gate = nullptr, *up = nullptr;
   int device = 0, act = 0, num_sm = 148;
-  int64_t M = 0, K = 0;
+  int64_t M = 0, K = 0, gate_values = 0, up_values = 0;
+  bool has_weights = false;
   char* w = nullptr;      // both weights in pairs
   int64_t up_byte = 0;    // where up's begin
   int* w_exp = nullptr;   // their exponent
@@ -205,7 +205,7 @@ vbsr_status make_panels(const PanelJob<A>& a, const PanelJob<C>& c, bool both, i
 
 template <bool DEVICE>
 vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cudaStream_t s) {
-  const int64_t ng = p->gate->d.nvalues, nu = p->up->d.nvalues;
+  const int64_t ng = p->gate_values, nu = p->up_values;
   const int n = ctas_for((ng + nu) / 8, kAmaxCtas);
   values_amax_kernel<<<n, 256, 0, s>>>(gate, ng, up, nu, p->w_partial);
   VBSR_CUDA(cudaGetLastError());
@@ -214,10 +214,10 @@ vbsr_status pack_weights(vbsr_gated* p, const float* gate, const float* up, cuda
   return VBSR_OK;
 }
 
-vbsr_status build_gated(vbsr_gated* p) {
-  const MatrixData* m[2] = {&p->gate->d, &p->up->d};
+vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData& up) {
+  const MatrixData* m[2] = {&gate, &up};
   const int R = m[0]->block_rows, S = m[0]->block_cols;
-  p->max_height = *std::max_element(p->gate->d.h_row_size.begin(), p->gate->d.h_row_size.end());
+  p->max_height = *std::max_element(gate.h_row_size.begin(), gate.h_row_size.end());
   VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
   for (const void* k : {reinterpret_cast<const void*>(pair_kernel<kForward>),
                         reinterpret_cast<const void*>(pair_kernel<kInputGrad>),
@@ -344,8 +344,11 @@ vbsr_status build_gated(vbsr_gated* p) {
   VBSR_CUDA(cudaMalloc(&p->w, p->up_byte + std::max<int64_t>(256, 4 * m[1]->nvalues)));
   VBSR_CUDA(cudaMalloc(&p->w_exp, sizeof(int)));
   VBSR_CUDA(cudaMalloc(&p->w_partial, kPartialBytes));
-  const vbsr_status st = pack_weights<true>(p, m[0]->d_values, m[1]->d_values, nullptr);
-  if (st != VBSR_OK) return st;
+  if ((!gate.structure_only && !up.structure_only) || gate.nvalues + up.nvalues == 0) {
+    const vbsr_status st = pack_weights<true>(p, gate.d_values, up.d_values, nullptr);
+    if (st != VBSR_OK) return st;
+    p->has_weights = true;
+  }
   VBSR_CUDA(cudaStreamSynchronize(nullptr));
   return VBSR_OK;
 }
@@ -396,8 +399,8 @@ vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, in
     return set_error(VBSR_INVALID_ARGUMENT, "gate and up have different block partitions");
   auto* p = new (std::nothrow) vbsr_gated;
   if (p == nullptr) return set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
-  p->gate = gate;
-  p->up = up;
+  p->gate_values = g.nvalues;
+  p->up_values = u.nvalues;
   p->device = g.device;
   p->act = activation;
   p->M = g.M;
@@ -405,7 +408,7 @@ vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, in
   DeviceGuard guard(p->device);
   vbsr_status st;
   try {
-    st = build_gated(p);
+    st = build_gated(p, g, u);
   } catch (const std::bad_alloc&) {
     st = set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
   }
@@ -427,12 +430,13 @@ vbsr_status vbsr_gated_set_values(vbsr_gated* p, const float* gate_values, const
                                   vbsr_stream_t stream) {
   clear_error();
   if (p == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null plan");
-  if ((gate_values == nullptr && p->gate->d.nvalues > 0) ||
-      (up_values == nullptr && p->up->d.nvalues > 0))
+  if ((gate_values == nullptr && p->gate_values > 0) || (up_values == nullptr && p->up_values > 0))
     return set_error(VBSR_INVALID_ARGUMENT, "null values");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return pack_weights<false>(p, gate_values, up_values, s);
+  const vbsr_status st = pack_weights<false>(p, gate_values, up_values, s);
+  p->has_weights |= st == VBSR_OK;
+  return st;
 }
 
 vbsr_status vbsr_gated_workspace_bytes(const vbsr_gated* p, int64_t tokens, int backward,
@@ -456,6 +460,7 @@ vbsr_status vbsr_gated_forward(const vbsr_gated* p, const float* B, int64_t toke
     return set_error(VBSR_INVALID_ARGUMENT, "G and U are given together or not at all");
   if (tokens == 0) return VBSR_OK;
   if (B == nullptr || H == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null B or H");
+  if (!p->has_weights) return set_error(VBSR_INVALID_ARGUMENT, "the plan has no weights yet");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -486,14 +491,14 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
     return set_error(VBSR_INVALID_ARGUMENT, "null B, G, U or dH");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const MatrixData &g = p->gate->d, &u = p->up->d;
   if (tokens == 0) {
     if (dgate != nullptr) {
-      VBSR_CUDA(cudaMemsetAsync(dgate, 0, 4 * g.nvalues, s));
-      VBSR_CUDA(cudaMemsetAsync(dup, 0, 4 * u.nvalues, s));
+      VBSR_CUDA(cudaMemsetAsync(dgate, 0, 4 * p->gate_values, s));
+      VBSR_CUDA(cudaMemsetAsync(dup, 0, 4 * p->up_values, s));
     }
     return VBSR_OK;
   }
+  if (!p->has_weights) return set_error(VBSR_INVALID_ARGUMENT, "the plan has no weights yet");
   char* ws = static_cast<char*>(workspace);
   const Panels n = panels_of(p, tokens, true);
   const auto dy = job_of(p, GateSource{G, U, dH, p->M, aligned16(G, U, dH), p->act}, n, tokens, ws, 1);

@@ -581,6 +581,7 @@ vbsr_status vbsr_matrix_quantize(const vbsr_matrix* m, int8_t* values, float* ro
                                  vbsr_stream_t stream) {
   clear_error();
   if (m == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null matrix");
+  if (m->d.structure_only) return set_error(VBSR_INVALID_ARGUMENT, "the matrix holds its structure only");
   if (row_scale == nullptr || (values == nullptr && m->d.nvalues > 0))
     return set_error(VBSR_INVALID_ARGUMENT, "null values or row_scale");
   DeviceGuard guard(m->d.device);

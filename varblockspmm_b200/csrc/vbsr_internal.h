@@ -103,6 +103,22 @@ struct DeviceGuard {
     if (prev >= 0) cudaSetDevice(prev);
   }
 };
+
+// A private non-blocking stream for the copies and kernels that build a matrix or a plan. Its work
+// is ordered only by itself, and finish() waits for exactly that work, so creation neither waits
+// for nor stalls other streams of the device (a legacy-stream cudaMemcpy from pageable memory or
+// cudaMemset may still be in flight when it returns, so creation does not use those).
+struct SetupStream {
+  cudaStream_t s = nullptr;
+  cudaError_t init() { return cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking); }
+  cudaError_t finish() { return s ? cudaStreamSynchronize(s) : cudaSuccess; }
+  ~SetupStream() {
+    if (s) {
+      cudaStreamSynchronize(s);
+      cudaStreamDestroy(s);
+    }
+  }
+};
 #endif
 
 // ---- owning matrix -------------------------------------------------------------------------
@@ -115,6 +131,7 @@ struct MatrixData {
   std::vector<int64_t> h_row_off, h_val_off_row, h_sum_w;
   std::vector<uint32_t> h_blk_desc;  // per block: col_scalar_off | (w/8 - 1)
   std::vector<int32_t> h_block_col, h_col_size;
+  bool structure_only = false;  // no values and no device arrays: the host copies are all there is
   // device arrays in the reference layout (device_view) ...
   int32_t *d_row_ptr = nullptr, *d_block_col = nullptr, *d_row_size = nullptr,
           *d_col_size = nullptr;

@@ -49,7 +49,6 @@ struct alignas(16) OrthoSlot {
 };
 
 struct vbsr_ortho {
-  const vbsr_matrix* m = nullptr;
   int device = 0, big_ctas = 0, small_ctas = 0;  // of blocks of more than 32 rows, which come first; others
   OrthoSlot* slots = nullptr;
   int* d_status = nullptr;
@@ -501,8 +500,7 @@ void free_ortho(vbsr_ortho* p) {
   delete p;
 }
 
-vbsr_status build_ortho(vbsr_ortho* p) {
-  const MatrixData& d = p->m->d;
+vbsr_status build_ortho(vbsr_ortho* p, const MatrixData& d) {
   VBSR_CUDA(cudaFuncSetAttribute(ortho_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem));
   VBSR_CUDA(cudaFuncSetAttribute(ortho_big_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBigSmem));
   std::vector<OrthoSlot> by_class[5][5];
@@ -550,12 +548,11 @@ vbsr_status vbsr_ortho_create(const vbsr_matrix* m, vbsr_ortho** out) {
   if (m == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null matrix");
   auto* p = new (std::nothrow) vbsr_ortho;
   if (p == nullptr) return set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
-  p->m = m;
   p->device = m->d.device;
   DeviceGuard guard(p->device);
   vbsr_status st;
   try {
-    st = build_ortho(p);
+    st = build_ortho(p, m->d);
   } catch (const std::bad_alloc&) {
     st = set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
   }
