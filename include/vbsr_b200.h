@@ -311,8 +311,8 @@ vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, in
                               vbsr_gated** out);
 vbsr_status vbsr_gated_destroy(vbsr_gated* p);
 /* Replaces the weights by packed device arrays (value_count floats each), as after an optimiser
- * step. Ordered on `stream`; calls of the plan on other streams must be ordered after it by the
- * caller. */
+ * step. Ordered on `stream`; calls of the plan on other streams, earlier ones and later ones, must be
+ * ordered with it by the caller. */
 vbsr_status vbsr_gated_set_values(vbsr_gated* p, const float* gate_values, const float* up_values,
                                   vbsr_stream_t stream);
 /* Workspace bytes of a forward call, or (backward != 0) the larger of a forward and a backward. */
@@ -337,14 +337,21 @@ vbsr_status vbsr_gated_backward(const vbsr_gated* p, const float* B, const float
 vbsr_status vbsr_gated_check_status(const vbsr_gated* p, vbsr_stream_t stream);
 
 /* Product in 8-bit integers, C[r, t] = row_scale[r] * token_scale[t] * sum_k Aq[r, k] Q[k, t]: the
- * sum is exact (32-bit integers), then rounded to fp32 and multiplied by the product of the scales. Weights are packed int8 device
- * values with one scale per scalar row (output channel), laid out at creation; `m` gives the
- * structure (its own values are not read) and must outlive the plan. A block row of
- * 131072 columns or more in total could overflow the 32-bit sum and is refused. */
+ * sum is exact (32-bit integers), then rounded to fp32 and multiplied by the product of the scales. Weights
+ * are packed int8 device values with one scale per scalar row (output channel); `m` gives the structure (its
+ * own values are not read) and is not needed after creation. The plan keeps its own copy of the weights,
+ * laid out for the kernels: from the arrays given at creation, which waits for all work on the device
+ * before it reads them, or, where both are NULL, from the first vbsr_int8_set_values (products before it
+ * are refused). A block row of 131072 columns or more in total could overflow the 32-bit sum and is
+ * refused. */
 typedef struct vbsr_int8 vbsr_int8;
 vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const float* row_scale,
                              vbsr_int8** out);
 vbsr_status vbsr_int8_destroy(vbsr_int8* p);
+/* Replaces the weights and their scales. Ordered on `stream`; calls of the plan on other streams, earlier
+ * ones and later ones, must be ordered with it by the caller. */
+vbsr_status vbsr_int8_set_values(vbsr_int8* p, const int8_t* values, const float* row_scale,
+                                 vbsr_stream_t stream);
 vbsr_status vbsr_int8_workspace_bytes(const vbsr_int8* p, int64_t tokens, int64_t* bytes);
 /* C from a quantised panel: Q is K x tokens int8 (ld K), token_scale has `tokens` floats. */
 vbsr_status vbsr_int8_execute(const vbsr_int8* p, const int8_t* Q, const float* token_scale,

@@ -87,3 +87,104 @@ def test_gated_plan_without_blocks_has_its_weights(cuda):
     plan.execute(panel(torch, 5, m.scalar_cols(), 1), H)
     plan.check_status()
     assert (H == 0).all()
+
+
+def int8_case(torch, tokens=19, seed=6):
+    m = ref.matrix(9, 11, 5, seed, empty=(4,))
+    rng = np.random.default_rng(seed)
+    q = [torch.from_numpy(rng.integers(-128, 128, len(m.values)).astype(np.int8)).cuda() for _ in range(2)]
+    s = [torch.from_numpy((rng.random(m.scalar_rows()) + 0.1).astype(np.float32)).cuda() for _ in range(2)]
+    Q = torch.from_numpy(rng.integers(-127, 128, (tokens, m.scalar_cols())).astype(np.int8)).cuda()
+    ts = torch.from_numpy((rng.random(tokens) + 0.1).astype(np.float32)).cuda()
+    want = [(Q.cpu().numpy().astype(np.float64) @ ref.dense(m, q[i].cpu().numpy()).T) *
+            (ts.cpu().numpy()[:, None].astype(np.float64) * s[i].cpu().numpy()) for i in range(2)]
+    return m, q, s, Q, ts, want
+
+
+def int8_close(C, want):
+    """The sum, the product of the scales and the result round once each."""
+    got = C.cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got - want) <= 4 * ref.U * np.abs(want))
+
+
+def test_int8_plan_from_structure_and_other_weights(cuda):
+    """No weights until set_values; set_values replaces them, captured and replayed too."""
+    torch = cuda
+    m, q, s, Q, ts, want = int8_case(torch)
+    plan = vb.Int8Plan(structure(m))
+    C = torch.full((len(Q), m.scalar_rows()), 5.0, device="cuda")
+    for call in (lambda: plan.execute(Q, ts, C), lambda: plan.execute_panel(Q.float(), C)):
+        with pytest.raises(vb.InvalidArgument, match="no weights"):
+            call()
+    torch.cuda.synchronize()
+    assert (C == 5).all()
+    for i in (0, 1, 0):
+        plan.set_values(q[i], s[i])
+        plan.execute(Q, ts, C)
+        plan.check_status()
+        int8_close(C, want[i])
+    g = torch.cuda.CUDAGraph()
+    values, scales = q[0].clone(), s[0].clone()
+    with torch.cuda.graph(g):
+        plan.set_values(values, scales, stream=torch.cuda.current_stream())
+        plan.execute(Q, ts, C, stream=torch.cuda.current_stream())
+    for i in (1, 0):
+        values.copy_(q[i])
+        scales.copy_(s[i])
+        g.replay()
+        torch.cuda.synchronize()
+        int8_close(C, want[i])
+
+
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_int8_weights_at_any_alignment(cuda, offset):
+    torch = cuda
+    m, q, s, Q, ts, want = int8_case(torch, 5, 8)
+    buf = torch.zeros(len(q[0]) + 16, dtype=torch.int8, device="cuda")
+    v = buf[offset:offset + len(q[0])]
+    v.copy_(q[0])
+    plan = vb.Int8Plan(structure(m), v, s[0])
+    C = torch.full((len(Q), m.scalar_rows()), float("nan"), device="cuda")
+    plan.execute(Q, ts, C)
+    plan.check_status()
+    int8_close(C, want[0])
+
+
+@pytest.mark.parametrize("size", [8, 16, 24, 40, 56, 64])
+def test_int8_layout_of_every_block_width(cuda, size):
+    torch = cuda
+    sizes = (8, 16, 24, 32, 40, 48, 56, 64)
+    m = ref.matrix(8, 8, 5, size, row_size=sizes, col_size=[size] * 8, repeat=True)
+    rng = np.random.default_rng(size)
+    q = rng.integers(-128, 128, len(m.values)).astype(np.int8)
+    Q = rng.integers(-127, 128, (3, m.scalar_cols())).astype(np.int8)
+    plan = vb.Int8Plan(structure(m), torch.from_numpy(q).cuda(), torch.ones(m.scalar_rows(), device="cuda"))
+    C = torch.full((3, m.scalar_rows()), float("nan"), device="cuda")
+    plan.execute(torch.from_numpy(Q).cuda(), torch.ones(3, device="cuda"), C)
+    plan.check_status()
+    # whole numbers below 2^24: exact
+    assert np.array_equal(C.cpu().numpy().astype(np.float64), Q.astype(np.float64) @ ref.dense(m, q).T)
+
+
+def test_int8_creation_waits_for_weights_made_on_another_stream(cuda):
+    """Weights whose quantisation is still behind other work on a side stream when the plan is made."""
+    torch = cuda
+    m = ref.matrix(9, 11, 5, 7)
+    M = vb.Matrix(m)
+    q, s = vb.quantize_values(M)
+    torch.cuda.synchronize()
+    X = panel(torch, 6, m.scalar_cols(), 9)
+    want = torch.empty(6, m.scalar_rows(), device="cuda")
+    vb.Int8Plan(M, q, s).execute_panel(X, want)
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(3):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(40):  # some tens of ms
+                busy = (busy @ busy).clamp_(-1, 1)
+        q2, s2 = vb.quantize_values(M, stream=side)
+        C = torch.empty_like(want)
+        vb.Int8Plan(M, q2, s2).execute_panel(X, C)
+        torch.cuda.synchronize()
+        assert torch.equal(C, want)

@@ -76,3 +76,7 @@ def test_matrix_of_structure_only():
     host.block_col = host.block_col + 7
     with pytest.raises(vb.InvalidArgument, match="out of range"):
         vb.Matrix(host, structure_only=True)
+
+
+def test_int8_set_values_of_a_null_plan():
+    refused(_lib.vbsr_int8_set_values(None, None, None, None), "null plan")

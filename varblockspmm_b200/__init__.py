@@ -187,6 +187,7 @@ _sig = {
     "vbsr_gated_check_status": [_vp, _vp],
     "vbsr_int8_create": [_vp, _vp, _vp, C.POINTER(_vp)],
     "vbsr_int8_destroy": [_vp],
+    "vbsr_int8_set_values": [_vp, _vp, _vp, _vp],
     "vbsr_int8_workspace_bytes": [_vp, C.c_int64, _p64],
     "vbsr_int8_execute": [_vp, _vp, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp],
     "vbsr_int8_execute_panel": [_vp, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp],
@@ -793,21 +794,26 @@ class Int8Plan:
         plan = Int8Plan(matrix, q, s)
         plan.execute_panel(X, C)                         # X [tokens, K] float32, quantised per token
         plan.execute(Q, token_scale, C)                  # or an int8 panel with its scales
+        plan.set_values(q, s, stream)                    # other weights, in stream order
 
-    `matrix` gives the structure (its own values are not read). Streams and workspaces as for
-    GatedPlan."""
+    `matrix` gives the structure (its own values are not read) and is not kept. Creation waits for the
+    device before it reads the weights; without weights, set_values comes before the first product.
+    Streams and workspaces as for GatedPlan."""
 
-    def __init__(self, matrix: Matrix, values, row_scale):
-        self._matrix = matrix  # keep it alive
+    def __init__(self, matrix: Matrix, values=None, row_scale=None):
         self._h = _vp()
         info = matrix.info()
         self._M, self._K, self._device = info.scalar_rows, info.scalar_cols, info.device
-        v = _panel(values, info.value_count, 1, "values", self._device, "int8")
-        s = _panel(row_scale, self._M, 1, "row_scale", self._device)
-        if hasattr(values, "device"):
-            import torch
-            torch.cuda.current_stream(values.device).synchronize()  # the layout runs on its own
-        _check(_lib.vbsr_int8_create(matrix._h, v, s, C.byref(self._h)))
+        self._values = info.value_count
+        _check(_lib.vbsr_int8_create(matrix._h, *self._weights(values, row_scale), C.byref(self._h)))
+
+    def _weights(self, values, row_scale):
+        return (_panel(values, self._values, 1, "values", self._device, "int8"),
+                _panel(row_scale, self._M, 1, "row_scale", self._device))
+
+    def set_values(self, values, row_scale, stream=None):
+        """Replaces the weights by packed int8 values and one scale per scalar row."""
+        _check(_lib.vbsr_int8_set_values(self._h, *self._weights(values, row_scale), _stream_ptr(stream)))
 
     def workspace_bytes(self, tokens: int) -> int:
         n = C.c_int64()

@@ -14,12 +14,22 @@
 
 using namespace vbsr_b200;
 
+// A block row in the packed layout and in ours (lay_weights_kernel).
+struct LayRow {
+  uint64_t val, out;   // first packed value, first byte
+  uint32_t c0, chunks; // of chunk_src
+  uint32_t row0, h;
+};
+
 struct vbsr_int8 {
-  const vbsr_matrix* m = nullptr;
-  int device = 0, num_sm = 148;
-  int64_t M = 0, K = 0;
+  int device = 0, num_sm = 148, block_rows = 0;
+  int64_t M = 0, K = 0, nvalues = 0;
+  bool has_weights = false;
   char* w = nullptr;  // weights in 16-column chunks
   uint32_t* chunk_col = nullptr;
+  // where the chunks' weights are in the packed layout
+  LayRow* lay = nullptr;
+  uint32_t* chunk_src = nullptr;
   RowUnit* rows[4] = {};
   int row_units[4] = {};
   int max_height = 64;
@@ -135,29 +145,46 @@ __host__ __device__ constexpr int64_t chunk_place(int64_t col8, int64_t K) {
   return (col8 & 1) * ((K / 8 + 1) / 2) + (col8 >> 1);
 }
 
-// Block row's weights from the packed layout: [chunk][h rows][16].
-struct LayRow {
-  uint64_t val, out;  // first packed value, first byte
-  uint32_t b0, b1, h, pad;
-};
-__global__ void __launch_bounds__(256) lay_weights_kernel(const LayRow* rows, const uint32_t* blk_desc,
-                                                          const int8_t* values, char* out) {
+// A block row's weights from the packed layout, [chunk][h rows][16], and its scales. The columns of a chunk are
+// neighbours in the packed layout; a thread takes 8 rows of a chunk, 8 bytes of every column, and turns them.
+// chunk_src: first column of a chunk among the columns of its block row's blocks, in eights, times 2; + 1 where
+// the chunk has 8 columns.
+__global__ void __launch_bounds__(128) lay_weights_kernel(const LayRow* rows, const uint32_t* chunk_src,
+                                                          const int8_t* values, int vec, const float* scale,
+                                                          char* out, float* scale_out) {
   const LayRow r = rows[blockIdx.x];
-  const int8_t* v = values + r.val;
-  char* o = out + r.out;
-  for (uint32_t b = r.b0; b < r.b1; ++b) {
-    const int w = int((blk_desc[b] & 7u) + 1u) * 8, chunks = (w + 15) / 16, h = int(r.h);
-    for (int i = threadIdx.x; i < chunks * h; i += blockDim.x) {
-      const int c = i / h, row = i % h;
-      union {
-        int8_t q[16];
-        uint4 u;
-      } x;
-      for (int k = 0; k < 16; ++k) x.q[k] = 16 * c + k < w ? v[(16 * c + k) * h + row] : int8_t(0);
-      *reinterpret_cast<uint4*>(o + 16 * i) = x.u;
+  const uint32_t h8 = r.h / 8;
+  if (threadIdx.x < r.h) scale_out[r.row0 + threadIdx.x] = scale[r.row0 + threadIdx.x];
+  for (uint32_t i = threadIdx.x; i < r.chunks * h8; i += blockDim.x) {
+    const uint32_t c = i / h8, g = i % h8, src = chunk_src[r.c0 + c];
+    const int8_t* v = values + r.val + (unsigned long long)(src >> 1) * 8 * r.h + 8 * g;
+    uint2 q[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      q[k] = make_uint2(0, 0);
+      if (k >= 8 && (src & 1)) continue;
+      if (vec) {
+        q[k] = *reinterpret_cast<const uint2*>(v + k * r.h);
+      } else {
+        for (int b = 0; b < 4; ++b) {
+          q[k].x |= uint32_t(uint8_t(v[k * r.h + b])) << 8 * b;
+          q[k].y |= uint32_t(uint8_t(v[k * r.h + 4 + b])) << 8 * b;
+        }
+      }
     }
-    v += h * w;
-    o += 16 * chunks * h;
+    uint4* o = reinterpret_cast<uint4*>(out + r.out + 16ull * (c * r.h + 8 * g));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // row j: byte j of every column
+      uint32_t w[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        auto half = [&](int k) { return j < 4 ? q[k].x : q[k].y; };
+        const uint32_t pick = uint32_t(j & 3) | uint32_t(4 + (j & 3)) << 4;
+        w[m] = __byte_perm(__byte_perm(half(4 * m), half(4 * m + 1), pick),
+                           __byte_perm(half(4 * m + 2), half(4 * m + 3), pick), 0x5410);
+      }
+      o[j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -403,19 +430,29 @@ void free_int8(vbsr_int8* p) {
   DeviceGuard guard(p->device);
   cudaFree(p->w);
   cudaFree(p->chunk_col);
+  cudaFree(p->lay);
+  cudaFree(p->chunk_src);
   for (RowUnit* r : p->rows) cudaFree(r);
   cudaFree(p->row_scale);
   cudaFree(p->d_status);
   delete p;
 }
 
-vbsr_status build_int8(vbsr_int8* p, const int8_t* values, const float* row_scale) {
-  const MatrixData& d = p->m->d;
-  p->max_height = *std::max_element(p->m->d.h_row_size.begin(), p->m->d.h_row_size.end());
+vbsr_status lay_weights(vbsr_int8* p, const int8_t* values, const float* row_scale, cudaStream_t s) {
+  lay_weights_kernel<<<unsigned(p->block_rows), 128, 0, s>>>(
+      p->lay, p->chunk_src, values, (reinterpret_cast<uintptr_t>(values) & 7u) == 0, row_scale, p->w, p->row_scale);
+  VBSR_CUDA(cudaGetLastError());
+  p->has_weights = true;
+  return VBSR_OK;
+}
+
+vbsr_status build_int8(vbsr_int8* p, const MatrixData& d, const int8_t* values, const float* row_scale) {
+  p->max_height = *std::max_element(d.h_row_size.begin(), d.h_row_size.end());
+  p->block_rows = d.block_rows;
   VBSR_CUDA(cudaDeviceGetAttribute(&p->num_sm, cudaDevAttrMultiProcessorCount, p->device));
   VBSR_CUDA(cudaFuncSetAttribute(pair_kernel<kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kPairSmem));
-  std::vector<uint32_t> cols;
+  std::vector<uint32_t> cols, src;
   std::vector<LayRow> lay;
   std::vector<RowUnit> whole(d.block_rows);
   uint64_t at = 0;
@@ -425,32 +462,36 @@ vbsr_status build_int8(vbsr_int8* p, const int8_t* values, const float* row_scal
     u.shape = uint32_t(d.h_row_size[i]);
     u.g0[0] = uint32_t(cols.size());
     u.w0[0] = at;
+    uint32_t before = 0;  // columns of the row's blocks so far, in eights
     for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
-      const int64_t col8 = d.h_blk_desc[b] >> 3, w8 = (d.h_blk_desc[b] & 7u) + 1u;
-      for (int64_t c = 0; c < w8; c += 2) cols.push_back(uint32_t(chunk_place(col8 + c, p->K)));
+      const uint32_t col8 = d.h_blk_desc[b] >> 3, w8 = (d.h_blk_desc[b] & 7u) + 1u;
+      for (uint32_t c = 0; c < w8; c += 2) {
+        cols.push_back(uint32_t(chunk_place(col8 + c, p->K)));
+        src.push_back((before + c) << 1 | (c + 1 == w8 ? 1u : 0u));
+      }
+      before += w8;
     }
     u.ng[0] = uint32_t(cols.size()) - u.g0[0];
-    lay.push_back({uint64_t(d.h_val_off_row[i]), at, uint32_t(d.h_row_ptr[i]),
-                   uint32_t(d.h_row_ptr[i + 1]), uint32_t(d.h_row_size[i]), 0});
+    lay.push_back({uint64_t(d.h_val_off_row[i]), at, u.g0[0], u.ng[0], uint32_t(d.h_row_off[i]),
+                   uint32_t(d.h_row_size[i])});
     at += uint64_t(16) * d.h_row_size[i] * u.ng[0];
   }
   VBSR_CUDA(upload_array(&p->chunk_col, cols));
+  VBSR_CUDA(upload_array(&p->chunk_src, src));
+  VBSR_CUDA(upload_array(&p->lay, lay));
   const vbsr_status st = upload_row_units(whole, p->rows, p->row_units);
   if (st != VBSR_OK) return st;
   VBSR_CUDA(cudaMalloc(&p->w, std::max<uint64_t>(256, at)));
   VBSR_CUDA(cudaMalloc(&p->row_scale, 4 * d.M));
   VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
   VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMemcpy(p->row_scale, row_scale, 4 * d.M, cudaMemcpyDeviceToDevice));
-  LayRow* d_lay = nullptr;
-  cudaError_t e = upload_array(&d_lay, lay);
-  if (e == cudaSuccess) {
-    lay_weights_kernel<<<unsigned(d.block_rows), 256>>>(d_lay, d.d_blk_desc, values, p->w);
-    e = cudaGetLastError();
+  if (row_scale != nullptr) {
+    // the caller's arrays may come from any stream
+    VBSR_CUDA(cudaDeviceSynchronize());
+    const vbsr_status laid = lay_weights(p, values, row_scale, nullptr);
+    if (laid != VBSR_OK) return laid;
   }
-  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
-  cudaFree(d_lay);
-  VBSR_CUDA(e);
+  VBSR_CUDA(cudaStreamSynchronize(nullptr));
   return VBSR_OK;
 }
 
@@ -464,7 +505,7 @@ vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const f
   if (out == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null output");
   *out = nullptr;
   if (m == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null matrix");
-  if (row_scale == nullptr || (values == nullptr && m->d.nvalues > 0))
+  if ((row_scale == nullptr) != (values == nullptr) && (row_scale == nullptr || m->d.nvalues > 0))
     return set_error(VBSR_INVALID_ARGUMENT, "null values or row_scale");
   for (int64_t w : m->d.h_sum_w)
     if (w > kMaxRowWidth)
@@ -472,14 +513,14 @@ vbsr_status vbsr_int8_create(const vbsr_matrix* m, const int8_t* values, const f
                        "a block row of 131072 columns or more could overflow the 32-bit sum");
   auto* p = new (std::nothrow) vbsr_int8;
   if (p == nullptr) return set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
-  p->m = m;
   p->device = m->d.device;
   p->M = m->d.M;
   p->K = m->d.K;
+  p->nvalues = m->d.nvalues;
   DeviceGuard guard(p->device);
   vbsr_status st;
   try {
-    st = build_int8(p, values, row_scale);
+    st = build_int8(p, m->d, values, row_scale);
   } catch (const std::bad_alloc&) {
     st = set_error(VBSR_OUT_OF_MEMORY, "host allocation failed");
   }
@@ -495,6 +536,16 @@ vbsr_status vbsr_int8_destroy(vbsr_int8* p) {
   clear_error();
   free_int8(p);
   return VBSR_OK;
+}
+
+vbsr_status vbsr_int8_set_values(vbsr_int8* p, const int8_t* values, const float* row_scale,
+                                 vbsr_stream_t stream) {
+  clear_error();
+  if (p == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null plan");
+  if (row_scale == nullptr || (values == nullptr && p->nvalues > 0))
+    return set_error(VBSR_INVALID_ARGUMENT, "null values or row_scale");
+  DeviceGuard guard(p->device);
+  return lay_weights(p, values, row_scale, reinterpret_cast<cudaStream_t>(stream));
 }
 
 vbsr_status vbsr_int8_workspace_bytes(const vbsr_int8* p, int64_t tokens, int64_t* bytes) {
@@ -517,6 +568,7 @@ vbsr_status vbsr_int8_execute(const vbsr_int8* p, const int8_t* Q, const float* 
   if (st != VBSR_OK || tokens == 0) return st;
   if (Q == nullptr || token_scale == nullptr || C == nullptr)
     return set_error(VBSR_INVALID_ARGUMENT, "null Q, token_scale or C");
+  if (!p->has_weights) return set_error(VBSR_INVALID_ARGUMENT, "the plan has no weights yet");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -535,6 +587,7 @@ vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t 
   if (st == VBSR_OK) st = check_workspace(workspace, workspace_bytes, need);
   if (st != VBSR_OK || tokens == 0) return st;
   if (B == nullptr || C == nullptr) return set_error(VBSR_INVALID_ARGUMENT, "null B or C");
+  if (!p->has_weights) return set_error(VBSR_INVALID_ARGUMENT, "the plan has no weights yet");
   DeviceGuard guard(p->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
