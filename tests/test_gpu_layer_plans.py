@@ -188,3 +188,32 @@ def test_int8_creation_waits_for_weights_made_on_another_stream(cuda):
         vb.Int8Plan(M, q2, s2).execute_panel(X, C)
         torch.cuda.synchronize()
         assert torch.equal(C, want)
+
+
+def test_new_plans_are_usable_from_any_stream_at_once(cuda):
+    """A plan's tables are complete when its creation returns, whatever stream runs its first call."""
+    torch = cuda
+    m = ref.matrix(300, 40, 12, 31)
+    bare, v = structure(m), torch.from_numpy(m.values).cuda()
+    X, dH = panel(torch, 9, m.scalar_cols(), 1), panel(torch, 9, m.scalar_rows(), 2)
+    rng = np.random.default_rng(3)
+    q = torch.from_numpy(rng.integers(-127, 128, len(m.values)).astype(np.int8)).cuda()
+    scale = torch.ones(m.scalar_rows(), device="cuda")
+    want = None
+    torch.cuda.synchronize()
+    for k in range(12):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            out = [torch.zeros_like(v) for _ in range(3)] + [torch.zeros_like(dH) for _ in range(4)]
+            vb.OrthoPlan(bare).execute(v, out[0], stream=s)
+            plan = vb.GatedPlan(bare, bare)
+            plan.set_values(v, v, stream=s)
+            plan.execute(X, *out[3:6], stream=s)
+            plan.backward(X, out[4], out[5], dH, None, out[1], out[2], stream=s)
+            i8 = vb.Int8Plan(bare)
+            i8.set_values(q, scale, stream=s)
+            i8.execute_panel(X, out[6], stream=s)
+        s.synchronize()
+        want = want or [t.clone() for t in out]
+        for a, b in zip(want, out):
+            assert torch.equal(a, b), k

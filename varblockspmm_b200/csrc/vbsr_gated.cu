@@ -88,7 +88,7 @@ struct vbsr_gated {
   uint32_t* group_col = nullptr;
   PackRow* pack = nullptr;
   int pack_rows = 0;
-  // work units with every block row (column) whole, and cut into 2, 4 and 8 parts
+  // work units with every block row (column) whole, and cut into 2, 4 and 8 parts, as far as calls choose them
   RowUnit* rows[4] = {};
   int row_units[4] = {};
   int max_height = 64;
@@ -98,6 +98,7 @@ struct vbsr_gated {
   GradUnit* grads = nullptr;
   int grad_units = 0;
   int* d_status = nullptr;
+  char* memory = nullptr;  // of all the above
 };
 
 namespace {
@@ -230,6 +231,8 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
   std::vector<uint32_t> group_col;
   std::vector<uint32_t> g0[2], ng[2];
   std::vector<PackRow> pack;
+  group_col.reserve(size_t(8 * (gate.nnzb + up.nnzb)));
+  pack.reserve(size_t(2 * R));
   for (int which = 0; which < 2; ++which) {
     const MatrixData& d = *m[which];
     for (int i = 0; i < R; ++i) {
@@ -248,10 +251,12 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
   }
   if (group_col.size() >= (size_t(1) << 31))
     return set_error(VBSR_INVALID_ARGUMENT, "matrices exceed the plan's index range");
-  VBSR_CUDA(upload_array(&p->group_col, group_col));
+  PlanMemory mem;
+  const size_t all_groups = group_col.size();
+  mem.table(&p->group_col, std::move(group_col));
   p->pack_rows = int(std::max<size_t>(1, pack.size()));
   if (pack.empty()) pack.push_back({0, 0, 8});
-  VBSR_CUDA(upload_array(&p->pack, pack));
+  mem.table(&p->pack, std::move(pack));
 
   std::vector<RowUnit> whole_rows(R);
   for (int i = 0; i < R; ++i) {
@@ -263,50 +268,51 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
       whole_rows[i].w0[which] = uint64_t(4 * m[which]->h_val_off_row[i] + (which ? p->up_byte : 0));
     }
   }
-  const vbsr_status su = upload_row_units(whole_rows, p->rows, p->row_units);
-  if (su != VBSR_OK) return su;
+  add_row_units(mem, whole_rows, p->num_sm, p->rows, p->row_units);
 
-  // blocks by block column, gate then up, in stages of at most 64 rows
-  std::vector<std::vector<ColEntry>> by_col(S);
-  for (int which = 0; which < 2; ++which) {
-    const MatrixData& d = *m[which];
-    for (int i = 0; i < R; ++i) {
-      int64_t val = d.h_val_off_row[i];
-      for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
-        const int h = d.h_row_size[i], c = d.h_block_col[b];
-        by_col[c].push_back({uint32_t((which ? p->M / 8 : 0) + d.h_row_off[i] / 8), uint32_t(h / 8),
-                             uint64_t(4 * val + (which ? p->up_byte : 0))});
-        val += int64_t(h) * d.h_col_size[c];
-      }
-    }
-  }
-  std::vector<ColEntry> entries;
+  // blocks by block column, gate then up, in stages of at most 64 rows: counted, then written
   std::vector<ColUnit> whole(S);
   std::vector<int64_t> col_rows(S, 0);
-  int64_t col0 = 0;
-  for (int c = 0; c < S; ++c) {
-    ColUnit& u = whole[c];
-    u.col0 = uint32_t(col0);
-    u.w = uint32_t(m[0]->h_col_size[c]);
-    u.s0 = uint32_t(entries.size() / kColEntries);
-    col0 += u.w;
-    uint32_t in_stage = 0, groups = 0;
-    for (const ColEntry& e : by_col[c]) {
-      if (in_stage == 0 || in_stage == kColEntries || groups + e.h8 > 8) {
-        entries.resize((entries.size() + kColEntries - 1) / kColEntries * kColEntries);
-        in_stage = groups = 0;
-        ++u.ns;
+  std::vector<ColEntry> entries;
+  struct Fill {
+    uint32_t stages = 0, entries = 0, groups = 0;  // entries and groups of the last stage
+  };
+  for (const bool write : {false, true}) {
+    std::vector<Fill> fill(S);
+    for (int which = 0; which < 2; ++which) {
+      const MatrixData& d = *m[which];
+      for (int i = 0; i < R; ++i) {
+        const uint32_t h = uint32_t(d.h_row_size[i]);
+        int64_t val = d.h_val_off_row[i];
+        for (int b = d.h_row_ptr[i]; b < d.h_row_ptr[i + 1]; ++b) {
+          const int c = d.h_block_col[b];
+          Fill& f = fill[c];
+          if (f.stages == 0 || f.entries == kColEntries || f.groups + h / 8 > 8) f = {f.stages + 1, 0, 0};
+          if (write)
+            entries[size_t(whole[c].s0 + f.stages - 1) * kColEntries + f.entries] = {
+                uint32_t((which ? p->M / 8 : 0) + d.h_row_off[i] / 8), h / 8,
+                uint64_t(4 * val + (which ? p->up_byte : 0))};
+          else
+            col_rows[c] += h;
+          ++f.entries;
+          f.groups += h / 8;
+          val += int64_t(h) * d.h_col_size[c];
+        }
       }
-      entries.push_back(e);
-      ++in_stage;
-      groups += e.h8;
-      col_rows[c] += 8 * e.h8;
     }
-    entries.resize((entries.size() + kColEntries - 1) / kColEntries * kColEntries);
+    if (write) break;
+    uint32_t col0 = 0, stages = 0;
+    for (int c = 0; c < S; ++c) {
+      whole[c] = ColUnit{col0, uint32_t(m[0]->h_col_size[c]), stages, fill[c].stages, 0, {}};
+      col0 += whole[c].w;
+      stages += whole[c].ns;
+    }
+    entries.resize(size_t(stages) * kColEntries);
   }
-  VBSR_CUDA(upload_array(&p->entries, entries));
-  for (int f = 0; f < 4; ++f) {
-    std::vector<std::pair<int64_t, ColUnit>> cols;
+  mem.table(&p->entries, std::move(entries));
+  std::vector<std::pair<int64_t, ColUnit>> cols;  // with the rows that it sums over
+  for (int f = 0; f < 4 && (f == 0 || finer_parts(p->col_units[f - 1], p->num_sm)); ++f) {
+    cols.clear();
     for (int c = 0; c < S; ++c) {
       const int w = int(whole[c].w), wp = std::max(8, (w / 8 + (1 << f) - 1) / (1 << f) * 8);
       for (int c0 = 0; c0 < w; c0 += wp) {
@@ -314,18 +320,20 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
         u.c0 = uint32_t(c0);
         u.col0 += u.c0;
         u.w = uint32_t(std::min(wp, w - c0));
-        cols.push_back({-col_rows[c] * (32 + int64_t(u.w)), u});
+        cols.push_back({col_rows[c], u});
       }
     }
-    std::stable_sort(cols.begin(), cols.end(),
-                     [](const auto& a, const auto& b) { return a.first < b.first; });
     std::vector<ColUnit> sorted;
-    for (const auto& c : cols) sorted.push_back(c.second);
-    VBSR_CUDA(upload_units(&p->cols[f], &p->col_units[f], sorted));
+    sorted.reserve(cols.size());
+    for (const auto& c : by_cost(cols, [](const auto& x) { return x.first * (32 + int64_t(x.second.w)); }))
+      sorted.push_back(c.second);
+    p->col_units[f] = int(sorted.size());
+    mem.table(&p->cols[f], std::move(sorted));
   }
 
-  // weight gradients: 16 groups (128 columns) of a block row at a time
+  // weight gradients: 16 groups (128 columns) of a block row at a time, the largest first
   std::vector<GradUnit> grads;
+  grads.reserve(all_groups / 16 + 2 * size_t(R));
   for (int which = 0; which < 2; ++which)
     for (int i = 0; i < R; ++i)
       for (uint32_t g = 0; g < ng[which][i]; g += 16) {
@@ -334,40 +342,29 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
                          uint32_t((which ? p->M / 8 : 0) + m[which]->h_row_off[i] / 8), uint32_t(h),
                          uint64_t(m[which]->h_val_off_row[i] + int64_t(g) * 8 * h), uint32_t(which), 0});
       }
-  std::stable_sort(grads.begin(), grads.end(), [](const GradUnit& a, const GradUnit& b) {
-    return (32 + a.h) * (8 + a.ng) > (32 + b.h) * (8 + b.ng);
-  });
-  VBSR_CUDA(upload_units(&p->grads, &p->grad_units, grads));
+  mem.table(&p->grads, by_cost(grads, [](const GradUnit& u) { return (32 + u.h) * (8 + u.ng); }));
+  p->grad_units = int(grads.size());
 
-  VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMalloc(&p->w, p->up_byte + std::max<int64_t>(256, 4 * m[1]->nvalues)));
-  VBSR_CUDA(cudaMalloc(&p->w_exp, sizeof(int)));
-  VBSR_CUDA(cudaMalloc(&p->w_partial, kPartialBytes));
+  mem.table(&p->d_status, std::vector<int>(kStatusWords));
+  mem.room(&p->w, p->up_byte + 4 * up.nvalues);
+  mem.room(&p->w_exp, sizeof(int));
+  mem.room(&p->w_partial, kPartialBytes);
+  SetupStream s;  // after `mem`: it waits before that goes
+  VBSR_CUDA(s.init());
+  VBSR_CUDA(mem.make(&p->memory, s.s));
   if ((!gate.structure_only && !up.structure_only) || gate.nvalues + up.nvalues == 0) {
-    const vbsr_status st = pack_weights<true>(p, gate.d_values, up.d_values, nullptr);
+    const vbsr_status st = pack_weights<true>(p, gate.d_values, up.d_values, s.s);
     if (st != VBSR_OK) return st;
     p->has_weights = true;
   }
-  VBSR_CUDA(cudaStreamSynchronize(nullptr));
+  VBSR_CUDA(s.finish());
   return VBSR_OK;
 }
 
 void free_gated(vbsr_gated* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
-  cudaFree(p->w);
-  cudaFree(p->w_exp);
-  cudaFree(p->w_partial);
-  cudaFree(p->group_col);
-  cudaFree(p->pack);
-  for (int f = 0; f < 4; ++f) {
-    cudaFree(p->rows[f]);
-    cudaFree(p->cols[f]);
-  }
-  cudaFree(p->entries);
-  cudaFree(p->grads);
-  cudaFree(p->d_status);
+  cudaFree(p->memory);
   delete p;
 }
 

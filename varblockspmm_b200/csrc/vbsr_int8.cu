@@ -35,6 +35,7 @@ struct vbsr_int8 {
   int max_height = 64;
   float* row_scale = nullptr;
   int* d_status = nullptr;
+  char* memory = nullptr;  // of all the above
 };
 
 namespace {
@@ -428,13 +429,7 @@ vbsr_status launch_chunks(const vbsr_int8* p, const Geometry& g, const void* src
 void free_int8(vbsr_int8* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
-  cudaFree(p->w);
-  cudaFree(p->chunk_col);
-  cudaFree(p->lay);
-  cudaFree(p->chunk_src);
-  for (RowUnit* r : p->rows) cudaFree(r);
-  cudaFree(p->row_scale);
-  cudaFree(p->d_status);
+  cudaFree(p->memory);
   delete p;
 }
 
@@ -476,22 +471,23 @@ vbsr_status build_int8(vbsr_int8* p, const MatrixData& d, const int8_t* values, 
                    uint32_t(d.h_row_size[i])});
     at += uint64_t(16) * d.h_row_size[i] * u.ng[0];
   }
-  VBSR_CUDA(upload_array(&p->chunk_col, cols));
-  VBSR_CUDA(upload_array(&p->chunk_src, src));
-  VBSR_CUDA(upload_array(&p->lay, lay));
-  const vbsr_status st = upload_row_units(whole, p->rows, p->row_units);
-  if (st != VBSR_OK) return st;
-  VBSR_CUDA(cudaMalloc(&p->w, std::max<uint64_t>(256, at)));
-  VBSR_CUDA(cudaMalloc(&p->row_scale, 4 * d.M));
-  VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
+  PlanMemory mem;
+  mem.table(&p->chunk_col, std::move(cols));
+  mem.table(&p->chunk_src, std::move(src));
+  mem.table(&p->lay, std::move(lay));
+  add_row_units(mem, whole, p->num_sm, p->rows, p->row_units);
+  mem.table(&p->d_status, std::vector<int>(kStatusWords));
+  mem.room(&p->w, int64_t(at));
+  mem.room(&p->row_scale, 4 * d.M);
+  SetupStream s;  // after `mem`: it waits before that goes
+  VBSR_CUDA(s.init());
+  VBSR_CUDA(mem.make(&p->memory, s.s));
   if (row_scale != nullptr) {
-    // the caller's arrays may come from any stream
-    VBSR_CUDA(cudaDeviceSynchronize());
-    const vbsr_status laid = lay_weights(p, values, row_scale, nullptr);
+    VBSR_CUDA(cudaDeviceSynchronize());  // the caller's arrays may come from any stream
+    const vbsr_status laid = lay_weights(p, values, row_scale, s.s);
     if (laid != VBSR_OK) return laid;
   }
-  VBSR_CUDA(cudaStreamSynchronize(nullptr));
+  VBSR_CUDA(s.finish());
   return VBSR_OK;
 }
 

@@ -3,10 +3,13 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <memory>
 #include <string>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "vbsr_internal.h"
@@ -27,14 +30,44 @@ inline vbsr_status check_workspace(const void* ws, int64_t bytes, int64_t need) 
   return VBSR_OK;
 }
 
-// Device copy of a host array (one element at least).
-template <class T>
-cudaError_t upload_array(T** dst, const std::vector<T>& src) {
-  const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(dst),
-                                   (src.empty() ? 1 : src.size()) * sizeof(T));
-  if (e != cudaSuccess || src.empty()) return e;
-  return cudaMemcpy(*dst, src.data(), src.size() * sizeof(T), cudaMemcpyHostToDevice);
-}
+// A plan's device memory: one allocation, with tables copied from the host and room for what kernels write, each
+// 256-byte aligned.
+class PlanMemory {
+ public:
+  template <class T>
+  void table(T** dst, std::vector<T> src) {
+    const auto kept = std::make_shared<std::vector<T>>(std::move(src));
+    add(reinterpret_cast<void**>(dst), kept->size() * sizeof(T), kept->data(), kept);
+  }
+  template <class T>
+  void room(T** dst, int64_t bytes) {
+    add(reinterpret_cast<void**>(dst), size_t(bytes), nullptr, nullptr);
+  }
+  // Allocates *base, sets the pointers and enqueues the copies. This object must live until `s` has been waited for.
+  cudaError_t make(char** base, cudaStream_t s) {
+    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(base), std::max<size_t>(bytes_, 1));
+    for (size_t i = 0; i < parts_.size() && e == cudaSuccess; ++i) {
+      const Part& p = parts_[i];
+      *p.dst = *base + p.at;
+      if (p.src != nullptr && p.bytes > 0) e = cudaMemcpyAsync(*p.dst, p.src, p.bytes, cudaMemcpyHostToDevice, s);
+    }
+    return e;
+  }
+
+ private:
+  struct Part {
+    void** dst;
+    size_t at, bytes;
+    const void* src;
+    std::shared_ptr<void> kept;
+  };
+  void add(void** dst, size_t bytes, const void* src, std::shared_ptr<void> kept) {
+    parts_.push_back({dst, bytes_, bytes, src, std::move(kept)});
+    bytes_ += size_t(align256(int64_t(std::max<size_t>(bytes, 1))));
+  }
+  std::vector<Part> parts_;
+  size_t bytes_ = 0;
+};
 
 // Reads and clears a plan's device status word after the work on `s`.
 inline vbsr_status read_status(int* d_status, cudaStream_t s) {

@@ -52,6 +52,7 @@ struct vbsr_ortho {
   int device = 0, big_ctas = 0, small_ctas = 0;  // of blocks of more than 32 rows, which come first; others
   OrthoSlot* slots = nullptr;
   int* d_status = nullptr;
+  char* memory = nullptr;  // of both
 };
 
 namespace {
@@ -495,8 +496,7 @@ __global__ void __launch_bounds__(128, 3) ortho_big_kernel(OrthoParams p) {
 void free_ortho(vbsr_ortho* p) {
   if (p == nullptr) return;
   DeviceGuard guard(p->device);
-  cudaFree(p->slots);
-  cudaFree(p->d_status);
+  cudaFree(p->memory);
   delete p;
 }
 
@@ -531,9 +531,13 @@ vbsr_status build_ortho(vbsr_ortho* p, const MatrixData& d) {
   for (int mt = 2; mt >= 1; --mt)
     for (int nt = 4; nt >= mt; --nt) pack(by_class[mt][nt], mt == 2 ? 2 : 4);
   p->small_ctas = int(slots.size() / 4) - p->big_ctas;
-  VBSR_CUDA(upload_array(&p->slots, slots));
-  VBSR_CUDA(cudaMalloc(&p->d_status, kStatusWords * sizeof(int)));
-  VBSR_CUDA(cudaMemset(p->d_status, 0, kStatusWords * sizeof(int)));
+  PlanMemory mem;
+  mem.table(&p->slots, std::move(slots));
+  mem.table(&p->d_status, std::vector<int>(kStatusWords));
+  SetupStream s;  // after `mem`: it waits before that goes
+  VBSR_CUDA(s.init());
+  VBSR_CUDA(mem.make(&p->memory, s.s));
+  VBSR_CUDA(s.finish());
   return VBSR_OK;
 }
 

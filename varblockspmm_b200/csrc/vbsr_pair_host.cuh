@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "vbsr_lm.cuh"
@@ -71,18 +72,29 @@ int aligned16(const P*... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
 }
 
-template <class T>
-cudaError_t upload_units(T** dst, int* count, const std::vector<T>& v) {
-  *count = int(v.size());
-  return upload_array(dst, v);
+// Sorted by falling cost, equal ones in their order.
+template <class T, class Cost>
+std::vector<T> by_cost(const std::vector<T>& v, Cost cost) {
+  std::vector<std::pair<uint64_t, uint32_t>> key(v.size());
+  for (size_t i = 0; i < v.size(); ++i) key[i] = {~uint64_t(cost(v[i])), uint32_t(i)};
+  std::sort(key.begin(), key.end());
+  std::vector<T> out;
+  out.reserve(v.size());
+  for (const auto& k : key) out.push_back(v[k.second]);
+  return out;
 }
 
+// Whether any call can choose parts finer than those that give `units` (parts_for, with one tile).
+inline bool finer_parts(int units, int num_sm) { return 2 * int64_t(units) < num_sm; }
+
 // Units of the block rows (given whole, shape = height), cut into 1, 2, 4 and 8 parts where their height
-// allows, the largest first: the grid strides over them, which evens out the SMs' shares. A unit's cost is
-// its weights' bytes and as much as 32 rows' for the activations.
-inline vbsr_status upload_row_units(const std::vector<RowUnit>& whole, RowUnit* (&rows)[4], int (&count)[4]) {
-  for (int f = 0; f < 4; ++f) {
-    std::vector<RowUnit> units;
+// allows and as far as calls can choose them, the largest first: the grid strides over them, which evens out
+// the SMs' shares. A unit's cost is its weights' bytes and as much as 32 rows' for the activations.
+inline void add_row_units(PlanMemory& mem, const std::vector<RowUnit>& whole, int num_sm, RowUnit* (&rows)[4],
+                          int (&count)[4]) {
+  std::vector<RowUnit> units;
+  for (int f = 0; f < 4 && (f == 0 || finer_parts(count[f - 1], num_sm)); ++f) {
+    units.clear();
     for (const RowUnit& w : whole) {
       const int h = int(w.shape), hp = std::max(8, (h / 8 + (1 << f) - 1) / (1 << f) * 8);
       for (int r0 = 0; r0 < h; r0 += hp) {
@@ -92,15 +104,11 @@ inline vbsr_status upload_row_units(const std::vector<RowUnit>& whole, RowUnit* 
         units.push_back(u);
       }
     }
-    std::stable_sort(units.begin(), units.end(), [](const RowUnit& a, const RowUnit& b) {
-      auto cost = [](const RowUnit& u) {
-        return uint64_t(u.ng[0] + u.ng[1]) * (32 + ((u.shape >> 8) & 255u));
-      };
-      return cost(a) > cost(b);
-    });
-    VBSR_CUDA(upload_units(&rows[f], &count[f], units));
+    mem.table(&rows[f], by_cost(units, [](const RowUnit& u) {
+                return uint64_t(u.ng[0] + u.ng[1]) * (32 + ((u.shape >> 8) & 255u));
+              }));
+    count[f] = int(units.size());
   }
-  return VBSR_OK;
 }
 
 }  // namespace vbsr_b200
