@@ -135,10 +135,11 @@ def _activations(tokens, features, g):
     return x
 
 
-def _host(vb, st, values):
-    return vb.HostMatrix(len(st["row_size"]), len(st["col_size"]), st["row_ptr"], st["block_col"],
-                         st["row_size"], st["col_size"], st["row_off"], st["col_off"],
-                         st["value_off"], values.cpu().numpy())
+def _matrix(vb, st):
+    """The structure alone: plans are made before there are values."""
+    host = vb.HostMatrix(len(st["row_size"]), len(st["col_size"]), st["row_ptr"], st["block_col"],
+                         st["row_size"], st["col_size"], st["row_off"], st["col_off"], st["value_off"])
+    return vb.Matrix(host, structure_only=True)
 
 
 def _inputs(case, seed):
@@ -182,8 +183,7 @@ def prepare(case, seed):
         if op in ("gated", "train"):
             act = {"silu": vb.Activation.SiLU, "gelu": vb.Activation.GELU, "relu": vb.Activation.ReLU,
                    "sigmoid": vb.Activation.Sigmoid}[case["act"]]
-            s["plan"] = vb.GatedPlan(vb.Matrix(_host(vb, st, s["gate"])),
-                                     vb.Matrix(_host(vb, s["st_up"], s["up"])), act)
+            s["plan"] = vb.GatedPlan(_matrix(vb, st), _matrix(vb, s["st_up"]), act)
             s["H"] = torch.empty(T, M, device=dev)
             need = s["plan"].workspace_bytes(T, backward=op == "train")
             s["workspace"] = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -192,12 +192,11 @@ def prepare(case, seed):
                 s["dX"] = torch.empty(T, K, device=dev)
                 s["dgate"], s["dup"] = torch.empty_like(s["gate"]), torch.empty_like(s["up"])
         elif op == "int8":
-            m = vb.Matrix(_host(vb, st, s["values"].float()))
-            s["plan"] = vb.Int8Plan(m, s["values"], s["row_scale"])
+            s["plan"] = vb.Int8Plan(_matrix(vb, st))
             s["C"] = torch.empty(T, M, device=dev)
             s["workspace"] = torch.empty(s["plan"].workspace_bytes(T), dtype=torch.uint8, device=dev)
         else:
-            s["plan"] = vb.OrthoPlan(vb.Matrix(_host(vb, st, s["grad"])))
+            s["plan"] = vb.OrthoPlan(_matrix(vb, st))
             s["out"] = torch.empty_like(s["grad"])
     elif op in ("gated", "train"):
         s["sub"], s["sub_up"] = _sub_blocks(st), _sub_blocks(s["st_up"])
@@ -269,8 +268,10 @@ def _newton_schulz(x):
 def run(s):
     op = s["case"]["op"]
     if own:
+        # the weights are packed values, as for the plain form: what the kernels make of them is part of the pass
         stream = torch.cuda.current_stream()
         if op == "gated":
+            s["plan"].set_values(s["gate"], s["up"], stream=stream)
             s["plan"].execute(s["X"], s["H"], workspace=s["workspace"], stream=stream)
             return s["H"]
         if op == "train":
@@ -280,6 +281,7 @@ def run(s):
                                workspace=s["workspace"], stream=stream)
             return {"H": s["H"], "dX": s["dX"], "dgate": s["dgate"], "dup": s["dup"]}
         if op == "int8":
+            s["plan"].set_values(s["values"], s["row_scale"], stream=stream)
             s["plan"].execute_panel(s["X"], s["C"], workspace=s["workspace"], stream=stream)
             return s["C"]
         s["plan"].execute(s["grad"], s["out"], steps=_STEPS, eps=_EPS, coefficients=_COEF, stream=stream)
