@@ -99,8 +99,8 @@ __device__ __forceinline__ void pair2(float x, float y, uint32_t& hi, uint32_t& 
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// |V| as 2^e |V / 2^e| with 2^e about the largest magnitude, so that the squares neither overflow nor vanish;
-// a NaN or infinity makes the sum NaN or infinite, and then the block.
+// |V| as 2^e |V / 2^e| with 2^e about the largest magnitude, so that the squares neither overflow nor vanish:
+// the sum is 0 for a block of zeros alone, and not finite only where a value is not.
 struct Norm {
   int e;
   float down;
@@ -113,10 +113,11 @@ struct Norm {
     const float y = v * down;
     return fmaf(y, y, sum);
   }
-  // kScale / (|V| + eps) times 2^e, 0 for a block of zeros without eps
+  // kScale / (|V| + eps) times 2^e; 0 for a block of zeros (kScale / eps may overflow), NaN for one with a NaN or
+  // an infinity
   __device__ __forceinline__ float inverse(float sum, float eps) const {
-    const float norm = sqrtf(sum) + eps * down;
-    return norm == 0.0f ? 0.0f : kScale / norm;
+    if (sum == 0.0f) return 0.0f;
+    return sum < __int_as_float(0x7f800000) ? kScale / (sqrtf(sum) + eps * down) : __int_as_float(0x7fc00000);
   }
   __device__ __forceinline__ float apply(float v, float inv) const { return v * down * inv; }
 };
