@@ -201,7 +201,11 @@ struct PanelJob {
   int dy_splits;
 };
 
-__device__ __forceinline__ float scale_for(int e) { return e < -126 ? 0.0f : pow2(e); }  // below: less than 1
+// 2^e down to the smallest subnormal number. A token of a stage's sums may have e below -126 where its x is near
+// the largest fp32 number; below -149 its products are under 2^-35 of the stage's largest.
+__device__ __forceinline__ float scale_for(int e) {
+  return e >= -126 ? pow2(e) : (e >= -149 ? __int_as_float(1 << (e + 149)) : 0.0f);
+}
 // A token's exponent, with the weights' exponent w.
 __device__ __forceinline__ int token_exponent(float amax, int w) {
   return min(126 - w, max(-126 - w, pair_exponent(amax)));
