@@ -62,3 +62,46 @@ def test_weight_gradients_of_activations_near_the_largest_number(cuda, tokens, l
     want = ref.sampled(m, want)
     for got in out:
         assert np.all(np.abs(got.cpu().numpy().astype(np.float64) - want) <= tol)
+
+
+@pytest.mark.parametrize("kind", [vb.Activation.SiLU, vb.Activation.Sigmoid])
+def test_activations_and_derivatives_in_their_tails(cuda, kind):
+    """act(G) U and act'(G) over the whole range of G, against 64 bits. Sigmoids of x and -x are each off by
+    (6 + 1.2 |x|) 2^-23 of themselves (see act_both), a product of them with one another or with x by the sum and
+    a rounding; dB passes through a product with the unit matrix, which holds values to 2^-23 twice, and, as a
+    token's gradients of gate and up share one power of two, to no better than 2^-50 of the largest of both:
+    that one is in [2^14, 2^15) as the high half, half a step of the low half's smallest numbers is
+    2^-25 2^-11 = 2^-36."""
+    torch = cuda
+    unit = vb.HostMatrix(1, 1, [0, 1], [0], [8], [8], [0, 8], [0, 8], [0, 64], np.eye(8, dtype=np.float32).reshape(-1))
+    none = vb.HostMatrix(1, 1, [0, 0], [], [8], [8], [0, 8], [0, 8], [0], [])
+    x = np.concatenate([np.linspace(-80, 80, 2001), np.linspace(-3, 3, 600), [0.0, -1e-30, 1e-30]]).astype(np.float32)
+    T = len(x)
+    G = torch.from_numpy(np.repeat(x[:, None], 8, axis=1)).cuda()  # a value to a token: each has its own scale
+    ones, dB = torch.ones(T, 8, device="cuda"), torch.full((T, 8), float("nan"), device="cuda")
+    # backward, up without blocks: dB = act'(G)
+    plan = vb.GatedPlan(vb.Matrix(unit), vb.Matrix(none), kind)
+    plan.backward(ones, G, ones, ones, dB)
+    plan.check_status()
+    x64 = x.astype(np.float64)
+    s, c = np.exp(-np.logaddexp(0, -x64)), np.exp(-np.logaddexp(0, x64))
+    rel = (6 + 1.2 * np.abs(x64)) * 2.0 ** -23
+    if kind == vb.Activation.Sigmoid:
+        want, size = s * c, s * c
+    else:
+        want, size = s * (1 + x64 * c), s * (1 + np.abs(x64) * c)
+    a64 = s if kind == vb.Activation.Sigmoid else np.abs(x64) * s  # dU
+    tol = (2 * rel + 6 * 2.0 ** -23) * size + 2.0 ** -50 * np.maximum(a64, np.abs(want)) + 1e-37
+    got = dB.cpu().numpy().astype(np.float64)
+    over = np.abs(got - want[:, None]) / tol[:, None]
+    assert over.max() <= 1, (x[over.max(axis=1).argmax()], over.max())
+    # forward, gate and up the unit matrix: H = act(G) U with the G and U that it returns
+    plan = vb.GatedPlan(vb.Matrix(unit), vb.Matrix(unit), kind)
+    H, Gf, Uf = (torch.full((T, 8), float("nan"), device="cuda") for _ in range(3))
+    plan.execute(G, H, Gf, Uf)
+    plan.check_status()
+    g, u = Gf.cpu().numpy().astype(np.float64), Uf.cpu().numpy().astype(np.float64)
+    s = np.exp(-np.logaddexp(0, -g))
+    want = (s if kind == vb.Activation.Sigmoid else g * s) * u
+    tol = ((6 + 1.2 * np.abs(g)) * 2.0 ** -23 + 2 * 2.0 ** -24) * np.abs(want) + 1e-37
+    assert np.all(np.abs(H.cpu().numpy() - want) <= tol)

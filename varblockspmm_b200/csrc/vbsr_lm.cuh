@@ -88,21 +88,11 @@ inline vbsr_device_matrix view_of(const MatrixData& d) {
           d.d_row_size, d.d_col_size, d.d_row_off, d.d_col_off, d.d_value_off, d.d_values};
 }
 
-// Row of block b: row_ptr[row] <= b < row_ptr[row + 1].
-__device__ __forceinline__ int row_of_block(const int32_t* row_ptr, int rows, int b) {
-  int lo = 0, hi = rows;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (row_ptr[mid] <= b) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
-// An activation and its derivative. The exponential and the quotient are the fast ones: exp is off by
-// about (4 + |x|) 2^-24 of itself and the quotient by 2^-23, so the sigmoid s by (6 + |x|) s (1 - s)
-// 2^-24 and x s by less than 3 |x| 2^-24, below what the products bring with them. exp overflows to
-// infinity for x < -88, where s is then 0, as it should be; the derivative of silu is written without
-// infinity times zero.
+// An activation and its derivative. The exponential and the quotient are the fast ones, whose documented errors
+// are (2 + 1.173 |x|) 2^-23 and 2^-22 of themselves. With t = exp(-|x|), the sigmoid of |x| is r = 1 / (1 + t) and
+// that of -|x| is t r, so neither it nor its complement is a difference: both are off by at most
+// (6 + 1.2 |x|) 2^-23 of themselves, and nothing overflows. GELU's (1 + erf) / 2 is off by about 2^-24 absolutely,
+// which for x far below zero is not small against it.
 template <int ACT>
 __device__ __forceinline__ void act_both(float x, float& a, float& da) {
   if (ACT == VBSR_ACT_RELU) {
@@ -113,13 +103,14 @@ __device__ __forceinline__ void act_both(float x, float& a, float& da) {
     a = x * cdf;
     da = cdf + x * __expf(-0.5f * x * x) * 0.39894228040143268f;
   } else {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-x));
+    const float t = __expf(-fabsf(x)), r = __fdividef(1.0f, 1.0f + t), q = t * r;
+    const float s = x >= 0.0f ? r : q, c = x >= 0.0f ? q : r;  // the sigmoids of x and of -x
     if (ACT == VBSR_ACT_SIGMOID) {
       a = s;
-      da = s * (1.0f - s);
+      da = s * c;
     } else {
       a = x * s;
-      da = s * (1.0f + x * (1.0f - s));
+      da = s * (1.0f + x * c);
     }
   }
 }
