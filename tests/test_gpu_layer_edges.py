@@ -105,3 +105,53 @@ def test_activations_and_derivatives_in_their_tails(cuda, kind):
     want = (s if kind == vb.Activation.Sigmoid else g * s) * u
     tol = ((6 + 1.2 * np.abs(g)) * 2.0 ** -23 + 2 * 2.0 ** -24) * np.abs(want) + 1e-37
     assert np.all(np.abs(H.cpu().numpy() - want) <= tol)
+
+
+def by_clusters(tokens, K):
+    """Which panels Int8Plan quantises by clusters of CTAs that hold two tokens each; others take two kernels."""
+    return K <= 38400 and (tokens <= max(128, K // 24) or K > 16384)
+
+
+@pytest.mark.parametrize("tokens,K,held", [
+    (1, 968, True), (128, 960, True), (129, 960, False),  # one piece of the lanes' registers, just full and over
+    (128, 2048, True), (129, 2048, False), (129, 3096, True), (341, 8184, True), (342, 8184, False),
+    (682, 16384, True), (683, 16384, False), (683, 16392, True),  # longer ones: any number of tokens
+    (3, 20008, True), (33, 30720, True), (131, 30728, True),
+    (2, 38400, True), (259, 38400, True), (2, 38408, False), (259, 38408, False)])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_int8_every_way_of_quantising(cuda, tokens, K, held, offset):
+    """Panels on both sides of every border of the choice, one token with a NaN, one with an infinity, one of
+    zeros, at aligned and unaligned places."""
+    torch = cuda
+    assert by_clusters(tokens, K) == held
+    col_size = [64] * (K // 64) + ([K % 64] if K % 64 else [])
+    m = ref.matrix(5, len(col_size), min(25, len(col_size)), 71, row_size=[8, 24, 64, 8, 16], col_size=col_size)
+    m.block_col[m.row_ptr[1] - 1] = len(col_size) - 1  # the last columns are read
+    m = vb.HostMatrix(m.block_rows, m.block_cols, m.row_ptr, m.block_col, m.row_size, m.col_size, m.row_scalar_off,
+                      m.col_scalar_off, np.concatenate([[0], np.cumsum(np.repeat(m.row_size, np.diff(m.row_ptr)) *
+                                                                       m.col_size[m.block_col])]), [])
+    rng = np.random.default_rng(tokens)
+    q = rng.integers(-128, 128, int(m.value_off[-1])).astype(np.int8)
+    rs = (rng.random(m.scalar_rows()) + 0.1).astype(np.float32)
+    X = (rng.standard_normal((tokens, K)) * np.exp(rng.standard_normal((tokens, 1)))).astype(np.float32)
+    bad = []
+    if tokens > 2:
+        X[tokens - 1, K - 1], X[1, 0], X[0] = np.nan, -np.inf, 0.0
+        bad = [1, tokens - 1]
+    with np.errstate(all="ignore"):
+        ts = np.abs(X).max(axis=1) * (np.float32(1) / np.float32(127))
+        Q = np.clip(np.where(ts[:, None] > 0, np.rint(X.astype(np.float64) / ts[:, None].astype(np.float64)), 0),
+                    -127, 127)
+        want = (np.where(np.isfinite(Q), Q, 0) @ ref.dense(m, q).T) * (ts[:, None].astype(np.float64) * rs)
+    buf = torch.zeros(tokens * K + 8, device="cuda")
+    x = buf[offset:offset + tokens * K]
+    x.copy_(torch.from_numpy(X).cuda().reshape(-1))
+    plan = vb.Int8Plan(vb.Matrix(m, structure_only=True), torch.from_numpy(q).cuda(), torch.from_numpy(rs).cuda())
+    C = torch.full((tokens, m.scalar_rows()), 7.0, device="cuda")
+    plan.execute_panel(x, C)
+    plan.check_status()
+    got = C.cpu().numpy().astype(np.float64)
+    good = np.setdiff1d(np.arange(tokens), bad)
+    # the sum, the product of the scales and the result round once each
+    assert np.all(np.abs(got[good] - want[good]) <= 4 * ref.U * np.abs(want[good]))
+    assert np.isnan(got[bad]).all()

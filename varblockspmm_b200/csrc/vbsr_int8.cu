@@ -288,12 +288,21 @@ __global__ void __launch_bounds__(256) chunk_panel_kernel(const void* src, long 
 // read until the CTAs have exchanged their largest magnitudes through distributed shared memory. A warp reads
 // 16 neighbouring groups and writes the 15 chunks that begin in the first 15, the second half of a chunk coming
 // from the lane of the next group: 16 bytes of both tokens side by side, a whole sector of 32. Against the two
-// kernels above (whole calls, 64 block rows of 4 blocks): 64 tokens of 8192 9.8 and 12.5 us, 777 of 16384 44 and
-// 48; but 777 of 2048, which fill a quarter of a cluster's lanes, 31 and 22, and 4000 of 16384 199 and 178. One
-// token of 147000, read twice by eight SMs: 39 us, and 32 by the two kernels.
+// kernels above it saves a launch and a read, but every two tokens take a cluster, whose lanes short tokens leave
+// idle. Whole calls, 64 block rows of 4 blocks, this and the two kernels, us:
+//   tokens  K = 2048    4096        8192        16384       24576       38400
+//   64      10.0  11.5  9.8   11.8  10.4  12.9  10.7  14.1  12.2  16.4  12.7  20.1
+//   128     9.9   11.6  10.6  12.5  10.9  13.9  13.1  16.4  14.4  20.6  16.5  26.7
+//   256     14.3  12.9  14.6  15.9  16.3  16.5  18.5  22.6  20.6  28.8  24.7  41.3
+//   512     20.6  15.8  22.3  16.5  24.7  22.6  28.8  29.1  33.1  45.0  41.1  63.0
+//   1024    34.5  18.5  37.0  22.6  41.1  30.7  51.3  51.3  59.2  69.4  71.8  102
+//   4096    117   41    128   58    144   93    179   155   208   223   255   328
+// So it takes up to 128 tokens, or one for every 24 features, and any number of tokens longer than 16384.
 constexpr int kTokenCtas = 8, kTokenThreads = 256, kTokenWarps = kTokenThreads / 32, kTokenHeld = 5;
 constexpr int64_t kHeldFeatures = 8ll * 15 * kTokenCtas * kTokenWarps * kTokenHeld;  // 38400
-constexpr int64_t kFewTokens = 256, kLongTokens = 16384;
+inline bool by_clusters(int64_t tokens, int64_t K) {
+  return K <= kHeldFeatures && (tokens <= std::max<int64_t>(128, K / 24) || K > 16384);
+}
 __global__ void __cluster_dims__(kTokenCtas) __launch_bounds__(kTokenThreads, 4)
     token_chunks_kernel(const float* B, long long tokens, long long rows, long long K, int R, int vec,
                         float* token_scale, char* out) {
@@ -589,7 +598,7 @@ vbsr_status vbsr_int8_execute_panel(const vbsr_int8* p, const float* B, int64_t 
   char* ws = static_cast<char*>(workspace);
   const Geometry g = geometry_of(p, tokens);
   const int vec = aligned16(B);
-  if (p->K <= kHeldFeatures && (tokens <= kFewTokens || p->K > kLongTokens)) {
+  if (by_clusters(tokens, p->K)) {
     const int64_t rows = g.tiles * g.R;
     token_chunks_kernel<<<unsigned((rows + 1) / 2 * kTokenCtas), kTokenThreads, 0, s>>>(
         B, tokens, rows, p->K, g.R, vec, reinterpret_cast<float*>(ws + g.scale_at), ws + g.panel_at);
