@@ -302,9 +302,16 @@ enum {
  * replaced by vbsr_gated_set_values; the matrices are not needed after creation. Where one of them holds
  * its structure only, the plan has no weights until the first vbsr_gated_set_values, and forward and
  * backward calls (of one token or more) are refused.
- * Products are formed at FP32 accuracy, each token's whatever the others hold; weights below 2^-28 of the
- * largest of both matrices, or activations below 2^-28 of their token's largest, are held to 2^-51 of
- * that. A token that holds a NaN or an infinity has results that are not finite in the rows that read it;
+ * Products are close to FP32 arithmetic, each token's whatever the others hold. Operands are held to 2^-23
+ * of themselves (FP32: 2^-24), and G, U and the gradients are off by 3e-7 to 4e-7 in the 2-norm, where
+ * plain FP32 arithmetic is off by 1.5e-7 to 6e-7. Small operands beside large ones are held less exactly:
+ * weights below 2^-27 of the largest of both matrices, activations below 2^-27 of their token's largest, and
+ * gradients dG and dU below 2^-27 of the largest of both in their token are held to 2^-50 of that. In the
+ * weight gradients, which sum over tokens, the same goes for a token whose largest product of activation
+ * and gradient is below 2^-27 of the largest such product of up to 64 tokens around it. The activations'
+ * exponentials and quotients are the fast ones: sigmoids are off by at most (6 + 1.2 |x|) 2^-23 of
+ * themselves, GELU's distribution function by about 2^-24 absolutely.
+ * A token that holds a NaN or an infinity has results that are not finite in the rows that read it;
  * the other tokens are not touched by it (the weight gradients sum over tokens and are). */
 typedef struct vbsr_gated vbsr_gated;
 vbsr_status vbsr_gated_create(const vbsr_matrix* gate, const vbsr_matrix* up, int activation,
@@ -379,8 +386,9 @@ vbsr_status vbsr_matrix_quantize(const vbsr_matrix* m, int8_t* values, float* ro
  * of the matrix's values) is replaced by `steps` Newton-Schulz steps
  *   X = V / (|V|_F + eps); then X <- a X + (b A + c A A) X with A = X X^T
  * with (a, b, c) = coefficients[0..2]. `out` may be `values` itself. A block of zeros gives zeros; one that
- * holds a NaN or an infinity gives NaN, the others are not touched by it. The products are at FP32
- * accuracy as long as the iterates' entries stay below 2^10 in magnitude and those of b A + c A A below
+ * holds a NaN or an infinity gives NaN, the others are not touched by it. Operands of the products are held
+ * to 2^-23 of themselves, and five steps are off by 1.1e-6 to 1.3e-6 in the 2-norm (plain FP32 arithmetic:
+ * 1.0e-6 to 1.1e-6), as long as the iterates' entries stay below 2^10 in magnitude and those of b A + c A A below
  * 2^5, as they do by far for coefficients that keep singular values near one; larger ones give
  * infinities or NaN. steps in [0, 64]; `m` gives the structure and is not needed after creation. */
 typedef struct vbsr_ortho vbsr_ortho;

@@ -287,7 +287,7 @@ __device__ __forceinline__ void orthogonalize(const OrthoParams& p, const OrthoS
     }
 }
 
-// Two to four warps a block: two blocks of more than 16 rows in a CTA, or four.
+// Two warps a block of more than 16 rows, two of them in a CTA, or one warp a block, four in a CTA.
 __global__ void __launch_bounds__(128, 4) ortho_small_kernel(OrthoParams p) {
   extern __shared__ __align__(16) char sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -3,12 +3,12 @@
 // FP32 accuracy from 16-bit tensor-core products. Every fp32 operand x is held as a pair of fp16
 // numbers: with a power of two 2^e that brings the largest magnitude (of the weights, or of a token's
 // activations or gradients) into [2^14, 2^15),
-//   hi = fp16(x 2^e),  lo = fp16((x 2^e - hi) 2^11),   x 2^e = hi + lo 2^-11 (1 + d), |d| <= 2^-12,
-// so the pair holds x to 2^-23 of itself (fp32 itself: 2^-24) for every |x| within 2^-28 of the
-// largest, and to 2^-51 of the largest below that. The factor 2^11 keeps lo out of fp16's
+//   hi = fp16(x 2^e),  lo = fp16((x 2^e - hi) 2^11),   x 2^e = hi + lo 2^-11 (1 + d), |d| <= 2^-11,
+// so the pair holds x to 2^-23 of itself (fp32 itself: 2^-24) for every |x| within 2^-27 of the
+// largest, and to 2^-50 of the largest below that. The factor 2^11 keeps lo out of fp16's
 // subnormals. A token has its own e because the tokens of a call may differ by any factor (padded places,
-// outliers); where tokens are summed over, see PanelJob (vbsr_panels.cuh). A product of two operands is hi hi + 2^-11 (hi lo + lo hi); lo lo is below 2^-22 of it
-// and left out. The two sums go to accumulators of their own (fp32, in TMEM) and are joined, and
+// outliers); where tokens are summed over, see PanelJob (vbsr_panels.cuh). A product of two operands is
+// hi hi + 2^-11 (hi lo + lo hi); lo lo is below 2^-22 of it and left out. The two sums go to accumulators of their own (fp32, in TMEM) and are joined, and
 // the powers of two taken back, in the epilogue. A pair is four bytes, as the fp32 number is: the
 // weights are laid out as pairs once (4 bytes per value streamed, no conversion in the kernel), the
 // activations by a pre-pass of each call. Against 3xTF32, which this replaces for these operators,
@@ -138,7 +138,10 @@ constexpr int kPairThreads = 32 * (kEpilogueWarp + 4 * kEpilogueGroups);
 // warpgroups: producers, MMA warps, and two of the epilogue.
 constexpr int kProducerRegs = 88, kMmaRegs = 40, kEpilogueRegs = 192;
 static_assert(kPairThreads == 512 && kProducerRegs + kMmaRegs + 2 * kEpilogueRegs <= 4 * 128, "registers");
-constexpr int kChunkSteps = 12;  // 8: error 3.0e-7, 1 token 49.8 us; 12: 4.6e-7, 42.9 us; 16: 6.1e-7, 42.3 us
+// Against 64 bits (2-norm) and fp32 arithmetic's 1.5e-7 to 3.3e-7, six shapes forward: 8 steps 2.9e-7 to 3.8e-7, 12
+// steps 4.3e-7 to 5.1e-7. 12 steps are faster for few tokens: 1 token 142 and 150 us with its weights laid out, 8
+// tokens of 256 rows 26.6 and 27.7, 32 tokens 290 and 293; 517 tokens and the training steps are the same within 1%.
+constexpr int kChunkSteps = 8;
 constexpr int kZeroBytes = 2048;   // 128 rows of 16 bytes
 constexpr int kTailBytes = 4096;   // MMAs read up to this far behind a tile's own rows
 constexpr int kGradTokens = 64;    // kWeightGrad: tokens per stage, at most
