@@ -231,7 +231,10 @@ vbsr_status build_gated(vbsr_gated* p, const MatrixData& gate, const MatrixData&
   std::vector<uint32_t> group_col;
   std::vector<uint32_t> g0[2], ng[2];
   std::vector<PackRow> pack;
-  group_col.reserve(size_t(8 * (gate.nnzb + up.nnzb)));
+  int64_t columns = 0;
+  for (const MatrixData* d : m)
+    for (const int64_t w : d->h_sum_w) columns += w;
+  group_col.reserve(size_t(columns / 8));
   pack.reserve(size_t(2 * R));
   for (int which = 0; which < 2; ++which) {
     const MatrixData& d = *m[which];

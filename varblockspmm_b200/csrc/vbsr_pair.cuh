@@ -43,7 +43,7 @@
 // are on the M side (64 or 128 rows): with weights there, blocks of 8 to 56 rows would leave most of an
 // MMA empty. What bounds it: the copies into shared memory. A weight group of 32 h bytes needs 32 R
 // bytes of activations, from L2, so few tokens run at the weights' HBM rate and many at the
-// L2-to-shared-memory rate, h / 2 operations per byte (517 tokens, 3.3 GB into shared memory: 11.8 TB/s).
+// L2-to-shared-memory rate, h / 2 operations per byte (517 tokens, 3.5 GB into shared memory: 12.5 TB/s).
 #pragma once
 #include <cuda_fp16.h>
 
