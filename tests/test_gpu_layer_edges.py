@@ -155,3 +155,104 @@ def test_int8_every_way_of_quantising(cuda, tokens, K, held, offset):
     # the sum, the product of the scales and the result round once each
     assert np.all(np.abs(got[good] - want[good]) <= 4 * ref.U * np.abs(want[good]))
     assert np.isnan(got[bad]).all()
+
+
+def long_case(torch, tokens, rows, cols, degree, seed):
+    m = ref.matrix(rows, cols, degree, seed)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    X = torch.randn(tokens, m.scalar_cols(), generator=g, device="cuda")
+    return m, X, g
+
+
+@pytest.mark.parametrize("tokens,rows,cols,degree", [
+    (4096, 12, 14, 6), (4097, 3, 4, 2), (65535, 2, 3, 2), (70001, 3, 4, 2), (1 << 22, 1, 1, 1)])
+def test_many_tokens(cuda, tokens, rows, cols, degree):
+    """Up to the largest number of tokens: all three directions and both ways of giving 8-bit activations."""
+    torch = cuda
+    m, X, g = long_case(torch, tokens, rows, cols, degree, 5 if tokens < 1 << 22 else 6)
+    M, K = m.scalar_rows(), m.scalar_cols()
+    A = torch.from_numpy(ref.dense(m)).cuda()
+    absA = A.abs()
+    bare, w = vb.Matrix(m, structure_only=True), torch.from_numpy(m.values).cuda()
+    plan = vb.GatedPlan(bare, bare, vb.Activation.ReLU)
+    plan.set_values(w, -w)
+    H, G, U = (torch.full((tokens, M), float("nan"), device="cuda") for _ in range(3))
+    plan.execute(X, H, G, U)
+    plan.check_status()
+    step = 1 << 16  # compared in pieces, in 64 bits
+
+    def held(got, want, tol):
+        assert bool(((got.double() - want).abs() <= tol + 1e-37).all())
+
+    n = ref.max_row_products(m)
+    for t in range(0, tokens, step):
+        x = X[t:t + step].double()
+        want = x @ A.T
+        tol = ref.product_tolerance(n, x.abs() @ absA.T)
+        held(G[t:t + step], want, tol)
+        held(U[t:t + step], -want, tol)
+        held(H[t:t + step], G[t:t + step].double().clamp(min=0) * U[t:t + step].double(), 2e-7 * want.square() + 1e-30)
+    dH = 1e-3 * torch.randn(tokens, M, generator=g, device="cuda")
+    dX = torch.full_like(X, float("nan"))
+    dw = [torch.full((len(m.values),), float("nan"), device="cuda") for _ in range(2)]
+    plan.backward(X, G, U, dH, dX, *dw)
+    plan.check_status()
+    sums, mags = [torch.zeros(M, K, dtype=torch.float64, device="cuda") for _ in range(2)], \
+        [torch.zeros(M, K, dtype=torch.float64, device="cuda") for _ in range(2)]
+    n = 2 * ref.max_col_products(m)
+    for t in range(0, tokens, step):
+        x, gg, u, dh = (v[t:t + step].double() for v in (X, G, U, dH))
+        d = [dh * u * (gg > 0), dh * gg.clamp(min=0)]
+        # dG and dU are rounded twice, then their product's bound
+        size = (d[0].abs() + d[1].abs()) @ absA
+        held(dX[t:t + step], (d[0] - d[1]) @ A, ref.product_tolerance(n, size) + 2 * ref.U * size)
+        for i in range(2):
+            sums[i] += d[i].T @ x
+            mags[i] += d[i].abs().T @ x.abs()
+    for i in range(2):
+        want, mag = ref.sampled(m, sums[i].cpu().numpy()), ref.sampled(m, mags[i].cpu().numpy())
+        got = dw[i].cpu().numpy().astype(np.float64)
+        # tokens are added 64 at a time
+        tol = ref.product_tolerance(min(tokens, 64) + tokens / 64, mag) + 2 * ref.U * mag
+        assert np.all(np.abs(got - want) <= tol), i
+    # 8 bits
+    q = torch.from_numpy(np.random.default_rng(1).integers(-127, 128, len(m.values)).astype(np.int8)).cuda()
+    rs = torch.rand(M, device="cuda") + 0.1
+    i8 = vb.Int8Plan(bare, q, rs)
+    C, C2, Q, ts = (torch.zeros(tokens, M, device="cuda"), torch.zeros(tokens, M, device="cuda"),
+                    torch.zeros(tokens, K, dtype=torch.int8, device="cuda"), torch.zeros(tokens, device="cuda"))
+    i8.execute_panel(X, C)
+    vb.quantize_panel(X, Q, ts, K)
+    i8.execute(Q, ts, C2)
+    i8.check_status()
+    assert torch.equal(C, C2)
+    Aq = torch.from_numpy(ref.dense(m, q.cpu().numpy())).cuda()
+    for t in range(0, tokens, step):
+        x = X[t:t + step]
+        want_ts = x.abs().amax(1) * torch.tensor(np.float32(1) / np.float32(127), device="cuda")
+        assert torch.equal(ts[t:t + step], want_ts)
+        want_q = torch.round(x.double() / want_ts.double()[:, None])
+        assert torch.equal(Q[t:t + step].double(), want_q)
+        want = (want_q @ Aq.T) * (want_ts.double()[:, None] * rs.double())
+        held(C[t:t + step], want, 4 * ref.U * want.abs())
+
+
+@pytest.mark.parametrize("tokens", [700, 4099])
+def test_int8_many_long_tokens(cuda, tokens):
+    """Clusters of held tokens, more than the GPU holds at once."""
+    torch = cuda
+    m = ref.matrix(4, 400, 30, 9, row_size=[8, 16, 64, 24], col_size=[48] * 400)
+    K = m.scalar_cols()
+    assert by_clusters(tokens, K)
+    X = torch.randn(tokens, K, device="cuda")
+    q = torch.from_numpy(np.random.default_rng(2).integers(-127, 128, len(m.values)).astype(np.int8)).cuda()
+    rs = torch.rand(m.scalar_rows(), device="cuda") + 0.1
+    plan = vb.Int8Plan(vb.Matrix(m, structure_only=True), q, rs)
+    C = torch.zeros(tokens, m.scalar_rows(), device="cuda")
+    plan.execute_panel(X, C)
+    plan.check_status()
+    ts = X.abs().amax(1) * torch.tensor(np.float32(1) / np.float32(127), device="cuda")
+    want = torch.round(X.double() / ts.double()[:, None]) @ torch.from_numpy(ref.dense(m, q.cpu().numpy())).cuda().T
+    want = want * (ts.double()[:, None] * rs.double())
+    assert bool(((C.double() - want).abs() <= 4 * ref.U * want.abs()).all())
