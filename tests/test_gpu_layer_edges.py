@@ -116,7 +116,7 @@ def by_clusters(tokens, K):
     (1, 968, True), (128, 960, True), (129, 960, False),  # one piece of the lanes' registers, just full and over
     (128, 2048, True), (129, 2048, False), (129, 3096, True), (341, 8184, True), (342, 8184, False),
     (682, 16384, True), (683, 16384, False), (683, 16392, True),  # longer ones: any number of tokens
-    (3, 20008, True), (33, 30720, True), (131, 30728, True),
+    (3, 20008, True), (33, 30712, True), (131, 30728, True),
     (2, 38400, True), (259, 38400, True), (2, 38408, False), (259, 38408, False)])
 @pytest.mark.parametrize("offset", [0, 1])
 def test_int8_every_way_of_quantising(cuda, tokens, K, held, offset):
