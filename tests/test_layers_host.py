@@ -80,3 +80,12 @@ def test_matrix_of_structure_only():
 
 def test_int8_set_values_of_a_null_plan():
     refused(_lib.vbsr_int8_set_values(None, None, None, None), "null plan")
+
+
+def test_int8_weights_and_scales_go_together():
+    """Refused before any array is read."""
+    import lm_reference as ref
+    m = vb.Matrix(ref.matrix(3, 4, 2, 1), structure_only=True)
+    for values, scale in ((256, None), (None, 256)):
+        with pytest.raises(vb.InvalidArgument, match="null values or row_scale"):
+            vb.Int8Plan(m, values, scale)
